@@ -392,6 +392,90 @@ typedef struct
 int tmi_dot_product_check(tmi_ctx_t* ctx, int32_t out_dtype, int64_t n, const void* imp_dev, const double* ref_dev,
                           const double* bnd_dev, int32_t ksb, int32_t set_number, tmi_dp_result_t* result);
 
+/* ---- the gated feed-forward block of transformers, in 16 and in 4 bits ----------------------------------
+ *
+ * Operators beside TOSA's, with no counterpart in the reference.  They keep this header's conventions: device pointers,
+ * TMI_ERROR with a message before anything is launched, launches on the context's stream and no wait.  Element type
+ * (dtype) TMI_FP16 or TMI_BF16 for every tensor that is not packed; tensors are aligned to their elements at least (16
+ * bytes for packed weights), rows may lie any number of elements apart.  Products are summed in 32 bits and results
+ * rounded once, to nearest with ties to even.  Equal calls give equal bits.  A call with no rows, or no features
+ * to write, does nothing. */
+
+/* act(g) */
+enum
+{
+    TMI_ACT_SILU      = 1, /* g / (1 + exp(-g))                                             */
+    TMI_ACT_GELU      = 2, /* g (1 + erf(g / sqrt 2)) / 2                                   */
+    TMI_ACT_GELU_TANH = 3, /* g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2             */
+    TMI_ACT_RELU      = 4, /* max(g, 0); NaN stays; slope 0 at 0                            */
+    TMI_ACT_SIGMOID   = 5  /* 1 / (1 + exp(-g))                                             */
+};
+
+/* h = act(x gate^T) * (x up^T): x [rows][in_features], gate and up [hidden_features][in_features], h [rows][hidden_features].
+ * A row stride counts elements from one row to the next, 0 means that rows lie side by side; a tensor's gradient has its
+ * stride: ld_x for x and its gradient, ld_w for gate, up and theirs, ld_h for h, the pre-activations and the gradient
+ * of h. */
+typedef struct
+{
+    int64_t ld_x, ld_w, ld_h;
+    int32_t dtype;
+    int32_t activation; /* TMI_ACT_* */
+    int32_t rows, in_features, hidden_features;
+} tmi_gated_ffn_desc_t;
+
+/* The block in one kernel.  pre_gate_dev and pre_up_dev receive x gate^T and x up^T, rounded to dtype, for
+ * tmi_gated_ffn_backward; both NULL: they are not stored.  h is computed from the sums before that rounding. */
+int tmi_gated_ffn(tmi_ctx_t* ctx, const tmi_gated_ffn_desc_t* d, const void* x_dev, const void* gate_dev, const void* up_dev,
+                  void* h_dev, void* pre_gate_dev, void* pre_up_dev);
+
+/* Its gradients, from the pre-activations g and u and the gradient dh of h:
+ *   du = dh act(g), dg = dh u act'(g), d_x = dg gate + du up, d_gate = dg^T x, d_up = du^T x
+ * in 32 bits, with dg and du rounded to dtype before the products.  d_x_dev NULL, or d_gate_dev and d_up_dev both NULL:
+ * that part is not computed (x_dev, or gate_dev and up_dev, may then be NULL).  dg and du live in the context's scratch buffer (see tmi_ctx_reserve_workspace), with
+ * partial sums where the work is split over a long sum. */
+int tmi_gated_ffn_backward(tmi_ctx_t* ctx, const tmi_gated_ffn_desc_t* d, const void* x_dev, const void* gate_dev,
+                           const void* up_dev, const void* pre_gate_dev, const void* pre_up_dev, const void* d_h_dev,
+                           void* d_x_dev, void* d_gate_dev, void* d_up_dev);
+
+/* Weights [out_features][in_features] in 4 bits: w[n][k] = scale[n][k / group] * v[n][k], v in -8 ... 7.
+ *
+ * The packed form is one buffer.  A tile holds 16 rows x 128 columns in 1024 bytes; tile (tn, tk) of ceil(out_features / 16) x
+ * ceil(in_features / 128) lies at 1024 (tn * ceil(in_features / 128) + tk).  In it the 16-byte unit 16 (k % 32 / 8) + n % 16
+ * holds in its 32-bit word k % 128 / 32 the columns k % 8 = e, as v + 8 at bit 4 (e / 2) + 16 (e % 2).  Behind the tiles
+ * lie the scales in dtype, [tn][tk][16 rows][128 / group].  Rows and columns that fill up the last tiles hold v = 0
+ * and scale 0. */
+typedef struct
+{
+    int32_t dtype; /* of the scales, and of activations and results */
+    int32_t group; /* 32, 64 or 128 */
+    int32_t out_features, in_features;
+} tmi_int4_desc_t;
+
+/* Bytes of the packed form. */
+int tmi_int4_packed_bytes(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, size_t* bytes);
+
+/* Packs weights w_dev of dtype, rows ld_w elements apart (0: side by side), with scale = max |w| / 7 over each group,
+ * rounded to dtype, and v = w / scale rounded to the nearest integer (ties to even) in -7 ... 7; v = 0 where the scale is 0
+ * or w / scale is no number.  A group with an infinite or NaN weight has a scale that is infinite or NaN. */
+int tmi_quantize_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, const void* w_dev, int64_t ld_w, void* packed_dev);
+
+/* Packs given values, one int8 an element as TOSA's INT4 tensors are held here (kept to -8 ... 7), and scales
+ * [out_features][ceil(in_features / group)] of dtype. */
+int tmi_pack_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, const int8_t* values_dev, int64_t ld_values, const void* scales_dev,
+                  void* packed_dev);
+
+/* The weights that a packed form stands for, rounded to dtype. */
+int tmi_dequantize_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, const void* packed_dev, void* w_dev, int64_t ld_w);
+
+/* y = x w^T for a few rows of x (single tokens): y[m][n] = sum_k x[m][k] w[n][k], x [rows][in_features] rows ld_x apart, y
+ * [rows][out_features] rows ld_y apart.  Any number of rows is taken; the weights are read once for every 64 of them. */
+int tmi_matvec_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, int32_t rows, const void* x_dev, int64_t ld_x, const void* packed_dev,
+                    void* y_dev, int64_t ld_y);
+
+/* The gated block on packed weights, in one kernel: h = act(x gate^T) * (x up^T), both matrices as d describes them. */
+int tmi_gated_ffn_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, int32_t activation, int32_t rows, const void* x_dev, int64_t ld_x,
+                       const void* gate_dev, const void* up_dev, void* h_dev, int64_t ld_h);
+
 /* ---- validation only (no launch) ---------------------------------------------------------------- */
 
 /* The checks OpConv2d / OpDepthwiseConv2d::checkTensorAttributes and the head of eval() perform

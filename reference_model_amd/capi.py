@@ -18,6 +18,7 @@ VALID, UNPREDICTABLE, ERROR = 0, 1, 2
 INT8, INT16, INT32, INT48, FP32, FP16, BF16 = 3, 4, 5, 6, 7, 8, 9
 ROUND_SINGLE, ROUND_INEXACT, ROUND_DOUBLE = 1, 2, 3
 FLAG_SCALE_MULTIPLIER, FLAG_SCALE_SHIFT, FLAG_SCALE_VALUE, FLAG_SCALE_RESULT, FLAG_ZP_RESULT = 1, 2, 4, 8, 16
+ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_RELU, ACT_SIGMOID = 1, 2, 3, 4, 5
 KERNEL_AUTO, KERNEL_DIRECT, KERNEL_MFMA, KERNEL_GEMM, KERNEL_SLAB, KERNEL_POINTWISE, KERNEL_STREAM = 0, 1, 2, 3, 4, 5, 6
 
 F64 = -64  # host-side tag of the fp64 buffers of the precise / bounds passes (not a TOSA element type)
@@ -37,6 +38,8 @@ EXPORTS = [
     "tmi_conv2d_precise", "tmi_depthwise_conv2d_precise", "tmi_matmul_precise", "tmi_dot_product_check",
     "tmi_ctx_reserve_workspace", "tmi_transpose_conv2d_noalloc", "tmi_ctx_set_level", "tmi_clamp_fp",
     "tmi_ctx_set_precise_mode", "tmi_ctx_workspace_bytes", "tmi_ctx_trim_workspace",
+    "tmi_int4_packed_bytes", "tmi_quantize_int4", "tmi_pack_int4", "tmi_dequantize_int4", "tmi_matvec_int4", "tmi_gated_ffn_int4",
+    "tmi_gated_ffn", "tmi_gated_ffn_backward",
     "tmi_debug_launch_empty", "tmi_debug_tile_decode", "tmi_debug_last_launch_shape", "tmi_debug_stream",
 ]
 
@@ -105,6 +108,15 @@ class RescaleDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in (
         "in_dtype", "out_dtype", "scale32", "rounding_mode", "per_channel", "input_unsigned", "output_unsigned",
         "in_zp", "out_zp", "n_multiplier", "n_shift")]
+
+
+class GatedFfnDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("ld_x", "ld_w", "ld_h")] + [
+        (n, ctypes.c_int32) for n in ("dtype", "activation", "rows", "in_features", "hidden_features")]
+
+
+class Int4Desc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "group", "out_features", "in_features")]
 
 
 class TmiError(RuntimeError):
@@ -176,6 +188,15 @@ def load_library() -> ctypes.CDLL:
     lib.tmi_depthwise_conv2d_precise.argtypes = [vp, ctypes.POINTER(ConvDesc), vp, vp, vp, i32, i32, vp]
     lib.tmi_matmul_precise.argtypes = [vp, i32, i32, i32, i32, i32, vp, vp, i32, vp]
     lib.tmi_dot_product_check.argtypes = [vp, i32, i64, vp, vp, vp, i32, i32, ctypes.POINTER(DpResult)]
+    ffn, int4 = ctypes.POINTER(GatedFfnDesc), ctypes.POINTER(Int4Desc)
+    lib.tmi_gated_ffn.argtypes = [vp, ffn] + [vp] * 6
+    lib.tmi_gated_ffn_backward.argtypes = [vp, ffn] + [vp] * 9
+    lib.tmi_int4_packed_bytes.argtypes = [vp, int4, ctypes.POINTER(ctypes.c_size_t)]
+    lib.tmi_quantize_int4.argtypes = [vp, int4, vp, i64, vp]
+    lib.tmi_pack_int4.argtypes = [vp, int4, vp, i64, vp, vp]
+    lib.tmi_dequantize_int4.argtypes = [vp, int4, vp, vp, i64]
+    lib.tmi_matvec_int4.argtypes = [vp, int4, i32, vp, i64, vp, vp, i64]
+    lib.tmi_gated_ffn_int4.argtypes = [vp, int4, i32, i32, vp, i64, vp, vp, vp, i64]
     lib.tmi_conv2d_check.argtypes = [vp, ctypes.POINTER(ConvDesc), i32]
     lib.tmi_rescale_check.argtypes = [vp, ctypes.POINTER(RescaleDesc), i32, i32]
     for name in EXPORTS:
@@ -403,6 +424,48 @@ class Context:
     def clamp_fp(self, dtype, n, inp, lo, hi, nan_mode, out) -> int:
         return self._check(self.lib.tmi_clamp_fp(self.handle, dtype, n, _ptr(inp), float(lo), float(hi), int(nan_mode),
                                                  _ptr(out)))
+
+    # -- the gated feed-forward block, in 16 and in 4 bits ---------------------------------------
+    # Row strides (ld_*) count elements; 0: rows lie side by side.
+    @staticmethod
+    def gated_ffn_desc(dtype, activation, rows, in_features, hidden_features, ld_x=0, ld_w=0, ld_h=0) -> GatedFfnDesc:
+        return GatedFfnDesc(ld_x, ld_w, ld_h, dtype, activation, rows, in_features, hidden_features)
+
+    @staticmethod
+    def int4_desc(dtype, group, out_features, in_features) -> Int4Desc:
+        return Int4Desc(dtype, group, out_features, in_features)
+
+    def gated_ffn(self, d: GatedFfnDesc, x, gate, up, h, pre_gate=None, pre_up=None) -> int:
+        """h = act(x gate^T) * (x up^T); pre_gate and pre_up receive the two products for gated_ffn_backward"""
+        return self._check(self.lib.tmi_gated_ffn(self.handle, ctypes.byref(d), _ptr(x), _ptr(gate), _ptr(up), _ptr(h), _ptr(pre_gate),
+                                                  _ptr(pre_up)))
+
+    def gated_ffn_backward(self, d: GatedFfnDesc, x, gate, up, pre_gate, pre_up, d_h, d_x, d_gate, d_up) -> int:
+        """the gradients of x, gate and up (None: not computed) from that of h"""
+        return self._check(self.lib.tmi_gated_ffn_backward(self.handle, ctypes.byref(d), _ptr(x), _ptr(gate), _ptr(up), _ptr(pre_gate),
+                                                           _ptr(pre_up), _ptr(d_h), _ptr(d_x), _ptr(d_gate), _ptr(d_up)))
+
+    def int4_packed_bytes(self, d: Int4Desc) -> int:
+        n = ctypes.c_size_t(0)
+        self._check(self.lib.tmi_int4_packed_bytes(self.handle, ctypes.byref(d), ctypes.byref(n)))
+        return n.value
+
+    def quantize_int4(self, d: Int4Desc, w, ld_w, packed) -> int:
+        return self._check(self.lib.tmi_quantize_int4(self.handle, ctypes.byref(d), _ptr(w), ld_w, _ptr(packed)))
+
+    def pack_int4(self, d: Int4Desc, values, ld_values, scales, packed) -> int:
+        return self._check(self.lib.tmi_pack_int4(self.handle, ctypes.byref(d), _ptr(values), ld_values, _ptr(scales), _ptr(packed)))
+
+    def dequantize_int4(self, d: Int4Desc, packed, w, ld_w) -> int:
+        return self._check(self.lib.tmi_dequantize_int4(self.handle, ctypes.byref(d), _ptr(packed), _ptr(w), ld_w))
+
+    def matvec_int4(self, d: Int4Desc, rows, x, ld_x, packed, y, ld_y) -> int:
+        """y = x w^T for a few rows of x"""
+        return self._check(self.lib.tmi_matvec_int4(self.handle, ctypes.byref(d), rows, _ptr(x), ld_x, _ptr(packed), _ptr(y), ld_y))
+
+    def gated_ffn_int4(self, d: Int4Desc, activation, rows, x, ld_x, gate, up, h, ld_h) -> int:
+        return self._check(self.lib.tmi_gated_ffn_int4(self.handle, ctypes.byref(d), activation, rows, _ptr(x), ld_x, _ptr(gate), _ptr(up),
+                                                       _ptr(h), ld_h))
 
     def stream_probe(self, mode, src, dst, nbytes) -> int:
         return self._check(self.lib.tmi_debug_stream(self.handle, mode, _ptr(src), _ptr(dst), nbytes))

@@ -1,0 +1,221 @@
+// Weights in 4 bits with a scale for each group of columns: from 16-bit floats, from given values and scales, and back.
+//
+//   scale = round16(max |w| / 7) over the group, v = rint(w / scale) in -7 ... 7 (0 where the scale is 0), w' = v * scale
+//
+// A wave owns one tile of 16 rows x 128 columns, lane 16 q + r the columns 32 j + 8 q + (0 ... 7) of row r, j = 0 ... 3: the 32 weights whose
+// 16 bytes it stores, so a tile goes out as one kilobyte in a row, and the maximum over a group of 32 is a maximum over the four lanes of a row.
+// Bound by the 16-bit side: 2 bytes a weight against half of one.
+#include "tmi_ffn.h"
+
+namespace tmi
+{
+namespace
+{
+
+struct Int4Args
+{
+    const void* in;
+    const uint16_t* scales;    // given values only: [n][groups]
+    void* out;
+    int64_t ld;                // elements between rows on the unpacked side
+    int64_t tiles, groups;
+    int32_t n, k, tiles_k;
+};
+
+constexpr int kWaves = 4;
+
+// the largest bit pattern of |w| over the four lanes of a row; NaN has the largest of all and stays
+__device__ __forceinline__ uint32_t row_max(uint32_t v)
+{
+    uint32_t o = (uint32_t)__shfl_xor((int)v, 16);
+    v          = v > o ? v : o;
+    o          = (uint32_t)__shfl_xor((int)v, 32);
+    return v > o ? v : o;
+}
+
+// GIVEN: int8 values (kept to -8 ... 7) and scales; else 16-bit weights
+template <typename T, int PER, bool GIVEN>
+__global__ __launch_bounds__(64 * kWaves) void int4_pack_kernel(Int4Args a)
+{
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    const int64_t tile = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (tile >= a.tiles)
+        return;
+    const int64_t tn = tile / a.tiles_k;
+    const int kt     = (int)(tile - tn * a.tiles_k);
+    const int64_t n  = tn * kInt4Rows + r;
+    const bool live  = n < a.n;
+    const int k0     = kt * kInt4Cols;
+    v4i packed;
+    uint16_t scale[PER];
+    if constexpr (GIVEN)
+    {
+        const int8_t* row = static_cast<const int8_t*>(a.in) + (live ? n : 0) * a.ld;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+        {
+            uint32_t w = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+            {
+                const int k = k0 + 32 * j + 8 * q + e;
+                int v       = live && k < a.k ? row[k] : 0;
+                v           = v < -8 ? -8 : (v > 7 ? 7 : v);
+                w |= (uint32_t)(v + 8) << (4 * (e >> 1) + 16 * (e & 1));
+            }
+            packed[j] = (int)w;
+        }
+#pragma unroll
+        for (int g = 0; g < PER; g++)
+        {
+            const int64_t at = (int64_t)kt * PER + g;
+            scale[g]         = live && at < a.groups ? a.scales[n * a.groups + at] : 0;
+        }
+    }
+    else
+    {
+        const uint16_t* row = static_cast<const uint16_t*>(a.in) + (live ? n : 0) * a.ld;
+        v4i w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            w[j] = load8(row, k0 + 32 * j + 8 * q, live ? a.k : 0);
+        uint32_t m[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+        {
+            m[j] = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+            {
+                const uint32_t b = half_of(w[j], e) & 0x7FFFu;
+                m[j]             = m[j] > b ? m[j] : b;
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < PER; g++)
+        {
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = g * 4 / PER; j < (g + 1) * 4 / PER; j++)
+                top = top > m[j] ? top : m[j];
+            scale[g]      = to_bits16<T>(from_bits16<T>((uint16_t)row_max(top)) / 7.0f);
+            const float s = from_bits16<T>(scale[g]);
+#pragma unroll
+            for (int j = g * 4 / PER; j < (g + 1) * 4 / PER; j++)
+            {
+                uint32_t word = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                {
+                    // a division, correctly rounded: no quotient of two 16-bit floats lies so near a half that rint could go the other way
+                    const float t = rintf(from_bits16<T>(half_of(w[j], e)) / s);
+                    const int v   = t == t ? (int)fminf(fmaxf(t, -7.0f), 7.0f) : 0;    // 0 / 0, inf / inf and what is divided by NaN
+                    word |= (uint32_t)(v + 8) << (4 * (e >> 1) + 16 * (e & 1));
+                }
+                packed[j] = (int)word;
+            }
+        }
+    }
+    uint8_t* out = static_cast<uint8_t*>(a.out);
+    *reinterpret_cast<v4i*>(out + tile * kInt4TileBytes + lane * 16) = packed;
+    if (q == 0)
+    {
+        uint16_t* s = reinterpret_cast<uint16_t*>(out + int4_scale_at(a.tiles, tile, PER)) + r * PER;
+#pragma unroll
+        for (int g = 0; g < PER; g++)
+            s[g] = scale[g];
+    }
+}
+
+template <typename T, int PER>
+__global__ __launch_bounds__(64 * kWaves) void int4_unpack_kernel(Int4Args a)
+{
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    const int64_t tile = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (tile >= a.tiles)
+        return;
+    const int64_t tn = tile / a.tiles_k;
+    const int kt     = (int)(tile - tn * a.tiles_k);
+    const int64_t n  = tn * kInt4Rows + r;
+    if (n >= a.n)
+        return;
+    const uint8_t* in  = static_cast<const uint8_t*>(a.in);
+    const v4i packed   = *reinterpret_cast<const v4i*>(in + tile * kInt4TileBytes + lane * 16);
+    const uint16_t* sc = reinterpret_cast<const uint16_t*>(in + int4_scale_at(a.tiles, tile, PER)) + r * PER;
+    uint16_t* row      = static_cast<uint16_t*>(a.out) + n * a.ld;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+    {
+        const float s = from_bits16<T>(sc[j * PER / 4]);
+        v4i w;
+#pragma unroll
+        for (int p = 0; p < 4; p++)
+        {
+            const uint32_t u = (uint32_t)packed[j] >> (4 * p);
+            w[p] = (int)pack16<T>((float)((int)(u & 15) - 8) * s, (float)((int)(u >> 16 & 15) - 8) * s);
+        }
+        store8(row, (int64_t)kt * kInt4Cols + 32 * j + 8 * q, a.k, w);
+    }
+}
+
+template <typename F>
+bool per_group(int group, F&& f)
+{
+    switch (group)
+    {
+        case 32:
+            return f(std::integral_constant<int, 4>()), true;
+        case 64:
+            return f(std::integral_constant<int, 2>()), true;
+        case 128:
+            return f(std::integral_constant<int, 1>()), true;
+        default:
+            return false;
+    }
+}
+
+Int4Args int4_args(int32_t n, int32_t k, int group, const void* in, int64_t ld, void* out)
+{
+    Int4Args a{};
+    a.in = in, a.out = out, a.ld = ld, a.n = n, a.k = k;
+    a.tiles_k = (int32_t)int4_tiles(k, kInt4Cols);
+    a.tiles   = int4_tiles(n, kInt4Rows) * a.tiles_k;
+    a.groups  = int4_tiles(k, group);
+    return a;
+}
+
+}    // namespace
+
+const char* launch_int4_pack(hipStream_t st, int32_t dtype, int32_t group, int32_t n, int32_t k, const void* w, int64_t ld, const void* scales,
+                             void* packed)
+{
+    Int4Args a    = int4_args(n, k, group, w, ld, packed);
+    a.scales      = static_cast<const uint16_t*>(scales);
+    const int grid = (int)int4_tiles(a.tiles, kWaves);
+    const bool ok  = per_group(group, [&](auto per) {
+        constexpr int PER = decltype(per)::value;
+        if (scales)
+            int4_pack_kernel<_Float16, PER, true><<<grid, 64 * kWaves, 0, st>>>(a);    // (the scales pass through as bits)
+        else if (dtype == TMI_BF16)
+            int4_pack_kernel<bf16_t, PER, false><<<grid, 64 * kWaves, 0, st>>>(a);
+        else
+            int4_pack_kernel<_Float16, PER, false><<<grid, 64 * kWaves, 0, st>>>(a);
+    });
+    return !ok ? nullptr : scales ? "int4_pack" : "int4_quantize";
+}
+
+const char* launch_int4_unpack(hipStream_t st, int32_t dtype, int32_t group, int32_t n, int32_t k, const void* packed, void* w, int64_t ld)
+{
+    const Int4Args a = int4_args(n, k, group, packed, ld, w);
+    const int grid   = (int)int4_tiles(a.tiles, kWaves);
+    const bool ok    = per_group(group, [&](auto per) {
+        constexpr int PER = decltype(per)::value;
+        if (dtype == TMI_BF16)
+            int4_unpack_kernel<bf16_t, PER><<<grid, 64 * kWaves, 0, st>>>(a);
+        else
+            int4_unpack_kernel<_Float16, PER><<<grid, 64 * kWaves, 0, st>>>(a);
+    });
+    return ok ? "int4_dequantize" : nullptr;
+}
+
+}    // namespace tmi

@@ -2034,4 +2034,262 @@ int tmi_clamp_fp(tmi_ctx_t* ctx, int32_t dtype, int64_t n, const void* in_dev, f
     return after_launch(ctx, launch_clamp_fp(ctx->stream, dtype, in_dev, out_dev, n, min_val, max_val, nan_mode));
 }
 
+// ---- the gated feed-forward block and 4-bit weights ----------------------------------------------------------------------
+
+constexpr int32_t kFfnFewRows = 64;    // up to here the gated block in 16 bits runs as products of a few rows
+
+static bool ffn_dtype(int32_t dtype)
+{
+    return dtype == TMI_FP16 || dtype == TMI_BF16;
+}
+
+static bool unaligned(const void* p, uintptr_t to)
+{
+    return ((uintptr_t)p & (to - 1)) != 0;
+}
+
+// The row stride `ld` of rows of `width` elements, 0 standing for `width`; false where rows would overlap, or where the last of `rows`
+// would end beyond 2^62 elements.
+static bool row_stride(int64_t& ld, int64_t width, int64_t rows)
+{
+    if (ld == 0)
+        ld = width;
+    return ld >= width && (ld == 0 || rows <= (int64_t(1) << 62) / ld);
+}
+
+static int validate_int4(tmi_ctx* ctx, const char* op, const tmi_int4_desc_t* d)
+{
+    if (!d)
+        return fail(ctx, "%s: null descriptor", op);
+    if (!ffn_dtype(d->dtype))
+        return fail(ctx, "%s: the data type must be FP16 or BF16", op);
+    if (d->group != 32 && d->group != 64 && d->group != 128)
+        return fail(ctx, "%s: groups of %d columns: 32, 64 or 128 are wanted", op, d->group);
+    if (d->out_features < 0 || d->in_features < 0)
+        return fail(ctx, "%s: negative tensor dimension", op);
+    const int64_t tiles_n = ((int64_t)d->out_features + 15) / 16, tiles_k = ((int64_t)d->in_features + 127) / 128;
+    if (tiles_n > (int64_t(1) << 22) || tiles_n * tiles_k > (int64_t(1) << 25))
+        return fail(ctx, "%s: %d x %d weights are more than one call takes (2^25 tiles of 16 x 128)", op, d->out_features, d->in_features);
+    return TMI_VALID;
+}
+
+static size_t int4_packed_size(const tmi_int4_desc_t* d)
+{
+    const size_t tiles = ((size_t)d->out_features + 15) / 16 * (((size_t)d->in_features + 127) / 128);
+    return tiles * (1024 + 32 * (128 / (size_t)d->group));
+}
+
+int tmi_int4_packed_bytes(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, size_t* bytes)
+{
+    if (!ctx)
+        return TMI_ERROR;
+    const int rc = validate_int4(ctx, "int4_packed_bytes", d);
+    if (rc != TMI_VALID)
+        return rc;
+    if (!bytes)
+        return fail(ctx, "int4_packed_bytes: null pointer");
+    *bytes = int4_packed_size(d);
+    return TMI_VALID;
+}
+
+// What packing and unpacking check in common; *empty: nothing to do
+static int check_int4_copy(tmi_ctx* ctx, const char* op, const tmi_int4_desc_t* d, const void* plain, uintptr_t align, int64_t& ld,
+                           const void* packed, bool* empty)
+{
+    const int rc = validate_int4(ctx, op, d);
+    if (rc != TMI_VALID)
+        return rc;
+    if (!row_stride(ld, d->in_features, d->out_features))
+        return fail(ctx, "%s: rows of %d elements cannot lie %lld apart", op, d->in_features, (long long)ld);
+    *empty = d->out_features == 0 || d->in_features == 0;
+    if (!*empty && (!plain || !packed))
+        return fail(ctx, "%s: null tensor pointer", op);
+    if (unaligned(plain, align))
+        return fail(ctx, "%s: a tensor is not aligned to its elements", op);
+    if (unaligned(packed, 16))
+        return fail(ctx, "%s: packed weights are not aligned to 16 bytes", op);
+    TMI_HIP(ctx, hipSetDevice(ctx->device));
+    if (*empty)
+        ctx->last_kernel = "empty";
+    return TMI_VALID;
+}
+
+int tmi_quantize_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, const void* w_dev, int64_t ld_w, void* packed_dev)
+{
+    if (!ctx)
+        return TMI_ERROR;
+    bool empty   = false;
+    const int rc = check_int4_copy(ctx, "quantize_int4", d, w_dev, 2, ld_w, packed_dev, &empty);
+    if (rc != TMI_VALID || empty)
+        return rc;
+    return after_launch(ctx, launch_int4_pack(ctx->stream, d->dtype, d->group, d->out_features, d->in_features, w_dev, ld_w, nullptr, packed_dev));
+}
+
+int tmi_pack_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, const int8_t* values_dev, int64_t ld_values, const void* scales_dev,
+                  void* packed_dev)
+{
+    if (!ctx)
+        return TMI_ERROR;
+    bool empty   = false;
+    const int rc = check_int4_copy(ctx, "pack_int4", d, values_dev, 1, ld_values, packed_dev, &empty);
+    if (rc != TMI_VALID || empty)
+        return rc;
+    if (!scales_dev)
+        return fail(ctx, "pack_int4: null tensor pointer");
+    if (unaligned(scales_dev, 2))
+        return fail(ctx, "pack_int4: a tensor is not aligned to its elements");
+    return after_launch(ctx, launch_int4_pack(ctx->stream, d->dtype, d->group, d->out_features, d->in_features, values_dev, ld_values, scales_dev,
+                                              packed_dev));
+}
+
+int tmi_dequantize_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, const void* packed_dev, void* w_dev, int64_t ld_w)
+{
+    if (!ctx)
+        return TMI_ERROR;
+    bool empty   = false;
+    const int rc = check_int4_copy(ctx, "dequantize_int4", d, w_dev, 2, ld_w, packed_dev, &empty);
+    if (rc != TMI_VALID || empty)
+        return rc;
+    return after_launch(ctx, launch_int4_unpack(ctx->stream, d->dtype, d->group, d->out_features, d->in_features, packed_dev, w_dev, ld_w));
+}
+
+// y = x w^T, or the gated block where `up` is given
+static int int4_rows(tmi_ctx* ctx, const char* op, const tmi_int4_desc_t* d, bool gated, int32_t activation, int32_t rows, const void* x, int64_t ld_x,
+                     const void* w, const void* up, void* out, int64_t ld_out)
+{
+    const int rc = validate_int4(ctx, op, d);
+    if (rc != TMI_VALID)
+        return rc;
+    if (gated && (activation < TMI_ACT_SILU || activation > TMI_ACT_SIGMOID))
+        return fail(ctx, "%s: unknown activation %d", op, activation);
+    if (rows < 0)
+        return fail(ctx, "%s: negative tensor dimension", op);
+    if (!row_stride(ld_x, d->in_features, rows) || !row_stride(ld_out, d->out_features, rows))
+        return fail(ctx, "%s: rows of %d or %d elements cannot lie %lld or %lld apart", op, d->in_features, d->out_features, (long long)ld_x,
+                    (long long)ld_out);
+    const bool empty = rows == 0 || d->out_features == 0;
+    if (!empty && (!out || (d->in_features > 0 && (!x || !w || (gated && !up)))))
+        return fail(ctx, "%s: null tensor pointer", op);
+    if (unaligned(x, 2) || unaligned(out, 2))
+        return fail(ctx, "%s: a tensor is not aligned to its elements", op);
+    if (unaligned(w, 16) || unaligned(up, 16))
+        return fail(ctx, "%s: packed weights are not aligned to 16 bytes", op);
+    TMI_HIP(ctx, hipSetDevice(ctx->device));
+    if (empty)
+    {
+        ctx->last_kernel = "empty";
+        return TMI_VALID;
+    }
+    return after_launch(ctx, launch_int4_rows(ctx->stream, d->dtype, d->group, gated, activation, rows, d->out_features, d->in_features, x, ld_x, w, up,
+                                              out, ld_out));
+}
+
+int tmi_matvec_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, int32_t rows, const void* x_dev, int64_t ld_x, const void* packed_dev,
+                    void* y_dev, int64_t ld_y)
+{
+    if (!ctx)
+        return TMI_ERROR;
+    return int4_rows(ctx, "matvec_int4", d, false, 0, rows, x_dev, ld_x, packed_dev, nullptr, y_dev, ld_y);
+}
+
+int tmi_gated_ffn_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, int32_t activation, int32_t rows, const void* x_dev, int64_t ld_x,
+                       const void* gate_dev, const void* up_dev, void* h_dev, int64_t ld_h)
+{
+    if (!ctx)
+        return TMI_ERROR;
+    return int4_rows(ctx, "gated_ffn_int4", d, true, activation, rows, x_dev, ld_x, gate_dev, up_dev, h_dev, ld_h);
+}
+
+// `d` checked, with its row strides filled in
+static int validate_gated_ffn(tmi_ctx* ctx, const char* op, const tmi_gated_ffn_desc_t* d, tmi_gated_ffn_desc_t& out)
+{
+    if (!d)
+        return fail(ctx, "%s: null descriptor", op);
+    if (!ffn_dtype(d->dtype))
+        return fail(ctx, "%s: the data type must be FP16 or BF16", op);
+    if (d->activation < TMI_ACT_SILU || d->activation > TMI_ACT_SIGMOID)
+        return fail(ctx, "%s: unknown activation %d", op, d->activation);
+    if (d->rows < 0 || d->in_features < 0 || d->hidden_features < 0)
+        return fail(ctx, "%s: negative tensor dimension", op);
+    out = *d;
+    if (!row_stride(out.ld_x, d->in_features, d->rows) || !row_stride(out.ld_w, d->in_features, d->hidden_features) ||
+        !row_stride(out.ld_h, d->hidden_features, d->rows))
+        return fail(ctx, "%s: rows of %d, %d and %d elements cannot lie %lld, %lld and %lld apart", op, d->in_features, d->in_features,
+                    d->hidden_features, (long long)d->ld_x, (long long)d->ld_w, (long long)d->ld_h);
+    // the tiles of a product are counted in 31 bits, and its summed index as well
+    const int64_t most = int64_t(1) << 28;
+    if (d->rows > most || d->in_features > most || d->hidden_features > most ||
+        ((int64_t)d->rows / 128 + 1) * ((int64_t)d->hidden_features / 64 + 1) > (int64_t(1) << 22) ||
+        ((int64_t)d->rows / 128 + 1) * ((int64_t)d->in_features / 64 + 1) > (int64_t(1) << 22) ||
+        ((int64_t)d->in_features / 128 + 1) * ((int64_t)d->hidden_features / 64 + 1) > (int64_t(1) << 22))
+        return fail(ctx, "%s: %d rows, %d x %d weights are more than one call takes", op, d->rows, d->hidden_features, d->in_features);
+    return TMI_VALID;
+}
+
+int tmi_gated_ffn(tmi_ctx_t* ctx, const tmi_gated_ffn_desc_t* desc, const void* x_dev, const void* gate_dev, const void* up_dev,
+                  void* h_dev, void* pre_gate_dev, void* pre_up_dev)
+{
+    if (!ctx)
+        return TMI_ERROR;
+    tmi_gated_ffn_desc_t d;
+    const int rc = validate_gated_ffn(ctx, "gated_ffn", desc, d);
+    if (rc != TMI_VALID)
+        return rc;
+    const bool empty = d.rows == 0 || d.hidden_features == 0;
+    if (!empty && (!h_dev || (d.in_features > 0 && (!x_dev || !gate_dev || !up_dev))))
+        return fail(ctx, "gated_ffn: null tensor pointer");
+    if (!pre_gate_dev != !pre_up_dev)
+        return fail(ctx, "gated_ffn: one of the pre-activations without the other");
+    for (const void* p : { x_dev, gate_dev, up_dev, (const void*)h_dev, (const void*)pre_gate_dev, (const void*)pre_up_dev })
+        if (unaligned(p, 2))
+            return fail(ctx, "gated_ffn: a tensor is not aligned to its elements");
+    TMI_HIP(ctx, hipSetDevice(ctx->device));
+    if (empty)
+    {
+        ctx->last_kernel = "empty";
+        return TMI_VALID;
+    }
+    if (d.rows <= kFfnFewRows)
+        return after_launch(ctx, launch_ffn_rows(ctx->stream, d.dtype, d.activation, d.rows, d.in_features, d.hidden_features, x_dev, d.ld_x, gate_dev,
+                                                 up_dev, d.ld_w, h_dev, pre_gate_dev, pre_up_dev, d.ld_h));
+    const size_t bytes = gated_ffn_scratch_bytes(d, x_dev, gate_dev, up_dev);
+    const bool parts   = bytes > 0 && optional_workspace(ctx, bytes);
+    return after_launch(ctx, launch_gated_ffn(ctx->stream, d, x_dev, gate_dev, up_dev, h_dev, pre_gate_dev, pre_up_dev,
+                                              parts ? ctx->workspace : nullptr, ctx->pages_dev));
+}
+
+int tmi_gated_ffn_backward(tmi_ctx_t* ctx, const tmi_gated_ffn_desc_t* desc, const void* x_dev, const void* gate_dev,
+                           const void* up_dev, const void* pre_gate_dev, const void* pre_up_dev, const void* d_h_dev,
+                           void* d_x_dev, void* d_gate_dev, void* d_up_dev)
+{
+    if (!ctx)
+        return TMI_ERROR;
+    tmi_gated_ffn_desc_t d;
+    const int rc = validate_gated_ffn(ctx, "gated_ffn_backward", desc, d);
+    if (rc != TMI_VALID)
+        return rc;
+    if (!d_gate_dev != !d_up_dev)
+        return fail(ctx, "gated_ffn_backward: one of the weights' gradients without the other");
+    // sums over no terms are zeros, so a gradient of some size is written whatever the other sizes are
+    const bool dx = d_x_dev && d.rows > 0 && d.in_features > 0, dw = d_gate_dev && d.hidden_features > 0 && d.in_features > 0;
+    if ((dx || dw) && d.rows > 0 && d.hidden_features > 0 &&
+        (!pre_gate_dev || !pre_up_dev || !d_h_dev || (dx && (!gate_dev || !up_dev)) || (dw && !x_dev)))
+        return fail(ctx, "gated_ffn_backward: null tensor pointer");
+    for (const void* p : { x_dev, gate_dev, up_dev, pre_gate_dev, pre_up_dev, d_h_dev, (const void*)d_x_dev, (const void*)d_gate_dev,
+                           (const void*)d_up_dev })
+        if (unaligned(p, 2))
+            return fail(ctx, "gated_ffn_backward: a tensor is not aligned to its elements");
+    TMI_HIP(ctx, hipSetDevice(ctx->device));
+    if (!dx && !dw)
+    {
+        ctx->last_kernel = "empty";
+        return TMI_VALID;
+    }
+    const int wrc = ensure_workspace(ctx, gated_ffn_backward_scratch_bytes(d, x_dev, gate_dev, up_dev, dx, dw));
+    if (wrc != TMI_VALID)
+        return wrc;
+    return after_launch(ctx, launch_gated_ffn_backward(ctx->stream, d, x_dev, gate_dev, up_dev, pre_gate_dev, pre_up_dev, d_h_dev, dx ? d_x_dev : nullptr,
+                                                       dw ? d_gate_dev : nullptr, dw ? d_up_dev : nullptr, ctx->workspace, ctx->pages_dev));
+}
+
 }    // extern "C"

@@ -1,0 +1,189 @@
+// What the feed-forward kernels share: the activations and their slopes, rounding to 16 bits, 16-byte loads at the ends of rows, the 16x16
+// matrix instruction of 16-bit floats, and the layout of 4-bit weights.
+#pragma once
+#include "tmi_mfma.h"
+
+namespace tmi
+{
+
+// act(g) in 32 bits.  The logistic forms hold where exp overflows: g / (1 + inf) is a zero.  GELU goes by erfc, which keeps its digits where
+// 1 + erf cancels, and its tanh form by (1 + tanh z) / 2 = 1 / (1 + exp(-2z)) for the same reason.
+__device__ __forceinline__ float logistic(float z)
+{
+    return 1.0f / (1.0f + expf(-z));
+}
+constexpr float kGeluTwoC  = 1.5957691216057308f;    // 2 sqrt(2 / pi)
+constexpr float kGeluCubic = 0.044715f;
+__device__ __forceinline__ float gelu_tanh_twice(float g)    // 2z
+{
+    return kGeluTwoC * (g + kGeluCubic * g * g * g);
+}
+__device__ __forceinline__ float act_value(int act, float g)
+{
+    switch (act)
+    {
+        case TMI_ACT_SILU:
+            return g / (1.0f + expf(-g));
+        case TMI_ACT_GELU:
+            return 0.5f * g * erfcf(-0.70710678118654752f * g);
+        case TMI_ACT_GELU_TANH:
+            return g / (1.0f + expf(-gelu_tanh_twice(g)));
+        case TMI_ACT_RELU:
+            return g < 0.0f ? 0.0f : g;    // (NaN stays)
+        default:
+            return logistic(g);
+    }
+}
+// act(g) and act'(g)
+__device__ __forceinline__ void act_both(int act, float g, float& value, float& slope)
+{
+    switch (act)
+    {
+        case TMI_ACT_SILU:
+        {
+            const float s = logistic(g);
+            value = g * s, slope = s * (1.0f + g * (1.0f - s));
+            return;
+        }
+        case TMI_ACT_GELU:
+        {
+            const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
+            value = g * cdf, slope = cdf + g * (expf(-0.5f * g * g) * 0.39894228040143268f);
+            return;
+        }
+        case TMI_ACT_GELU_TANH:
+        {
+            const float p = logistic(gelu_tanh_twice(g)), pq = p * (1.0f - p);
+            // far out p is 0 or 1 and g * g may be infinite
+            value = g * p, slope = pq == 0.0f ? p : p + g * pq * (kGeluTwoC * (1.0f + 3.0f * kGeluCubic * g * g));
+            return;
+        }
+        case TMI_ACT_RELU:
+            value = g < 0.0f ? 0.0f : g, slope = g > 0.0f ? 1.0f : 0.0f;
+            return;
+        default:
+        {
+            const float s = logistic(g);
+            value = s, slope = s * (1.0f - s);
+            return;
+        }
+    }
+}
+
+// ---- 16-bit floats: T is _Float16 or bf16_t (its bits) -----------------------------------------------------------------------
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+
+template <typename T>
+__device__ __forceinline__ uint16_t to_bits16(float v)    // rounded to nearest, ties to even
+{
+    if constexpr (sizeof(T) == 2 && !__is_same(T, bf16_t))
+        return __builtin_bit_cast(uint16_t, (_Float16)v);
+    else
+        return __builtin_bit_cast(uint16_t, (__bf16)v);
+}
+template <typename T>
+__device__ __forceinline__ float from_bits16(uint16_t b)
+{
+    if constexpr (__is_same(T, bf16_t))
+        return __uint_as_float((uint32_t)b << 16);
+    else
+        return (float)__builtin_bit_cast(_Float16, b);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi)
+{
+    return (uint32_t)to_bits16<T>(lo) | (uint32_t)to_bits16<T>(hi) << 16;
+}
+__device__ __forceinline__ uint16_t half_of(v4i v, int e)    // e a constant
+{
+    return (uint16_t)((uint32_t)v[e >> 1] >> (16 * (e & 1)));
+}
+
+// Eight elements of a row from column k on; zeros at and behind `end`, where nothing is read.  The row may begin at any element.
+__device__ __forceinline__ v4i load8(const uint16_t* row, int64_t k, int64_t end)
+{
+    if (k + 8 <= end)
+        return load16(reinterpret_cast<const uint8_t*>(row + k));
+    v4i v = { 0, 0, 0, 0 };
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        if (k + e < end)
+            v[e >> 1] |= (int)((uint32_t)row[k + e] << (16 * (e & 1)));
+    return v;
+}
+// the same way out
+__device__ __forceinline__ void store8(uint16_t* row, int64_t k, int64_t end, v4i v)
+{
+    if (k + 8 <= end)
+    {
+        __builtin_memcpy(row + k, &v, 16);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        if (k + e < end)
+            row[k + e] = half_of(v, e);
+}
+
+// One 16x16 step over 32 columns: lane l holds columns [8 (l / 16), + 8) of row l % 16 of either operand; of the result row 4 (l / 16) + i
+// of the first operand against row l % 16 of the second, i = 0..3.
+template <typename T>
+__device__ __forceinline__ v4f mma16(v4i a, v4i b, v4f c)
+{
+    if constexpr (__is_same(T, bf16_t))
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+// ---- 4-bit weights: the layout that tosa_mi355.h gives --------------------------------------------------------------------------
+constexpr int kInt4Rows = 16, kInt4Cols = 128, kInt4TileBytes = 1024;
+
+__host__ __device__ inline int64_t int4_tiles(int64_t n, int64_t per)
+{
+    return (n + per - 1) / per;
+}
+// byte of the scales of tile (row tile, column tile); `tiles` = all tiles, `per` = groups of a tile
+__host__ __device__ inline int64_t int4_scale_at(int64_t tiles, int64_t tile, int per)
+{
+    return tiles * kInt4TileBytes + tile * (kInt4Rows * 2) * per;
+}
+
+// The eight weights of a word as 16-bit floats, times kInt4Unit.  fp16: a nibble in the mantissa of 1024 gives 1024 + u, one four bits higher
+// 1024 + 16 u; u - 8 is then one exact packed operation.  bf16 has seven bits of mantissa and no packed arithmetic: the conversion of a signed
+// nibble to 32 bits (a sixteenth of its value), of which the upper halves are the bf16 numbers.
+template <typename T>
+constexpr float kInt4Unit = __is_same(T, bf16_t) ? 1.0f / 16 : 1.0f;
+
+template <typename T>
+__device__ __forceinline__ v4i int4_unpack(uint32_t w)
+{
+    v4i r;
+    if constexpr (__is_same(T, bf16_t))
+    {
+        const uint32_t s = w ^ 0x88888888u;    // v + 8 -> v, two's complement
+#pragma unroll
+        for (int p = 0; p < 4; p++)
+        {
+            const float lo = __builtin_amdgcn_cvt_off_f32_i4((int)(s >> (4 * p))), hi = __builtin_amdgcn_cvt_off_f32_i4((int)(s >> (16 + 4 * p)));
+            r[p] = (int)__builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+        }
+    }
+    else
+    {
+        const v2h off0 = { (_Float16)-1032.0f, (_Float16)-1032.0f }, off1 = { (_Float16)-72.0f, (_Float16)-72.0f };
+        const v2h sixteenth = { (_Float16)0.0625f, (_Float16)0.0625f };
+#pragma unroll
+        for (int p = 0; p < 4; p += 2)
+        {
+            const uint32_t s = w >> (4 * p);
+            const v2h lo = __builtin_bit_cast(v2h, (s & 0x000F000Fu) | 0x64006400u), hi = __builtin_bit_cast(v2h, (s & 0x00F000F0u) | 0x64006400u);
+            r[p]     = __builtin_bit_cast(int, lo + off0);
+            r[p + 1] = __builtin_bit_cast(int, __builtin_elementwise_fma(hi, sixteenth, off1));
+        }
+    }
+    return r;
+}
+
+}    // namespace tmi
