@@ -12,7 +12,6 @@
 // instructions for eight), their products are summed in 32 bits, and the sum over a group is multiplied by its scale: no weight is
 // rounded, and an infinite or NaN x does to a row what it does in the formula.
 #include "tmi_ffn.h"
-#include <type_traits>
 
 namespace tmi
 {
@@ -190,29 +189,38 @@ __global__ __launch_bounds__(64 * kMostWaves) void few_rows_kernel(RowsArgs a)
             for (int i = 0; i < 4; i++)
                 red[((wave * S + s) * MT + mt) * 256 + i * 64 + lane] = acc[s][mt][i];
     __syncthreads();
-    for (int o = threadIdx.x; o < NT * MT * 256; o += blockDim.x)
-    {
-        const int t = o / (MT * 256), mt = o / 256 % MT, ln = o & 63;
-        const int64_t n = ((int64_t)nb * NT + t) * 16 + (ln & 15);
-        const int64_t m = row0 + 16 * mt + (ln >> 4) * 4 + (o >> 6 & 3);
-        if (n >= a.n || m >= a.rows)
-            continue;
-        constexpr float unit = DENSE ? 1.0f : 1.0f / kInt4Unit<T>;
-        float v[2] = { 0.0f, 0.0f };
-#pragma unroll
-        for (int half = 0; half < (GATED ? 2 : 1); half++)
+    auto results = [&](auto ACT) {
+        for (int o = threadIdx.x; o < NT * MT * 256; o += blockDim.x)
         {
-            const int s = GATED ? 2 * t + half : t;
-            for (int w = 0; w < waves; w++)
-                v[half] += red[((w * S + s) * MT + mt) * 256 + (o & 255)];
-            v[half] *= unit;
+            const int t = o / (MT * 256), mt = o / 256 % MT, ln = o & 63;
+            const int64_t n = ((int64_t)nb * NT + t) * 16 + (ln & 15);
+            const int64_t m = row0 + 16 * mt + (ln >> 4) * 4 + (o >> 6 & 3);
+            if (n >= a.n || m >= a.rows)
+                continue;
+            constexpr float unit = DENSE ? 1.0f : 1.0f / kInt4Unit<T>;
+            float v[2] = { 0.0f, 0.0f };
+#pragma unroll
+            for (int half = 0; half < (GATED ? 2 : 1); half++)
+            {
+                const int s = GATED ? 2 * t + half : t;
+                for (int w = 0; w < waves; w++)
+                    v[half] += red[((w * S + s) * MT + mt) * 256 + (o & 255)];
+                v[half] *= unit;
+            }
+            const int64_t at = m * a.ldo + n;
+            if constexpr (GATED)
+                a.out[at] = to_bits16<T>(act_value<decltype(ACT)::value>(v[0]) * v[1]);
+            else
+                a.out[at] = to_bits16<T>(v[0]);
+            if constexpr (GATED && DENSE)
+                if (a.pre_gate)
+                    a.pre_gate[at] = to_bits16<T>(v[0]), a.pre_up[at] = to_bits16<T>(v[1]);
         }
-        const int64_t at = m * a.ldo + n;
-        a.out[at]        = to_bits16<T>(GATED ? act_value(a.act, v[0]) * v[1] : v[0]);
-        if constexpr (GATED && DENSE)
-            if (a.pre_gate)
-                a.pre_gate[at] = to_bits16<T>(v[0]), a.pre_up[at] = to_bits16<T>(v[1]);
-    }
+    };
+    if constexpr (GATED)
+        for_act(a.act, results);
+    else
+        results(0);
 }
 
 template <typename T, int PER, int MT, int NT, bool GATED>

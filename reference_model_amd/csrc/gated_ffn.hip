@@ -1,23 +1,24 @@
 // The gated feed-forward block on many rows, and its gradients, on the matrix cores:
 //
 //   forward    h[m][f]  = act(sum_d x[m][d] gate[f][d]) * (sum_d x[m][d] up[f][d])
-//   slopes     dp[m]    = [ dh u act'(g) | dh act(g) ], rows of 2 FP elements, FP = F up to whole blocks of 64, zeros behind F
+//   slopes     dp[m]    = [ dh u act'(g) | dh act(g) ], 2 FP elements, FP = F up to whole blocks of 64, zeros behind F
 //   d_x        dx[m][d] = sum_f dp[m][f] gate[f][d] + dp[m][FP + f] up[f][d]
 //   d_w        dw[f][d] = sum_m dp[m][f] x[m][d], f over gate and up
 //
 // One kernel makes all three products.  The operand whose index runs along an output row ("columns": weights, weights, x) is the first of the
-// 32x32x16 matrix instruction, so that a lane owns 16 neighbouring results of one row; the other ("rows": x, dp, dp) is the second.  An operand
+// 16x16x32 matrix instruction, so that a lane owns four neighbouring results of one row; the other ("rows": x, dp, dp) is the second.  (32x32x16
+// does as many operations a clock, but takes more power for them: 1.82 PFLOP/s on random bf16 numbers and nothing else, against 2.03.)  An operand
 // lies in memory with the summed index innermost (forward: both; d_x: dp) or outermost (d_x: the weights; d_w: both).  Either way 16-byte pieces
 // go to LDS as they lie; an outermost one comes out through the transposing reads ds_read_b64_tr_b16.  So nothing is transposed in memory.
 //
-// The forward pass deals gate and up rows of the same 32 features to one wave as its two column tiles: activation and product are done on the
+// The forward pass deals gate and up rows of the same 32 features to one wave as its four column tiles: activation and product are done on the
 // accumulators, and the pre-activations leave the chip only if they are asked for.
 //
-// LDS: a stage holds 64 of the summed index.  Innermost: rows of 128 bytes, 16-byte piece c of row r at c ^ (r / 2 % 8).  Outermost: 64 rows
-// of the tile's width, their 64-byte segments moved by the row's number mod 4.  Both keep the 16 (32) lanes that the LDS serves at once on
-// banks of their own.
+// LDS is a ring of stages of 32 of the summed index (96 KB of operands in flight behind the one in use at 256 x 256).  Innermost: rows of 64
+// bytes, their 16-byte pieces permuted by the row.  Outermost: 32 rows of the tile's width, their 32-byte segments permuted by the row.  Both keep
+// the 16 (32) lanes that the LDS serves at once on banks of their own.  Pieces that are whole go from global memory straight into LDS; where
+// rows begin at any element or end inside a piece they go through registers, two blocks ahead.
 #include "tmi_ffn.h"
-#include <type_traits>
 
 namespace tmi
 {
@@ -44,36 +45,53 @@ struct GemmFfnArgs
     int32_t K;                 // summed index (of one half, for d_x)
     int32_t half;              // FP, the columns of each half of dp
     int32_t features;          // F
-    int32_t blocks;            // of 64 of the summed index
+    int32_t blocks;            // of 32 of the summed index
     int32_t tiles_m, tiles_n, tiles, per_xcd;
     int32_t splits, per_split; // blocks of a split
     int32_t act;
 };
 
+// Innermost: piece c of row r lies at c ^ swizzle_in(r).  The LDS serves 16-byte reads of 16 lanes at once, of each half wave the quads (4 lanes)
+// {0, 3, 5, 6} and then {1, 2, 4, 7}; lane l reads piece l / 16 of row l % 16.  Rows of a quad differ in r % 4, that is in which 64 of 256
+// bytes they use; of the quads of a set two are of the first piece and two of the second, and 0, 3, 2, 1 for the rows' r / 4 keeps all four apart.
 __device__ __forceinline__ int swizzle_in(int r)
 {
-    return (r >> 1) & 7;
+    const int q = (r >> 2) & 3;
+    return (q ^ (q << 1)) & 3;
+}
+// Outermost: 32-byte segment c of row k lies at c ^ swizzle_out(k).  A transposing read serves 32 lanes at once: 32 bytes of the rows k % 8 = 0 ... 3
+// (or 4 ... 7) of two neighbouring eights.
+__device__ __forceinline__ int swizzle_out(int k)
+{
+    return (k & 3) | (k >> 1 & 4);
 }
 
 constexpr int kGroup = 8;    // row tiles that neighbouring workgroups share column tiles over
+constexpr int kBlock = 32;   // of the summed index
 
-template <typename T, int OP, int WC, int WR, int RT, bool FAST>
+// stages of the ring: all of the LDS for one workgroup of eight waves or two of four; through registers, what that needs
+template <bool DIRECT>
+constexpr int kRing = DIRECT ? 5 : 4;
+
+// WC x WR waves (columns x rows) of 64 columns and 16 RT rows each
+template <typename T, int OP, int WC, int WR, int RT, bool DIRECT>
 __global__ __launch_bounds__(64 * WC * WR, 2) void gated_gemm_kernel(GemmFfnArgs a)
 {
-    constexpr int THREADS  = 64 * WC * WR;
-    constexpr int BN       = 64 * WC, BM = 32 * RT * WR;
-    constexpr bool CIN     = OP == OP_FORWARD;    // summed index innermost: columns operand
-    constexpr bool RIN     = OP != OP_DW;         // rows operand
-    constexpr int CB       = BN * 128, STAGE = (BN + BM) * 128;
-    constexpr int CL       = BN * 8 / THREADS, RL = BM * 8 / THREADS;    // 16-byte loads of a thread and block
-    constexpr int TN       = CIN ? BN / 2 : BN;    // results a tile's columns make
-    static_assert(CL * THREADS == BN * 8 && RL * THREADS == BM * 8, "a block must split evenly over the threads");
+    constexpr int THREADS = 64 * WC * WR;
+    constexpr int BN = 64 * WC, BM = 16 * RT * WR;
+    constexpr int CT = 4;    // column tiles of a wave (forward: gate, gate, up, up)
+    constexpr bool CIN = OP == OP_FORWARD;    // summed index innermost: columns operand
+    constexpr bool RIN = OP != OP_DW;         // rows operand
+    constexpr int CB = BN * 64, STAGE = (BN + BM) * 64, RING = kRing<DIRECT>;
+    constexpr int CL = BN * 4 / THREADS, RL = BM * 4 / THREADS, LOADS = CL + RL;    // 16-byte loads of a thread and block
+    constexpr int TN = CIN ? BN / 2 : BN;                                            // results a tile's columns make
+    static_assert(CL * THREADS == BN * 4 && RL * THREADS == BM * 4 && RT >= 4, "a block must split evenly over the threads");
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wc = wave % WC, wr = wave / WC;
-    const int rho = lane & 31, h = lane >> 5;
+    const int l16 = lane & 15, q4 = lane >> 4;
 
     // workgroups go round-robin to the 8 XCDs; each takes a contiguous range of the tile list, along rows in groups of kGroup
     const int t = (blockIdx.x & 7) * a.per_xcd + (blockIdx.x >> 3);
@@ -86,6 +104,8 @@ __global__ __launch_bounds__(64 * WC * WR, 2) void gated_gemm_kernel(GemmFfnArgs
     const int64_t n0 = (int64_t)tn * TN, m0 = (int64_t)tm * BM;
     const int block0 = split * a.per_split;
     const int block1 = block0 + a.per_split < a.blocks ? block0 + a.per_split : a.blocks;
+    const int second = OP == OP_DX ? a.half / kBlock : INT32_MAX;    // first block of the second half
+    auto block_k = [&](int n) { return (n >= second ? n - second : n) * kBlock; };    // its first index, within its half
 
     // ---- what a thread loads: 16-byte unit u = j * THREADS + tid of either operand's part of a stage -------------------------
     struct Unit
@@ -97,43 +117,39 @@ __global__ __launch_bounds__(64 * WC * WR, 2) void gated_gemm_kernel(GemmFfnArgs
         const int u = j * THREADS + tid;
         if constexpr (CIN)
         {
-            const int r     = u >> 3;
+            const int r     = u >> 2;
             const int64_t f = n0 + (r >> 6) * 32 + (r & 31);    // rows 0..31 of 64 are gate's, the others up's
-            return Unit{ f < a.N ? f : a.N - 1, ((u & 7) ^ swizzle_in(r)) * 8 };
+            return Unit{ f < a.N ? f : a.N - 1, ((u & 3) ^ swizzle_in(r)) * 8 };
         }
         else
         {
             const int k = u / (BN / 8);
-            return Unit{ k, ((u % (BN / 8)) ^ ((k & 3) << 2)) * 8 };
+            return Unit{ k, ((u % (BN / 8)) ^ (swizzle_out(k) << 1)) * 8 };
         }
     };
     auto row_unit = [&](int j) {
         const int u = j * THREADS + tid;
         if constexpr (RIN)
         {
-            const int r     = u >> 3;
+            const int r     = u >> 2;
             const int64_t m = m0 + r;
-            return Unit{ m < a.M ? m : a.M - 1, ((u & 7) ^ swizzle_in(r)) * 8 };
+            return Unit{ m < a.M ? m : a.M - 1, ((u & 3) ^ swizzle_in(r)) * 8 };
         }
         else
         {
             const int k = u / (BM / 8);
-            return Unit{ k, ((u % (BM / 8)) ^ ((k & 3) << 2)) * 8 };
+            return Unit{ k, ((u % (BM / 8)) ^ (swizzle_out(k) << 1)) * 8 };
         }
     };
-    // which of the two column operands load j of this wave (forward), or block n (d_x), comes from
-    auto col_base = [&](int j, int n) {
-        if constexpr (CIN)
-            return a.col[((j * THREADS + wave * 64) >> 3 >> 5) & 1];
-        else
-            return a.col[OP == OP_DX && n * 64 >= a.half ? 1 : 0];
-    };
-    // first of the summed index of block n, within its half, and where it ends
-    auto block_k = [&](int n) { return OP == OP_DX && n * 64 >= a.half ? n * 64 - a.half : n * 64; };
+    // the column operand of load j of this wave (forward), or of block n (d_x)
+    auto col_base = [&](int j, int n) { return CIN ? a.col[(j * THREADS + wave * 64) >> 7 & 1] : a.col[n >= second ? 1 : 0]; };
 
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-    uint32_t cvoff[FAST ? CL : 1], rvoff[FAST ? RL : 1];
-    if constexpr (FAST)
+    // DIRECT: running addresses of the block to be requested next, and the thread's offsets from them
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave * 1024;
+    uint32_t cvoff[DIRECT ? CL : 1], rvoff[DIRECT ? RL : 1];
+    const uint16_t *cat[DIRECT ? (CIN ? CL : 1) : 1], *rat = nullptr;
+    int ahead = block0, astage = 0;    // the block, and the stage it goes to
+    if constexpr (DIRECT)
     {
 #pragma unroll
         for (int j = 0; j < CL; j++)
@@ -153,103 +169,105 @@ __global__ __launch_bounds__(64 * WC * WR, 2) void gated_gemm_kernel(GemmFfnArgs
             else
                 rvoff[j] = (uint32_t)(u.row * a.ldr + (u.col < a.M - 8 - m0 ? u.col : a.M - 8 - m0)) * 2;
         }
+#pragma unroll
+        for (int j = 0; j < (CIN ? CL : 1); j++)
+            cat[j] = col_base(j, block0) + (CIN ? n0 * a.ldc + block0 * kBlock : (int64_t)block_k(block0) * a.ldc + n0);
+        rat = a.row + (RIN ? m0 * a.ldr + block0 * kBlock : (int64_t)block0 * kBlock * a.ldr + m0);
     }
-    auto direct = [&](const uint16_t* base, uint32_t voff, uint32_t dst) {
+    // load q of the block `ahead`; EDGE: the summed index ends in it, and zeros come from there on (dp holds its own)
+    auto request = [&](int q, auto EDGE) {
+        const bool is_c      = q < CL;
+        const int j          = is_c ? q : q - CL;
+        const uint32_t dst   = lds0 + astage * STAGE + (is_c ? 0 : CB) + j * THREADS * 16;
+        const uint16_t* base = is_c ? cat[CIN ? j : 0] : rat;
+        const uint32_t voff  = is_c ? cvoff[j] : rvoff[j];
+        if constexpr (decltype(EDGE)::value)
+        {
+            if (is_c || OP != OP_DX)
+            {
+                const Unit u       = is_c ? col_unit(j) : row_unit(j);
+                const bool inside  = block_k(ahead) + ((is_c ? CIN : RIN) ? u.col : (int)u.row) < a.K;
+                const uint8_t* src = inside ? reinterpret_cast<const uint8_t*>(base) + voff : a.zeros;
+                asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(dst) : "memory");
+                return;
+            }
+        }
         asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(base), "s"(dst) : "memory");
     };
-    auto direct_or_zero = [&](const uint16_t* base, uint32_t voff, bool inside, uint32_t dst) {
-        const uint8_t* src = inside ? reinterpret_cast<const uint8_t*>(base) + voff : a.zeros;
-        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(dst) : "memory");
+    // Past the last block it is requested again, into stages nobody reads: the loads in flight are then as many in every block.
+    auto advance = [&]() {
+        astage = astage + 1 < RING ? astage + 1 : 0;
+        if (++ahead < block1)
+        {
+#pragma unroll
+            for (int j = 0; j < (CIN ? CL : 1); j++)
+                cat[j] += CIN ? kBlock : kBlock * a.ldc;
+            if (OP == OP_DX && ahead == second)
+                cat[0] = a.col[1] + n0;
+            rat += RIN ? kBlock : kBlock * a.ldr;
+        }
+        else
+            ahead = block1 - 1;
     };
-    // FAST: all loads of block n into stage s, straight to LDS
-    auto issue = [&](int n, int s) {
-        const int k0         = block_k(n);
-        const bool whole     = k0 + 64 <= a.K;
-        const uint32_t stage = lds0 + s * STAGE + wave * 1024;
+
+    // Otherwise through registers, in two sets
+    v4i creg[DIRECT ? 1 : 2][DIRECT ? 1 : CL], rreg[DIRECT ? 1 : 2][DIRECT ? 1 : RL];
+    // (pieces that all lie inside their rows need no look at each element)
+    const bool inner = (CIN || n0 + BN <= a.N) && (RIN || m0 + BM <= a.M);
+    auto fetch = [&](auto SET, int n) {
+        constexpr int P  = decltype(SET)::value;
+        const int k0     = block_k(n);
+        const bool plain = inner && k0 + kBlock <= a.K;
 #pragma unroll
         for (int j = 0; j < CL; j++)
         {
-            const uint16_t* base = col_base(j, n) + (CIN ? n0 * a.ldc + k0 : k0 * a.ldc + n0);
-            const uint32_t dst   = stage + j * THREADS * 16;
-            if (whole)
-                direct(base, cvoff[j], dst);
+            const Unit u        = col_unit(j);
+            const uint16_t* row = col_base(j, n) + (CIN ? u.row : k0 + u.row) * a.ldc;
+            const int64_t c     = CIN ? k0 + u.col : n0 + u.col;
+            if (plain)
+                creg[P][j] = load16(reinterpret_cast<const uint8_t*>(row + c));
             else
-            {
-                const Unit u = col_unit(j);
-                direct_or_zero(base, cvoff[j], k0 + (CIN ? u.col : (int)u.row) < a.K, dst);
-            }
-        }
-        const int rk = OP == OP_DX ? n * 64 : k0;    // dp holds both halves, filled up with zeros
-#pragma unroll
-        for (int j = 0; j < RL; j++)
-        {
-            const uint16_t* base = a.row + (RIN ? m0 * a.ldr + rk : rk * a.ldr + m0);
-            const uint32_t dst   = stage + CB + j * THREADS * 16;
-            if (whole || OP == OP_DX)
-                direct(base, rvoff[j], dst);
-            else
-            {
-                const Unit u = row_unit(j);
-                direct_or_zero(base, rvoff[j], k0 + (RIN ? u.col : (int)u.row) < a.K, dst);
-            }
-        }
-    };
-    // otherwise through registers: rows that begin at any element, and that end inside a piece
-    v4i creg[FAST ? 1 : CL], rreg[FAST ? 1 : RL];
-    auto fetch = [&](int n) {
-        const int k0 = block_k(n);
-#pragma unroll
-        for (int j = 0; j < CL; j++)
-        {
-            const Unit u         = col_unit(j);
-            const uint16_t* base = col_base(j, n);
-            if constexpr (CIN)
-                creg[j] = load8(base + u.row * a.ldc, k0 + u.col, a.K);
-            else
-                creg[j] = load8(base + (k0 + u.row) * a.ldc, n0 + u.col, k0 + u.row < a.K ? a.N : 0);
+                creg[P][j] = load8(row, c, CIN ? a.K : k0 + u.row < a.K ? a.N : 0);
         }
 #pragma unroll
         for (int j = 0; j < RL; j++)
         {
-            const Unit u = row_unit(j);
-            if constexpr (OP == OP_DX)
-                rreg[j] = *reinterpret_cast<const v4i*>(a.row + u.row * a.ldr + n * 64 + u.col);
-            else if constexpr (RIN)
-                rreg[j] = load8(a.row + u.row * a.ldr, k0 + u.col, a.K);
+            const Unit u        = row_unit(j);
+            const uint16_t* row = a.row + (RIN ? u.row : k0 + u.row) * a.ldr;
+            const int64_t c     = OP == OP_DX ? n * kBlock + u.col : RIN ? k0 + u.col : m0 + u.col;
+            if (OP == OP_DX || plain)
+                rreg[P][j] = load16(reinterpret_cast<const uint8_t*>(row + c));
             else
-                rreg[j] = load8(a.row + (k0 + u.row) * a.ldr, m0 + u.col, k0 + u.row < a.K ? a.M : 0);
+                rreg[P][j] = load8(row, c, RIN ? a.K : k0 + u.row < a.K ? a.M : 0);
         }
     };
-    auto put = [&](int s) {
-        uint8_t* stage = lds + s * STAGE;
+    auto put = [&](auto SET, int stage) {
+        constexpr int P = decltype(SET)::value;
+        uint8_t* to     = lds + stage * STAGE + tid * 16;
 #pragma unroll
         for (int j = 0; j < CL; j++)
-            *reinterpret_cast<v4i*>(stage + (j * THREADS + tid) * 16) = creg[j];
+            *reinterpret_cast<v4i*>(to + j * THREADS * 16) = creg[P][j];
 #pragma unroll
         for (int j = 0; j < RL; j++)
-            *reinterpret_cast<v4i*>(stage + CB + (j * THREADS + tid) * 16) = rreg[j];
+            *reinterpret_cast<v4i*>(to + CB + j * THREADS * 16) = rreg[P][j];
     };
 
     // ---- what a lane reads --------------------------------------------------------------------------------------------------
-    const int crow = channel_of_row(rho);
-    const int sl = lane & 15, m4 = sl >> 2, a4 = sl & 3, brho = (lane >> 4) & 1;
-    uint32_t caddr[CIN ? 4 : 2], raddr[RIN ? 4 : RT];    // by step, or by tile
+    // innermost: piece q4 of row l16 of a tile; outermost: as source lane, four columns of row l16 / 4 of the first four of the eight rows q4
+    uint32_t caddr[CIN ? 1 : CT], raddr[RIN ? 1 : RT];    // (outermost: by tile)
+    const int k8 = 8 * q4 + (l16 >> 2), seg = swizzle_out(k8);
     if constexpr (CIN)
-#pragma unroll
-        for (int s = 0; s < 4; s++)
-            caddr[s] = (wc * 64 + crow) * 128 + (((2 * s + h) ^ swizzle_in(crow)) * 16);
+        caddr[0] = (wc * 64 + l16) * 64 + ((q4 ^ swizzle_in(l16)) * 16);
     else
 #pragma unroll
-        for (int c = 0; c < 2; c++)    // source lane: row m4 of four, columns of the lanes 4 a4 ... 4 a4 + 3
-            caddr[c] = (8 * h + m4) * (BN * 2) + (((wc * 2 + c) ^ m4) << 6) + 2 * (16 * (a4 & 1) + 4 * (2 * brho + (a4 >> 1)));
+        for (int c = 0; c < CT; c++)
+            caddr[c] = k8 * (BN * 2) + (((wc * CT + c) ^ seg) << 5) + 8 * (l16 & 3);
     if constexpr (RIN)
-#pragma unroll
-        for (int s = 0; s < 4; s++)
-            raddr[s] = CB + (wr * 32 * RT + rho) * 128 + (((2 * s + h) ^ swizzle_in(rho)) * 16);
+        raddr[0] = CB + (wr * 16 * RT + l16) * 64 + ((q4 ^ swizzle_in(l16)) * 16);
     else
 #pragma unroll
         for (int i = 0; i < RT; i++)
-            raddr[i] = CB + (8 * h + m4) * (BM * 2) + (((wr * RT + i) ^ m4) << 6) + 2 * (16 * brho + 4 * a4);
+            raddr[i] = CB + k8 * (BM * 2) + (((wr * RT + i) ^ seg) << 5) + 8 * (l16 & 3);
     auto transposed = [&](const uint8_t* at, int rows_apart) {
         typedef __attribute__((address_space(3))) v4s lds_v4s;
         const v2i lo = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at));
@@ -257,195 +275,307 @@ __global__ __launch_bounds__(64 * WC * WR, 2) void gated_gemm_kernel(GemmFfnArgs
         return v4i{ lo.x, lo.y, hi.x, hi.y };
     };
 
-    v16f acc[2][RT];
+    v4f acc[CT][RT];
 #pragma unroll
-    for (int c = 0; c < 2; c++)
+    for (int c = 0; c < CT; c++)
 #pragma unroll
         for (int i = 0; i < RT; i++)
-#pragma unroll
-            for (int e = 0; e < 16; e++)
-                acc[c][i][e] = 0.0f;
+            acc[c][i] = v4f{ 0.0f, 0.0f, 0.0f, 0.0f };
 
-    auto multiply = [&](int stage) {
-        const uint8_t* sb = lds + stage * STAGE;
-#pragma unroll
-        for (int s = 0; s < 4; s++)
-        {
-            v4i fc[2], fr[RT];
-#pragma unroll
-            for (int c = 0; c < 2; c++)
-                if constexpr (CIN)
-                    fc[c] = *reinterpret_cast<const v4i*>(sb + caddr[s] + c * 4096);
-                else
-                    fc[c] = transposed(sb + caddr[c] + 16 * s * (BN * 2), 4 * (BN * 2));
-#pragma unroll
-            for (int i = 0; i < RT; i++)
-                if constexpr (RIN)
-                    fr[i] = *reinterpret_cast<const v4i*>(sb + raddr[s] + i * 4096);
-                else
-                    fr[i] = transposed(sb + raddr[i] + 16 * s * (BM * 2), 4 * (BM * 2));
-#pragma unroll
-            for (int i = 0; i < RT; i++)
-#pragma unroll
-                for (int c = 0; c < 2; c++)
-                    acc[c][i] = Mma<T>::mma(fc[c], fr[i], acc[c][i]);
-        }
+    // ---- main loop ------------------------------------------------------------------------------------------------------------
+    // A block is one matrix instruction deep.  A wave takes it row tile by row tile; when a row tile is done its fragment is read from the next
+    // block, a block ahead of its use, and the column tiles' fragments into a second set.  The barrier that publishes block n + 1 stands behind
+    // the first row tile of block n; past it every wave is done with block n - 1, whose stage takes the loads of block n + RING - 1.  Reads and
+    // loads stand behind matrix instructions one by one, and are kept there: their wait for a slot passes while the matrix cores work.
+    v4i fc[2][CT], fr[RT];
+    auto read_col = [&](int set, const uint8_t* sb, int c) {
+        if constexpr (CIN)
+            fc[set][c] = *reinterpret_cast<const v4i*>(sb + caddr[0] + c * 1024);
+        else
+            fc[set][c] = transposed(sb + caddr[c], 4 * (BN * 2));
     };
-
-    if constexpr (FAST)
-    {
-        if (block0 < block1)
-            issue(block0, 0);
-        for (int n = block0; n < block1; n++)
-        {
-            // block n has landed, and every wave is past block n - 1, whose stage the next loads overwrite
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (n + 1 < block1)
-                issue(n + 1, (n + 1 - block0) & 1);
-            multiply((n - block0) & 1);
-        }
-    }
-    else
-    {
-        if (block0 < block1)
-        {
-            fetch(block0);
-            put(0);
-        }
-        __syncthreads();
-        for (int n = block0; n < block1; n++)
-        {
-            if (n + 1 < block1)
-                fetch(n + 1);
-            multiply((n - block0) & 1);
-            if (n + 1 < block1)
-                put((n + 1 - block0) & 1);
-            __syncthreads();
-        }
-    }
-
-    // ---- results: a lane has 16 neighbours of a row from each accumulator tile -----------------------------------------------
-    auto store16 = [&](uint16_t* row, int64_t at, int64_t end, const float* v) {
-#pragma unroll
-        for (int q = 0; q < 2; q++)
-        {
-            v4i w;
-#pragma unroll
-            for (int p = 0; p < 4; p++)
-                w[p] = (int)pack16<T>(v[8 * q + 2 * p], v[8 * q + 2 * p + 1]);
-            store8(row, at + 8 * q, end, w);
-        }
+    auto read_row = [&](const uint8_t* sb, int i) {
+        if constexpr (RIN)
+            fr[i] = *reinterpret_cast<const v4i*>(sb + raddr[0] + i * 1024);
+        else
+            fr[i] = transposed(sb + raddr[i], 4 * (BM * 2));
     };
-    auto store_part = [&](int which, int64_t m, int64_t at, const v16f& v) {
-        float* row = a.part + (((int64_t)split * (CIN ? 2 : 1) + which) * a.M + m) * a.N;
+    // a block whose column fragments are in set P, with the reads of the next one from `next`; publish() behind the first row tile, and NL loads
+    auto block = [&](auto SET, const uint8_t* next, auto&& publish, auto NL_tag, auto&& load) {
+        constexpr int P = decltype(SET)::value, NL = decltype(NL_tag)::value;
 #pragma unroll
-        for (int q = 0; q < 4; q++)
+        for (int i = 0; i < RT; i++)
         {
-            const v4f w = { v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3] };
-            if (at + 4 * q + 4 <= a.N)
-                __builtin_memcpy(row + at + 4 * q, &w, 16);
-            else
 #pragma unroll
-                for (int e = 0; e < 3; e++)
-                    if (at + 4 * q + e < a.N)
-                        row[at + 4 * q + e] = w[e];
-        }
-    };
-#pragma unroll
-    for (int i = 0; i < RT; i++)
-    {
-        const int64_t m = m0 + (wr * RT + i) * 32 + rho;
-        if (m >= a.M)
-            continue;
-        if constexpr (OP == OP_FORWARD)
-        {
-            const int64_t f = n0 + wc * 32 + 16 * h;
-            if (a.splits > 1)
+            for (int k = 0; k < CT; k++)
             {
-                store_part(0, m, f, acc[0][i]);
-                store_part(1, m, f, acc[1][i]);
-                continue;
+                const int c = i & 1 ? CT - 1 - k : k;    // (one operand changes at a time)
+                acc[c][i]   = mma16<T>(fc[P][c], fr[i], acc[c][i]);
+                if (i > 0 && k == 1)
+#pragma unroll
+                    for (int q = 0; q < NL; q++)
+                        if (1 + q * (RT - 1) / (NL ? NL : 1) == i)
+                            load(q);
+                if (k == 2 && i < CT && i > 0)
+                    read_col(1 - P, next, i);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            float v[16];
-            if (a.pre_gate)
+            if (i == 0)
             {
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    v[e] = acc[0][i][e];
-                store16(a.pre_gate + m * a.ldo, f, a.N, v);
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    v[e] = acc[1][i][e];
-                store16(a.pre_up + m * a.ldo, f, a.N, v);
+                publish();
+                read_col(1 - P, next, 0);
             }
+            read_row(next, i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto first_reads = [&]() {
 #pragma unroll
-            for (int e = 0; e < 16; e++)
-                v[e] = act_value(a.act, acc[0][i][e]) * acc[1][i][e];
-            store16(a.out[0] + m * a.ldo, f, a.N, v);
+        for (int c = 0; c < CT; c++)
+            read_col(0, lds, c);
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+            read_row(lds, i);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    constexpr std::integral_constant<int, 0> zero{};
+    constexpr std::integral_constant<int, 1> one{};
+    auto next_of = [&](int s) { return s + 1 < RING ? s + 1 : 0; };
+
+    if (block0 < block1)
+    {
+        int cur = 0;
+        if constexpr (DIRECT)
+        {
+            auto whole = [&]() { return block_k(ahead) + kBlock <= a.K; };
+#pragma unroll 1
+            for (int b = 0; b < RING - 1; b++)
+            {
+                if (whole())
+#pragma unroll
+                    for (int q = 0; q < LOADS; q++)
+                        request(q, std::false_type());
+                else
+#pragma unroll
+                    for (int q = 0; q < LOADS; q++)
+                        request(q, std::true_type());
+                advance();
+            }
+            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((RING - 2) * LOADS) : "memory");
+            first_reads();
+            auto one_block = [&](auto SET) {
+                cur          = next_of(cur);
+                const bool w = whole();
+                // (a bare barrier: the reads in flight are of the block in use)
+                auto publish = [&]() { asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((RING - 3) * LOADS) : "memory"); };
+                block(SET, lds + cur * STAGE, publish, std::integral_constant<int, LOADS>(), [&](int q) {
+                    if (w)
+                        request(q, std::false_type());
+                    else
+                        request(q, std::true_type());
+                });
+                advance();
+            };
+#pragma unroll 1
+            for (int n = block0; n < block1; n += 2)
+            {
+                one_block(zero);
+                if (n + 1 < block1)
+                    one_block(one);
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
         else
         {
-            uint16_t* row = a.out[0];
-            int64_t r     = m;
-            if constexpr (OP == OP_DW)
+            // blocks 0 and 1 in LDS, 2 and 3 in the registers; behind its barrier a block n writes block n + 2, and fetches n + 4
+            fetch(zero, block0);
+            if (block0 + 1 < block1)
+                fetch(one, block0 + 1);
+            put(zero, 0);
+            put(one, 1);
+            if (block0 + 2 < block1)
+                fetch(zero, block0 + 2);
+            if (block0 + 3 < block1)
+                fetch(one, block0 + 3);
+            __syncthreads();
+            first_reads();
+            auto one_block = [&](auto SET, int n) {
+                cur          = next_of(cur);
+                auto publish = [&]() {
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    put(SET, next_of(cur));
+                    if (n + 4 < block1)
+                        fetch(SET, n + 4);
+                };
+                block(SET, lds + cur * STAGE, publish, zero, [](int) {});
+            };
+#pragma unroll 1
+            for (int n = block0; n < block1; n += 2)
             {
-                // rows of dp's halves behind their F features are none of a gradient's
-                const int half = m >= a.half ? 1 : 0;
-                r              = m - (half ? a.half : 0);
-                row            = a.out[half];
-                if (r >= a.features)
-                    continue;
-            }
-#pragma unroll
-            for (int c = 0; c < 2; c++)
-            {
-                const int64_t d = n0 + wc * 64 + c * 32 + 16 * h;
-                if (a.splits > 1)
-                {
-                    store_part(0, m, d, acc[c][i]);
-                    continue;
-                }
-                float v[16];
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    v[e] = acc[c][i][e];
-                store16(row + r * a.ldo, d, a.N, v);
+                one_block(zero, n);
+                if (n + 1 < block1)
+                    one_block(one, n + 1);
             }
         }
     }
+
+    // ---- results ------------------------------------------------------------------------------------------------------------
+    // A lane has four neighbours of a row from each accumulator tile.  They go through LDS as a tile of whole rows (piece p of row r at p ^ r), and
+    // from there in whole lines.  W words of 32 bits hold a lane's four results: 4 as floats (parts of a split sum), 2 rounded.
+    auto through_lds = [&](int width, auto W_tag, auto&& words, auto&& store) {
+        constexpr int W  = decltype(W_tag)::value;
+        constexpr int TC = CIN && W == 2 ? CT / 2 : CT;    // tiles that results come from (forward: of gate and up together)
+        const int pieces = width * W / 16;                  // 16-byte pieces of a row
+        // what does not fit at once goes in two halves of each wave's row tiles
+        constexpr int PASSES = BM * BN * W * (CIN && W == 2 ? 2 : 4) / 4 > RING * STAGE ? 2 : 1, RP = RT / PASSES;
+#pragma unroll
+        for (int i0 = 0; i0 < RT; i0 += RP)
+        {
+            __syncthreads();    // the ring, or the tile before, is read
+#pragma unroll
+            for (int i = 0; i < RP; i++)
+#pragma unroll
+                for (int c = 0; c < TC; c++)
+                {
+                    const int r = (wr * RP + i) * 16 + l16, col = (wc * TC + c) * 16 + 4 * q4;
+                    uint32_t v[W];
+                    words(c, i0 + i, v);
+                    uint8_t* at = lds + (r * pieces + ((col * W / 16) ^ (r & (pieces - 1)))) * 16 + (W == 2 ? 8 * (q4 & 1) : 0);
+                    if constexpr (W == 2)
+                        *reinterpret_cast<v2i*>(at) = v2i{ (int)v[0], (int)v[1] };
+                    else
+                        *reinterpret_cast<v4i*>(at) = v4i{ (int)v[0], (int)v[1], (int)v[2], (int)v[3] };
+                }
+            __syncthreads();
+#pragma unroll 2
+            for (int u = tid; u < BM / PASSES * pieces; u += THREADS)
+            {
+                const int r = u / pieces, p = u % pieces;
+                const int64_t m = m0 + (PASSES == 1 ? r : (r / (16 * RP) * RT + i0) * 16 + r % (16 * RP));
+                if (m < a.M)
+                    store(m, p, *reinterpret_cast<const v4i*>(lds + (r * pieces + (p ^ (r & (pieces - 1)))) * 16));
+            }
+        }
+    };
+    constexpr std::integral_constant<int, 2> rounded{};
+    auto round4 = [&](v4f v, uint32_t* w) { w[0] = pack16<T>(v[0], v[1]), w[1] = pack16<T>(v[2], v[3]); };
+    if (a.splits > 1)
+    {
+        through_lds(BN, std::integral_constant<int, 4>(), [&](int c, int i, uint32_t* v) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                v[e] = __float_as_uint(acc[c][i][e]);
+        }, [&](int64_t m, int p, v4i v) {
+            // forward: of every 64 columns 32 are gate's sums, the others up's
+            const int col   = 4 * p, which = CIN ? col >> 5 & 1 : 0;
+            const int64_t n = n0 + (CIN ? (col >> 6) * 32 + (col & 31) : col);
+            float* row      = a.part + (((int64_t)split * (CIN ? 2 : 1) + which) * a.M + m) * a.N;
+            if (n + 4 <= a.N)
+                __builtin_memcpy(row + n, &v, 16);
+            else
+#pragma unroll
+                for (int e = 0; e < 3; e++)
+                    if (n + e < a.N)
+                        row[n + e] = __int_as_float(v[e]);
+        });
+        return;
+    }
+    if constexpr (OP == OP_FORWARD)
+    {
+        auto to = [&](uint16_t* out) { return [=](int64_t m, int p, v4i v) { store8(out + m * a.ldo, n0 + 8 * p, a.N, v); }; };
+        if (a.pre_gate)
+        {
+            through_lds(TN, rounded, [&](int c, int i, uint32_t* w) { round4(acc[c][i], w); }, to(a.pre_gate));
+            through_lds(TN, rounded, [&](int c, int i, uint32_t* w) { round4(acc[c + CT / 2][i], w); }, to(a.pre_up));
+        }
+        for_act(a.act, [&](auto ACT) {
+            through_lds(TN, rounded, [&](int c, int i, uint32_t* w) {
+                v4f v;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    v[e] = act_value<decltype(ACT)::value>(acc[c][i][e]) * acc[c + CT / 2][i][e];
+                round4(v, w);
+            }, to(a.out[0]));
+        });
+    }
+    else
+        through_lds(TN, rounded, [&](int c, int i, uint32_t* w) {
+            round4(acc[c][i], w);
+        }, [&](int64_t m, int p, v4i v) {
+            uint16_t* out = a.out[0];
+            if constexpr (OP == OP_DW)
+            {
+                // rows of dp's halves behind their F features are none of a gradient's
+                if (m >= a.half)
+                    m -= a.half, out = a.out[1];
+                if (m >= a.features)
+                    return;
+            }
+            store8(out + m * a.ldo, n0 + 8 * p, a.N, v);
+        });
 }
 
-// Results of a sum that was split: the parts in the order of the splits, then what the unsplit kernel does with a sum.
+// Results of a sum that was split, four of a row a thread: the parts in the order of the splits, then what the unsplit kernel does with a sum.
 template <typename T, int OP>
 __global__ __launch_bounds__(256) void gated_join_kernel(GemmFfnArgs a)
 {
-    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x, m = blockIdx.y;
+    const int64_t n = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, m = blockIdx.y;
     if (n >= a.N)
         return;
     constexpr int W     = OP == OP_FORWARD ? 2 : 1;
     const int64_t plane = (int64_t)a.M * a.N;
     const float* part   = a.part + m * a.N + n;
-    float v[W];
+    const int live      = a.N - n < 4 ? (int)(a.N - n) : 4;
+    v4f v[W];
 #pragma unroll
     for (int w = 0; w < W; w++)
-        v[w] = 0.0f;
+        v[w] = v4f{ 0.0f, 0.0f, 0.0f, 0.0f };
     for (int s = 0; s < a.splits; s++)
 #pragma unroll
         for (int w = 0; w < W; w++)
-            v[w] += part[(s * W + w) * plane];
+        {
+            v4f t = { 0.0f, 0.0f, 0.0f, 0.0f };
+            const float* at = part + (s * W + w) * plane;
+            if (live == 4)
+                __builtin_memcpy(&t, at, 16);
+            else
+#pragma unroll
+                for (int e = 0; e < 3; e++)
+                    if (e < live)
+                        t[e] = at[e];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                v[w][e] += t[e];
+        }
+    auto store = [&](uint16_t* to, v4f r) {
+        const v2i bits = { (int)pack16<T>(r[0], r[1]), (int)pack16<T>(r[2], r[3]) };
+        if (live == 4)
+            __builtin_memcpy(to, &bits, 8);
+        else
+#pragma unroll
+            for (int e = 0; e < 3; e++)
+                if (e < live)
+                    to[e] = to_bits16<T>(r[e]);
+    };
     if constexpr (OP == OP_FORWARD)
     {
         const int64_t at = m * a.ldo + n;
         if (a.pre_gate)
-            a.pre_gate[at] = to_bits16<T>(v[0]), a.pre_up[at] = to_bits16<T>(v[W - 1]);
-        a.out[0][at] = to_bits16<T>(act_value(a.act, v[0]) * v[W - 1]);
+            store(a.pre_gate + at, v[0]), store(a.pre_up + at, v[W - 1]);
+        for_act(a.act, [&](auto ACT) {
+            v4f h;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                h[e] = act_value<decltype(ACT)::value>(v[0][e]) * v[W - 1][e];
+            store(a.out[0] + at, h);
+        });
     }
     else
     {
         const int half  = OP == OP_DW && m >= a.half ? 1 : 0;
         const int64_t r = m - (half ? a.half : 0);
         if (OP == OP_DX || r < a.features)
-            a.out[half][r * a.ldo + n] = to_bits16<T>(v[0]);
+            store(a.out[half] + r * a.ldo + n, v[0]);
     }
 }
 
@@ -454,7 +584,7 @@ struct SlopeArgs
 {
     const uint16_t *pre_gate, *pre_up, *dh;
     uint16_t* dp;
-    int64_t ld, units;    // units: rows * half / 8
+    int64_t ld, ldp, units;    // elements between rows of the inputs and of dp; units: rows * half / 8
     int32_t features, half, act;
 };
 
@@ -469,25 +599,27 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(SlopeArgs a)
         const v4i g = load8(a.pre_gate + m * a.ld, f, a.features), up = load8(a.pre_up + m * a.ld, f, a.features),
                   dh = load8(a.dh + m * a.ld, f, a.features);
         v4i dg, du;
+        for_act(a.act, [&](auto ACT) {
 #pragma unroll
-        for (int p = 0; p < 4; p++)
-        {
-            float x[2], y[2];
-#pragma unroll
-            for (int e = 0; e < 2; e++)
+            for (int p = 0; p < 4; p++)
             {
-                float value, slope;
-                act_both(a.act, from_bits16<T>(half_of(g, 2 * p + e)), value, slope);
-                const float d = from_bits16<T>(half_of(dh, 2 * p + e));
-                x[e] = d * from_bits16<T>(half_of(up, 2 * p + e)) * slope;
-                y[e] = d * value;
-                if (f + 2 * p + e >= a.features)
-                    x[e] = 0.0f, y[e] = 0.0f;
+                float x[2], y[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                {
+                    float value, slope;
+                    act_both<decltype(ACT)::value>(from_bits16<T>(half_of(g, 2 * p + e)), value, slope);
+                    const float d = from_bits16<T>(half_of(dh, 2 * p + e));
+                    x[e] = d * from_bits16<T>(half_of(up, 2 * p + e)) * slope;
+                    y[e] = d * value;
+                    if (f + 2 * p + e >= a.features)
+                        x[e] = 0.0f, y[e] = 0.0f;
+                }
+                dg[p] = (int)pack16<T>(x[0], x[1]);
+                du[p] = (int)pack16<T>(y[0], y[1]);
             }
-            dg[p] = (int)pack16<T>(x[0], x[1]);
-            du[p] = (int)pack16<T>(y[0], y[1]);
-        }
-        uint16_t* row = a.dp + m * 2 * a.half + f;
+        });
+        uint16_t* row = a.dp + m * a.ldp + f;
         *reinterpret_cast<v4i*>(row)          = dg;
         *reinterpret_cast<v4i*>(row + a.half) = du;
     }
@@ -495,39 +627,58 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(SlopeArgs a)
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 
+enum
+{
+    TILE_256,        // 256 x 256 results, eight waves
+    TILE_256_128,    // 256 rows x 128 columns, eight waves
+    TILE_128         // 128 x 128, four waves, two workgroups a CU
+};
 struct Shape
 {
-    bool large;      // 256 x 256 (eight waves) or 128 x 128 (four waves, two workgroups a CU)
+    int tile;
     int splits, per_split;
     int tiles_m, tiles_n;
 };
 
-// 256 x 256 where that fills two thirds of the CUs.  Smaller products go to 128 x 128, and where those are few and the sum is long it is split,
-// into parts of eight blocks (512 of the summed index) at least.  Operands that are read through registers take 128 x 128: the others' accumulators
-// leave no room.
+// The tile, and into how many parts the sum is split, by the time that follows from what was measured (us, over 4096 x 2048 x 8192 and halves to
+// eighths of each size): a block of 32 costs a workgroup of the three tiles 0.62, 0.39 and 0.33 on an empty chip and 0.80, 0.48 and 0.58 on
+// a full one (the smaller ones ask L2 for more, the weights' gradients' least), a tile 12, 7 and 6 beside them, and a split its partial sums
+// out and in at 4.5 TB/s and a launch.  Both sides, us: d_x 4096 x 2048 x 8192 (128, 256 and 512 tiles) 240 with the largest tile and two parts, 332, 317
+// and 359 in one part of each; of half the size 73 with four parts, 90 at best in one; forward 512 x 4096 x 2048 81, 52 and 43 in one part, 38, 32
+// and 32 in the best number of parts; 4096 x 2048 x 8192 243, 301 and 328.  Operands that go through registers take the smallest tile: the
+// others' accumulators leave no room.
 Shape shape_of(int op, int64_t M, int64_t N, int blocks, bool fast)
 {
-    Shape s{};
-    auto tiles = [&](int size) {
-        s.tiles_m = (int)((M + size - 1) / size);
-        const int tn = op == OP_FORWARD ? size / 2 : size;
-        s.tiles_n = (int)((N + tn - 1) / tn);
-        return (int64_t)s.tiles_m * s.tiles_n;
-    };
-    s.large = fast && tiles(256) >= 170;
-    s.splits = 1, s.per_split = blocks;
-    if (!s.large)
+    static const struct
     {
-        const int64_t n = tiles(128);
-        int64_t want = n >= 256 || n < 1 ? 1 : (512 + n - 1) / n;    // (a product of no results is planned too)
-        want         = want < blocks / 8 ? want : blocks / 8;
-        if (want > 1)
+        int bm, bn, slots;
+        double empty, full, tile;
+    } of[3] = { { 256, 256, 256, 0.62, 0.80, 12 }, { 256, 128, 256, 0.39, 0.48, 7 }, { 128, 128, 512, 0.33, 0.58, 6 } };
+    Shape best{};
+    double least = 0;
+    for (int tile = fast ? TILE_256 : TILE_128; tile <= TILE_128; tile++)
+    {
+        const int tn = op == OP_FORWARD ? of[tile].bn / 2 : of[tile].bn;
+        Shape s{};
+        s.tile = tile, s.tiles_m = (int)((M + of[tile].bm - 1) / of[tile].bm), s.tiles_n = (int)((N + tn - 1) / tn);
+        for (int want = 1; want <= 16 && (want == 1 || blocks >= 16 * want); want++)
         {
-            s.per_split = (int)((blocks + want - 1) / want);
-            s.splits    = (blocks + s.per_split - 1) / s.per_split;
+            s.per_split      = (blocks + want - 1) / want;
+            s.splits         = s.per_split ? (blocks + s.per_split - 1) / s.per_split : 1;
+            const int64_t n  = (int64_t)s.tiles_m * s.tiles_n * s.splits;
+            const int64_t rounds = (n + of[tile].slots - 1) / of[tile].slots;
+            // (of the smallest tile the first 256 have a CU each)
+            const double busy = n >= of[tile].slots ? 1 : tile == TILE_128 ? (n > 256 ? n / 256.0 - 1 : 0) : (double)n / of[tile].slots;
+            double us         = rounds * (s.per_split * (of[tile].empty + (of[tile].full - of[tile].empty) * busy) + of[tile].tile);
+            if (s.splits > 1)
+                us += 3 + (double)M * N * (op == OP_FORWARD ? 2 : 1) * 4 * 2 * s.splits / 4.5e6;
+            if (!best.tiles_m || us < least)
+                least = us, best = s;
         }
+        if (!best.tiles_m)    // no rows
+            best = s;
     }
-    return s;
+    return best;
 }
 
 size_t part_bytes(int op, const Shape& s, int64_t M, int64_t N)
@@ -538,7 +689,7 @@ size_t part_bytes(int op, const Shape& s, int64_t M, int64_t N)
 template <typename T, int OP, int WC, int WR, int RT, bool FAST>
 bool launch_tiles(hipStream_t st, const GemmFfnArgs& a)
 {
-    constexpr size_t lds = 2 * (64 * WC + 32 * RT * WR) * 128;
+    constexpr size_t lds = kRing<FAST> * (64 * WC + 16 * RT * WR) * 64;
     if (!ensure_dynamic_lds<gated_gemm_kernel<T, OP, WC, WR, RT, FAST>>(lds))
         return false;
     gated_gemm_kernel<T, OP, WC, WR, RT, FAST><<<a.per_xcd * 8, 64 * WC * WR, lds, st>>>(a);
@@ -554,12 +705,14 @@ bool launch_product(hipStream_t st, int32_t dtype, GemmFfnArgs a, const Shape& s
     auto typed = [&](auto type) {
         using T = decltype(type);
         bool ok;
-        if (s.large)
-            ok = launch_tiles<T, OP, 4, 2, 4, true>(st, a);
+        if (s.tile == TILE_256)
+            ok = launch_tiles<T, OP, 4, 2, 8, true>(st, a);
+        else if (s.tile == TILE_256_128)
+            ok = launch_tiles<T, OP, 2, 4, 4, true>(st, a);
         else
-            ok = fast ? launch_tiles<T, OP, 2, 2, 2, true>(st, a) : launch_tiles<T, OP, 2, 2, 2, false>(st, a);
+            ok = fast ? launch_tiles<T, OP, 2, 2, 4, true>(st, a) : launch_tiles<T, OP, 2, 2, 4, false>(st, a);
         if (ok && s.splits > 1)
-            gated_join_kernel<T, OP><<<dim3((a.N + 255) / 256, a.M), 256, 0, st>>>(a);
+            gated_join_kernel<T, OP><<<dim3((a.N + 1023) / 1024, a.M), 256, 0, st>>>(a);
         return ok;
     };
     return dtype == TMI_BF16 ? typed(bf16_t{}) : typed(_Float16{});
@@ -581,14 +734,14 @@ struct ForwardPlan
 ForwardPlan forward_plan(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up)
 {
     ForwardPlan p;
-    p.blocks = (int)(((int64_t)d.in_features + 63) / 64);
+    p.blocks = (int)(((int64_t)d.in_features + kBlock - 1) / kBlock);
     p.fast   = whole_pieces(x, d.in_features, d.ld_x) && whole_pieces(gate, d.in_features, d.ld_w) && whole_pieces(up, d.in_features, d.ld_w);
     p.shape  = shape_of(OP_FORWARD, d.rows, d.hidden_features, p.blocks, p.fast);
     return p;
 }
 struct BackwardPlan
 {
-    int64_t half;
+    int64_t half, ldp;
     size_t dp_bytes;
     int dx_blocks, dw_blocks;
     bool dx_fast, dw_fast;
@@ -598,10 +751,13 @@ BackwardPlan backward_plan(const tmi_gated_ffn_desc_t& d, const void* x, const v
 {
     BackwardPlan p;
     p.half           = ((int64_t)d.hidden_features + 63) / 64 * 64;
-    p.dp_bytes       = (size_t)d.rows * 2 * p.half * 2;
-    p.dx_blocks      = (int)(2 * p.half / 64);
-    p.dw_blocks      = (int)(((int64_t)d.rows + 63) / 64);
-    const bool near  = 2 * p.half < (int64_t(1) << 22);
+    // Rows of dp lie 128 bytes further apart than they are long: the 256 rows that a tile reads 64 bytes of at a time would otherwise lie a power
+    // of two apart where F is one, on few channels of the memory.
+    p.ldp            = 2 * p.half + 64;
+    p.dp_bytes       = (size_t)d.rows * p.ldp * 2;
+    p.dx_blocks      = (int)(2 * p.half / kBlock);
+    p.dw_blocks      = (int)(((int64_t)d.rows + kBlock - 1) / kBlock);
+    const bool near  = p.ldp < (int64_t(1) << 22);
     p.dx_fast        = near && whole_pieces(gate, d.in_features, d.ld_w) && whole_pieces(up, d.in_features, d.ld_w);
     p.dw_fast        = near && whole_pieces(x, d.in_features, d.ld_x);
     p.dx             = shape_of(OP_DX, d.rows, d.in_features, p.dx_blocks, p.dx_fast);
@@ -648,7 +804,7 @@ const char* launch_gated_ffn_backward(hipStream_t st, const tmi_gated_ffn_desc_t
     const BackwardPlan p = backward_plan(d, x, gate, up);
     SlopeArgs q{};
     q.pre_gate = static_cast<const uint16_t*>(pre_gate), q.pre_up = static_cast<const uint16_t*>(pre_up), q.dh = static_cast<const uint16_t*>(d_h);
-    q.dp = static_cast<uint16_t*>(scratch), q.ld = d.ld_h, q.units = d.rows * (p.half / 8);
+    q.dp = static_cast<uint16_t*>(scratch), q.ld = d.ld_h, q.ldp = p.ldp, q.units = d.rows * (p.half / 8);
     q.features = d.hidden_features, q.half = (int32_t)p.half, q.act = d.activation;
     const int64_t groups = (q.units + 255) / 256;
     const int grid       = (int)(groups < 4096 ? groups : 4096);
@@ -658,7 +814,7 @@ const char* launch_gated_ffn_backward(hipStream_t st, const tmi_gated_ffn_desc_t
         gated_slope_kernel<_Float16><<<grid, 256, 0, st>>>(q);
 
     GemmFfnArgs a{};
-    a.row = q.dp, a.ldr = 2 * p.half, a.half = (int32_t)p.half, a.features = d.hidden_features;
+    a.row = q.dp, a.ldr = p.ldp, a.half = (int32_t)p.half, a.features = d.hidden_features;
     a.part  = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + p.dp_bytes);
     a.zeros = static_cast<const uint8_t*>(zeros);
     a.N     = d.in_features;

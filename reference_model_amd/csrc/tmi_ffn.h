@@ -2,15 +2,27 @@
 // matrix instruction of 16-bit floats, and the layout of 4-bit weights.
 #pragma once
 #include "tmi_mfma.h"
+#include <type_traits>
 
 namespace tmi
 {
 
-// act(g) in 32 bits.  The logistic forms hold where exp overflows: g / (1 + inf) is a zero.  GELU goes by erfc, which keeps its digits where
-// 1 + erf cancels, and its tanh form by (1 + tanh z) / 2 = 1 / (1 + exp(-2z)) for the same reason.
+// act(g) in 32 bits, to a few units of the last place.  GELU goes by erfc, which keeps its digits where 1 + erf cancels, and its tanh form by
+// (1 + tanh z) / 2 = 1 / (1 + exp(-2z)) for the same reason.
+//
+// 1 / (1 + exp(-z)) without a division and without a library's exp (which take twice as many instructions): with E = exp(-|z|) in [0, 1] it is
+// 1 / (1 + E) or E / (1 + E), and the reciprocal's argument lies in [1, 2].  E is the square of 2^(-|z| log2(e) / 2), so that it may be subnormal,
+// put right by what rounding the exponent took.  |z| is cut where E has long been 0, for the difference of infinities that an infinite one would make.
 __device__ __forceinline__ float logistic(float z)
 {
-    return 1.0f / (1.0f + expf(-z));
+    constexpr float c = -0.72134752044448170f;    // -log2(e) / 2
+    const float a     = fabsf(z) > 512.0f ? 512.0f : fabsf(z);    // (NaN stays)
+    const float m     = a * c, off = __builtin_fmaf(a, c, -m);
+    const float q     = __builtin_amdgcn_exp2f(m);
+    float e           = q * q;
+    e                 = __builtin_fmaf(e, off * 1.38629436111989062f, e);    // 2 ln 2
+    const float r     = __builtin_amdgcn_rcpf(1.0f + e);
+    return z < 0.0f ? e * r : r;
 }
 constexpr float kGeluTwoC  = 1.5957691216057308f;    // 2 sqrt(2 / pi)
 constexpr float kGeluCubic = 0.044715f;
@@ -18,55 +30,64 @@ __device__ __forceinline__ float gelu_tanh_twice(float g)    // 2z
 {
     return kGeluTwoC * (g + kGeluCubic * g * g * g);
 }
-__device__ __forceinline__ float act_value(int act, float g)
+// act(g); ACT a constant, so that a kernel chooses once and not for each element (for_act)
+template <int ACT>
+__device__ __forceinline__ float act_value(float g)
 {
-    switch (act)
-    {
-        case TMI_ACT_SILU:
-            return g / (1.0f + expf(-g));
-        case TMI_ACT_GELU:
-            return 0.5f * g * erfcf(-0.70710678118654752f * g);
-        case TMI_ACT_GELU_TANH:
-            return g / (1.0f + expf(-gelu_tanh_twice(g)));
-        case TMI_ACT_RELU:
-            return g < 0.0f ? 0.0f : g;    // (NaN stays)
-        default:
-            return logistic(g);
-    }
+    if constexpr (ACT == TMI_ACT_SILU)
+        return g * logistic(g);
+    else if constexpr (ACT == TMI_ACT_GELU)
+        return 0.5f * g * erfcf(-0.70710678118654752f * g);
+    else if constexpr (ACT == TMI_ACT_GELU_TANH)
+        return g * logistic(gelu_tanh_twice(g));
+    else if constexpr (ACT == TMI_ACT_RELU)
+        return g < 0.0f ? 0.0f : g;    // (NaN stays)
+    else
+        return logistic(g);
 }
 // act(g) and act'(g)
-__device__ __forceinline__ void act_both(int act, float g, float& value, float& slope)
+template <int ACT>
+__device__ __forceinline__ void act_both(float g, float& value, float& slope)
+{
+    if constexpr (ACT == TMI_ACT_SILU)
+    {
+        const float s = logistic(g);
+        value = g * s, slope = s * (1.0f + g * (1.0f - s));
+    }
+    else if constexpr (ACT == TMI_ACT_GELU)
+    {
+        const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
+        value = g * cdf, slope = cdf + g * (expf(-0.5f * g * g) * 0.39894228040143268f);
+    }
+    else if constexpr (ACT == TMI_ACT_GELU_TANH)
+    {
+        const float p = logistic(gelu_tanh_twice(g)), pq = p * (1.0f - p);
+        // far out p is 0 or 1 and g * g may be infinite
+        value = g * p, slope = pq == 0.0f ? p : p + g * pq * (kGeluTwoC * (1.0f + 3.0f * kGeluCubic * g * g));
+    }
+    else if constexpr (ACT == TMI_ACT_RELU)
+        value = g < 0.0f ? 0.0f : g, slope = g > 0.0f ? 1.0f : 0.0f;
+    else
+    {
+        const float s = logistic(g);
+        value = s, slope = s * (1.0f - s);
+    }
+}
+template <typename F>
+__device__ __forceinline__ void for_act(int act, F&& f)
 {
     switch (act)
     {
         case TMI_ACT_SILU:
-        {
-            const float s = logistic(g);
-            value = g * s, slope = s * (1.0f + g * (1.0f - s));
-            return;
-        }
+            return f(std::integral_constant<int, TMI_ACT_SILU>());
         case TMI_ACT_GELU:
-        {
-            const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
-            value = g * cdf, slope = cdf + g * (expf(-0.5f * g * g) * 0.39894228040143268f);
-            return;
-        }
+            return f(std::integral_constant<int, TMI_ACT_GELU>());
         case TMI_ACT_GELU_TANH:
-        {
-            const float p = logistic(gelu_tanh_twice(g)), pq = p * (1.0f - p);
-            // far out p is 0 or 1 and g * g may be infinite
-            value = g * p, slope = pq == 0.0f ? p : p + g * pq * (kGeluTwoC * (1.0f + 3.0f * kGeluCubic * g * g));
-            return;
-        }
+            return f(std::integral_constant<int, TMI_ACT_GELU_TANH>());
         case TMI_ACT_RELU:
-            value = g < 0.0f ? 0.0f : g, slope = g > 0.0f ? 1.0f : 0.0f;
-            return;
+            return f(std::integral_constant<int, TMI_ACT_RELU>());
         default:
-        {
-            const float s = logistic(g);
-            value = s, slope = s * (1.0f - s);
-            return;
-        }
+            return f(std::integral_constant<int, TMI_ACT_SIGMOID>());
     }
 }
 
