@@ -99,7 +99,8 @@ __global__ __launch_bounds__(64 * kMostWaves) void few_rows_kernel(RowsArgs a)
                 const uint16_t* row = reinterpret_cast<const uint16_t*>(wbase[s]);
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    t.w[s][j] = load8(row, (int64_t)kt * 128 + 32 * j + 8 * q, decltype(tail)::value ? (int64_t)a.k : INT64_MAX);
+                    t.w[s][j] = decltype(tail)::value ? load8(row, (int64_t)kt * 128 + 32 * j + 8 * q, a.k)
+                                                      : load16(reinterpret_cast<const uint8_t*>(row + (int64_t)kt * 128 + 32 * j + 8 * q));
             }
             else
             {
@@ -114,9 +115,12 @@ __global__ __launch_bounds__(64 * kMostWaves) void few_rows_kernel(RowsArgs a)
 #pragma unroll
             for (int j = 0; j < 4; j++)
             {
-                t.x[mt][j] = v4i{ 0, 0, 0, 0 };
-                if (live[mt])
-                    t.x[mt][j] = load8(xrow[mt], (int64_t)kt * 128 + 32 * j + 8 * q, decltype(tail)::value ? (int64_t)a.k : INT64_MAX);
+                t.x[mt][j]      = v4i{ 0, 0, 0, 0 };
+                const int64_t k = (int64_t)kt * 128 + 32 * j + 8 * q;
+                if constexpr (decltype(tail)::value)
+                    t.x[mt][j] = load8(xrow[mt], k, a.k, live[mt]);
+                else if (live[mt])
+                    t.x[mt][j] = load16(reinterpret_cast<const uint8_t*>(xrow[mt] + k));
             }
     };
     auto multiply = [&](const Tile& t) {

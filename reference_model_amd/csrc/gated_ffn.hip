@@ -43,6 +43,7 @@ struct GemmFfnArgs
     int64_t ldc, ldr, ldo;     // elements
     int32_t M, N;              // results: rows and columns (features of h; d; d)
     int32_t K;                 // summed index (of one half, for d_x)
+    int32_t width;             // elements of a row of an outermost columns operand: N, or 8 where N is less and it was copied
     int32_t half;              // FP, the columns of each half of dp
     int32_t features;          // F
     int32_t blocks;            // of 32 of the summed index
@@ -158,7 +159,7 @@ __global__ __launch_bounds__(64 * WC * WR, 2) void gated_gemm_kernel(GemmFfnArgs
             if constexpr (CIN)
                 cvoff[j] = (uint32_t)((u.row - n0) * a.ldc + u.col) * 2;
             else    // pieces past the row's end repeat the last one; never stored
-                cvoff[j] = (uint32_t)(u.row * a.ldc + (u.col < a.N - 8 - n0 ? u.col : a.N - 8 - n0)) * 2;
+                cvoff[j] = (uint32_t)(u.row * a.ldc + (u.col < a.width - 8 - n0 ? u.col : a.width - 8 - n0)) * 2;
         }
 #pragma unroll
         for (int j = 0; j < RL; j++)
@@ -212,38 +213,62 @@ __global__ __launch_bounds__(64 * WC * WR, 2) void gated_gemm_kernel(GemmFfnArgs
 
     // Otherwise through registers, in two sets
     v4i creg[DIRECT ? 1 : 2][DIRECT ? 1 : CL], rreg[DIRECT ? 1 : 2][DIRECT ? 1 : RL];
-    // (pieces that all lie inside their rows need no look at each element)
-    const bool inner = (CIN || n0 + BN <= a.N) && (RIN || m0 + BM <= a.M);
+    // Pieces that their rows end in, and rows that are none, are put right on their way into LDS, when they are there; a block whose pieces all lie
+    // inside needs no look at them.
+    const bool inner = (CIN || n0 + BN <= a.width) && (RIN || m0 + BM <= a.M);
+    struct Piece
+    {
+        const uint16_t* row;
+        int64_t at, end;
+        bool inside;
+    };
+    auto col_piece = [&](int j, int n) {
+        const Unit u      = col_unit(j);
+        const int k0      = block_k(n);
+        const bool inside = CIN || k0 + u.row < a.K;
+        return Piece{ col_base(j, n) + (CIN ? u.row : inside ? k0 + u.row : a.K - 1) * a.ldc, CIN ? k0 + u.col : n0 + u.col, CIN ? a.K : a.width, inside };
+    };
+    auto row_piece = [&](int j, int n) {
+        const Unit u      = row_unit(j);
+        const int k0      = block_k(n);
+        const bool inside = RIN || k0 + u.row < a.K;
+        return Piece{ a.row + (RIN ? u.row : inside ? k0 + u.row : a.K - 1) * a.ldr, OP == OP_DX ? n * kBlock + u.col : RIN ? k0 + u.col : m0 + u.col,
+                      OP == OP_DX ? a.ldr : RIN ? a.K : a.M, inside };
+    };
     auto fetch = [&](auto SET, int n) {
-        constexpr int P  = decltype(SET)::value;
-        const int k0     = block_k(n);
-        const bool plain = inner && k0 + kBlock <= a.K;
+        constexpr int P = decltype(SET)::value;
 #pragma unroll
         for (int j = 0; j < CL; j++)
         {
-            const Unit u        = col_unit(j);
-            const uint16_t* row = col_base(j, n) + (CIN ? u.row : k0 + u.row) * a.ldc;
-            const int64_t c     = CIN ? k0 + u.col : n0 + u.col;
-            if (plain)
-                creg[P][j] = load16(reinterpret_cast<const uint8_t*>(row + c));
-            else
-                creg[P][j] = load8(row, c, CIN ? a.K : k0 + u.row < a.K ? a.N : 0);
+            const Piece p = col_piece(j, n);
+            creg[P][j]    = load8_raw(p.row, p.at, p.end);
         }
 #pragma unroll
         for (int j = 0; j < RL; j++)
         {
-            const Unit u        = row_unit(j);
-            const uint16_t* row = a.row + (RIN ? u.row : k0 + u.row) * a.ldr;
-            const int64_t c     = OP == OP_DX ? n * kBlock + u.col : RIN ? k0 + u.col : m0 + u.col;
-            if (OP == OP_DX || plain)
-                rreg[P][j] = load16(reinterpret_cast<const uint8_t*>(row + c));
-            else
-                rreg[P][j] = load8(row, c, RIN ? a.K : k0 + u.row < a.K ? a.M : 0);
+            const Piece p = row_piece(j, n);
+            rreg[P][j]    = load8_raw(p.row, p.at, p.end);
         }
     };
-    auto put = [&](auto SET, int stage) {
+    auto put = [&](auto SET, int n, int stage) {
         constexpr int P = decltype(SET)::value;
-        uint8_t* to     = lds + stage * STAGE + tid * 16;
+        if (!(inner && block_k(n) + kBlock <= a.K))
+        {
+#pragma unroll
+            for (int j = 0; j < CL; j++)
+            {
+                const Piece p = col_piece(j, n);
+                creg[P][j]    = settle8(creg[P][j], p.at, p.end, p.inside);
+            }
+#pragma unroll
+            for (int j = 0; j < RL; j++)
+                if (OP != OP_DX)
+                {
+                    const Piece p = row_piece(j, n);
+                    rreg[P][j]    = settle8(rreg[P][j], p.at, p.end, p.inside);
+                }
+        }
+        uint8_t* to = lds + stage * STAGE + tid * 16;
 #pragma unroll
         for (int j = 0; j < CL; j++)
             *reinterpret_cast<v4i*>(to + j * THREADS * 16) = creg[P][j];
@@ -387,35 +412,35 @@ __global__ __launch_bounds__(64 * WC * WR, 2) void gated_gemm_kernel(GemmFfnArgs
         }
         else
         {
-            // blocks 0 and 1 in LDS, 2 and 3 in the registers; behind its barrier a block n writes block n + 2, and fetches n + 4
+            // Blocks 0 and 1 in LDS, 2 and 3 in the registers; behind its barrier a block n writes block n + 2, and fetches n + 4.  Past the last block
+            // that one is fetched again, so that no branch stands between the loads and the count of those to wait for.
+            auto last = [&](int n) { return n < block1 ? n : block1 - 1; };
             fetch(zero, block0);
-            if (block0 + 1 < block1)
-                fetch(one, block0 + 1);
-            put(zero, 0);
-            put(one, 1);
-            if (block0 + 2 < block1)
-                fetch(zero, block0 + 2);
-            if (block0 + 3 < block1)
-                fetch(one, block0 + 3);
+            fetch(one, last(block0 + 1));
+            put(zero, block0, 0);
+            put(one, last(block0 + 1), 1);
+            fetch(zero, last(block0 + 2));
+            fetch(one, last(block0 + 3));
             __syncthreads();
             first_reads();
             auto one_block = [&](auto SET, int n) {
                 cur          = next_of(cur);
                 auto publish = [&]() {
                     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                    put(SET, next_of(cur));
-                    if (n + 4 < block1)
-                        fetch(SET, n + 4);
+                    put(SET, last(n + 2), next_of(cur));
+                    fetch(SET, last(n + 4));
                 };
                 block(SET, lds + cur * STAGE, publish, zero, [](int) {});
             };
+            int n = block0;
 #pragma unroll 1
-            for (int n = block0; n < block1; n += 2)
+            for (; n + 1 < block1; n += 2)
             {
                 one_block(zero, n);
-                if (n + 1 < block1)
-                    one_block(one, n + 1);
+                one_block(one, n + 1);
             }
+            if (n < block1)
+                one_block(zero, n);
         }
     }
 
@@ -625,6 +650,20 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(SlopeArgs a)
     }
 }
 
+// Rows of less than eight elements, filled up with zeros to eight
+__global__ __launch_bounds__(256) void gated_widen_kernel(const uint16_t* in, int64_t ld, int width, int64_t rows, uint16_t* out)
+{
+    const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (m >= rows)
+        return;
+    v4i v = { 0, 0, 0, 0 };
+#pragma unroll
+    for (int e = 0; e < 7; e++)
+        if (e < width)
+            v[e >> 1] |= (int)((uint32_t)in[m * ld + e] << (16 * (e & 1)));
+    *reinterpret_cast<v4i*>(out + m * 8) = v;
+}
+
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 
 enum
@@ -667,8 +706,8 @@ Shape shape_of(int op, int64_t M, int64_t N, int blocks, bool fast)
             s.splits         = s.per_split ? (blocks + s.per_split - 1) / s.per_split : 1;
             const int64_t n  = (int64_t)s.tiles_m * s.tiles_n * s.splits;
             const int64_t rounds = (n + of[tile].slots - 1) / of[tile].slots;
-            // (of the smallest tile the first 256 have a CU each)
-            const double busy = n >= of[tile].slots ? 1 : tile == TILE_128 ? (n > 256 ? n / 256.0 - 1 : 0) : (double)n / of[tile].slots;
+            // (of the smallest tile 256 have a CU each; of more some share one, and the last of those counts)
+            const double busy = tile == TILE_128 ? n > 256 : n >= 256 ? 1 : n / 256.0;
             double us         = rounds * (s.per_split * (of[tile].empty + (of[tile].full - of[tile].empty) * busy) + of[tile].tile);
             if (s.splits > 1)
                 us += 3 + (double)M * N * (op == OP_FORWARD ? 2 : 1) * 4 * 2 * s.splits / 4.5e6;
@@ -743,6 +782,7 @@ struct BackwardPlan
 {
     int64_t half, ldp;
     size_t dp_bytes;
+    size_t x_bytes, w_bytes;    // of copies of x, and of gate or up: rows of less than eight elements
     int dx_blocks, dw_blocks;
     bool dx_fast, dw_fast;
     Shape dx, dw;
@@ -757,9 +797,12 @@ BackwardPlan backward_plan(const tmi_gated_ffn_desc_t& d, const void* x, const v
     p.dp_bytes       = (size_t)d.rows * p.ldp * 2;
     p.dx_blocks      = (int)(2 * p.half / kBlock);
     p.dw_blocks      = (int)(((int64_t)d.rows + kBlock - 1) / kBlock);
+    const bool few   = d.in_features < 8;
+    p.x_bytes        = few ? (size_t)d.rows * 16 : 0;
+    p.w_bytes        = few ? (size_t)d.hidden_features * 16 : 0;
     const bool near  = p.ldp < (int64_t(1) << 22);
-    p.dx_fast        = near && whole_pieces(gate, d.in_features, d.ld_w) && whole_pieces(up, d.in_features, d.ld_w);
-    p.dw_fast        = near && whole_pieces(x, d.in_features, d.ld_x);
+    p.dx_fast        = near && (few || (whole_pieces(gate, d.in_features, d.ld_w) && whole_pieces(up, d.in_features, d.ld_w)));
+    p.dw_fast        = near && (few || whole_pieces(x, d.in_features, d.ld_x));
     p.dx             = shape_of(OP_DX, d.rows, d.in_features, p.dx_blocks, p.dx_fast);
     p.dw             = shape_of(OP_DW, 2 * p.half, d.in_features, p.dw_blocks, p.dw_fast);
     return p;
@@ -788,13 +831,13 @@ const char* launch_gated_ffn(hipStream_t st, const tmi_gated_ffn_desc_t& d, cons
     return launch_product<OP_FORWARD>(st, d.dtype, a, p.shape, p.fast) ? "gated_ffn" : nullptr;
 }
 
-// dp, then the partial sums of one product after the other
+// dp, then copies of narrow operands, then the partial sums of one product after the other
 size_t gated_ffn_backward_scratch_bytes(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up, bool dx, bool dw)
 {
     const BackwardPlan p = backward_plan(d, x, gate, up);
     const size_t of_dx   = dx ? part_bytes(OP_DX, p.dx, d.rows, d.in_features) : 0;
     const size_t of_dw   = dw ? part_bytes(OP_DW, p.dw, 2 * p.half, d.in_features) : 0;
-    return p.dp_bytes + (of_dx > of_dw ? of_dx : of_dw);
+    return p.dp_bytes + p.x_bytes + 2 * p.w_bytes + (of_dx > of_dw ? of_dx : of_dw);
 }
 
 const char* launch_gated_ffn_backward(hipStream_t st, const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up,
@@ -815,20 +858,31 @@ const char* launch_gated_ffn_backward(hipStream_t st, const tmi_gated_ffn_desc_t
 
     GemmFfnArgs a{};
     a.row = q.dp, a.ldr = p.ldp, a.half = (int32_t)p.half, a.features = d.hidden_features;
-    a.part  = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + p.dp_bytes);
+    uint8_t* narrow = static_cast<uint8_t*>(scratch) + p.dp_bytes;
+    auto copied     = [&](const void* v, int64_t ld, int64_t rows, size_t bytes) {
+        if (!bytes)
+            return static_cast<const uint16_t*>(v);
+        gated_widen_kernel<<<(int)((rows + 255) / 256), 256, 0, st>>>(static_cast<const uint16_t*>(v), ld, d.in_features, rows, reinterpret_cast<uint16_t*>(narrow));
+        narrow += bytes;
+        return reinterpret_cast<const uint16_t*>(narrow - bytes);
+    };
+    a.part  = reinterpret_cast<float*>(narrow + p.x_bytes + 2 * p.w_bytes);
     a.zeros = static_cast<const uint8_t*>(zeros);
     a.N     = d.in_features;
+    a.width = d.in_features < 8 ? 8 : d.in_features;
     bool ok = true;
     if (d_x)
     {
-        a.col[0] = static_cast<const uint16_t*>(gate), a.col[1] = static_cast<const uint16_t*>(up), a.ldc = d.ld_w;
+        a.col[0] = copied(gate, d.ld_w, d.hidden_features, p.w_bytes), a.col[1] = copied(up, d.ld_w, d.hidden_features, p.w_bytes);
+        a.ldc    = d.in_features < 8 ? 8 : d.ld_w;
         a.out[0] = static_cast<uint16_t*>(d_x), a.out[1] = nullptr, a.ldo = d.ld_x;
         a.M = d.rows, a.K = d.hidden_features, a.blocks = p.dx_blocks;
         ok = launch_product<OP_DX>(st, d.dtype, a, p.dx, p.dx_fast);
     }
     if (ok && d_gate)
     {
-        a.col[0] = a.col[1] = static_cast<const uint16_t*>(x), a.ldc = d.ld_x;
+        a.col[0] = a.col[1] = copied(x, d.ld_x, d.rows, p.x_bytes);
+        a.ldc    = d.in_features < 8 ? 8 : d.ld_x;
         a.out[0] = static_cast<uint16_t*>(d_gate), a.out[1] = static_cast<uint16_t*>(d_up), a.ldo = d.ld_w;
         a.M = (int32_t)(2 * p.half), a.K = d.rows, a.blocks = p.dw_blocks;
         ok = launch_product<OP_DW>(st, d.dtype, a, p.dw, p.dw_fast);

@@ -78,7 +78,7 @@ __global__ __launch_bounds__(64 * kWaves) void int4_pack_kernel(Int4Args a)
         v4i w[4];
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            w[j] = load8(row, k0 + 32 * j + 8 * q, live ? a.k : 0);
+            w[j] = load8(row, k0 + 32 * j + 8 * q, a.k, live);
         uint32_t m[4];
 #pragma unroll
         for (int j = 0; j < 4; j++)

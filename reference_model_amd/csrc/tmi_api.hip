@@ -2249,7 +2249,7 @@ int tmi_gated_ffn(tmi_ctx_t* ctx, const tmi_gated_ffn_desc_t* desc, const void* 
         ctx->last_kernel = "empty";
         return TMI_VALID;
     }
-    if (d.rows <= kFfnFewRows)
+    if (d.rows <= kFfnFewRows || d.in_features < 8)    // (the other kernel reads rows of eight elements at least)
         return after_launch(ctx, launch_ffn_rows(ctx->stream, d.dtype, d.activation, d.rows, d.in_features, d.hidden_features, x_dev, d.ld_x, gate_dev,
                                                  up_dev, d.ld_w, h_dev, pre_gate_dev, pre_up_dev, d.ld_h));
     const size_t bytes = gated_ffn_scratch_bytes(d, x_dev, gate_dev, up_dev);
