@@ -810,6 +810,11 @@ BackwardPlan backward_plan(const tmi_gated_ffn_desc_t& d, const void* x, const v
 
 }    // namespace
 
+void launch_widen_rows(hipStream_t st, const void* in, int64_t ld, int32_t width, int64_t rows, void* out)
+{
+    gated_widen_kernel<<<(int)((rows + 255) / 256), 256, 0, st>>>(static_cast<const uint16_t*>(in), ld, width, rows, static_cast<uint16_t*>(out));
+}
+
 size_t gated_ffn_scratch_bytes(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up)
 {
     return part_bytes(OP_FORWARD, forward_plan(d, x, gate, up).shape, d.rows, d.hidden_features);
@@ -862,7 +867,7 @@ const char* launch_gated_ffn_backward(hipStream_t st, const tmi_gated_ffn_desc_t
     auto copied     = [&](const void* v, int64_t ld, int64_t rows, size_t bytes) {
         if (!bytes)
             return static_cast<const uint16_t*>(v);
-        gated_widen_kernel<<<(int)((rows + 255) / 256), 256, 0, st>>>(static_cast<const uint16_t*>(v), ld, d.in_features, rows, reinterpret_cast<uint16_t*>(narrow));
+        launch_widen_rows(st, v, ld, d.in_features, rows, narrow);
         narrow += bytes;
         return reinterpret_cast<const uint16_t*>(narrow - bytes);
     };

@@ -2036,7 +2036,7 @@ int tmi_clamp_fp(tmi_ctx_t* ctx, int32_t dtype, int64_t n, const void* in_dev, f
 
 // ---- the gated feed-forward block and 4-bit weights ----------------------------------------------------------------------
 
-constexpr int32_t kFfnFewRows = 64;    // up to here the gated block in 16 bits runs as products of a few rows
+constexpr int32_t kFfnFewRows = 32;    // up to here the gated block in 16 bits runs as products of a few rows
 
 static bool ffn_dtype(int32_t dtype)
 {
@@ -2180,8 +2180,17 @@ static int int4_rows(tmi_ctx* ctx, const char* op, const tmi_int4_desc_t* d, boo
         ctx->last_kernel = "empty";
         return TMI_VALID;
     }
-    return after_launch(ctx, launch_int4_rows(ctx->stream, d->dtype, d->group, gated, activation, rows, d->out_features, d->in_features, x, ld_x, w, up,
-                                              out, ld_out));
+    int32_t k = d->in_features;
+    if (k > 0 && k < 8)
+    {
+        // the kernel reads rows of eight elements at least: a copy that ends in zeros, as the packed rows do
+        const int wrc = ensure_workspace(ctx, (size_t)rows * 16);
+        if (wrc != TMI_VALID)
+            return wrc;
+        launch_widen_rows(ctx->stream, x, ld_x, k, rows, ctx->workspace);
+        x = ctx->workspace, ld_x = k = 8;
+    }
+    return after_launch(ctx, launch_int4_rows(ctx->stream, d->dtype, d->group, gated, activation, rows, d->out_features, k, x, ld_x, w, up, out, ld_out));
 }
 
 int tmi_matvec_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, int32_t rows, const void* x_dev, int64_t ld_x, const void* packed_dev,
@@ -2249,7 +2258,21 @@ int tmi_gated_ffn(tmi_ctx_t* ctx, const tmi_gated_ffn_desc_t* desc, const void* 
         ctx->last_kernel = "empty";
         return TMI_VALID;
     }
-    if (d.rows <= kFfnFewRows || d.in_features < 8)    // (the other kernel reads rows of eight elements at least)
+    if (d.in_features > 0 && d.in_features < 8)
+    {
+        // the kernels read rows of eight elements at least: copies that end in zeros
+        const size_t x_bytes = (size_t)d.rows * 16, w_bytes = (size_t)d.hidden_features * 16;
+        const int wrc        = ensure_workspace(ctx, x_bytes + 2 * w_bytes);
+        if (wrc != TMI_VALID)
+            return wrc;
+        uint8_t* to = static_cast<uint8_t*>(ctx->workspace);
+        launch_widen_rows(ctx->stream, x_dev, d.ld_x, d.in_features, d.rows, to);
+        launch_widen_rows(ctx->stream, gate_dev, d.ld_w, d.in_features, d.hidden_features, to + x_bytes);
+        launch_widen_rows(ctx->stream, up_dev, d.ld_w, d.in_features, d.hidden_features, to + x_bytes + w_bytes);
+        return after_launch(ctx, launch_ffn_rows(ctx->stream, d.dtype, d.activation, d.rows, 8, d.hidden_features, to, 8, to + x_bytes,
+                                                 to + x_bytes + w_bytes, 8, h_dev, pre_gate_dev, pre_up_dev, d.ld_h));
+    }
+    if (d.rows <= kFfnFewRows)
         return after_launch(ctx, launch_ffn_rows(ctx->stream, d.dtype, d.activation, d.rows, d.in_features, d.hidden_features, x_dev, d.ld_x, gate_dev,
                                                  up_dev, d.ld_w, h_dev, pre_gate_dev, pre_up_dev, d.ld_h));
     const size_t bytes = gated_ffn_scratch_bytes(d, x_dev, gate_dev, up_dev);

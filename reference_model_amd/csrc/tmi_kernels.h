@@ -316,13 +316,15 @@ const char* launch_matmul_i16_direct(hipStream_t st, int32_t N, int32_t H, int32
 const char* launch_matmul_direct(hipStream_t st, int32_t in_dtype, int32_t N, int32_t H, int32_t C, int32_t W,
                                  const void* a, const void* b, int32_t a_zp, int32_t b_zp, void* out);
 
-// few_rows.hip: products of a few rows with 4-bit weights (`up` not read), the gated block on them, and the gated block on 16-bit weights
+// few_rows.hip (rows of x of 8 elements at least, or of none): products of a few rows with 4-bit weights (`up` not read), the gated block on them, and the gated block on 16-bit weights
 const char* launch_int4_rows(hipStream_t st, int32_t dtype, int32_t group, bool gated, int32_t act, int32_t rows, int32_t n, int32_t k,
                              const void* x, int64_t ldx, const void* w, const void* up, void* out, int64_t ldo);
 const char* launch_ffn_rows(hipStream_t st, int32_t dtype, int32_t act, int32_t rows, int32_t d, int32_t f, const void* x, int64_t ldx,
                             const void* gate, const void* up, int64_t ldw, void* out, void* pre_gate, void* pre_up, int64_t ldo);
 // gated_ffn.hip: the gated block on many rows and its gradients (row strides of the descriptors filled in).  `scratch`: of as many bytes as the
 // functions before say (forward: nullptr does too, with the sum in one piece); zeros: 64 bytes of them
+// rows of `width` < 8 elements of 16 bits, filled up with zeros to 8
+void launch_widen_rows(hipStream_t st, const void* in, int64_t ld, int32_t width, int64_t rows, void* out);
 size_t gated_ffn_scratch_bytes(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up);
 const char* launch_gated_ffn(hipStream_t st, const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up, void* h, void* pre_gate,
                              void* pre_up, void* scratch, const void* zeros);

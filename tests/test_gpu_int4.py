@@ -204,3 +204,37 @@ def test_what_is_refused(ctx):
     refused("negative", ctx.matvec_int4, ctx.int4_desc(*ok), -1, p, 0, p, p, 0)
     refused("null tensor", ctx.pack_int4, ctx.int4_desc(*ok), p, 0, None, p)
     assert ctx.sync() == capi.VALID
+
+
+@pytest.mark.parametrize("shape", [(1, 16 * 1030, 4100, 128), (3, 16 * 1030, 4100, 32), (16, 16 * 600 + 5, 2050, 64), (13, 4099, 4111, 64), (9, 200, 33000, 128), (33, 5500, 2048, 32),
+                                   (64, 4099, 4100, 128), (50, 2000, 1111, 64), (64, 40, 9000, 32)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_large_matrices(ctx, kind, shape):
+    """blocks of weight rows one after the other, columns of x a part at a time, row tiles of x in one or several workgroups; some of the results"""
+    kind, (m, n, k, group) = KINDS[kind], shape
+    rng = np.random.default_rng(n)
+    x = kind.wide(kind.narrow(rng.normal(0, 1, (m, k))))
+    desc = ctx.int4_desc(kind.dtype, group, n, k)
+    pick = np.unique(np.r_[0:20, rng.integers(0, n, 40), n - 20:n])
+    packs, w = [], []
+    for _ in range(2):
+        v, scales = rng.integers(-8, 8, (n, k), np.int8), kind.narrow(rng.uniform(0.01, 0.1, (n, -(-k // group))))
+        dv, ds = ctx.upload(v), ctx.upload(scales, kind.dtype)
+        to = ctx.upload(np.zeros(ctx.int4_packed_bytes(desc), np.uint8))
+        ctx.pack_int4(desc, dv, 0, ds, to)
+        assert ctx.sync() == capi.VALID
+        dv.free(), ds.free()
+        packs.append(to)
+        w.append(ref.weights(kind, v[pick].astype(np.int64), scales[pick], group))
+    dev, out = Rows(ctx, kind, (m, k), x, 3, 1), Rows(ctx, kind, (m, n), None, 8, 0)
+    ctx.matvec_int4(desc, m, dev.at, k + 3, packs[0], out.at, n + 8)
+    assert ctx.sync() == capi.VALID
+    got = out.values()
+    near(got[:, pick], ref.product(kind, x, w[0]))
+    ctx.matvec_int4(desc, m, dev.at, k + 3, packs[0], out.at, n + 8)
+    assert ctx.sync() == capi.VALID and np.array_equal(out.values(), got)
+    ctx.gated_ffn_int4(desc, capi.ACT_GELU_TANH, m, dev.at, k + 3, *packs, out.at, n + 8)
+    assert ctx.sync() == capi.VALID
+    near(out.values()[:, pick], ref.gated(kind, "gelu_tanh", x, *w)[0])
+    for t in [dev, out] + packs:
+        t.free()
