@@ -252,6 +252,7 @@ __global__ __launch_bounds__(64 * kShortWaves) void few_rows_kernel(RowsArgs a)
         store_rows<T, DENSE, MT, GATED>(a, red, waves, o, (int64_t)tn * 16, row0);
 }
 
+constexpr int kAhead = 4;                              // pieces of x that a lane asks for at once
 constexpr int kLds = 156 * 1024, kLdsHalf = 78 * 1024;    // for one workgroup of a CU, and for two
 
 // MT: tiles of 16 rows of x; PER: groups of a tile; U: column tiles in flight
@@ -297,14 +298,14 @@ __global__ __launch_bounds__(1024) void int4_stream_kernel(RowsArgs a)
             const uint16_t* row = a.x + (row0 + m) * a.ldx + (int64_t)from * 128;
             const int end       = a.k - from * 128;
 #pragma unroll 1
-            for (int c0 = wave / apart * 64 + lane; c0 < pieces; c0 += 4 * lanes)
+            for (int c0 = wave / apart * 64 + lane; c0 < pieces; c0 += kAhead * lanes)
             {
-                v4i v[4];
+                v4i v[kAhead];
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                for (int i = 0; i < kAhead; i++)
                     v[i] = load8_raw(row, 8 * (c0 + i * lanes), end);
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                for (int i = 0; i < kAhead; i++)
                     if (c0 + i * lanes < pieces)
                         *reinterpret_cast<v4i*>(lds + unit_of(c0 + i * lanes, m) * 16) = settle8(v[i], 8 * (c0 + i * lanes), end, true);
             }

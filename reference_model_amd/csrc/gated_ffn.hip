@@ -43,7 +43,7 @@ struct GemmFfnArgs
     int64_t ldc, ldr, ldo;     // elements
     int32_t M, N;              // results: rows and columns (features of h; d; d)
     int32_t K;                 // summed index (of one half, for d_x)
-    int32_t width;             // elements of a row of an outermost columns operand: N, or 8 where N is less and it was copied
+    int32_t width;             // elements of a row of an outermost columns operand: N, or of its copy
     int32_t half;              // FP, the columns of each half of dp
     int32_t features;          // F
     int32_t blocks;            // of 32 of the summed index
@@ -650,18 +650,18 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(SlopeArgs a)
     }
 }
 
-// Rows of less than eight elements, filled up with zeros to eight
-__global__ __launch_bounds__(256) void gated_widen_kernel(const uint16_t* in, int64_t ld, int width, int64_t rows, uint16_t* out)
+// Rows filled up with zeros to whole pieces of eight elements: up to three matrices of one width
+__global__ __launch_bounds__(256) void gated_widen_kernel(WidenRows a)
 {
-    const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (m >= rows)
-        return;
-    v4i v = { 0, 0, 0, 0 };
-#pragma unroll
-    for (int e = 0; e < 7; e++)
-        if (e < width)
-            v[e >> 1] |= (int)((uint32_t)in[m * ld + e] << (16 * (e & 1)));
-    *reinterpret_cast<v4i*>(out + m * 8) = v;
+    const int per_row = (a.width + 7) / 8;
+    const uint16_t* in = static_cast<const uint16_t*>(a.in[blockIdx.y]);
+    const int64_t ld = a.ld[blockIdx.y], units = a.rows[blockIdx.y] * per_row, step = (int64_t)gridDim.x * 256;
+    v4i* out = static_cast<v4i*>(a.out[blockIdx.y]);
+    for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < units; u += step)
+    {
+        const int64_t m = u / per_row;
+        out[u]          = load8(in + m * ld, (u - m * per_row) * 8, a.width);
+    }
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
@@ -682,11 +682,11 @@ struct Shape
 // The tile, and into how many parts the sum is split, by the time that follows from what was measured (us, over 4096 x 2048 x 8192 and halves to
 // eighths of each size): a block of 32 costs a workgroup of the three tiles 0.62, 0.39 and 0.33 on an empty chip and 0.80, 0.48 and 0.58 on
 // a full one (the smaller ones ask L2 for more, the weights' gradients' least), a tile 12, 7 and 6 beside them, and a split its partial sums
-// out and in at 4.5 TB/s and a launch.  Both sides, us: d_x 4096 x 2048 x 8192 (128, 256 and 512 tiles) 240 with the largest tile and two parts, 332, 317
+// out and in at 4.5 TB/s and a launch.  Operands that go through
+// registers cost 1.4 times as much, and take the smallest tile: the others' accumulators leave no room.  Both sides, us: d_x 4096 x 2048 x 8192 (128, 256 and 512 tiles) 240 with the largest tile and two parts, 332, 317
 // and 359 in one part of each; of half the size 73 with four parts, 90 at best in one; forward 512 x 4096 x 2048 81, 52 and 43 in one part, 38, 32
-// and 32 in the best number of parts; 4096 x 2048 x 8192 243, 301 and 328.  Operands that go through registers take the smallest tile: the
-// others' accumulators leave no room.
-Shape shape_of(int op, int64_t M, int64_t N, int blocks, bool fast)
+// and 32 in the best number of parts; 4096 x 2048 x 8192 243, 301 and 328.
+Shape shape_of(int op, int64_t M, int64_t N, int blocks, bool fast, double& least)
 {
     static const struct
     {
@@ -694,7 +694,7 @@ Shape shape_of(int op, int64_t M, int64_t N, int blocks, bool fast)
         double empty, full, tile;
     } of[3] = { { 256, 256, 256, 0.62, 0.80, 12 }, { 256, 128, 256, 0.39, 0.48, 7 }, { 128, 128, 512, 0.33, 0.58, 6 } };
     Shape best{};
-    double least = 0;
+    least = 0;
     for (int tile = fast ? TILE_256 : TILE_128; tile <= TILE_128; tile++)
     {
         const int tn = op == OP_FORWARD ? of[tile].bn / 2 : of[tile].bn;
@@ -717,6 +717,7 @@ Shape shape_of(int op, int64_t M, int64_t N, int blocks, bool fast)
         if (!best.tiles_m)    // no rows
             best = s;
     }
+    least *= fast ? 1 : 1.4;
     return best;
 }
 
@@ -763,86 +764,130 @@ bool whole_pieces(const void* p, int64_t width, int64_t ld)
     return ((uintptr_t)p & 15) == 0 && width % 8 == 0 && ld % 8 == 0 && ld < (int64_t(1) << 22);
 }
 
+int64_t whole_of(int64_t n, int64_t per)
+{
+    return (n + per - 1) / per * per;
+}
+
+// A product's way: of operands that lie in whole pieces, as they are; of others through registers, or on copies that end in zeros, read and written at 3.5
+// TB/s with 8 us for a launch more.  us forward 4096 x 2047 x 8192 460 through registers, 263 on copies, its gradients 905 and 536; 777 x 1111 x 2731 32 and
+// 38, 512 x 4095 x 4096 61 and 87.  (Rows of less than eight elements are always copied: the loads through registers take eight.)
+struct Way
+{
+    bool fast, copies;
+    size_t bytes;     // of the copies
+    Shape shape;
+};
+Way way_of(int op, int64_t M, int64_t N, int blocks, bool whole, int64_t copied_rows, int64_t d)
+{
+    Way w{};
+    double direct = 0, registers = 0;
+    w.shape = shape_of(op, M, N, blocks, true, direct);
+    w.fast  = true;
+    if (whole)
+        return w;
+    const Shape other  = shape_of(op, M, N, blocks, false, registers);
+    const size_t bytes = (size_t)copied_rows * whole_of(d, 8) * 2;
+    if (d < 8 || direct + 2 * (double)bytes / 3.5e6 + 8 < registers)
+        w.copies = true, w.bytes = bytes;
+    else
+        w.fast = false, w.shape = other;
+    return w;
+}
+
 // What a call launches, from its sizes, strides and addresses
 struct ForwardPlan
 {
     int blocks;
-    bool fast;
-    Shape shape;
+    Way way;
 };
 ForwardPlan forward_plan(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up)
 {
     ForwardPlan p;
-    p.blocks = (int)(((int64_t)d.in_features + kBlock - 1) / kBlock);
-    p.fast   = whole_pieces(x, d.in_features, d.ld_x) && whole_pieces(gate, d.in_features, d.ld_w) && whole_pieces(up, d.in_features, d.ld_w);
-    p.shape  = shape_of(OP_FORWARD, d.rows, d.hidden_features, p.blocks, p.fast);
+    const bool whole = whole_pieces(x, d.in_features, d.ld_x) && whole_pieces(gate, d.in_features, d.ld_w) && whole_pieces(up, d.in_features, d.ld_w);
+    p.blocks         = (int)(whole_of(d.in_features, kBlock) / kBlock);
+    p.way            = way_of(OP_FORWARD, d.rows, d.hidden_features, p.blocks, whole, (int64_t)d.rows + 2 * (int64_t)d.hidden_features, d.in_features);
     return p;
 }
 struct BackwardPlan
 {
     int64_t half, ldp;
     size_t dp_bytes;
-    size_t x_bytes, w_bytes;    // of copies of x, and of gate or up: rows of less than eight elements
     int dx_blocks, dw_blocks;
-    bool dx_fast, dw_fast;
-    Shape dx, dw;
+    Way dx, dw;
 };
 BackwardPlan backward_plan(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up)
 {
     BackwardPlan p;
-    p.half           = ((int64_t)d.hidden_features + 63) / 64 * 64;
+    p.half           = whole_of(d.hidden_features, 64);
     // Rows of dp lie 128 bytes further apart than they are long: the 256 rows that a tile reads 64 bytes of at a time would otherwise lie a power
     // of two apart where F is one, on few channels of the memory.
     p.ldp            = 2 * p.half + 64;
     p.dp_bytes       = (size_t)d.rows * p.ldp * 2;
     p.dx_blocks      = (int)(2 * p.half / kBlock);
-    p.dw_blocks      = (int)(((int64_t)d.rows + kBlock - 1) / kBlock);
-    const bool few   = d.in_features < 8;
-    p.x_bytes        = few ? (size_t)d.rows * 16 : 0;
-    p.w_bytes        = few ? (size_t)d.hidden_features * 16 : 0;
-    const bool near  = p.ldp < (int64_t(1) << 22);
-    p.dx_fast        = near && (few || (whole_pieces(gate, d.in_features, d.ld_w) && whole_pieces(up, d.in_features, d.ld_w)));
-    p.dw_fast        = near && (few || whole_pieces(x, d.in_features, d.ld_x));
-    p.dx             = shape_of(OP_DX, d.rows, d.in_features, p.dx_blocks, p.dx_fast);
-    p.dw             = shape_of(OP_DW, 2 * p.half, d.in_features, p.dw_blocks, p.dw_fast);
+    p.dw_blocks      = (int)(whole_of(d.rows, kBlock) / kBlock);
+    const int64_t D  = d.in_features, F = d.hidden_features;
+    p.dx             = way_of(OP_DX, d.rows, D, p.dx_blocks, whole_pieces(gate, D, d.ld_w) && whole_pieces(up, D, d.ld_w), 2 * F, D);
+    p.dw             = way_of(OP_DW, 2 * p.half, D, p.dw_blocks, whole_pieces(x, D, d.ld_x), d.rows, D);
     return p;
 }
 
 }    // namespace
 
-void launch_widen_rows(hipStream_t st, const void* in, int64_t ld, int32_t width, int64_t rows, void* out)
+void launch_widen_rows(hipStream_t st, const WidenRows& a)
 {
-    gated_widen_kernel<<<(int)((rows + 255) / 256), 256, 0, st>>>(static_cast<const uint16_t*>(in), ld, width, rows, static_cast<uint16_t*>(out));
+    int64_t most = 0;
+    for (int i = 0; i < a.n; i++)
+        most = most > a.rows[i] ? most : a.rows[i];
+    const int64_t groups = (most * ((a.width + 7) / 8) + 255) / 256;
+    if (groups > 0)
+        gated_widen_kernel<<<dim3((int)(groups < 2048 ? groups : 2048), a.n), 256, 0, st>>>(a);
 }
 
 size_t gated_ffn_scratch_bytes(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up)
 {
-    return part_bytes(OP_FORWARD, forward_plan(d, x, gate, up).shape, d.rows, d.hidden_features);
+    const Way w = forward_plan(d, x, gate, up).way;
+    return w.bytes + part_bytes(OP_FORWARD, w.shape, d.rows, d.hidden_features);
 }
 
 const char* launch_gated_ffn(hipStream_t st, const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up, void* h, void* pre_gate,
                              void* pre_up, void* scratch, const void* zeros)
 {
     ForwardPlan p = forward_plan(d, x, gate, up);
+    if (!scratch && p.way.copies)
+    {
+        double us;
+        p.way.copies = p.way.fast = false;
+        p.way.shape = shape_of(OP_FORWARD, d.rows, d.hidden_features, p.blocks, false, us);
+    }
     if (!scratch)
-        p.shape.splits = 1, p.shape.per_split = p.blocks;
+        p.way.shape.splits = 1, p.way.shape.per_split = p.blocks;
     GemmFfnArgs a{};
     a.col[0] = static_cast<const uint16_t*>(gate), a.col[1] = static_cast<const uint16_t*>(up), a.row = static_cast<const uint16_t*>(x);
     a.out[0] = static_cast<uint16_t*>(h);
     a.pre_gate = static_cast<uint16_t*>(pre_gate), a.pre_up = static_cast<uint16_t*>(pre_up);
-    a.part = static_cast<float*>(scratch), a.zeros = static_cast<const uint8_t*>(zeros);
+    a.zeros = static_cast<const uint8_t*>(zeros);
     a.ldc = d.ld_w, a.ldr = d.ld_x, a.ldo = d.ld_h;
     a.M = d.rows, a.N = d.hidden_features, a.K = d.in_features, a.blocks = p.blocks, a.act = d.activation;
-    return launch_product<OP_FORWARD>(st, d.dtype, a, p.shape, p.fast) ? "gated_ffn" : nullptr;
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + p.way.bytes);
+    if (p.way.copies)
+    {
+        // (columns that fill up the last piece are zeros on both sides of the products)
+        const int64_t wide = whole_of(d.in_features, 8);
+        uint16_t *cx = static_cast<uint16_t*>(scratch), *cg = cx + d.rows * wide, *cu = cg + d.hidden_features * wide;
+        launch_widen_rows(st, WidenRows{ 3, d.in_features, { x, gate, up }, { d.ld_x, d.ld_w, d.ld_w }, { d.rows, d.hidden_features, d.hidden_features }, { cx, cg, cu } });
+        a.row = cx, a.col[0] = cg, a.col[1] = cu, a.ldr = a.ldc = wide, a.K = (int32_t)wide;
+    }
+    return launch_product<OP_FORWARD>(st, d.dtype, a, p.way.shape, p.way.fast) ? "gated_ffn" : nullptr;
 }
 
-// dp, then copies of narrow operands, then the partial sums of one product after the other
+// dp, then copies, then the partial sums of one product after the other
 size_t gated_ffn_backward_scratch_bytes(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up, bool dx, bool dw)
 {
     const BackwardPlan p = backward_plan(d, x, gate, up);
-    const size_t of_dx   = dx ? part_bytes(OP_DX, p.dx, d.rows, d.in_features) : 0;
-    const size_t of_dw   = dw ? part_bytes(OP_DW, p.dw, 2 * p.half, d.in_features) : 0;
-    return p.dp_bytes + p.x_bytes + 2 * p.w_bytes + (of_dx > of_dw ? of_dx : of_dw);
+    const size_t of_dx   = dx ? part_bytes(OP_DX, p.dx.shape, d.rows, d.in_features) : 0;
+    const size_t of_dw   = dw ? part_bytes(OP_DW, p.dw.shape, 2 * p.half, d.in_features) : 0;
+    return p.dp_bytes + p.dx.bytes + p.dw.bytes + (of_dx > of_dw ? of_dx : of_dw);
 }
 
 const char* launch_gated_ffn_backward(hipStream_t st, const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up,
@@ -861,36 +906,39 @@ const char* launch_gated_ffn_backward(hipStream_t st, const tmi_gated_ffn_desc_t
     else if (grid > 0)
         gated_slope_kernel<_Float16><<<grid, 256, 0, st>>>(q);
 
+    const int64_t wide = whole_of(d.in_features, 8);
+    uint16_t* copies   = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(scratch) + p.dp_bytes);
     GemmFfnArgs a{};
     a.row = q.dp, a.ldr = p.ldp, a.half = (int32_t)p.half, a.features = d.hidden_features;
-    uint8_t* narrow = static_cast<uint8_t*>(scratch) + p.dp_bytes;
-    auto copied     = [&](const void* v, int64_t ld, int64_t rows, size_t bytes) {
-        if (!bytes)
-            return static_cast<const uint16_t*>(v);
-        launch_widen_rows(st, v, ld, d.in_features, rows, narrow);
-        narrow += bytes;
-        return reinterpret_cast<const uint16_t*>(narrow - bytes);
-    };
-    a.part  = reinterpret_cast<float*>(narrow + p.x_bytes + 2 * p.w_bytes);
+    a.part  = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(copies) + p.dx.bytes + p.dw.bytes);
     a.zeros = static_cast<const uint8_t*>(zeros);
     a.N     = d.in_features;
-    a.width = d.in_features < 8 ? 8 : d.in_features;
     bool ok = true;
     if (d_x)
     {
-        a.col[0] = copied(gate, d.ld_w, d.hidden_features, p.w_bytes), a.col[1] = copied(up, d.ld_w, d.hidden_features, p.w_bytes);
-        a.ldc    = d.in_features < 8 ? 8 : d.ld_w;
+        a.col[0] = static_cast<const uint16_t*>(gate), a.col[1] = static_cast<const uint16_t*>(up), a.ldc = d.ld_w, a.width = d.in_features;
+        if (p.dx.copies)
+        {
+            launch_widen_rows(st, WidenRows{ 2, d.in_features, { gate, up }, { d.ld_w, d.ld_w }, { d.hidden_features, d.hidden_features },
+                                             { copies, copies + d.hidden_features * wide } });
+            a.col[0] = copies, a.col[1] = copies + d.hidden_features * wide, a.ldc = wide, a.width = (int32_t)wide;
+        }
         a.out[0] = static_cast<uint16_t*>(d_x), a.out[1] = nullptr, a.ldo = d.ld_x;
         a.M = d.rows, a.K = d.hidden_features, a.blocks = p.dx_blocks;
-        ok = launch_product<OP_DX>(st, d.dtype, a, p.dx, p.dx_fast);
+        ok = launch_product<OP_DX>(st, d.dtype, a, p.dx.shape, p.dx.fast);
     }
     if (ok && d_gate)
     {
-        a.col[0] = a.col[1] = copied(x, d.ld_x, d.rows, p.x_bytes);
-        a.ldc    = d.in_features < 8 ? 8 : d.ld_x;
+        a.col[0] = a.col[1] = static_cast<const uint16_t*>(x), a.ldc = d.ld_x, a.width = d.in_features;
+        if (p.dw.copies)
+        {
+            uint16_t* cx = copies + p.dx.bytes / 2;
+            launch_widen_rows(st, WidenRows{ 1, d.in_features, { x }, { d.ld_x }, { d.rows }, { cx } });
+            a.col[0] = a.col[1] = cx, a.ldc = wide, a.width = (int32_t)wide;
+        }
         a.out[0] = static_cast<uint16_t*>(d_gate), a.out[1] = static_cast<uint16_t*>(d_up), a.ldo = d.ld_w;
         a.M = (int32_t)(2 * p.half), a.K = d.rows, a.blocks = p.dw_blocks;
-        ok = launch_product<OP_DW>(st, d.dtype, a, p.dw, p.dw_fast);
+        ok = launch_product<OP_DW>(st, d.dtype, a, p.dw.shape, p.dw.fast);
     }
     return ok ? "gated_ffn_backward" : nullptr;
 }

@@ -24,6 +24,16 @@ struct Int4Args
 
 constexpr int kWaves = 4;
 
+typedef unsigned short v2us __attribute__((ext_vector_type(2)));
+
+// v_cvt_i32_f32 itself: what C leaves undefined is defined there, NaN to 0 and the others to the nearest int32
+__device__ __forceinline__ int to_int(float t)
+{
+    int v;
+    asm("v_cvt_i32_f32 %0, %1" : "=v"(v) : "v"(t));
+    return v;
+}
+
 // the largest bit pattern of |w| over the four lanes of a row; NaN has the largest of all and stays
 __device__ __forceinline__ uint32_t row_max(uint32_t v)
 {
@@ -38,92 +48,97 @@ template <typename T, int PER, bool GIVEN>
 __global__ __launch_bounds__(64 * kWaves) void int4_pack_kernel(Int4Args a)
 {
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-    const int64_t tile = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (tile >= a.tiles)
-        return;
-    const int64_t tn = tile / a.tiles_k;
-    const int kt     = (int)(tile - tn * a.tiles_k);
-    const int64_t n  = tn * kInt4Rows + r;
-    const bool live  = n < a.n;
-    const int k0     = kt * kInt4Cols;
-    v4i packed;
-    uint16_t scale[PER];
-    if constexpr (GIVEN)
+    for (int64_t tile = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); tile < a.tiles; tile += (int64_t)gridDim.x * kWaves)
     {
-        const int8_t* row = static_cast<const int8_t*>(a.in) + (live ? n : 0) * a.ld;
-#pragma unroll
-        for (int j = 0; j < 4; j++)
+        const int64_t tn = tile / a.tiles_k;
+        const int kt     = (int)(tile - tn * a.tiles_k);
+        const int64_t n  = tn * kInt4Rows + r;
+        const bool live  = n < a.n;
+        const int k0     = kt * kInt4Cols;
+        v4i packed;
+        uint16_t scale[PER];
+        if constexpr (GIVEN)
         {
-            uint32_t w = 0;
+            const int8_t* row = static_cast<const int8_t*>(a.in) + (live ? n : 0) * a.ld;
 #pragma unroll
-            for (int e = 0; e < 8; e++)
+            for (int j = 0; j < 4; j++)
             {
-                const int k = k0 + 32 * j + 8 * q + e;
-                int v       = live && k < a.k ? row[k] : 0;
-                v           = v < -8 ? -8 : (v > 7 ? 7 : v);
-                w |= (uint32_t)(v + 8) << (4 * (e >> 1) + 16 * (e & 1));
-            }
-            packed[j] = (int)w;
-        }
-#pragma unroll
-        for (int g = 0; g < PER; g++)
-        {
-            const int64_t at = (int64_t)kt * PER + g;
-            scale[g]         = live && at < a.groups ? a.scales[n * a.groups + at] : 0;
-        }
-    }
-    else
-    {
-        const uint16_t* row = static_cast<const uint16_t*>(a.in) + (live ? n : 0) * a.ld;
-        v4i w[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            w[j] = load8(row, k0 + 32 * j + 8 * q, a.k, live);
-        uint32_t m[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-        {
-            m[j] = 0;
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-            {
-                const uint32_t b = half_of(w[j], e) & 0x7FFFu;
-                m[j]             = m[j] > b ? m[j] : b;
-            }
-        }
-#pragma unroll
-        for (int g = 0; g < PER; g++)
-        {
-            uint32_t top = 0;
-#pragma unroll
-            for (int j = g * 4 / PER; j < (g + 1) * 4 / PER; j++)
-                top = top > m[j] ? top : m[j];
-            scale[g]      = to_bits16<T>(from_bits16<T>((uint16_t)row_max(top)) / 7.0f);
-            const float s = from_bits16<T>(scale[g]);
-#pragma unroll
-            for (int j = g * 4 / PER; j < (g + 1) * 4 / PER; j++)
-            {
-                uint32_t word = 0;
+                uint32_t w = 0;
 #pragma unroll
                 for (int e = 0; e < 8; e++)
                 {
-                    // a division, correctly rounded: no quotient of two 16-bit floats lies so near a half that rint could go the other way
-                    const float t = rintf(from_bits16<T>(half_of(w[j], e)) / s);
-                    const int v   = t == t ? (int)fminf(fmaxf(t, -7.0f), 7.0f) : 0;    // 0 / 0, inf / inf and what is divided by NaN
-                    word |= (uint32_t)(v + 8) << (4 * (e >> 1) + 16 * (e & 1));
+                    const int k = k0 + 32 * j + 8 * q + e;
+                    int v       = live && k < a.k ? row[k] : 0;
+                    v           = v < -8 ? -8 : (v > 7 ? 7 : v);
+                    w |= (uint32_t)(v + 8) << (4 * (e >> 1) + 16 * (e & 1));
                 }
-                packed[j] = (int)word;
+                packed[j] = (int)w;
+            }
+#pragma unroll
+            for (int g = 0; g < PER; g++)
+            {
+                const int64_t at = (int64_t)kt * PER + g;
+                scale[g]         = live && at < a.groups ? a.scales[n * a.groups + at] : 0;
             }
         }
-    }
-    uint8_t* out = static_cast<uint8_t*>(a.out);
-    *reinterpret_cast<v4i*>(out + tile * kInt4TileBytes + lane * 16) = packed;
-    if (q == 0)
-    {
-        uint16_t* s = reinterpret_cast<uint16_t*>(out + int4_scale_at(a.tiles, tile, PER)) + r * PER;
+        else
+        {
+            const uint16_t* row = static_cast<const uint16_t*>(a.in) + (live ? n : 0) * a.ld;
+            v4i w[4];
 #pragma unroll
-        for (int g = 0; g < PER; g++)
-            s[g] = scale[g];
+            for (int j = 0; j < 4; j++)
+                w[j] = load8(row, k0 + 32 * j + 8 * q, a.k, live);
+            v2us m[4];    // of |w|, by halves: bit patterns order like the numbers, and NaN above all
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+            {
+                m[j] = v2us{ 0, 0 };
+#pragma unroll
+                for (int p = 0; p < 4; p++)
+                    m[j] = __builtin_elementwise_max(m[j], __builtin_bit_cast(v2us, w[j][p] & 0x7FFF7FFF));
+            }
+#pragma unroll
+            for (int g = 0; g < PER; g++)
+            {
+                v2us top = { 0, 0 };
+#pragma unroll
+                for (int j = g * 4 / PER; j < (g + 1) * 4 / PER; j++)
+                    top = __builtin_elementwise_max(top, m[j]);
+                scale[g] = to_bits16<T>(from_bits16<T>((uint16_t)row_max(top.x > top.y ? top.x : top.y)) / 7.0f);
+                // rint(w / scale) without 32 divisions.  A quotient of two 16-bit floats between -11 and 11 is a half or 2^-13 from one at least, and w times
+                // the reciprocal is off by 2^-19 at most: rounded to a multiple of 2^-14 (768 + t has no finer ones) halves are halves again, and no other
+                // quotient crosses one.  (bf16 scales may be so small that their reciprocal is none: both sides times 2^64.)
+                const float s    = from_bits16<T>(scale[g]);
+                const float wide = __is_same(T, bf16_t) && s < 0x1p-60f ? 0x1p64f : 1.0f;
+                const float r    = s == 0.0f ? 0.0f : 1.0f / (s * wide);
+#pragma unroll
+                for (int j = g * 4 / PER; j < (g + 1) * 4 / PER; j++)
+                {
+                    uint32_t word = 0x88888888u;
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                    {
+                        float t = from_bits16<T>(half_of(w[j], e));
+                        if constexpr (__is_same(T, bf16_t))
+                            t *= wide;
+                        t = rintf((t * r + 768.0f) - 768.0f);
+                        // (the conversion makes 0 of NaN: of inf * 0, and of what is multiplied by NaN)
+                        const int v = clamp_med3(to_int(t), -7, 7);
+                        word += (uint32_t)v << (4 * (e >> 1) + 16 * (e & 1));
+                    }
+                    packed[j] = (int)word;
+                }
+            }
+        }
+        uint8_t* out = static_cast<uint8_t*>(a.out);
+        *reinterpret_cast<v4i*>(out + tile * kInt4TileBytes + lane * 16) = packed;
+        if (q == 0)
+        {
+            uint16_t* s = reinterpret_cast<uint16_t*>(out + int4_scale_at(a.tiles, tile, PER)) + r * PER;
+#pragma unroll
+            for (int g = 0; g < PER; g++)
+                s[g] = scale[g];
+        }
     }
 }
 
@@ -174,6 +189,14 @@ bool per_group(int group, F&& f)
     }
 }
 
+// Eight workgroups a CU, each wave with several tiles where there are more: 16384 x 4096 37.5 us, 48.9 a tile a wave.  (The way back, whose stores nothing
+// waits for, is the other way round: 57 and 42.)
+int grid_of(int64_t tiles)
+{
+    const int64_t n = int4_tiles(tiles, kWaves);
+    return (int)(n < 2048 ? n : 2048);
+}
+
 Int4Args int4_args(int32_t n, int32_t k, int group, const void* in, int64_t ld, void* out)
 {
     Int4Args a{};
@@ -191,7 +214,7 @@ const char* launch_int4_pack(hipStream_t st, int32_t dtype, int32_t group, int32
 {
     Int4Args a    = int4_args(n, k, group, w, ld, packed);
     a.scales      = static_cast<const uint16_t*>(scales);
-    const int grid = (int)int4_tiles(a.tiles, kWaves);
+    const int grid = grid_of(a.tiles);
     const bool ok  = per_group(group, [&](auto per) {
         constexpr int PER = decltype(per)::value;
         if (scales)

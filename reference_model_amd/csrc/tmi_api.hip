@@ -2187,7 +2187,7 @@ static int int4_rows(tmi_ctx* ctx, const char* op, const tmi_int4_desc_t* d, boo
         const int wrc = ensure_workspace(ctx, (size_t)rows * 16);
         if (wrc != TMI_VALID)
             return wrc;
-        launch_widen_rows(ctx->stream, x, ld_x, k, rows, ctx->workspace);
+        launch_widen_rows(ctx->stream, WidenRows{ 1, k, { x }, { ld_x }, { rows }, { ctx->workspace } });
         x = ctx->workspace, ld_x = k = 8;
     }
     return after_launch(ctx, launch_int4_rows(ctx->stream, d->dtype, d->group, gated, activation, rows, d->out_features, k, x, ld_x, w, up, out, ld_out));
@@ -2266,9 +2266,8 @@ int tmi_gated_ffn(tmi_ctx_t* ctx, const tmi_gated_ffn_desc_t* desc, const void* 
         if (wrc != TMI_VALID)
             return wrc;
         uint8_t* to = static_cast<uint8_t*>(ctx->workspace);
-        launch_widen_rows(ctx->stream, x_dev, d.ld_x, d.in_features, d.rows, to);
-        launch_widen_rows(ctx->stream, gate_dev, d.ld_w, d.in_features, d.hidden_features, to + x_bytes);
-        launch_widen_rows(ctx->stream, up_dev, d.ld_w, d.in_features, d.hidden_features, to + x_bytes + w_bytes);
+        launch_widen_rows(ctx->stream, WidenRows{ 3, d.in_features, { x_dev, gate_dev, up_dev }, { d.ld_x, d.ld_w, d.ld_w },
+                                                  { d.rows, d.hidden_features, d.hidden_features }, { to, to + x_bytes, to + x_bytes + w_bytes } });
         return after_launch(ctx, launch_ffn_rows(ctx->stream, d.dtype, d.activation, d.rows, 8, d.hidden_features, to, 8, to + x_bytes,
                                                  to + x_bytes + w_bytes, 8, h_dev, pre_gate_dev, pre_up_dev, d.ld_h));
     }

@@ -323,8 +323,15 @@ const char* launch_ffn_rows(hipStream_t st, int32_t dtype, int32_t act, int32_t 
                             const void* gate, const void* up, int64_t ldw, void* out, void* pre_gate, void* pre_up, int64_t ldo);
 // gated_ffn.hip: the gated block on many rows and its gradients (row strides of the descriptors filled in).  `scratch`: of as many bytes as the
 // functions before say (forward: nullptr does too, with the sum in one piece); zeros: 64 bytes of them
-// rows of `width` < 8 elements of 16 bits, filled up with zeros to 8
-void launch_widen_rows(hipStream_t st, const void* in, int64_t ld, int32_t width, int64_t rows, void* out);
+// n matrices of rows of `width` elements of 16 bits, copied to rows filled up with zeros to whole pieces of 8
+struct WidenRows
+{
+    int32_t n, width;
+    const void* in[3];
+    int64_t ld[3], rows[3];
+    void* out[3];
+};
+void launch_widen_rows(hipStream_t st, const WidenRows& a);
 size_t gated_ffn_scratch_bytes(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up);
 const char* launch_gated_ffn(hipStream_t st, const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up, void* h, void* pre_gate,
                              void* pre_up, void* scratch, const void* zeros);
