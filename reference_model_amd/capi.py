@@ -209,7 +209,8 @@ def load_library() -> ctypes.CDLL:
     except ModuleNotFoundError:
         _calls = None
     if _calls:
-        _calls.install(Context, DeviceTensor, TmiError, ctypes.ArgumentError, ConvDesc, TconvDesc, Conv3dDesc, PoolDesc, RescaleDesc)
+        _calls.install(Context, DeviceTensor, TmiError, ctypes.ArgumentError, ConvDesc, TconvDesc, Conv3dDesc, PoolDesc, RescaleDesc,
+                       GatedFfnDesc, Int4Desc)
     _lib = lib
     return lib
 
@@ -349,8 +350,8 @@ class Context:
         return r
 
     # -- operators (device pointers in, status out) ------------------------------------------
-    # load_library() puts native methods (csrc/host/pycalls.cc) in the place of those named in PLAIN_OPERATORS, with the same
-    # arguments, results and errors.
+    # load_library() puts native methods (csrc/host/pycalls.cc) in the place of those named in PLAIN_OPERATORS and PLAIN_FEED_FORWARD, with the
+    # same arguments, results and errors.
     def conv2d(self, d: ConvDesc, inp, w, bias, in_zp, w_zp, out) -> int:
         return self._check(self.lib.tmi_conv2d(self.handle, ctypes.byref(d), _ptr(inp), _ptr(w), _ptr(bias), in_zp, w_zp, _ptr(out)))
 
@@ -491,6 +492,9 @@ class Context:
 PLAIN_OPERATORS = {name: vars(Context)[name] for name in (
     "conv2d", "depthwise_conv2d", "transpose_conv2d", "conv3d", "conv2d_rescale_clamp", "depthwise_conv2d_rescale_clamp", "matmul",
     "rescale", "clamp", "avg_pool2d", "max_pool2d")}
+
+PLAIN_FEED_FORWARD = {name: vars(Context)[name] for name in (
+    "gated_ffn", "gated_ffn_backward", "quantize_int4", "dequantize_int4", "matvec_int4", "gated_ffn_int4")}
 
 
 def _stored(zp: int, dtype: int) -> int:

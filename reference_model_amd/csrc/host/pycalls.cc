@@ -203,7 +203,8 @@ constexpr int arity(int (*)(A...))
     return sizeof...(A);
 }
 
-template <auto Fn>
+// OPTIONAL: how many of the last arguments may be left out, for None
+template <auto Fn, int OPTIONAL = 0>
 struct Operator
 {
     static constexpr int n = arity(Fn);
@@ -212,15 +213,17 @@ struct Operator
     static PyObject* run(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames)
     {
         PyObject* at[n];
-        if (!collect(name, names, n, 0, args, nargs, kwnames, at))
+        if (!collect(name, names, n, OPTIONAL, args, nargs, kwnames, at))
             return nullptr;
+        for (int i = n - OPTIONAL; i < n; i++)
+            at[i] = at[i] ? at[i] : Py_None;
         return call<Fn>(Fn, at, std::make_index_sequence<n>{});
     }
 };
-template <auto Fn>
-const char* Operator<Fn>::name = nullptr;
-template <auto Fn>
-const char* const* Operator<Fn>::names = nullptr;
+template <auto Fn, int OPTIONAL>
+const char* Operator<Fn, OPTIONAL>::name = nullptr;
+template <auto Fn, int OPTIONAL>
+const char* const* Operator<Fn, OPTIONAL>::names = nullptr;
 
 // CONV2D / DEPTHWISE_CONV2D + RESCALE (+ CLAMP): `clamp` is None or a pair (lowest, highest)
 template <auto Fn>
@@ -275,13 +278,14 @@ PyObject* run_depthwise_fused(PyObject*, PyObject* const* args, Py_ssize_t nargs
     return run_fused<tmi_depthwise_conv2d_rescale_clamp>("depthwise_conv2d_rescale_clamp", args, nargs, kwnames);
 }
 
-template <auto Fn, size_t N>
+template <auto Fn, int OPTIONAL = 0, size_t N>
 PyMethodDef op(const char* name, const char* const (&names)[N], const char* doc)
 {
-    static_assert(N == Operator<Fn>::n, "one name for each argument of the entry point");
-    Operator<Fn>::name  = name;
-    Operator<Fn>::names = names;
-    return PyMethodDef{ name, (PyCFunction)(void (*)())Operator<Fn>::run, METH_FASTCALL | METH_KEYWORDS, doc };
+    using O = Operator<Fn, OPTIONAL>;
+    static_assert(N == O::n, "one name for each argument of the entry point");
+    O::name  = name;
+    O::names = names;
+    return PyMethodDef{ name, (PyCFunction)(void (*)())O::run, METH_FASTCALL | METH_KEYWORDS, doc };
 }
 
 const char* const kConv[]    = { "self", "d", "inp", "w", "bias", "in_zp", "w_zp", "out" };
@@ -290,6 +294,12 @@ const char* const kRescale[] = { "self", "r", "rank", "rows", "c", "inp", "mult"
 const char* const kClamp[]   = { "self", "dtype", "n", "inp", "lo", "hi", "out" };
 const char* const kAvg[]     = { "self", "d", "inp", "in_zp", "out_zp", "out" };
 const char* const kMax[]     = { "self", "d", "inp", "out" };
+const char* const kFfn[]     = { "self", "d", "x", "gate", "up", "h", "pre_gate", "pre_up" };
+const char* const kFfnBack[] = { "self", "d", "x", "gate", "up", "pre_gate", "pre_up", "d_h", "d_x", "d_gate", "d_up" };
+const char* const kQuant[]   = { "self", "d", "w", "ld_w", "packed" };
+const char* const kDequant[] = { "self", "d", "packed", "w", "ld_w" };
+const char* const kMatvec[]  = { "self", "d", "rows", "x", "ld_x", "packed", "y", "ld_y" };
+const char* const kFfnInt4[] = { "self", "d", "activation", "rows", "x", "ld_x", "gate", "up", "h", "ld_h" };
 
 PyMethodDef g_methods[] = {
     op<tmi_conv2d>("conv2d", kConv, "conv2d($self, d, inp, w, bias, in_zp, w_zp, out)\n--\n\nCONV2D; d: ConvDesc"),
@@ -301,6 +311,16 @@ PyMethodDef g_methods[] = {
     op<tmi_clamp>("clamp", kClamp, "clamp($self, dtype, n, inp, lo, hi, out)\n--\n\nCLAMP of integers"),
     op<tmi_avg_pool2d>("avg_pool2d", kAvg, "avg_pool2d($self, d, inp, in_zp, out_zp, out)\n--\n\nAVG_POOL2D; d: PoolDesc"),
     op<tmi_max_pool2d>("max_pool2d", kMax, "max_pool2d($self, d, inp, out)\n--\n\nMAX_POOL2D; d: PoolDesc"),
+    op<tmi_gated_ffn, 2>("gated_ffn", kFfn, "gated_ffn($self, d, x, gate, up, h, pre_gate=None, pre_up=None)\n--\n\n"
+                                            "h = act(x gate^T) * (x up^T); d: GatedFfnDesc; pre_gate and pre_up receive the two products for gated_ffn_backward"),
+    op<tmi_gated_ffn_backward>("gated_ffn_backward", kFfnBack,
+                               "gated_ffn_backward($self, d, x, gate, up, pre_gate, pre_up, d_h, d_x, d_gate, d_up)\n--\n\n"
+                               "the gradients of x, gate and up (None: not computed) from that of h; d: GatedFfnDesc"),
+    op<tmi_quantize_int4>("quantize_int4", kQuant, "quantize_int4($self, d, w, ld_w, packed)\n--\n\n16-bit weights into 4 bits; d: Int4Desc"),
+    op<tmi_dequantize_int4>("dequantize_int4", kDequant, "dequantize_int4($self, d, packed, w, ld_w)\n--\n\nthe weights that a packed form stands for; d: Int4Desc"),
+    op<tmi_matvec_int4>("matvec_int4", kMatvec, "matvec_int4($self, d, rows, x, ld_x, packed, y, ld_y)\n--\n\ny = x w^T for a few rows of x; d: Int4Desc"),
+    op<tmi_gated_ffn_int4>("gated_ffn_int4", kFfnInt4,
+                           "gated_ffn_int4($self, d, activation, rows, x, ld_x, gate, up, h, ld_h)\n--\n\nthe gated block on 4-bit weights; d: Int4Desc"),
     { "conv2d_rescale_clamp", (PyCFunction)(void (*)())run_conv_fused, METH_FASTCALL | METH_KEYWORDS,
       "conv2d_rescale_clamp($self, d, inp, w, bias, in_zp, w_zp, r, mult, shift, out, clamp=None)\n--\n\nCONV2D + RESCALE (+ CLAMP)" },
     { "depthwise_conv2d_rescale_clamp", (PyCFunction)(void (*)())run_depthwise_fused, METH_FASTCALL | METH_KEYWORDS,
@@ -308,18 +328,19 @@ PyMethodDef g_methods[] = {
       "DEPTHWISE_CONV2D + RESCALE (+ CLAMP)" },
 };
 
-// install(Context, DeviceTensor, TmiError, ctypes.ArgumentError, ConvDesc, TconvDesc, Conv3dDesc, PoolDesc, RescaleDesc):
+// install(Context, DeviceTensor, TmiError, ctypes.ArgumentError, ConvDesc, TconvDesc, Conv3dDesc, PoolDesc, RescaleDesc, GatedFfnDesc, Int4Desc):
 // the operators become methods of Context
 PyObject* install(PyObject*, PyObject* args)
 {
     PyObject *context, **kept[] = { &g_tensor, &g_error, &g_argument_error, &g_desc<tmi_conv_desc_t>, &g_desc<tmi_tconv_desc_t>,
-                                    &g_desc<tmi_conv3d_desc_t>, &g_desc<tmi_pool_desc_t>, &g_desc<tmi_rescale_desc_t> };
-    PyObject* got[8];
-    if (!PyArg_ParseTuple(args, "OOOOOOOOO", &context, &got[0], &got[1], &got[2], &got[3], &got[4], &got[5], &got[6], &got[7]))
+                                    &g_desc<tmi_conv3d_desc_t>, &g_desc<tmi_pool_desc_t>, &g_desc<tmi_rescale_desc_t>,
+                                    &g_desc<tmi_gated_ffn_desc_t>, &g_desc<tmi_int4_desc_t> };
+    PyObject* got[10];
+    if (!PyArg_ParseTuple(args, "OOOOOOOOOOO", &context, &got[0], &got[1], &got[2], &got[3], &got[4], &got[5], &got[6], &got[7], &got[8], &got[9]))
         return nullptr;
     const Py_ssize_t sizes[] = { sizeof(tmi_conv_desc_t), sizeof(tmi_tconv_desc_t), sizeof(tmi_conv3d_desc_t), sizeof(tmi_pool_desc_t),
-                                 sizeof(tmi_rescale_desc_t) };
-    for (int i = 0; i < 8; i++)
+                                 sizeof(tmi_rescale_desc_t), sizeof(tmi_gated_ffn_desc_t), sizeof(tmi_int4_desc_t) };
+    for (int i = 0; i < 10; i++)
     {
         if (!PyType_Check(got[i]))
             return PyErr_Format(PyExc_TypeError, "install: argument %d is no type", i + 2), nullptr;
