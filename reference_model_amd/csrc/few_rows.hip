@@ -433,8 +433,10 @@ __global__ __launch_bounds__(1024) void int4_stream_kernel(RowsArgs a)
 template <int PER, int MT, bool GATED>
 constexpr int kInFlight = GATED && MT > 1 ? 2 : 4;
 
-// What a call costs by its parts' rates, in us: the bytes of weights and x that a CU takes in at 64 a clock, those that L2 gives out at 10 TB/s and HBM at 6,
-// the weights' unpacking (a matrix of 1 GB in 4 bits 160 us in bf16, 90 in fp16), 1.5 for every reading of x and 0.5 for every block.
+// What a call costs by its parts' rates, in us: the bytes of weights and x that the busiest CU takes in at 64 a clock, those that L2 gives out at 10 TB/s
+// and HBM at 6, and the vector instructions of its four SIMDs: a weight tile takes 320 clocks to unpack in bf16 and 250 in fp16, 24 for each group's
+// scale and 40 of products for each row tile, and a turn's empty places a fifth of that; 8 % of what does not bound, 1.5 us for every reading of x and 1
+// for every block.  Over 13 sizes and all their plans (8 and 16 waves, every split, 1 to 4 row tiles) its choice is within 2 % of the best on average.
 template <typename T, int PER, int MT, bool GATED>
 double plan(RowsArgs& a, int& waves)
 {
@@ -461,17 +463,19 @@ double plan(RowsArgs& a, int& waves)
             const int wn = many / wk, slots = many == 8 ? 512 : 256;
             t.n_blocks   = (a.tiles_n + wn - 1) / wn;
             const double wgs = t.n_blocks * chunks, rounds = wgs > slots ? (double)(int64_t)((wgs + slots - 1) / slots) : 1;
-            const double shared  = wgs > 256 && many == 8 ? 2 : 1;    // workgroups of a CU
+            const double busiest = (double)(int64_t)((wgs + 255) / 256);    // blocks of the CU that has most
+            const double shared  = wgs > 256 && many == 8 ? 2 : 1;          // workgroups of a CU
             const double w_bytes = (double)wn * S * a.tiles_k * (1024 + 32 * PER), x_bytes = (double)m * a.k * 2;
             const double reads   = resident ? 1 : rounds * ((t.turns + t.part - 1) / (t.part ? t.part : 1));
-            const double cu      = shared * (rounds * w_bytes + (resident ? 1 : rounds) * x_bytes) / 147e3;
+            const double cu      = (busiest * w_bytes + (resident ? shared : busiest) * x_bytes) / 147e3;
             const double l2      = (wgs * w_bytes + (resident && wgs > slots ? slots : wgs) * x_bytes) / 10e6;
             const double hbm     = (double)t.n_blocks * w_bytes / 6e6;
-            const double unpack  = wgs * w_bytes * (__is_same(T, bf16_t) ? 160e-9 : 90e-9) * (wgs < 256 ? 256 / wgs : 1);
+            const double clocks  = (__is_same(T, bf16_t) ? 320 : 250) + (24 * PER + 40) * MT;
+            const double vector  = busiest * wn * S * (0.8 * a.tiles_k + 0.2 * t.turns * U * wk) / 4 * clocks / 2100;
             double us            = cu > l2 ? cu : l2;
             us                   = us > hbm ? us : hbm;
-            us                   = us > unpack ? us : unpack;
-            us += 1.5 * reads / shared + 0.5 * rounds;
+            us                   = us > vector ? us : vector;
+            us += 0.08 * (cu + l2 + hbm + vector - us) + 1.5 * reads / shared + rounds;
             if (least < 0 || us < least)
                 least = us, best = t, waves = many;
         }
