@@ -219,11 +219,17 @@ __device__ __forceinline__ v4i int4_unpack(uint32_t w)
     v4i r;
     if constexpr (__is_same(T, bf16_t))
     {
-        const uint32_t s = w ^ 0x88888888u;    // v + 8 -> v, two's complement
+        uint32_t s[2] = { w ^ 0x88888888u };    // v + 8 -> v, two's complement
+        // (one operation each: the conversion itself picks the byte)
+        asm("" : "+v"(s[0]));
+        s[1] = s[0] >> 4;
+        asm("" : "+v"(s[1]));
 #pragma unroll
         for (int p = 0; p < 4; p++)
         {
-            const float lo = __builtin_amdgcn_cvt_off_f32_i4((int)(s >> (4 * p))), hi = __builtin_amdgcn_cvt_off_f32_i4((int)(s >> (16 + 4 * p)));
+            const int byte = 8 * (p >> 1);
+            const float lo = __builtin_amdgcn_cvt_off_f32_i4((int)__builtin_amdgcn_ubfe(s[p & 1], byte, 8));
+            const float hi = __builtin_amdgcn_cvt_off_f32_i4((int)__builtin_amdgcn_ubfe(s[p & 1], byte + 16, 8));
             r[p] = (int)__builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
         }
     }
@@ -231,11 +237,14 @@ __device__ __forceinline__ v4i int4_unpack(uint32_t w)
     {
         const v2h off0 = { (_Float16)-1032.0f, (_Float16)-1032.0f }, off1 = { (_Float16)-72.0f, (_Float16)-72.0f };
         const v2h sixteenth = { (_Float16)0.0625f, (_Float16)0.0625f };
+        // (held in registers, so that a mask and the exponent are one operation: an instruction takes one constant)
+        uint32_t low = 0x000F000Fu, high = 0x00F000F0u, exponent = 0x64006400u;
+        asm("" : "+s"(low), "+s"(high), "+v"(exponent));
 #pragma unroll
         for (int p = 0; p < 4; p += 2)
         {
             const uint32_t s = w >> (4 * p);
-            const v2h lo = __builtin_bit_cast(v2h, (s & 0x000F000Fu) | 0x64006400u), hi = __builtin_bit_cast(v2h, (s & 0x00F000F0u) | 0x64006400u);
+            const v2h lo = __builtin_bit_cast(v2h, (s & low) | exponent), hi = __builtin_bit_cast(v2h, (s & high) | exponent);
             r[p]     = __builtin_bit_cast(int, lo + off0);
             r[p + 1] = __builtin_bit_cast(int, __builtin_elementwise_fma(hi, sixteenth, off1));
         }
