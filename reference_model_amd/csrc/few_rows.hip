@@ -83,9 +83,31 @@ __device__ __forceinline__ void store_rows(const RowsArgs& a, const float* red, 
 
 constexpr int kShortWaves = 8;
 
-// PER: groups of a 4-bit tile, 0 = 16-bit weights; MT: tiles of 16 rows of x; U: column tiles whose loads a wave has in flight together
-template <typename T, int PER, int MT, bool GATED, int U>
-__global__ __launch_bounds__(64 * kShortWaves) void few_rows_kernel(RowsArgs a)
+// A row that begins at an odd element is read in words: 16 bytes from the word on that it begins in, and the one word behind them where that one
+// holds more of the row; joined() then moves the halves.  Loads of 16 bytes that begin inside a word take the caches more than twice as long.
+struct Halves
+{
+    const uint8_t* base;
+    uint32_t shift;    // 0 or 16
+    __device__ __forceinline__ const uint16_t* row() const { return reinterpret_cast<const uint16_t*>(base + (shift >> 3)); }
+    // of the 16 bytes at `at`: the fifth word, or the fourth again
+    __device__ __forceinline__ int next(int64_t at) const { return *reinterpret_cast<const int*>(base + at + 12 + (shift >> 2)); }
+};
+__device__ __forceinline__ Halves halves_of(const uint8_t* row)
+{
+    const uint32_t odd = (uint32_t)reinterpret_cast<uintptr_t>(row) & 2;
+    return { row - odd, 8 * odd };
+}
+__device__ __forceinline__ v4i joined(v4i v, int next, uint32_t shift)
+{
+    return v4i{ (int)__builtin_amdgcn_alignbit(v[1], v[0], shift), (int)__builtin_amdgcn_alignbit(v[2], v[1], shift),
+                (int)__builtin_amdgcn_alignbit(v[3], v[2], shift), (int)__builtin_amdgcn_alignbit(next, v[3], shift) };
+}
+
+// PER: groups of a 4-bit tile, 0 = 16-bit weights; MT: tiles of 16 rows of x; U: column tiles whose loads a wave has in flight together;
+// ODD: rows of x or of 16-bit weights begin at odd elements
+template <typename T, int PER, int MT, bool GATED, int U, bool ODD>
+__global__ __launch_bounds__(64 * kShortWaves, PER ? 1 : 4) void few_rows_kernel(RowsArgs a)
 {
     constexpr bool DENSE = PER == 0;
     constexpr int S      = GATED ? 2 : 1;    // streams of weights: gate and up
@@ -137,7 +159,15 @@ __global__ __launch_bounds__(64 * kShortWaves) void few_rows_kernel(RowsArgs a)
         v4i x[MT][4];
         v4i w[S][WV];
         scales_t<PER> scale[S];
+        int x_next[MT][ODD ? 4 : 1], w_next[S][ODD && DENSE ? WV : 1];
     };
+    Halves xhalf[MT], whalf[S];
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++)
+        xhalf[mt] = halves_of(reinterpret_cast<const uint8_t*>(xrow[mt]));
+#pragma unroll
+    for (int s = 0; s < S; s++)
+        whalf[s] = halves_of(wbase[s]);
     // Rows of 16-bit weights may lie a power of two apart: workgroups that begin at different columns meet on different channels of the
     // memory.  us of one row with 2 x 32768 x 8192: 230 all from the first column, 178 so.  (In 4 bits a tile of rows lies in one piece.)
     const int turn = DENSE && full ? (int)((blockIdx.x * 5u) % (uint32_t)full) : 0;
@@ -149,12 +179,20 @@ __global__ __launch_bounds__(64 * kShortWaves) void few_rows_kernel(RowsArgs a)
         {
             if constexpr (DENSE)
             {
-                const uint16_t* row = reinterpret_cast<const uint16_t*>(wbase[s]);
+                const uint16_t* row = ODD ? whalf[s].row() : reinterpret_cast<const uint16_t*>(wbase[s]);
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                 {
                     const int64_t k = (int64_t)kt * 128 + 32 * j + 8 * q;
-                    t.w[s][j]       = decltype(TAIL)::value ? settle8(load8_raw(row, k, a.k), k, a.k, true) : load16(reinterpret_cast<const uint8_t*>(row + k));
+                    if constexpr (decltype(TAIL)::value)
+                        t.w[s][j] = settle8(load8_raw(row, k, a.k), k, a.k, true);
+                    else if constexpr (ODD)
+                    {
+                        t.w[s][j]      = load16(whalf[s].base + 2 * k);
+                        t.w_next[s][j] = whalf[s].next(2 * k);
+                    }
+                    else
+                        t.w[s][j] = load16(reinterpret_cast<const uint8_t*>(row + k));
                 }
             }
             else
@@ -173,9 +211,32 @@ __global__ __launch_bounds__(64 * kShortWaves) void few_rows_kernel(RowsArgs a)
                 const int64_t k = (int64_t)kt * 128 + 32 * j + 8 * q;
                 t.x[mt][j]      = v4i{ 0, 0, 0, 0 };
                 if constexpr (decltype(TAIL)::value)
-                    t.x[mt][j] = settle8(load8_raw(xrow[mt], k, a.k), k, a.k, live[mt]);
+                    t.x[mt][j] = settle8(load8_raw(ODD ? xhalf[mt].row() : xrow[mt], k, a.k), k, a.k, live[mt]);
+                else if constexpr (ODD)
+                {
+                    t.x_next[mt][j] = 0;
+                    if (live[mt])
+                    {
+                        t.x[mt][j]      = load16(xhalf[mt].base + 2 * k);
+                        t.x_next[mt][j] = xhalf[mt].next(2 * k);
+                    }
+                }
                 else if (live[mt])
                     t.x[mt][j] = load16(reinterpret_cast<const uint8_t*>(xrow[mt] + k));
+            }
+    };
+    auto join = [&](Tile& t) {
+        if constexpr (ODD)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+            {
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+                    t.x[mt][j] = joined(t.x[mt][j], t.x_next[mt][j], xhalf[mt].shift);
+                if constexpr (DENSE)
+#pragma unroll
+                    for (int s = 0; s < S; s++)
+                        t.w[s][j] = joined(t.w[s][j], t.w_next[s][j], whalf[s].shift);
             }
     };
     auto multiply = [&](const Tile& t) {
@@ -230,7 +291,10 @@ __global__ __launch_bounds__(64 * kShortWaves) void few_rows_kernel(RowsArgs a)
 #pragma unroll
         for (int u = 0; u < U; u++)
             if (k0 + u * waves < full)
+            {
+                join(t[u]);
                 multiply(t[u]);
+            }
     }
     if (full < a.tiles_k && full % waves == wave)
     {
@@ -506,13 +570,13 @@ bool launch_stream(hipStream_t st, const RowsArgs& a, int waves)
     return true;
 }
 
-template <typename T, int PER, int MT, bool GATED>
+template <typename T, int PER, int MT, bool GATED, bool ODD>
 bool launch_short(hipStream_t st, const RowsArgs& a)
 {
-    constexpr int U = PER ? 4 : MT == 1 ? 2 : 1, S = GATED ? 2 : 1;
+    constexpr int U = PER ? 4 : MT == 1 && !ODD ? 2 : 1, S = GATED ? 2 : 1;
     const int waves  = a.tiles_k < 1 ? 1 : a.tiles_k < kShortWaves ? a.tiles_k : kShortWaves;
     const size_t lds = (size_t)waves * S * MT * 1024;
-    if (!ensure_dynamic_lds<few_rows_kernel<T, PER, MT, GATED, U>>(lds))
+    if (!ensure_dynamic_lds<few_rows_kernel<T, PER, MT, GATED, U, ODD>>(lds))
         return false;
     // a grid has 2^16 chunks of rows, and 2^32 threads
     const int64_t chunks = ((int64_t)a.rows + 16 * MT - 1) / (16 * MT), most = (int64_t(1) << 22) / a.tiles_n < 1 << 14 ? (int64_t(1) << 22) / a.tiles_n : 1 << 14;
@@ -525,9 +589,20 @@ bool launch_short(hipStream_t st, const RowsArgs& a)
         part.x += m * a.ldx, part.out += m * a.ldo;
         if (a.pre_gate)
             part.pre_gate += m * a.ldo, part.pre_up += m * a.ldo;
-        few_rows_kernel<T, PER, MT, GATED, U><<<dim3(a.tiles_n, (int)(chunks - c < step ? chunks - c : step)), 64 * waves, lds, st>>>(part);
+        few_rows_kernel<T, PER, MT, GATED, U, ODD><<<dim3(a.tiles_n, (int)(chunks - c < step ? chunks - c : step)), 64 * waves, lds, st>>>(part);
     }
     return true;
+}
+
+// Rows that begin at odd elements, us with one load for 16 bytes / in words: 1, 16 and 32 rows with 2 x 8192 x 2047 in bf16 28.2, 38.9, 51.4 / 15.1, 18.8, 24.4,
+// 16 rows with 2 x 2000 x 2048 in 4 bits 7.4 / 5.6.
+template <typename T, int PER, int MT, bool GATED>
+bool launch_short(hipStream_t st, const RowsArgs& a)
+{
+    bool odd = ((a.ldx & 1) && a.rows > 1) || (reinterpret_cast<uintptr_t>(a.x) & 2);
+    if (PER == 0)
+        odd |= (a.ldw & 1) || ((reinterpret_cast<uintptr_t>(a.w[0]) | reinterpret_cast<uintptr_t>(a.w[1])) & 2);
+    return odd ? launch_short<T, PER, MT, GATED, true>(st, a) : launch_short<T, PER, MT, GATED, false>(st, a);
 }
 
 // The short kernel up to four rows and 32 MB of weights, and up to 16 rows and 8 MB (x goes to it once for every 16 weight rows).  us short /
