@@ -83,27 +83,6 @@ __device__ __forceinline__ void store_rows(const RowsArgs& a, const float* red, 
 
 constexpr int kShortWaves = 8;
 
-// A row that begins at an odd element is read in words: 16 bytes from the word on that it begins in, and the one word behind them where that one
-// holds more of the row; joined() then moves the halves.  Loads of 16 bytes that begin inside a word take the caches more than twice as long.
-struct Halves
-{
-    const uint8_t* base;
-    uint32_t shift;    // 0 or 16
-    __device__ __forceinline__ const uint16_t* row() const { return reinterpret_cast<const uint16_t*>(base + (shift >> 3)); }
-    // of the 16 bytes at `at`: the fifth word, or the fourth again
-    __device__ __forceinline__ int next(int64_t at) const { return *reinterpret_cast<const int*>(base + at + 12 + (shift >> 2)); }
-};
-__device__ __forceinline__ Halves halves_of(const uint8_t* row)
-{
-    const uint32_t odd = (uint32_t)reinterpret_cast<uintptr_t>(row) & 2;
-    return { row - odd, 8 * odd };
-}
-__device__ __forceinline__ v4i joined(v4i v, int next, uint32_t shift)
-{
-    return v4i{ (int)__builtin_amdgcn_alignbit(v[1], v[0], shift), (int)__builtin_amdgcn_alignbit(v[2], v[1], shift),
-                (int)__builtin_amdgcn_alignbit(v[3], v[2], shift), (int)__builtin_amdgcn_alignbit(next, v[3], shift) };
-}
-
 // PER: groups of a 4-bit tile, 0 = 16-bit weights; MT: tiles of 16 rows of x; U: column tiles whose loads a wave has in flight together;
 // ODD: rows of x or of 16-bit weights begin at odd elements
 template <typename T, int PER, int MT, bool GATED, int U, bool ODD>
