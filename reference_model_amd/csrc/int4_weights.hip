@@ -4,7 +4,10 @@
 //
 // A wave owns one tile of 16 rows x 128 columns, lane 16 q + r the columns 32 j + 8 q + (0 ... 7) of row r, j = 0 ... 3: the 32 weights whose
 // 16 bytes it stores, so a tile goes out as one kilobyte in a row, and the maximum over a group of 32 is a maximum over the four lanes of a row.
-// Bound by the 16-bit side: 2 bytes a weight against half of one.
+// The tiles of a workgroup lie side by side, and their 16-bit side passes through LDS (piece p of row r at p ^ r), so that it is read and written
+// in whole kilobytes of a row: where rows begin inside a cache line those meet one line more than they fill, where tile by tile every 64 bytes of
+// a row do.  Bound by the 16-bit side: 2 bytes a weight against half of one.  16384 x 4096 takes 36.3 us into 4 bits (4.6 TB/s) and 31.6 back
+// (5.3); tile by tile they were 37.5 and 42, and with rows of 4095 57.9 and 74 against 38.4 and 46.8 now.
 #include "tmi_ffn.h"
 
 namespace tmi
@@ -19,7 +22,8 @@ struct Int4Args
     void* out;
     int64_t ld;                // elements between rows on the unpacked side
     int64_t tiles, groups;
-    int32_t n, k, tiles_k;
+    int64_t blocks;            // of 16 rows x 512 columns
+    int32_t n, k, tiles_k, across;
 };
 
 constexpr int kWaves = 4;
@@ -47,14 +51,39 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v)
 template <typename T, int PER, bool GIVEN, bool ODD>
 __global__ __launch_bounds__(64 * kWaves) void int4_pack_kernel(Int4Args a)
 {
-    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-    for (int64_t tile = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); tile < a.tiles; tile += (int64_t)gridDim.x * kWaves)
+    __shared__ v4i lds[GIVEN ? 1 : kInt4Rows * kWaves * 16];
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int64_t b = blockIdx.x; b < a.blocks; b += gridDim.x)
     {
-        const int64_t tn = tile / a.tiles_k;
-        const int kt     = (int)(tile - tn * a.tiles_k);
-        const int64_t n  = tn * kInt4Rows + r;
-        const bool live  = n < a.n;
-        const int k0     = kt * kInt4Cols;
+        const int64_t tn   = b / a.across;
+        const int kt0      = (int)(b - tn * a.across) * kWaves, kt = kt0 + wave;
+        const int64_t tile = tn * a.tiles_k + kt;
+        const int64_t n    = tn * kInt4Rows + r;
+        const bool live    = n < a.n;
+        const int k0       = kt * kInt4Cols;
+        if constexpr (!GIVEN)
+        {
+            v4i in[kInt4Rows / kWaves];
+#pragma unroll
+            for (int i = 0; i < kInt4Rows / kWaves; i++)
+            {
+                const int64_t m     = tn * kInt4Rows + wave * (kInt4Rows / kWaves) + i;
+                const uint16_t* row = static_cast<const uint16_t*>(a.in) + (m < a.n ? m : 0) * a.ld;
+                const int k         = kt0 * kInt4Cols + 8 * lane;
+                in[i]               = ODD ? load8_words(row, k, a.k, m < a.n) : load8(row, k, a.k, m < a.n);
+            }
+            if (b != blockIdx.x)
+                __syncthreads();    // the last block is read
+#pragma unroll
+            for (int i = 0; i < kInt4Rows / kWaves; i++)
+            {
+                const int row                           = wave * (kInt4Rows / kWaves) + i;
+                lds[row * (kWaves * 16) + (lane ^ row)] = in[i];
+            }
+            __syncthreads();
+        }
+        if (kt >= a.tiles_k)
+            continue;
         v4i packed;
         uint16_t scale[PER];
         if constexpr (GIVEN)
@@ -83,11 +112,10 @@ __global__ __launch_bounds__(64 * kWaves) void int4_pack_kernel(Int4Args a)
         }
         else
         {
-            const uint16_t* row = static_cast<const uint16_t*>(a.in) + (live ? n : 0) * a.ld;
             v4i w[4];
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                w[j] = ODD ? load8_words(row, k0 + 32 * j + 8 * q, a.k, live) : load8(row, k0 + 32 * j + 8 * q, a.k, live);
+                w[j] = lds[r * (kWaves * 16) + ((wave * 16 + 4 * j + q) ^ r)];
             v2us m[4];    // of |w|, by halves: bit patterns order like the numbers, and NaN above all
 #pragma unroll
             for (int j = 0; j < 4; j++)
@@ -145,31 +173,43 @@ __global__ __launch_bounds__(64 * kWaves) void int4_pack_kernel(Int4Args a)
 template <typename T, int PER>
 __global__ __launch_bounds__(64 * kWaves) void int4_unpack_kernel(Int4Args a)
 {
-    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-    const int64_t tile = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (tile >= a.tiles)
-        return;
-    const int64_t tn = tile / a.tiles_k;
-    const int kt     = (int)(tile - tn * a.tiles_k);
-    const int64_t n  = tn * kInt4Rows + r;
-    if (n >= a.n)
-        return;
-    const uint8_t* in  = static_cast<const uint8_t*>(a.in);
-    const v4i packed   = *reinterpret_cast<const v4i*>(in + tile * kInt4TileBytes + lane * 16);
-    const uint16_t* sc = reinterpret_cast<const uint16_t*>(in + int4_scale_at(a.tiles, tile, PER)) + r * PER;
-    uint16_t* row      = static_cast<uint16_t*>(a.out) + n * a.ld;
-#pragma unroll
-    for (int j = 0; j < 4; j++)
+    __shared__ v4i lds[kInt4Rows * kWaves * 16];
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int64_t b = blockIdx.x; b < a.blocks; b += gridDim.x)
     {
-        const float s = from_bits16<T>(sc[j * PER / 4]);
-        v4i w;
-#pragma unroll
-        for (int p = 0; p < 4; p++)
+        const int64_t tn = b / a.across;
+        const int kt0    = (int)(b - tn * a.across) * kWaves;
+        if (kt0 + wave < a.tiles_k)
         {
-            const uint32_t u = (uint32_t)packed[j] >> (4 * p);
-            w[p] = (int)pack16<T>((float)((int)(u & 15) - 8) * s, (float)((int)(u >> 16 & 15) - 8) * s);
+            const int64_t tile = tn * a.tiles_k + kt0 + wave;
+            const uint8_t* in  = static_cast<const uint8_t*>(a.in);
+            const v4i packed   = *reinterpret_cast<const v4i*>(in + tile * kInt4TileBytes + lane * 16);
+            const uint16_t* sc = reinterpret_cast<const uint16_t*>(in + int4_scale_at(a.tiles, tile, PER)) + r * PER;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+            {
+                const float s = from_bits16<T>(sc[j * PER / 4]);
+                v4i w;
+#pragma unroll
+                for (int p = 0; p < 4; p++)
+                {
+                    const uint32_t u = (uint32_t)packed[j] >> (4 * p);
+                    w[p] = (int)pack16<T>((float)((int)(u & 15) - 8) * s, (float)((int)(u >> 16 & 15) - 8) * s);
+                }
+                lds[r * (kWaves * 16) + ((wave * 16 + 4 * j + q) ^ r)] = w;
+            }
         }
-        store8(row, (int64_t)kt * kInt4Cols + 32 * j + 8 * q, a.k, w);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kInt4Rows / kWaves; i++)
+        {
+            const int row   = wave * (kInt4Rows / kWaves) + i;
+            const int64_t n = tn * kInt4Rows + row;
+            if (n < a.n)
+                store8(static_cast<uint16_t*>(a.out) + n * a.ld, (int64_t)kt0 * kInt4Cols + lane * 8, a.k, lds[row * (kWaves * 16) + (lane ^ row)]);
+        }
+        if (b + gridDim.x < a.blocks)
+            __syncthreads();    // the block is read
     }
 }
 
@@ -189,12 +229,11 @@ bool per_group(int group, F&& f)
     }
 }
 
-// Eight workgroups a CU, each wave with several tiles where there are more: 16384 x 4096 37.5 us, 48.9 a tile a wave.  (The way back, whose stores nothing
-// waits for, is the other way round: 57 and 42.)
-int grid_of(int64_t tiles)
+// Eight workgroups a CU, which go on to further blocks: 16384 x 4096 36.3 us, 43.0 with a workgroup for each.  (The way back, whose stores nothing waits
+// for, takes one for each.)
+int grid_of(int64_t blocks)
 {
-    const int64_t n = int4_tiles(tiles, kWaves);
-    return (int)(n < 2048 ? n : 2048);
+    return (int)(blocks < 2048 ? blocks : 2048);
 }
 
 Int4Args int4_args(int32_t n, int32_t k, int group, const void* in, int64_t ld, void* out)
@@ -204,6 +243,8 @@ Int4Args int4_args(int32_t n, int32_t k, int group, const void* in, int64_t ld, 
     a.tiles_k = (int32_t)int4_tiles(k, kInt4Cols);
     a.tiles   = int4_tiles(n, kInt4Rows) * a.tiles_k;
     a.groups  = int4_tiles(k, group);
+    a.across  = (int32_t)int4_tiles(a.tiles_k, kWaves);
+    a.blocks  = int4_tiles(n, kInt4Rows) * a.across;
     return a;
 }
 
@@ -214,8 +255,7 @@ const char* launch_int4_pack(hipStream_t st, int32_t dtype, int32_t group, int32
 {
     Int4Args a    = int4_args(n, k, group, w, ld, packed);
     a.scales      = static_cast<const uint16_t*>(scales);
-    const int grid = grid_of(a.tiles);
-    // 16384 x 4095 57.9 us with loads of 16 bytes from odd elements, 50.4 in words, 4096 x 8191 29.9 and 21.1
+    const int grid = grid_of(a.blocks);
     const bool odd = !scales && ((ld & 1) || (reinterpret_cast<uintptr_t>(w) & 2));
     const bool ok  = per_group(group, [&](auto per) {
         constexpr int PER = decltype(per)::value;
@@ -234,7 +274,7 @@ const char* launch_int4_pack(hipStream_t st, int32_t dtype, int32_t group, int32
 const char* launch_int4_unpack(hipStream_t st, int32_t dtype, int32_t group, int32_t n, int32_t k, const void* packed, void* w, int64_t ld)
 {
     const Int4Args a = int4_args(n, k, group, packed, ld, w);
-    const int grid   = (int)int4_tiles(a.tiles, kWaves);
+    const int grid   = (int)(a.blocks < 1 << 23 ? a.blocks : 1 << 23);    // (2^32 threads at most)
     const bool ok    = per_group(group, [&](auto per) {
         constexpr int PER = decltype(per)::value;
         if (dtype == TMI_BF16)
