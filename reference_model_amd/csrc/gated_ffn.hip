@@ -76,7 +76,7 @@ constexpr int kRing = DIRECT ? 5 : 4;
 
 // WC x WR waves (columns x rows) of 64 columns and 16 RT rows each
 template <typename T, int OP, int WC, int WR, int RT, bool DIRECT>
-__global__ __launch_bounds__(64 * WC * WR, 2) void gated_gemm_kernel(GemmFfnArgs a)
+__device__ __forceinline__ void gated_gemm(const GemmFfnArgs& a, int workgroup)
 {
     constexpr int THREADS = 64 * WC * WR;
     constexpr int BN = 64 * WC, BM = 16 * RT * WR;
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(64 * WC * WR, 2) void gated_gemm_kernel(GemmFfnArgs
     const int l16 = lane & 15, q4 = lane >> 4;
 
     // workgroups go round-robin to the 8 XCDs; each takes a contiguous range of the tile list, along rows in groups of kGroup
-    const int t = (blockIdx.x & 7) * a.per_xcd + (blockIdx.x >> 3);
+    const int t = (workgroup & 7) * a.per_xcd + (workgroup >> 3);
     if (t >= a.tiles * a.splits)
         return;
     const int split = t / a.tiles, tile = t - split * a.tiles;
@@ -540,6 +540,23 @@ __global__ __launch_bounds__(64 * WC * WR, 2) void gated_gemm_kernel(GemmFfnArgs
         });
 }
 
+template <typename T, int OP, int WC, int WR, int RT, bool DIRECT>
+__global__ __launch_bounds__(64 * WC * WR, 2) void gated_gemm_kernel(GemmFfnArgs a)
+{
+    gated_gemm<T, OP, WC, WR, RT, DIRECT>(a, blockIdx.x);
+}
+
+// d_x and the weights' gradients side by side in tiles of 128 x 128, where neither fills the chip: the first dx.per_xcd * 8 workgroups are d_x's
+template <typename T, bool DIRECT>
+__global__ __launch_bounds__(256, 2) void gated_gradients_kernel(GemmFfnArgs dx, GemmFfnArgs dw)
+{
+    const int of_dx = dx.per_xcd * 8;
+    if ((int)blockIdx.x < of_dx)
+        gated_gemm<T, OP_DX, 2, 2, 4, DIRECT>(dx, blockIdx.x);
+    else
+        gated_gemm<T, OP_DW, 2, 2, 4, DIRECT>(dw, blockIdx.x - of_dx);
+}
+
 // Results of a sum that was split, four of a row a thread: the parts in the order of the splits, then what the unsplit kernel does with a sum.
 template <typename T, int OP>
 __global__ __launch_bounds__(256) void gated_join_kernel(GemmFfnArgs a)
@@ -678,6 +695,28 @@ struct Shape
     int splits, per_split;
     int tiles_m, tiles_n;
 };
+constexpr struct
+{
+    int bm, bn, slots;
+    double empty, full, tile;    // us: of a block of 32 on an empty and on a full chip, and of a tile beside them
+} kTiles[3] = { { 256, 256, 256, 0.62, 0.80, 12 }, { 256, 128, 256, 0.39, 0.48, 7 }, { 128, 128, 512, 0.33, 0.58, 6 } };
+constexpr double kThroughRegisters = 1.4;
+constexpr int kMostSplits = 16, kLeastBlocks = 16;    // parts of a sum, and blocks of a part
+
+void split(Shape& s, int blocks, int parts)
+{
+    s.per_split = (blocks + parts - 1) / parts;
+    s.splits    = s.per_split ? (blocks + s.per_split - 1) / s.per_split : 1;
+}
+// what splitting costs: the partial sums out and in, and a launch
+double join_us(int op, int64_t M, int64_t N, int splits)
+{
+    return splits > 1 ? 3 + (double)M * N * (op == OP_FORWARD ? 2 : 1) * 4 * 2 * splits / 4.5e6 : 0;
+}
+bool may_split(int64_t M, int blocks, int parts)
+{
+    return parts == 1 || (blocks >= kLeastBlocks * parts && M < 65536);    // (a grid's second side)
+}
 
 // The tile, and into how many parts the sum is split, by the time that follows from what was measured (us, over 4096 x 2048 x 8192 and halves to
 // eighths of each size): a block of 32 costs a workgroup of the three tiles 0.62, 0.39 and 0.33 on an empty chip and 0.80, 0.48 and 0.58 on
@@ -688,11 +727,7 @@ struct Shape
 // and 32 in the best number of parts; 4096 x 2048 x 8192 243, 301 and 328.
 Shape shape_of(int op, int64_t M, int64_t N, int blocks, bool fast, double& least)
 {
-    static const struct
-    {
-        int bm, bn, slots;
-        double empty, full, tile;
-    } of[3] = { { 256, 256, 256, 0.62, 0.80, 12 }, { 256, 128, 256, 0.39, 0.48, 7 }, { 128, 128, 512, 0.33, 0.58, 6 } };
+    const auto& of = kTiles;
     Shape best{};
     least = 0;
     for (int tile = fast ? TILE_256 : TILE_128; tile <= TILE_128; tile++)
@@ -700,24 +735,22 @@ Shape shape_of(int op, int64_t M, int64_t N, int blocks, bool fast, double& leas
         const int tn = op == OP_FORWARD ? of[tile].bn / 2 : of[tile].bn;
         Shape s{};
         s.tile = tile, s.tiles_m = (int)((M + of[tile].bm - 1) / of[tile].bm), s.tiles_n = (int)((N + tn - 1) / tn);
-        for (int want = 1; want <= 16 && (want == 1 || blocks >= 16 * want); want++)
+        for (int want = 1; want <= kMostSplits && may_split(M, blocks, want); want++)
         {
-            s.per_split      = (blocks + want - 1) / want;
-            s.splits         = s.per_split ? (blocks + s.per_split - 1) / s.per_split : 1;
+            split(s, blocks, want);
             const int64_t n  = (int64_t)s.tiles_m * s.tiles_n * s.splits;
             const int64_t rounds = (n + of[tile].slots - 1) / of[tile].slots;
             // (of the smallest tile 256 have a CU each; of more some share one, and the last of those counts)
             const double busy = tile == TILE_128 ? n > 256 : n >= 256 ? 1 : n / 256.0;
             double us         = rounds * (s.per_split * (of[tile].empty + (of[tile].full - of[tile].empty) * busy) + of[tile].tile);
-            if (s.splits > 1)
-                us += 3 + (double)M * N * (op == OP_FORWARD ? 2 : 1) * 4 * 2 * s.splits / 4.5e6;
+            us += join_us(op, M, N, s.splits);
             if (!best.tiles_m || us < least)
                 least = us, best = s;
         }
         if (!best.tiles_m)    // no rows
             best = s;
     }
-    least *= fast ? 1 : 1.4;
+    least *= fast ? 1 : kThroughRegisters;
     return best;
 }
 
@@ -736,12 +769,44 @@ bool launch_tiles(hipStream_t st, const GemmFfnArgs& a)
     return true;
 }
 
-template <int OP>
-bool launch_product(hipStream_t st, int32_t dtype, GemmFfnArgs a, const Shape& s, bool fast)
+void set_shape(GemmFfnArgs& a, const Shape& s)
 {
     a.tiles_m = s.tiles_m, a.tiles_n = s.tiles_n, a.tiles = s.tiles_m * s.tiles_n;
     a.splits = s.splits, a.per_split = s.per_split;
     a.per_xcd = (a.tiles * a.splits + 7) / 8;
+}
+
+template <int OP>
+void launch_join(hipStream_t st, int32_t dtype, const GemmFfnArgs& a)
+{
+    const dim3 grid((a.N + 1023) / 1024, a.M);
+    if (a.splits > 1 && dtype == TMI_BF16)
+        gated_join_kernel<bf16_t, OP><<<grid, 256, 0, st>>>(a);
+    else if (a.splits > 1)
+        gated_join_kernel<_Float16, OP><<<grid, 256, 0, st>>>(a);
+}
+
+bool launch_gradients(hipStream_t st, int32_t dtype, const GemmFfnArgs& dx, const GemmFfnArgs& dw, bool fast)
+{
+    auto typed = [&](auto type, auto FAST) {
+        using T = decltype(type);
+        constexpr bool DIRECT = decltype(FAST)::value;
+        constexpr size_t lds  = kRing<DIRECT> * 256 * 64;
+        if (!ensure_dynamic_lds<gated_gradients_kernel<T, DIRECT>>(lds))
+            return false;
+        gated_gradients_kernel<T, DIRECT><<<(dx.per_xcd + dw.per_xcd) * 8, 256, lds, st>>>(dx, dw);
+        return true;
+    };
+    const bool ok = dtype == TMI_BF16 ? (fast ? typed(bf16_t{}, std::true_type()) : typed(bf16_t{}, std::false_type()))
+                                      : (fast ? typed(_Float16{}, std::true_type()) : typed(_Float16{}, std::false_type()));
+    if (ok)
+        launch_join<OP_DX>(st, dtype, dx), launch_join<OP_DW>(st, dtype, dw);
+    return ok;
+}
+
+template <int OP>
+bool launch_product(hipStream_t st, int32_t dtype, const GemmFfnArgs& a, const Shape& s, bool fast)
+{
     auto typed = [&](auto type) {
         using T = decltype(type);
         bool ok;
@@ -751,11 +816,12 @@ bool launch_product(hipStream_t st, int32_t dtype, GemmFfnArgs a, const Shape& s
             ok = launch_tiles<T, OP, 2, 4, 4, true>(st, a);
         else
             ok = fast ? launch_tiles<T, OP, 2, 2, 4, true>(st, a) : launch_tiles<T, OP, 2, 2, 4, false>(st, a);
-        if (ok && s.splits > 1)
-            gated_join_kernel<T, OP><<<dim3((a.N + 1023) / 1024, a.M), 256, 0, st>>>(a);
         return ok;
     };
-    return dtype == TMI_BF16 ? typed(bf16_t{}) : typed(_Float16{});
+    const bool ok = dtype == TMI_BF16 ? typed(bf16_t{}) : typed(_Float16{});
+    if (ok)
+        launch_join<OP>(st, dtype, a);
+    return ok;
 }
 
 // whether rows of `width` elements, `ld` apart, are whole 16-byte pieces, and near enough for 32-bit offsets over a tile
@@ -778,21 +844,52 @@ struct Way
     size_t bytes;     // of the copies
     Shape shape;
 };
-Way way_of(int op, int64_t M, int64_t N, int blocks, bool whole, int64_t copied_rows, int64_t d)
+Way way_of(int op, int64_t M, int64_t N, int blocks, bool whole, int64_t copied_rows, int64_t d, double& us)
 {
     Way w{};
     double direct = 0, registers = 0;
     w.shape = shape_of(op, M, N, blocks, true, direct);
     w.fast  = true;
+    us      = direct;
     if (whole)
         return w;
     const Shape other  = shape_of(op, M, N, blocks, false, registers);
     const size_t bytes = (size_t)copied_rows * whole_of(d, 8) * 2;
     if (d < 8 || direct + 2 * (double)bytes / 3.5e6 + 8 < registers)
-        w.copies = true, w.bytes = bytes;
+        w.copies = true, w.bytes = bytes, us += 2 * (double)bytes / 3.5e6 + 8;
     else
-        w.fast = false, w.shape = other;
+        w.fast = false, w.shape = other, us = registers;
     return w;
+}
+
+// Both gradients in one launch, if that takes less than `apart`, one after the other, and 4 us for the other launch: in tiles of 128 x 128, of which
+// 512 have a place, with parts of the sums as long as those that are there together allow.
+bool side_by_side(Way& dx, int64_t dx_rows, int dx_blocks, Way& dw, int64_t dw_rows, int dw_blocks, int64_t N, double apart)
+{
+    const auto& tile    = kTiles[TILE_128];
+    const double slower = dx.fast ? 1 : kThroughRegisters;
+    double least        = apart + 4;
+    bool better         = false;
+    Shape x{}, w{};
+    x.tile = w.tile = TILE_128;
+    x.tiles_m = (int)((dx_rows + tile.bm - 1) / tile.bm), w.tiles_m = (int)((dw_rows + tile.bm - 1) / tile.bm);
+    x.tiles_n = w.tiles_n = (int)((N + tile.bn - 1) / tile.bn);
+    if ((int64_t)(x.tiles_m + (int64_t)w.tiles_m) * x.tiles_n > 2 * tile.slots || !x.tiles_n || !x.tiles_m || !w.tiles_m)
+        return false;
+    for (int px = 1; px <= kMostSplits && may_split(dx_rows, dx_blocks, px); px++)
+        for (int pw = 1; pw <= kMostSplits && may_split(dw_rows, dw_blocks, pw); pw++)
+        {
+            split(x, dx_blocks, px), split(w, dw_blocks, pw);
+            const double nx = (double)x.tiles_m * x.tiles_n * x.splits, nw = (double)w.tiles_m * w.tiles_n * w.splits;
+            const double block = (nx + nw > 256 ? tile.full : tile.empty) * slower;
+            const double one_x = x.per_split * block + tile.tile, one_w = w.per_split * block + tile.tile;
+            // the longest of them, and what all of them take from the places
+            const double longest = one_x > one_w ? one_x : one_w, all = (nx * one_x + nw * one_w) / tile.slots;
+            const double us = (nx + nw <= tile.slots ? longest : all + longest / 2) + join_us(OP_DX, dx_rows, N, x.splits) + join_us(OP_DW, dw_rows, N, w.splits);
+            if (us < least)
+                least = us, better = true, dx.shape = x, dw.shape = w;
+        }
+    return better;
 }
 
 // What a call launches, from its sizes, strides and addresses
@@ -806,7 +903,8 @@ ForwardPlan forward_plan(const tmi_gated_ffn_desc_t& d, const void* x, const voi
     ForwardPlan p;
     const bool whole = whole_pieces(x, d.in_features, d.ld_x) && whole_pieces(gate, d.in_features, d.ld_w) && whole_pieces(up, d.in_features, d.ld_w);
     p.blocks         = (int)(whole_of(d.in_features, kBlock) / kBlock);
-    p.way            = way_of(OP_FORWARD, d.rows, d.hidden_features, p.blocks, whole, (int64_t)d.rows + 2 * (int64_t)d.hidden_features, d.in_features);
+    double us;
+    p.way            = way_of(OP_FORWARD, d.rows, d.hidden_features, p.blocks, whole, (int64_t)d.rows + 2 * (int64_t)d.hidden_features, d.in_features, us);
     return p;
 }
 struct BackwardPlan
@@ -815,8 +913,9 @@ struct BackwardPlan
     size_t dp_bytes;
     int dx_blocks, dw_blocks;
     Way dx, dw;
+    bool together;    // in one launch
 };
-BackwardPlan backward_plan(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up)
+BackwardPlan backward_plan(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up, bool want_dx, bool want_dw)
 {
     BackwardPlan p;
     p.half           = whole_of(d.hidden_features, 64);
@@ -827,8 +926,12 @@ BackwardPlan backward_plan(const tmi_gated_ffn_desc_t& d, const void* x, const v
     p.dx_blocks      = (int)(2 * p.half / kBlock);
     p.dw_blocks      = (int)(whole_of(d.rows, kBlock) / kBlock);
     const int64_t D  = d.in_features, F = d.hidden_features;
-    p.dx             = way_of(OP_DX, d.rows, D, p.dx_blocks, whole_pieces(gate, D, d.ld_w) && whole_pieces(up, D, d.ld_w), 2 * F, D);
-    p.dw             = way_of(OP_DW, 2 * p.half, D, p.dw_blocks, whole_pieces(x, D, d.ld_x), d.rows, D);
+    double us_dx, us_dw;
+    p.dx             = way_of(OP_DX, d.rows, D, p.dx_blocks, whole_pieces(gate, D, d.ld_w) && whole_pieces(up, D, d.ld_w), 2 * F, D, us_dx);
+    p.dw             = way_of(OP_DW, 2 * p.half, D, p.dw_blocks, whole_pieces(x, D, d.ld_x), d.rows, D, us_dw);
+    p.together       = false;
+    if (want_dx && want_dw && !p.dx.copies && !p.dw.copies && p.dx.fast == p.dw.fast)
+        p.together = side_by_side(p.dx, d.rows, p.dx_blocks, p.dw, 2 * p.half, p.dw_blocks, D, us_dx + us_dw);
     return p;
 }
 
@@ -878,23 +981,24 @@ const char* launch_gated_ffn(hipStream_t st, const tmi_gated_ffn_desc_t& d, cons
         launch_widen_rows(st, WidenRows{ 3, d.in_features, { x, gate, up }, { d.ld_x, d.ld_w, d.ld_w }, { d.rows, d.hidden_features, d.hidden_features }, { cx, cg, cu } });
         a.row = cx, a.col[0] = cg, a.col[1] = cu, a.ldr = a.ldc = wide, a.K = (int32_t)wide;
     }
+    set_shape(a, p.way.shape);
     return launch_product<OP_FORWARD>(st, d.dtype, a, p.way.shape, p.way.fast) ? "gated_ffn" : nullptr;
 }
 
-// dp, then copies, then the partial sums of one product after the other
+// dp, then copies, then the partial sums: of one product after the other, or of both
 size_t gated_ffn_backward_scratch_bytes(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up, bool dx, bool dw)
 {
-    const BackwardPlan p = backward_plan(d, x, gate, up);
+    const BackwardPlan p = backward_plan(d, x, gate, up, dx, dw);
     const size_t of_dx   = dx ? part_bytes(OP_DX, p.dx.shape, d.rows, d.in_features) : 0;
     const size_t of_dw   = dw ? part_bytes(OP_DW, p.dw.shape, 2 * p.half, d.in_features) : 0;
-    return p.dp_bytes + p.dx.bytes + p.dw.bytes + (of_dx > of_dw ? of_dx : of_dw);
+    return p.dp_bytes + p.dx.bytes + p.dw.bytes + (p.together ? of_dx + of_dw : of_dx > of_dw ? of_dx : of_dw);
 }
 
 const char* launch_gated_ffn_backward(hipStream_t st, const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up,
                                       const void* pre_gate, const void* pre_up, const void* d_h, void* d_x, void* d_gate, void* d_up, void* scratch,
                                       const void* zeros)
 {
-    const BackwardPlan p = backward_plan(d, x, gate, up);
+    const BackwardPlan p = backward_plan(d, x, gate, up, d_x, d_gate);
     SlopeArgs q{};
     q.pre_gate = static_cast<const uint16_t*>(pre_gate), q.pre_up = static_cast<const uint16_t*>(pre_up), q.dh = static_cast<const uint16_t*>(d_h);
     q.dp = static_cast<uint16_t*>(scratch), q.ld = d.ld_h, q.ldp = p.ldp, q.units = d.rows * (p.half / 8);
@@ -913,32 +1017,45 @@ const char* launch_gated_ffn_backward(hipStream_t st, const tmi_gated_ffn_desc_t
     a.part  = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(copies) + p.dx.bytes + p.dw.bytes);
     a.zeros = static_cast<const uint8_t*>(zeros);
     a.N     = d.in_features;
-    bool ok = true;
+    GemmFfnArgs of_x = a, of_w = a;
     if (d_x)
     {
-        a.col[0] = static_cast<const uint16_t*>(gate), a.col[1] = static_cast<const uint16_t*>(up), a.ldc = d.ld_w, a.width = d.in_features;
+        of_x.col[0] = static_cast<const uint16_t*>(gate), of_x.col[1] = static_cast<const uint16_t*>(up), of_x.ldc = d.ld_w, of_x.width = d.in_features;
         if (p.dx.copies)
         {
             launch_widen_rows(st, WidenRows{ 2, d.in_features, { gate, up }, { d.ld_w, d.ld_w }, { d.hidden_features, d.hidden_features },
                                              { copies, copies + d.hidden_features * wide } });
-            a.col[0] = copies, a.col[1] = copies + d.hidden_features * wide, a.ldc = wide, a.width = (int32_t)wide;
+            of_x.col[0] = copies, of_x.col[1] = copies + d.hidden_features * wide, of_x.ldc = wide, of_x.width = (int32_t)wide;
         }
-        a.out[0] = static_cast<uint16_t*>(d_x), a.out[1] = nullptr, a.ldo = d.ld_x;
-        a.M = d.rows, a.K = d.hidden_features, a.blocks = p.dx_blocks;
-        ok = launch_product<OP_DX>(st, d.dtype, a, p.dx.shape, p.dx.fast);
+        of_x.out[0] = static_cast<uint16_t*>(d_x), of_x.ldo = d.ld_x;
+        of_x.M = d.rows, of_x.K = d.hidden_features, of_x.blocks = p.dx_blocks;
+        set_shape(of_x, p.dx.shape);
     }
-    if (ok && d_gate)
+    if (d_gate)
     {
-        a.col[0] = a.col[1] = static_cast<const uint16_t*>(x), a.ldc = d.ld_x, a.width = d.in_features;
+        of_w.col[0] = of_w.col[1] = static_cast<const uint16_t*>(x), of_w.ldc = d.ld_x, of_w.width = d.in_features;
         if (p.dw.copies)
         {
             uint16_t* cx = copies + p.dx.bytes / 2;
             launch_widen_rows(st, WidenRows{ 1, d.in_features, { x }, { d.ld_x }, { d.rows }, { cx } });
-            a.col[0] = a.col[1] = cx, a.ldc = wide, a.width = (int32_t)wide;
+            of_w.col[0] = of_w.col[1] = cx, of_w.ldc = wide, of_w.width = (int32_t)wide;
         }
-        a.out[0] = static_cast<uint16_t*>(d_gate), a.out[1] = static_cast<uint16_t*>(d_up), a.ldo = d.ld_w;
-        a.M = (int32_t)(2 * p.half), a.K = d.rows, a.blocks = p.dw_blocks;
-        ok = launch_product<OP_DW>(st, d.dtype, a, p.dw.shape, p.dw.fast);
+        of_w.out[0] = static_cast<uint16_t*>(d_gate), of_w.out[1] = static_cast<uint16_t*>(d_up), of_w.ldo = d.ld_w;
+        of_w.M = (int32_t)(2 * p.half), of_w.K = d.rows, of_w.blocks = p.dw_blocks;
+        set_shape(of_w, p.dw.shape);
+    }
+    bool ok = true;
+    if (p.together)
+    {
+        of_w.part += part_bytes(OP_DX, p.dx.shape, d.rows, d.in_features) / 4;
+        ok = launch_gradients(st, d.dtype, of_x, of_w, p.dx.fast);
+    }
+    else
+    {
+        if (d_x)
+            ok = launch_product<OP_DX>(st, d.dtype, of_x, p.dx.shape, p.dx.fast);
+        if (ok && d_gate)
+            ok = launch_product<OP_DW>(st, d.dtype, of_w, p.dw.shape, p.dw.fast);
     }
     return ok ? "gated_ffn_backward" : nullptr;
 }
