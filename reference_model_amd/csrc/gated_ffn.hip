@@ -74,6 +74,14 @@ constexpr int kBlock = 32;   // of the summed index
 template <bool DIRECT>
 constexpr int kRing = DIRECT ? 5 : 4;
 
+// a pointer that is the same in every lane, where the compiler does not see it
+__device__ __forceinline__ const uint16_t* uniform(const uint16_t* p)
+{
+    const uint64_t v  = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return reinterpret_cast<const uint16_t*>((uint64_t)hi << 32 | lo);
+}
+
 // WC x WR waves (columns x rows) of 64 columns and 16 RT rows each
 template <typename T, int OP, int WC, int WR, int RT, bool DIRECT>
 __device__ __forceinline__ void gated_gemm(const GemmFfnArgs& a, int workgroup)
@@ -86,7 +94,7 @@ __device__ __forceinline__ void gated_gemm(const GemmFfnArgs& a, int workgroup)
     constexpr int CB = BN * 64, STAGE = (BN + BM) * 64, RING = kRing<DIRECT>;
     constexpr int CL = BN * 4 / THREADS, RL = BM * 4 / THREADS, LOADS = CL + RL;    // 16-byte loads of a thread and block
     constexpr int TN = CIN ? BN / 2 : BN;                                            // results a tile's columns make
-    static_assert(CL * THREADS == BN * 4 && RL * THREADS == BM * 4 && RT >= 4, "a block must split evenly over the threads");
+    static_assert(CL * THREADS == BN * 4 && RL * THREADS == BM * 4 && (RT == 2 || RT >= CT), "a block must split evenly over the threads");
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
 
     const int tid = threadIdx.x, lane = tid & 63;
@@ -193,7 +201,7 @@ __device__ __forceinline__ void gated_gemm(const GemmFfnArgs& a, int workgroup)
                 return;
             }
         }
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(base), "s"(dst) : "memory");
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(uniform(base)), "s"(dst) : "memory");
     };
     // Past the last block it is requested again, into stages nobody reads: the loads in flight are then as many in every block.
     auto advance = [&]() {
@@ -341,8 +349,8 @@ __device__ __forceinline__ void gated_gemm(const GemmFfnArgs& a, int workgroup)
                     for (int q = 0; q < NL; q++)
                         if (1 + q * (RT - 1) / (NL ? NL : 1) == i)
                             load(q);
-                if (k == 2 && i < CT && i > 0)
-                    read_col(1 - P, next, i);
+                if (i > 0 && (RT >= CT ? k == 2 && i < CT : k >= 1))
+                    read_col(1 - P, next, RT >= CT ? i : k);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (i == 0)
@@ -815,7 +823,8 @@ bool launch_product(hipStream_t st, int32_t dtype, const GemmFfnArgs& a, const S
         else if (s.tile == TILE_256_128)
             ok = launch_tiles<T, OP, 2, 4, 4, true>(st, a);
         else
-            ok = fast ? launch_tiles<T, OP, 2, 2, 4, true>(st, a) : launch_tiles<T, OP, 2, 2, 4, false>(st, a);
+            ok = a.tiles * a.splits > 256 ? (fast ? launch_tiles<T, OP, 2, 2, 4, true>(st, a) : launch_tiles<T, OP, 2, 2, 4, false>(st, a))
+                                          : (fast ? launch_tiles<T, OP, 2, 4, 2, true>(st, a) : launch_tiles<T, OP, 2, 4, 2, false>(st, a));
         return ok;
     };
     const bool ok = dtype == TMI_BF16 ? typed(bf16_t{}) : typed(_Float16{});
