@@ -399,7 +399,14 @@ int tmi_dot_product_check(tmi_ctx_t* ctx, int32_t out_dtype, int64_t n, const vo
  * (dtype) TMI_FP16 or TMI_BF16 for every tensor that is not packed; tensors are aligned to their elements at least (16
  * bytes for packed weights), rows may lie any number of elements apart.  Products are summed in 32 bits and results
  * rounded once, to nearest with ties to even.  Equal calls give equal bits.  A call with no rows, or no features
- * to write, does nothing. */
+ * to write, does nothing.
+ *
+ * Some calls use the context's scratch buffer (tmi_ctx_reserve_workspace; the rules for graphs and for several of them are
+ * those of every call that does): tmi_gated_ffn_backward always; tmi_gated_ffn on more than 32 rows, for partial sums where few
+ * tiles meet a long sum and for copies of large operands whose rows are no whole pieces of 16 bytes; tmi_gated_ffn,
+ * tmi_matvec_int4 and tmi_gated_ffn_int4 for copies of rows of fewer than eight elements.  While a graph is captured the buffer
+ * cannot grow: a call that needs more is then refused, but for tmi_gated_ffn on rows of eight elements or more, which goes on
+ * without it (its sums are then added in another order). */
 
 /* act(g) */
 enum
@@ -431,8 +438,8 @@ int tmi_gated_ffn(tmi_ctx_t* ctx, const tmi_gated_ffn_desc_t* d, const void* x_d
 /* Its gradients, from the pre-activations g and u and the gradient dh of h:
  *   du = dh act(g), dg = dh u act'(g), d_x = dg gate + du up, d_gate = dg^T x, d_up = du^T x
  * in 32 bits, with dg and du rounded to dtype before the products.  d_x_dev NULL, or d_gate_dev and d_up_dev both NULL:
- * that part is not computed (x_dev, or gate_dev and up_dev, may then be NULL).  dg and du live in the context's scratch buffer (see tmi_ctx_reserve_workspace), with
- * partial sums where the work is split over a long sum. */
+ * that part is not computed (x_dev, or gate_dev and up_dev, may then be NULL).  dg and du live in the scratch buffer, 4
+ * (rows) (hidden_features up to whole 64s) bytes and 128 more a row, with partial sums and copies as above. */
 int tmi_gated_ffn_backward(tmi_ctx_t* ctx, const tmi_gated_ffn_desc_t* d, const void* x_dev, const void* gate_dev,
                            const void* up_dev, const void* pre_gate_dev, const void* pre_up_dev, const void* d_h_dev,
                            void* d_x_dev, void* d_gate_dev, void* d_up_dev);
@@ -468,7 +475,8 @@ int tmi_pack_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, const int8_t* values
 int tmi_dequantize_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, const void* packed_dev, void* w_dev, int64_t ld_w);
 
 /* y = x w^T for a few rows of x (single tokens): y[m][n] = sum_k x[m][k] w[n][k], x [rows][in_features] rows ld_x apart, y
- * [rows][out_features] rows ld_y apart.  Any number of rows is taken; the weights are read once for every 64 of them. */
+ * [rows][out_features] rows ld_y apart.  Any number of rows is taken; the weights are read once for every 16, 32 or 64 of
+ * them. */
 int tmi_matvec_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, int32_t rows, const void* x_dev, int64_t ld_x, const void* packed_dev,
                     void* y_dev, int64_t ld_y);
 
