@@ -7,20 +7,20 @@
 //
 // 16x16x32 instructions take the rows of x as first operand and the weights as second: a single row wastes 15/16 of the matrix cores, which at 512
 // weights an instruction still run four times as many weights as HBM delivers, and any other number of rows up to 16 costs the same.  4-bit
-// weights become 16-bit integers (exact; 9 to 14 instructions for eight), their products are summed in 32 bits, and the sum over a group is
+// weights become 16-bit integers (exact; 8 or 13 instructions for eight), their products are summed in 32 bits, and the sum over a group is
 // multiplied by its scale: no weight is rounded, and an infinite or NaN x does to a row what it does in the formula.
 //
 // Two kernels share this.  In both, what the waves of a workgroup have summed meets in LDS in the order of the waves, so equal calls give equal bits.
 //
 // few_rows_kernel: a workgroup of up to eight waves has one tile of 16 weight rows (of both matrices, if gated), a wave every eighth tile of 128
 // columns of it; weights and x go straight to registers, the loads of U column tiles at once, with nothing to wait for in between.  Its
-// calls are short: 2.5 us for 512 x 512 in 4 bits, 4.0 for 4096 x 4096.
+// calls are short: 2.4 us for 512 x 512 in 4 bits, 3.8 for 4096 x 4096.
 //
 // int4_stream_kernel: for large matrices and more rows.  A workgroup goes through blocks of WN tiles of 16 weight rows; WK of its waves share
 // a tile, each with every WK-th tile of 128 columns.  A wave's weights go round in U sets of registers, the loads of the next U column tiles in
 // flight, from one block of rows into the next and past the barriers (the other kernel's waves load, wait and compute in turn: 2 x 32768 x 8192 in
-// bf16 69 us there, 56 here, one row).  x lies in LDS, all of its columns or a part of them at a time: read by each wave from L2 its rows are up to
-// eight times the weights' bytes (16 rows, 16384 x 4096: 18.6 us there, 12.6 here).  Where x takes less than half of the LDS two workgroups of eight
+// bf16 69 us there, 55 here, one row: 5.0 TB/s).  x lies in LDS, all of its columns or a part of them at a time: read by each wave from L2 its rows are up to
+// eight times the weights' bytes (16 rows, 16384 x 4096: 18.9 us there, 11.8 here).  Where x takes less than half of the LDS two workgroups of eight
 // waves share a CU, otherwise one of sixteen has it.
 #include "tmi_ffn.h"
 
@@ -585,8 +585,8 @@ bool launch_short(hipStream_t st, const RowsArgs& a)
 }
 
 // The short kernel up to four rows and 32 MB of weights, and up to 16 rows and 8 MB (x goes to it once for every 16 weight rows).  us short /
-// stream: one row 512 x 512 2.5 / 4.0, 4096 x 4096 4.0 / 5.0, 12000 x 4096 9.2 / 10.7, 16384 x 4096 11.1 / 10.8, 65536 x 8192 74 / 61; 13 rows 12000 x
-// 4096 13.0 / 12.0, 16 rows 16384 x 4096 18.6 / 12.6, 2 x 5500 x 2048 10.2 / 8.3.
+// stream: one row 512 x 512 2.4 / 4.0, 4096 x 4096 4.1 / 5.4, 12000 x 4096 8.5 / 9.2, 16384 x 4096 10.1 / 10.4, 65536 x 8192 68 / 60, 2 x 11000 x 4096
+// 16.0 / 14.7; 4 rows 8192 x 4096 7.1 / 8.4; 16 rows 4096 x 4096 6.7 / 8.6, 12000 x 4096 13.0 / 11.2, 2 x 5500 x 2048 9.4 / 8.1.
 template <typename T, int PER, bool GATED>
 bool choose(hipStream_t st, const RowsArgs& a)
 {

@@ -910,14 +910,14 @@ struct ForwardPlan
 {
     int blocks;
     Way way;
+    double us;
 };
 ForwardPlan forward_plan(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up)
 {
     ForwardPlan p;
     const bool whole = whole_pieces(x, d.in_features, d.ld_x) && whole_pieces(gate, d.in_features, d.ld_w) && whole_pieces(up, d.in_features, d.ld_w);
     p.blocks         = (int)(whole_of(d.in_features, kBlock) / kBlock);
-    double us;
-    p.way            = way_of(OP_FORWARD, d.rows, d.hidden_features, p.blocks, whole, (int64_t)d.rows + 2 * (int64_t)d.hidden_features, d.in_features, us);
+    p.way            = way_of(OP_FORWARD, d.rows, d.hidden_features, p.blocks, whole, (int64_t)d.rows + 2 * (int64_t)d.hidden_features, d.in_features, p.us);
     return p;
 }
 struct BackwardPlan
@@ -958,6 +958,21 @@ void launch_widen_rows(hipStream_t st, const WidenRows& a)
     const int64_t groups = (most * ((a.width + 7) / 8) + 255) / 256;
     if (groups > 0)
         gated_widen_kernel<<<dim3((int)(groups < 2048 ? groups : 2048), a.n), 256, 0, st>>>(a);
+}
+
+// The products of a few rows against the tiles here.  A workgroup of those takes 1024 columns of 16 weight rows and 32 rows of x in 3.6 us, 512 have a
+// place, and the weights come in at 4.3 TB/s for each 32 rows; 1.4 times that from odd elements.  us few rows / tiles: 32 rows 512 x 512 4.9 / 8.3, 1024 x
+// 4096 6.7 / 11.6, 4096 x 1024 16.6 / 13.9, 8000 x 500 30.9 / 16.4, 2048 x 8192 17.8 / 17.2; 48 rows 1024 x 2000 6.7 / 11.5; 40 rows 2048 x 8192 27.4 / 18.2.
+bool gated_ffn_few_rows_lead(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up)
+{
+    if (d.rows <= 16 || d.in_features < 8)
+        return true;
+    if (d.rows > 64)
+        return false;
+    const double chunks = (d.rows + 31) / 32, workgroups = chunks * ((d.hidden_features + 15) / 16), places = workgroups > 512 ? workgroups / 512 : 1;
+    const double chain  = ((d.in_features + 1023) / 1024) * 3.6 * places, bytes = chunks * 4.0 * d.in_features * d.hidden_features / 4.3e6;
+    const bool odd      = ((d.ld_x | d.ld_w) & 1) || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(gate) | reinterpret_cast<uintptr_t>(up)) & 2);
+    return 1.7 + (chain > bytes ? chain : bytes) * (odd ? 1.4 : 1) < forward_plan(d, x, gate, up).us;
 }
 
 size_t gated_ffn_scratch_bytes(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up)

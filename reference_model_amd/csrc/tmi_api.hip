@@ -2036,7 +2036,6 @@ int tmi_clamp_fp(tmi_ctx_t* ctx, int32_t dtype, int64_t n, const void* in_dev, f
 
 // ---- the gated feed-forward block and 4-bit weights ----------------------------------------------------------------------
 
-constexpr int32_t kFfnFewRows = 32;    // up to here the gated block in 16 bits runs as products of a few rows
 
 static bool ffn_dtype(int32_t dtype)
 {
@@ -2271,7 +2270,7 @@ int tmi_gated_ffn(tmi_ctx_t* ctx, const tmi_gated_ffn_desc_t* desc, const void* 
         return after_launch(ctx, launch_ffn_rows(ctx->stream, d.dtype, d.activation, d.rows, 8, d.hidden_features, to, 8, to + x_bytes,
                                                  to + x_bytes + w_bytes, 8, h_dev, pre_gate_dev, pre_up_dev, d.ld_h));
     }
-    if (d.rows <= kFfnFewRows)
+    if (gated_ffn_few_rows_lead(d, x_dev, gate_dev, up_dev))
         return after_launch(ctx, launch_ffn_rows(ctx->stream, d.dtype, d.activation, d.rows, d.in_features, d.hidden_features, x_dev, d.ld_x, gate_dev,
                                                  up_dev, d.ld_w, h_dev, pre_gate_dev, pre_up_dev, d.ld_h));
     const size_t bytes = gated_ffn_scratch_bytes(d, x_dev, gate_dev, up_dev);

@@ -332,6 +332,8 @@ struct WidenRows
     void* out[3];
 };
 void launch_widen_rows(hipStream_t st, const WidenRows& a);
+// whether launch_ffn_rows takes less time than launch_gated_ffn
+bool gated_ffn_few_rows_lead(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up);
 size_t gated_ffn_scratch_bytes(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up);
 const char* launch_gated_ffn(hipStream_t st, const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up, void* h, void* pre_gate,
                              void* pre_up, void* scratch, const void* zeros);
