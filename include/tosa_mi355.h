@@ -402,11 +402,11 @@ int tmi_dot_product_check(tmi_ctx_t* ctx, int32_t out_dtype, int64_t n, const vo
  * to write, does nothing.
  *
  * Some calls use the context's scratch buffer (tmi_ctx_reserve_workspace; the rules for graphs and for several of them are
- * those of every call that does): tmi_gated_ffn_backward always; tmi_gated_ffn on more than 16 rows, for partial sums where few
- * tiles meet a long sum and for copies of large operands whose rows are no whole pieces of 16 bytes; tmi_gated_ffn,
- * tmi_matvec_int4 and tmi_gated_ffn_int4 for copies of rows of fewer than eight elements.  While a graph is captured the buffer
- * cannot grow: a call that needs more is then refused, but for tmi_gated_ffn on rows of eight elements or more, which goes on
- * without it (its sums are then added in another order). */
+ * those of every call that does): tmi_gated_ffn_backward always; tmi_gated_ffn, tmi_matvec_int4 and tmi_gated_ffn_int4 for partial
+ * sums where few results meet a long sum, and for copies of rows of fewer than eight elements; tmi_gated_ffn for copies of large
+ * operands whose rows are no whole pieces of 16 bytes.  While a graph is captured the buffer cannot grow: a call that needs more is
+ * then refused, but for the last three on rows of eight elements or more, which go on without it (their sums are then added in
+ * another order). */
 
 /* act(g) */
 enum

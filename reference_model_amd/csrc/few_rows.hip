@@ -39,6 +39,10 @@ struct RowsArgs
     int32_t rows, n, k;
     int32_t tiles_n, tiles_k;
     int32_t act;
+    // few_rows_kernel: where a row's column tiles are shared by workgroups, `splits` of them, their sums as store_rows takes them from one workgroup's waves
+    int32_t splits;
+    int32_t per_split;        // column tiles
+    float* sums;              // [row tile of x][weight row tile][split]
     // int4_stream_kernel
     int32_t n_blocks;
     int32_t wk;               // waves of a tile
@@ -84,9 +88,9 @@ __device__ __forceinline__ void store_rows(const RowsArgs& a, const float* red, 
 constexpr int kShortWaves = 8;
 
 // PER: groups of a 4-bit tile, 0 = 16-bit weights; MT: tiles of 16 rows of x; U: column tiles whose loads a wave has in flight together;
-// ODD: rows of x or of 16-bit weights begin at odd elements
-template <typename T, int PER, int MT, bool GATED, int U, bool ODD>
-__global__ __launch_bounds__(64 * kShortWaves, PER ? 1 : 4) void few_rows_kernel(RowsArgs a)
+// ODD: rows of x or of 16-bit weights begin at odd elements; SHARED: workgroups may share a row's columns (16 bits: 0.2 us a call where they do not)
+template <typename T, int PER, int MT, bool GATED, int U, bool ODD, bool SHARED>
+__global__ __launch_bounds__(64 * kShortWaves, PER || SHARED ? 1 : 4) void few_rows_kernel(RowsArgs a)
 {
     constexpr bool DENSE = PER == 0;
     constexpr int S      = GATED ? 2 : 1;    // streams of weights: gate and up
@@ -149,7 +153,7 @@ __global__ __launch_bounds__(64 * kShortWaves, PER ? 1 : 4) void few_rows_kernel
         whalf[s] = halves_of(wbase[s]);
     // Rows of 16-bit weights may lie a power of two apart: workgroups that begin at different columns meet on different channels of the
     // memory.  us of one row with 2 x 32768 x 8192: 230 all from the first column, 178 so.  (In 4 bits a tile of rows lies in one piece.)
-    const int turn = DENSE && full ? (int)((blockIdx.x * 5u) % (uint32_t)full) : 0;
+    const int turn = DENSE && full && !SHARED ? (int)((blockIdx.x * 5u) % (uint32_t)full) : 0;
     auto turned    = [&](int kt) { return DENSE ? (kt + turn < full ? kt + turn : kt + turn - full) : kt; };
     // TAIL: the column tile that K ends in
     auto fetch_w = [&](Tile& t, int kt, auto TAIL) {
@@ -256,26 +260,28 @@ __global__ __launch_bounds__(64 * kShortWaves, PER ? 1 : 4) void few_rows_kernel
             }
     };
 
-    for (int k0 = wave; k0 < full; k0 += U * waves)
+    const int first = SHARED ? blockIdx.z * a.per_split : 0, behind = SHARED && first + a.per_split < a.tiles_k ? first + a.per_split : a.tiles_k;
+    const int whole = behind < full ? behind : full;
+    for (int k0 = first + wave; k0 < whole; k0 += U * waves)
     {
         Tile t[U];
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (k0 + u * waves < full)
+            if (k0 + u * waves < whole)
                 fetch_w(t[u], turned(k0 + u * waves), std::false_type());
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (k0 + u * waves < full)
+            if (k0 + u * waves < whole)
                 fetch_x(t[u], turned(k0 + u * waves), std::false_type());
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (k0 + u * waves < full)
+            if (k0 + u * waves < whole)
             {
                 join(t[u]);
                 multiply(t[u]);
             }
     }
-    if (full < a.tiles_k && full % waves == wave)
+    if (whole < behind && (whole - first) % waves == wave)
     {
         Tile t;
         fetch_w(t, full, std::true_type());
@@ -291,8 +297,29 @@ __global__ __launch_bounds__(64 * kShortWaves, PER ? 1 : 4) void few_rows_kernel
             for (int i = 0; i < 4; i++)
                 red[((wave * S + s) * MT + mt) * 256 + i * 64 + lane] = acc[s][mt][i];
     __syncthreads();
-    for (int o = threadIdx.x; o < MT * 256; o += blockDim.x)
-        store_rows<T, DENSE, MT, GATED>(a, red, waves, o, (int64_t)tn * 16, row0);
+    if (!SHARED || a.splits == 1)
+    {
+        for (int o = threadIdx.x; o < MT * 256; o += blockDim.x)
+            store_rows<T, DENSE, MT, GATED>(a, red, waves, o, (int64_t)tn * 16, row0);
+        return;
+    }
+    float* part = a.sums + (((int64_t)blockIdx.y * a.tiles_n + tn) * a.splits + blockIdx.z) * (S * MT * 256);
+    for (int o = threadIdx.x; o < S * MT * 256; o += blockDim.x)
+    {
+        float v = 0.0f;
+        for (int p = 0; p < waves; p++)
+            v += red[p * (S * MT * 256) + o];
+        part[o] = v;
+    }
+}
+
+// results of column tiles that workgroups shared
+template <typename T, bool DENSE, int MT, bool GATED>
+__global__ __launch_bounds__(256) void few_rows_join_kernel(RowsArgs a)
+{
+    const float* part = a.sums + ((int64_t)blockIdx.y * a.tiles_n + blockIdx.x) * a.splits * ((GATED ? 2 : 1) * MT * 256);
+    for (int o = threadIdx.x; o < MT * 256; o += 256)
+        store_rows<T, DENSE, MT, GATED>(a, part, a.splits, o, (int64_t)blockIdx.x * 16, (int64_t)blockIdx.y * (16 * MT));
 }
 
 constexpr int kAhead = 4;                              // pieces of x that a lane asks for at once
@@ -549,13 +576,13 @@ bool launch_stream(hipStream_t st, const RowsArgs& a, int waves)
     return true;
 }
 
-template <typename T, int PER, int MT, bool GATED, bool ODD>
+template <typename T, int PER, int MT, bool GATED, bool ODD, bool SHARED>
 bool launch_short(hipStream_t st, const RowsArgs& a)
 {
     constexpr int U = PER ? 4 : MT == 1 && !ODD ? 2 : 1, S = GATED ? 2 : 1;
-    const int waves  = a.tiles_k < 1 ? 1 : a.tiles_k < kShortWaves ? a.tiles_k : kShortWaves;
+    const int waves  = a.per_split < 1 ? 1 : a.per_split < kShortWaves ? a.per_split : kShortWaves;
     const size_t lds = (size_t)waves * S * MT * 1024;
-    if (!ensure_dynamic_lds<few_rows_kernel<T, PER, MT, GATED, U, ODD>>(lds))
+    if (!ensure_dynamic_lds<few_rows_kernel<T, PER, MT, GATED, U, ODD, SHARED>>(lds))
         return false;
     // a grid has 2^16 chunks of rows, and 2^32 threads
     const int64_t chunks = ((int64_t)a.rows + 16 * MT - 1) / (16 * MT), most = (int64_t(1) << 22) / a.tiles_n < 1 << 14 ? (int64_t(1) << 22) / a.tiles_n : 1 << 14;
@@ -568,8 +595,11 @@ bool launch_short(hipStream_t st, const RowsArgs& a)
         part.x += m * a.ldx, part.out += m * a.ldo;
         if (a.pre_gate)
             part.pre_gate += m * a.ldo, part.pre_up += m * a.ldo;
-        few_rows_kernel<T, PER, MT, GATED, U, ODD><<<dim3(a.tiles_n, (int)(chunks - c < step ? chunks - c : step)), 64 * waves, lds, st>>>(part);
+        few_rows_kernel<T, PER, MT, GATED, U, ODD, SHARED><<<dim3(a.tiles_n, (int)(chunks - c < step ? chunks - c : step), a.splits), 64 * waves, lds, st>>>(part);
     }
+    // (sums are split only where one launch has all rows)
+    if (a.splits > 1)
+        few_rows_join_kernel<T, PER == 0, MT, GATED><<<dim3(a.tiles_n, (int)chunks), 256, 0, st>>>(a);
     return true;
 }
 
@@ -581,7 +611,9 @@ bool launch_short(hipStream_t st, const RowsArgs& a)
     bool odd = ((a.ldx & 1) && a.rows > 1) || (reinterpret_cast<uintptr_t>(a.x) & 2);
     if (PER == 0)
         odd |= (a.ldw & 1) || ((reinterpret_cast<uintptr_t>(a.w[0]) | reinterpret_cast<uintptr_t>(a.w[1])) & 2);
-    return odd ? launch_short<T, PER, MT, GATED, true>(st, a) : launch_short<T, PER, MT, GATED, false>(st, a);
+    if (PER || a.splits > 1)
+        return odd ? launch_short<T, PER, MT, GATED, true, true>(st, a) : launch_short<T, PER, MT, GATED, false, true>(st, a);
+    return odd ? launch_short<T, PER, MT, GATED, true, PER != 0>(st, a) : launch_short<T, PER, MT, GATED, false, PER != 0>(st, a);
 }
 
 // The short kernel up to four rows and 32 MB of weights, and up to 16 rows and 8 MB (x goes to it once for every 16 weight rows).  us short /
@@ -590,6 +622,8 @@ bool launch_short(hipStream_t st, const RowsArgs& a)
 template <typename T, int PER, bool GATED>
 bool choose(hipStream_t st, const RowsArgs& a)
 {
+    if (a.splits > 1)
+        return launch_short<T, PER, 1, GATED>(st, a);
     const int64_t kb = a.tiles * (GATED ? 2 : 1);
     if (a.rows <= 16 && kb <= (a.rows <= 4 ? 32768 : 8192))
         return launch_short<T, PER, 1, GATED>(st, a);
@@ -621,25 +655,58 @@ RowsArgs rows_args(int32_t rows, int32_t n, int32_t k, const void* x, int64_t ld
     a.ldx = ldx, a.ldo = ldo, a.rows = rows, a.n = n, a.k = k;
     a.tiles_n = (int32_t)int4_tiles(n, kInt4Rows), a.tiles_k = (int32_t)int4_tiles(k, kInt4Cols);
     a.tiles   = (int64_t)a.tiles_n * a.tiles_k;
+    a.splits  = 1, a.per_split = a.tiles_k;
     return a;
+}
+
+// How many workgroups share the columns of a weight row tile.  Few tiles with long rows leave most of the chip idle while each of eight waves goes through
+// its columns in turns of U tiles, 2 to 4 us each; joining the parts is a launch more, which two turns do not pay.  More than 16 rows of x in 4 bits would
+// otherwise go to the stream, whose workgroups have more rows.  us with all columns in one workgroup / shared, in 4 bits: 14 rows 256 x 24008 18.4 / 7.5,
+// one row 512 x 16384 (four turns) 9.1 / 6.1, 1024 x 8192 (two) 5.4 / 6.0, 19 rows 2 x 104 x 4636 13.4 / 7.6; in 16 bits: one row 2 x 1000 x 8192 (four) 18.5
+// / 11.7, 2 x 2000 x 4096 (two) 10.7 / 11.4.
+int few_rows_splits(bool dense, int32_t rows, int32_t n, int32_t k)
+{
+    const int at_once      = kShortWaves * (dense ? (rows <= 16 ? 2 : 1) : 4), of_x = dense && rows > 16 ? 32 : 16;
+    const int64_t tiles_k  = int4_tiles(k, kInt4Cols), tiles = int4_tiles(n, kInt4Rows) * int4_tiles(rows, of_x);
+    const int64_t turns    = int4_tiles(tiles_k, at_once), places = 512 / (tiles > 0 ? tiles : 1);
+    if (tiles > 128 || tiles_k <= (!dense && rows > 16 ? 1 : 2) * at_once)
+        return 1;
+    return (int)(turns < places ? turns : places);
+}
+
+void share_columns(RowsArgs& a, int splits, float* sums)
+{
+    a.per_split = (int32_t)int4_tiles(a.tiles_k, splits);
+    a.splits    = (int32_t)int4_tiles(a.tiles_k, a.per_split);
+    a.sums      = sums;
 }
 
 }    // namespace
 
+size_t few_rows_scratch_bytes(bool dense, bool gated, int32_t rows, int32_t n, int32_t k)
+{
+    const int splits = few_rows_splits(dense, rows, n, k), of_x = dense && rows > 16 ? 32 : 16;
+    return splits == 1 ? 0 : (size_t)int4_tiles(n, kInt4Rows) * int4_tiles(rows, of_x) * splits * (gated ? 2 : 1) * of_x * 64;
+}
+
 const char* launch_int4_rows(hipStream_t st, int32_t dtype, int32_t group, bool gated, int32_t act, int32_t rows, int32_t n, int32_t k, const void* x,
-                             int64_t ldx, const void* w, const void* up, void* out, int64_t ldo)
+                             int64_t ldx, const void* w, const void* up, void* out, int64_t ldo, void* scratch)
 {
     RowsArgs a = rows_args(rows, n, k, x, ldx, w, up, out, ldo);
     a.act      = act;
+    if (scratch)
+        share_columns(a, few_rows_splits(false, rows, n, k), static_cast<float*>(scratch));
     const bool ok = group == 32 ? choose<4>(st, dtype, gated, a) : group == 64 ? choose<2>(st, dtype, gated, a) : choose<1>(st, dtype, gated, a);
     return !ok ? nullptr : gated ? "int4_rows_gated" : "int4_rows";
 }
 
 const char* launch_ffn_rows(hipStream_t st, int32_t dtype, int32_t act, int32_t rows, int32_t d, int32_t f, const void* x, int64_t ldx,
-                            const void* gate, const void* up, int64_t ldw, void* out, void* pre_gate, void* pre_up, int64_t ldo)
+                            const void* gate, const void* up, int64_t ldw, void* out, void* pre_gate, void* pre_up, int64_t ldo, void* scratch)
 {
     RowsArgs a = rows_args(rows, f, d, x, ldx, gate, up, out, ldo);
     a.act = act, a.ldw = ldw;
+    if (scratch)
+        share_columns(a, few_rows_splits(true, rows, f, d), static_cast<float*>(scratch));
     a.pre_gate = static_cast<uint16_t*>(pre_gate), a.pre_up = static_cast<uint16_t*>(pre_up);
     bool ok;
     if (rows <= 16)

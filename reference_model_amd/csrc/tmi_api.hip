@@ -2189,7 +2189,11 @@ static int int4_rows(tmi_ctx* ctx, const char* op, const tmi_int4_desc_t* d, boo
         launch_widen_rows(ctx->stream, WidenRows{ 1, k, { x }, { ld_x }, { rows }, { ctx->workspace } });
         x = ctx->workspace, ld_x = k = 8;
     }
-    return after_launch(ctx, launch_int4_rows(ctx->stream, d->dtype, d->group, gated, activation, rows, d->out_features, k, x, ld_x, w, up, out, ld_out));
+    // (rows of fewer than eight elements have one column tile: nothing to share, and the scratch buffer is theirs alone)
+    const size_t bytes = few_rows_scratch_bytes(false, gated, rows, d->out_features, k);
+    const bool parts   = bytes > 0 && optional_workspace(ctx, bytes);
+    return after_launch(ctx, launch_int4_rows(ctx->stream, d->dtype, d->group, gated, activation, rows, d->out_features, k, x, ld_x, w, up, out, ld_out,
+                                              parts ? ctx->workspace : nullptr));
 }
 
 int tmi_matvec_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, int32_t rows, const void* x_dev, int64_t ld_x, const void* packed_dev,
@@ -2268,11 +2272,15 @@ int tmi_gated_ffn(tmi_ctx_t* ctx, const tmi_gated_ffn_desc_t* desc, const void* 
         launch_widen_rows(ctx->stream, WidenRows{ 3, d.in_features, { x_dev, gate_dev, up_dev }, { d.ld_x, d.ld_w, d.ld_w },
                                                   { d.rows, d.hidden_features, d.hidden_features }, { to, to + x_bytes, to + x_bytes + w_bytes } });
         return after_launch(ctx, launch_ffn_rows(ctx->stream, d.dtype, d.activation, d.rows, 8, d.hidden_features, to, 8, to + x_bytes,
-                                                 to + x_bytes + w_bytes, 8, h_dev, pre_gate_dev, pre_up_dev, d.ld_h));
+                                                 to + x_bytes + w_bytes, 8, h_dev, pre_gate_dev, pre_up_dev, d.ld_h, nullptr));
     }
     if (gated_ffn_few_rows_lead(d, x_dev, gate_dev, up_dev))
+    {
+        const size_t bytes = few_rows_scratch_bytes(true, true, d.rows, d.hidden_features, d.in_features);
+        const bool parts   = bytes > 0 && optional_workspace(ctx, bytes);
         return after_launch(ctx, launch_ffn_rows(ctx->stream, d.dtype, d.activation, d.rows, d.in_features, d.hidden_features, x_dev, d.ld_x, gate_dev,
-                                                 up_dev, d.ld_w, h_dev, pre_gate_dev, pre_up_dev, d.ld_h));
+                                                 up_dev, d.ld_w, h_dev, pre_gate_dev, pre_up_dev, d.ld_h, parts ? ctx->workspace : nullptr));
+    }
     const size_t bytes = gated_ffn_scratch_bytes(d, x_dev, gate_dev, up_dev);
     const bool parts   = bytes > 0 && optional_workspace(ctx, bytes);
     return after_launch(ctx, launch_gated_ffn(ctx->stream, d, x_dev, gate_dev, up_dev, h_dev, pre_gate_dev, pre_up_dev,

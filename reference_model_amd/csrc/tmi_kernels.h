@@ -316,11 +316,13 @@ const char* launch_matmul_i16_direct(hipStream_t st, int32_t N, int32_t H, int32
 const char* launch_matmul_direct(hipStream_t st, int32_t in_dtype, int32_t N, int32_t H, int32_t C, int32_t W,
                                  const void* a, const void* b, int32_t a_zp, int32_t b_zp, void* out);
 
-// few_rows.hip (rows of x of 8 elements at least, or of none): products of a few rows with 4-bit weights (`up` not read), the gated block on them, and the gated block on 16-bit weights
+// few_rows.hip (rows of x of 8 elements at least, or of none): products of a few rows with 4-bit weights (`up` not read), the gated block on them, and the gated block on 16-bit weights.
+// `scratch`: of as many bytes as few_rows_scratch_bytes says, or nullptr: all columns of a weight row in one workgroup
+size_t few_rows_scratch_bytes(bool dense, bool gated, int32_t rows, int32_t n, int32_t k);
 const char* launch_int4_rows(hipStream_t st, int32_t dtype, int32_t group, bool gated, int32_t act, int32_t rows, int32_t n, int32_t k,
-                             const void* x, int64_t ldx, const void* w, const void* up, void* out, int64_t ldo);
+                             const void* x, int64_t ldx, const void* w, const void* up, void* out, int64_t ldo, void* scratch);
 const char* launch_ffn_rows(hipStream_t st, int32_t dtype, int32_t act, int32_t rows, int32_t d, int32_t f, const void* x, int64_t ldx,
-                            const void* gate, const void* up, int64_t ldw, void* out, void* pre_gate, void* pre_up, int64_t ldo);
+                            const void* gate, const void* up, int64_t ldw, void* out, void* pre_gate, void* pre_up, int64_t ldo, void* scratch);
 // gated_ffn.hip: the gated block on many rows and its gradients (row strides of the descriptors filled in).  `scratch`: of as many bytes as the
 // functions before say (forward: nullptr does too, with the sum in one piece); zeros: 64 bytes of them
 // n matrices of rows of `width` elements of 16 bits, copied to rows filled up with zeros to whole pieces of 8

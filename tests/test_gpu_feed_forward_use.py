@@ -240,3 +240,30 @@ def test_example():
     # a group's largest weight is 7 steps, so a rounding is off by a fourteenth of it at most, 2.9 / 14 / sqrt(3) of a normal number's deviation at 32 a group and about
     # half of that in the mean; three such matrices make an answer
     assert 0.02 < got["weights_off"] < 0.12 and got["answers_off"] < 0.35
+
+
+# few results from long rows, whose columns workgroups share; the last rows of tiles and the last column tiles empty, one column past a tile, one short of it
+LONG = [(1, 6001, 40), (14, 8193, 17), (16, 2111, 100), (5, 4095, 16), (31, 5000, 9), (60, 3001, 33)]
+
+
+@pytest.mark.parametrize("shape", LONG, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_few_results_of_long_rows(ctx, kind, shape):
+    kind, (m, k, n), group = KINDS[kind], shape, 64
+    rng = np.random.default_rng(k)
+    x, gate, up = operands(kind, m, k, n, k)
+    for v, want in zip(forward(ctx, kind, "gelu", x, gate, up), ref.gated(kind, "gelu", x, gate, up)):
+        near(kind.wide(v), want)
+    desc, held, packed = ctx.int4_desc(kind.dtype, group, n, k), [], []
+    for _ in range(2):
+        v, scales = rng.integers(-8, 8, (n, k)), kind.narrow(rng.normal(0, 0.2 / np.sqrt(k), (n, -(-k // group))))
+        packed.append(ref.weights(kind, v, scales, group))
+        held.append(ctx.upload(ref.packed(kind, v, scales, group)))
+    dev, y, h = Rows(ctx, kind, (m, k), x, 1, 0), Rows(ctx, kind, (m, n), None, 3, 0), Rows(ctx, kind, (m, n), None, 3, 0)
+    ctx.matvec_int4(desc, m, dev.at, k + 1, held[0], y.at, n + 3)
+    ctx.gated_ffn_int4(desc, capi.ACT_SILU, m, dev.at, k + 1, *held, h.at, n + 3)
+    assert ctx.sync() == capi.VALID
+    near(y.values(), ref.product(kind, x, packed[0]))
+    near(h.values(), ref.gated(kind, "silu", x, *packed)[0])
+    for t in held + [dev, y, h]:
+        t.free()
