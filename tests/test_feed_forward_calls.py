@@ -9,6 +9,7 @@ import pytest
 
 from reference_model_amd import TmiError, build, capi
 
+pytest.importorskip("torch")    # first: the library then shares its HIP runtime; loaded behind the library it would bring a second one, which finds no GPU
 capi.load_library()
 NATIVE = {name: vars(capi.Context)[name] for name in capi.PLAIN_FEED_FORWARD}
 FFN, INT4 = capi.GatedFfnDesc(), capi.Int4Desc()
