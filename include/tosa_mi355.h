@@ -543,6 +543,14 @@ void tmi_debug_last_launch_shape(int32_t* out3);
 int tmi_debug_tile_decode(int64_t grid, uint32_t n_ocb, uint32_t tiles_x, uint32_t tiles_y, uint32_t block,
                           int32_t* out4);
 
+/* Host arithmetic only, no GPU call: how tmi_gated_ffn (product 0) or tmi_gated_ffn_backward, called for all gradients (1: d_x, 2: those of the
+ * weights), runs on tensors at these addresses, of which nothing is read.  out8 receives rows and columns of a tile (0: the kernel of few
+ * rows has the call), waves of a workgroup, parts of the sum, whether operands go straight into LDS, whether they are copied first, whether both
+ * gradients are one launch, and the bytes that an offset held in 32 bits reaches over.  TMI_ERROR where the call is refused.
+ * Used by the unit tests, which choose their sizes by it. */
+int tmi_debug_gated_ffn_plan(const tmi_gated_ffn_desc_t* d, const void* x_dev, const void* gate_dev, const void* up_dev, int32_t product,
+                             int64_t* out8);
+
 /* Library build identification, e.g. "tosa_mi355 gfx950". */
 const char* tmi_version(void);
 

@@ -40,7 +40,7 @@ EXPORTS = [
     "tmi_ctx_set_precise_mode", "tmi_ctx_workspace_bytes", "tmi_ctx_trim_workspace",
     "tmi_int4_packed_bytes", "tmi_quantize_int4", "tmi_pack_int4", "tmi_dequantize_int4", "tmi_matvec_int4", "tmi_gated_ffn_int4",
     "tmi_gated_ffn", "tmi_gated_ffn_backward",
-    "tmi_debug_launch_empty", "tmi_debug_tile_decode", "tmi_debug_last_launch_shape", "tmi_debug_stream",
+    "tmi_debug_launch_empty", "tmi_debug_tile_decode", "tmi_debug_last_launch_shape", "tmi_debug_stream", "tmi_debug_gated_ffn_plan",
 ]
 
 NOALLOC_SCRATCH_BYTES = 16 << 20  # TMI_NOALLOC_SCRATCH_BYTES
@@ -191,6 +191,7 @@ def load_library() -> ctypes.CDLL:
     ffn, int4 = ctypes.POINTER(GatedFfnDesc), ctypes.POINTER(Int4Desc)
     lib.tmi_gated_ffn.argtypes = [vp, ffn] + [vp] * 6
     lib.tmi_gated_ffn_backward.argtypes = [vp, ffn] + [vp] * 9
+    lib.tmi_debug_gated_ffn_plan.argtypes = [ffn] + [vp] * 3 + [i32, ctypes.POINTER(i64)]
     lib.tmi_int4_packed_bytes.argtypes = [vp, int4, ctypes.POINTER(ctypes.c_size_t)]
     lib.tmi_quantize_int4.argtypes = [vp, int4, vp, i64, vp]
     lib.tmi_pack_int4.argtypes = [vp, int4, vp, i64, vp, vp]

@@ -778,6 +778,12 @@ bool launch_tiles(hipStream_t st, const GemmFfnArgs& a)
     return true;
 }
 
+// Tiles of 128 x 128 through registers: with two workgroups to a CU four waves are enough, and read LDS less (777 x 1111 x 2731 34.4 us with eight, 32.2)
+bool four_waves(const Shape& s)
+{
+    return s.tiles_m * s.tiles_n * s.splits > 256;
+}
+
 void set_shape(GemmFfnArgs& a, const Shape& s)
 {
     a.tiles_m = s.tiles_m, a.tiles_n = s.tiles_n, a.tiles = s.tiles_m * s.tiles_n;
@@ -825,10 +831,9 @@ bool launch_product(hipStream_t st, int32_t dtype, const GemmFfnArgs& a, const S
             ok = launch_tiles<T, OP, 2, 4, 4, true>(st, a);
         else
             // Eight waves, whose reads and matrix instructions hide each other's waits: us forward 1024 x 1024 x 1024 13.3 with eight and 15.2 with four, 500 x
-            // 1111 x 2731 through registers 17.2 and 20.9.  Through registers with two workgroups to a CU four are enough, and read LDS less: 777 x
-            // 1111 x 2731 34.4 and 32.2.
+            // 1111 x 2731 through registers 17.2 and 20.9.
             ok = fast ? launch_tiles<T, OP, 2, 4, 2, true>(st, a)
-                      : a.tiles * a.splits > 256 ? launch_tiles<T, OP, 2, 2, 4, false>(st, a) : launch_tiles<T, OP, 2, 4, 2, false>(st, a);
+                      : four_waves(s) ? launch_tiles<T, OP, 2, 2, 4, false>(st, a) : launch_tiles<T, OP, 2, 4, 2, false>(st, a);
         return ok;
     };
     const bool ok = dtype == TMI_BF16 ? typed(bf16_t{}) : typed(_Float16{});
@@ -837,10 +842,13 @@ bool launch_product(hipStream_t st, int32_t dtype, const GemmFfnArgs& a, const S
     return ok;
 }
 
-// whether rows of `width` elements, `ld` apart, are whole 16-byte pieces, and near enough for 32-bit offsets over a tile
+// Loads straight into LDS take a lane's offset from a tile's first element in 32 bits: over the 256 rows of the largest tile 2^31 bytes from here on.
+constexpr int64_t kFarRows = int64_t(1) << 22;
+
+// whether rows of `width` elements, `ld` apart, are whole 16-byte pieces, and near enough for those offsets
 bool whole_pieces(const void* p, int64_t width, int64_t ld)
 {
-    return ((uintptr_t)p & 15) == 0 && width % 8 == 0 && ld % 8 == 0 && ld < (int64_t(1) << 22);
+    return ((uintptr_t)p & 15) == 0 && width % 8 == 0 && ld % 8 == 0 && ld < kFarRows;
 }
 
 int64_t whole_of(int64_t n, int64_t per)
@@ -850,28 +858,31 @@ int64_t whole_of(int64_t n, int64_t per)
 
 // A product's way: of operands that lie in whole pieces, as they are; of others through registers, or on copies that end in zeros, read and written at 3.5
 // TB/s with 8 us for a launch more.  us forward 4096 x 2047 x 8192 460 through registers, 263 on copies, its gradients 905 and 536; 777 x 1111 x 2731 32 and
-// 38, 512 x 4095 x 4096 61 and 87.  (Rows of less than eight elements are always copied: the loads through registers take eight.)
+// 38, 512 x 4095 x 4096 61 and 87.  (Rows of less than eight elements are always copied: the loads through registers take eight.)  Where the rows of a copy,
+// or of dp (`ldp`, 0 where it is no operand), lie too far apart for the offsets of the direct loads, the product takes the registers' 64-bit addresses.
 struct Way
 {
     bool fast, copies;
     size_t bytes;     // of the copies
     Shape shape;
 };
-Way way_of(int op, int64_t M, int64_t N, int blocks, bool whole, int64_t copied_rows, int64_t d, double& us)
+Way way_of(int op, int64_t M, int64_t N, int blocks, bool whole, int64_t ldp, int64_t copied_rows, int64_t d, double& us)
 {
     Way w{};
     double direct = 0, registers = 0;
     w.shape = shape_of(op, M, N, blocks, true, direct);
     w.fast  = true;
     us      = direct;
-    if (whole)
+    const bool near = ldp < kFarRows;
+    if (whole && near)
         return w;
     const Shape other  = shape_of(op, M, N, blocks, false, registers);
     const size_t bytes = (size_t)copied_rows * whole_of(d, 8) * 2;
-    if (d < 8 || direct + 2 * (double)bytes / 3.5e6 + 8 < registers)
-        w.copies = true, w.bytes = bytes, us += 2 * (double)bytes / 3.5e6 + 8;
-    else
-        w.fast = false, w.shape = other, us = registers;
+    const double copy  = 2 * (double)bytes / 3.5e6 + 8;
+    if (d < 8 || (near && whole_of(d, 8) < kFarRows && direct + copy < registers))
+        w.copies = true, w.bytes = bytes, us += copy;
+    if (!near || !w.copies)
+        w.fast = false, w.shape = other, us = registers + (w.copies ? copy : 0);
     return w;
 }
 
@@ -917,7 +928,7 @@ ForwardPlan forward_plan(const tmi_gated_ffn_desc_t& d, const void* x, const voi
     ForwardPlan p;
     const bool whole = whole_pieces(x, d.in_features, d.ld_x) && whole_pieces(gate, d.in_features, d.ld_w) && whole_pieces(up, d.in_features, d.ld_w);
     p.blocks         = (int)(whole_of(d.in_features, kBlock) / kBlock);
-    p.way            = way_of(OP_FORWARD, d.rows, d.hidden_features, p.blocks, whole, (int64_t)d.rows + 2 * (int64_t)d.hidden_features, d.in_features, p.us);
+    p.way            = way_of(OP_FORWARD, d.rows, d.hidden_features, p.blocks, whole, 0, (int64_t)d.rows + 2 * (int64_t)d.hidden_features, d.in_features, p.us);
     return p;
 }
 struct BackwardPlan
@@ -940,8 +951,8 @@ BackwardPlan backward_plan(const tmi_gated_ffn_desc_t& d, const void* x, const v
     p.dw_blocks      = (int)(whole_of(d.rows, kBlock) / kBlock);
     const int64_t D  = d.in_features, F = d.hidden_features;
     double us_dx, us_dw;
-    p.dx             = way_of(OP_DX, d.rows, D, p.dx_blocks, whole_pieces(gate, D, d.ld_w) && whole_pieces(up, D, d.ld_w), 2 * F, D, us_dx);
-    p.dw             = way_of(OP_DW, 2 * p.half, D, p.dw_blocks, whole_pieces(x, D, d.ld_x), d.rows, D, us_dw);
+    p.dx             = way_of(OP_DX, d.rows, D, p.dx_blocks, whole_pieces(gate, D, d.ld_w) && whole_pieces(up, D, d.ld_w), p.ldp, 2 * F, D, us_dx);
+    p.dw             = way_of(OP_DW, 2 * p.half, D, p.dw_blocks, whole_pieces(x, D, d.ld_x), p.ldp, d.rows, D, us_dw);
     p.together       = false;
     if (want_dx && want_dw && !p.dx.copies && !p.dw.copies && p.dx.fast == p.dw.fast)
         p.together = side_by_side(p.dx, d.rows, p.dx_blocks, p.dw, 2 * p.half, p.dw_blocks, D, us_dx + us_dw);
@@ -973,6 +984,37 @@ bool gated_ffn_few_rows_lead(const tmi_gated_ffn_desc_t& d, const void* x, const
     const double chain  = ((d.in_features + 1023) / 1024) * 3.6 * places, bytes = chunks * 4.0 * d.in_features * d.hidden_features / 4.3e6;
     const bool odd      = ((d.ld_x | d.ld_w) & 1) || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(gate) | reinterpret_cast<uintptr_t>(up)) & 2);
     return 1.7 + (chain > bytes ? chain : bytes) * (odd ? 1.4 : 1) < forward_plan(d, x, gate, up).us;
+}
+
+GatedFfnPlan gated_ffn_plan(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up, int product)
+{
+    GatedFfnPlan r{};
+    if (product == OP_FORWARD && gated_ffn_few_rows_lead(d, x, gate, up))
+        return r;
+    Way w{};
+    int64_t M = d.rows, col_rows = kBlock, row_rows = kBlock, ldc = product == OP_DW ? d.ld_x : d.ld_w, ldr = d.ld_x;
+    if (product == OP_FORWARD)
+        w = forward_plan(d, x, gate, up).way;
+    else
+    {
+        const BackwardPlan p = backward_plan(d, x, gate, up, true, true);
+        w = product == OP_DX ? p.dx : p.dw, ldr = p.ldp, r.together = p.together;
+        M = product == OP_DX ? d.rows : 2 * p.half;
+    }
+    const auto& tile = kTiles[w.shape.tile];
+    if (w.copies)
+        ldc = whole_of(d.in_features, 8), ldr = product == OP_FORWARD ? ldc : ldr;
+    if (product == OP_FORWARD)
+        col_rows = d.hidden_features < tile.bn / 2 ? d.hidden_features : tile.bn / 2;
+    if (product != OP_DW)
+        row_rows = M < tile.bm ? M : tile.bm;
+    r.bm = tile.bm, r.bn = tile.bn, r.fast = w.fast, r.copies = w.copies, r.splits = w.shape.splits;
+    r.waves = !w.fast && !r.together && four_waves(w.shape) ? 4 : 8;
+    // (a tile's rows are read 64 bytes at a time where the summed index is innermost, else whole)
+    const int64_t of_col = (col_rows - 1) * ldc * 2 + (product == OP_FORWARD ? 2 * kBlock : 2 * tile.bn),
+                  of_row = (row_rows - 1) * ldr * 2 + (product == OP_DW ? 2 * tile.bm : 2 * kBlock);
+    r.span = w.fast ? (of_col > of_row ? of_col : of_row) : 0;
+    return r;
 }
 
 size_t gated_ffn_scratch_bytes(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up)

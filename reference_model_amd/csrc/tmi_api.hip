@@ -2238,6 +2238,18 @@ static int validate_gated_ffn(tmi_ctx* ctx, const char* op, const tmi_gated_ffn_
     return TMI_VALID;
 }
 
+int tmi_debug_gated_ffn_plan(const tmi_gated_ffn_desc_t* desc, const void* x_dev, const void* gate_dev, const void* up_dev, int32_t product,
+                             int64_t* out8)
+{
+    tmi_gated_ffn_desc_t d;
+    if (!out8 || product < 0 || product > 2 || validate_gated_ffn(nullptr, "gated_ffn", desc, d) != TMI_VALID)
+        return TMI_ERROR;
+    const GatedFfnPlan p = gated_ffn_plan(d, x_dev, gate_dev, up_dev, product);
+    out8[0] = p.bm, out8[1] = p.bn, out8[2] = p.waves, out8[3] = p.splits;
+    out8[4] = p.fast, out8[5] = p.copies, out8[6] = p.together, out8[7] = p.span;
+    return TMI_VALID;
+}
+
 int tmi_gated_ffn(tmi_ctx_t* ctx, const tmi_gated_ffn_desc_t* desc, const void* x_dev, const void* gate_dev, const void* up_dev,
                   void* h_dev, void* pre_gate_dev, void* pre_up_dev)
 {

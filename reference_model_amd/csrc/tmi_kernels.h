@@ -336,6 +336,15 @@ struct WidenRows
 void launch_widen_rows(hipStream_t st, const WidenRows& a);
 // whether launch_ffn_rows takes less time than launch_gated_ffn
 bool gated_ffn_few_rows_lead(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up);
+// what a product (0: forward, 1: d_x, 2: the weights' gradients) of a call for all of them launches: its tile (0: launch_ffn_rows takes the call), waves of a
+// workgroup, operands straight into LDS, on copies, parts of the sum, both gradients in one launch, bytes that a lane's 32-bit offset reaches over
+struct GatedFfnPlan
+{
+    int32_t bm, bn, waves, splits;
+    bool fast, copies, together;
+    int64_t span;
+};
+GatedFfnPlan gated_ffn_plan(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up, int product);
 size_t gated_ffn_scratch_bytes(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up);
 const char* launch_gated_ffn(hipStream_t st, const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up, void* h, void* pre_gate,
                              void* pre_up, void* scratch, const void* zeros);
