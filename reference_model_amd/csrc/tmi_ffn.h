@@ -13,16 +13,23 @@ namespace tmi
 // 1 / (1 + exp(-z)) without a division and without a library's exp (which take twice as many instructions): with E = exp(-|z|) in [0, 1] it is
 // 1 / (1 + E) or E / (1 + E), and the reciprocal's argument lies in [1, 2].  E is the square of 2^(-|z| log2(e) / 2), so that it may be subnormal,
 // put right by what rounding the exponent took.  |z| is cut where E has long been 0, for the difference of infinities that an infinite one would make.
-__device__ __forceinline__ float logistic(float z)
+// Of the value p and its complement q = 1 / (1 + exp(z)) each has all its digits: 1 - p would lose those of q for positive z, all of them from 17.3 on.
+__device__ __forceinline__ void logistic_both(float z, float& p, float& q)
 {
     constexpr float c = -0.72134752044448170f;    // -log2(e) / 2
     const float a     = fabsf(z) > 512.0f ? 512.0f : fabsf(z);    // (NaN stays)
     const float m     = a * c, off = __builtin_fmaf(a, c, -m);
-    const float q     = __builtin_amdgcn_exp2f(m);
-    float e           = q * q;
+    const float root  = __builtin_amdgcn_exp2f(m);
+    float e           = root * root;
     e                 = __builtin_fmaf(e, off * 1.38629436111989062f, e);    // 2 ln 2
-    const float r     = __builtin_amdgcn_rcpf(1.0f + e);
-    return z < 0.0f ? e * r : r;
+    const float r     = __builtin_amdgcn_rcpf(1.0f + e), er = e * r;
+    p = z < 0.0f ? er : r, q = z < 0.0f ? r : er;
+}
+__device__ __forceinline__ float logistic(float z)
+{
+    float p, q;
+    logistic_both(z, p, q);
+    return p;
 }
 // Phi(g), the normal distribution's cdf, and its density.  The tail beyond a = |g| is exp(-a^2 / 2) t S(t) with t = 1 / (1 + 0.32 a): S is a
 // polynomial of degree 9 fitted to it for the least relative error over all a (3e-8; in 32 bits 6 units of the last place).
@@ -72,8 +79,9 @@ __device__ __forceinline__ void act_both(float g, float& value, float& slope)
 {
     if constexpr (ACT == TMI_ACT_SILU)
     {
-        const float s = logistic(g);
-        value = g * s, slope = s * (1.0f + g * (1.0f - s));
+        float p, q;
+        logistic_both(g, p, q);
+        value = g * p, slope = p * (1.0f + g * q);
     }
     else if constexpr (ACT == TMI_ACT_GELU)
     {
@@ -83,7 +91,9 @@ __device__ __forceinline__ void act_both(float g, float& value, float& slope)
     }
     else if constexpr (ACT == TMI_ACT_GELU_TANH)
     {
-        const float p = logistic(gelu_tanh_twice(g)), pq = p * (1.0f - p);
+        float p, q;
+        logistic_both(gelu_tanh_twice(g), p, q);
+        const float pq = p * q;
         // far out p is 0 or 1 and g * g may be infinite
         value = g * p, slope = pq == 0.0f ? p : p + g * pq * (kGeluTwoC * (1.0f + 3.0f * kGeluCubic * g * g));
     }
@@ -91,8 +101,9 @@ __device__ __forceinline__ void act_both(float g, float& value, float& slope)
         value = g < 0.0f ? 0.0f : g, slope = g > 0.0f ? 1.0f : 0.0f;
     else
     {
-        const float s = logistic(g);
-        value = s, slope = s * (1.0f - s);
+        float p, q;
+        logistic_both(g, p, q);
+        value = p, slope = p * q;
     }
 }
 template <typename F>

@@ -1,7 +1,12 @@
-"""The feed-forward operators at the ends of their ranges: rows that lie gigabytes apart."""
+"""The feed-forward operators at the ends of their ranges: rows that lie gigabytes apart, pre-activations far out."""
+import math
+
+import numpy as np
 import pytest
 
+import ffn_reference as ref
 from reference_model_amd import Context, capi
+from test_gpu_gated_ffn import KINDS, backward, near
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -32,3 +37,37 @@ def test_gradients_of_rows_that_lie_4_gib_apart_over_a_tile(ctx):
     want = torch.zeros(f, d, device="cuda", dtype=torch.float64)
     want[features] = torch.mm(few.t().contiguous(), x.double())
     assert torch.equal(d_gate.double(), want) and torch.equal(d_up.double(), want)
+
+
+def slope_off(name, g, slope):
+    """How far act'(g) may be off in 32 bits: 32 units in 2^24 of what it is summed from, of which every factor has all its digits; an exponent z multiplies the
+    rounding of its argument by |z|, taken four times (GELU: z = g^2 / 2; its tanh form: z = 2 sqrt(2 / pi) (g + 0.044715 g^3))."""
+    with np.errstate(over="ignore", under="ignore"):
+        if name == "relu":
+            return 0 * g
+        if name == "gelu":
+            z, parts = g * g / 2, ref.act(name, -np.abs(g))[0] / -np.maximum(np.abs(g), 1e-30) + np.abs(g) * np.exp(-g * g / 2) / math.sqrt(2 * math.pi)
+            return ref.EPS * ((32 + 4 * z) * parts + 32 * np.abs(slope))
+        z, factor = g, 1.0
+        if name == "gelu_tanh":
+            z, factor = 2 * math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3), 2 * math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * g ** 2)
+        p, q = 1 / (1 + np.exp(-z)), 1 / (1 + np.exp(z))
+        if name == "sigmoid":
+            return ref.EPS * 32 * slope
+        return ref.EPS * (32 + (4 * np.abs(z) if name == "gelu_tanh" else 0)) * (np.minimum(p, q) + np.abs(g) * p * q * factor) + ref.EPS * 32 * np.abs(slope)
+
+
+@pytest.mark.parametrize("name", list(ref.ACTS))
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_slopes_over_their_range(ctx, kind, name):
+    """g from -30 to 30; one row whose first element is 1, u = dh = 1: the gradients of the weights are act'(g) and act(g) themselves, one term each"""
+    kind = KINDS[kind]
+    g = kind.wide(kind.narrow(np.r_[np.linspace(-30, 30, 601), np.linspace(9, 20, 100)]))[None]
+    f, one, w = g.shape[1], np.eye(1, 8), np.zeros((g.shape[1], 8))
+    _, d_gate, d_up = (kind.wide(v) for v in backward(ctx, kind, name, one, w, w, g, np.ones((1, f)), np.ones((1, f))))
+    value, slope = (v[0] for v in ref.act(name, g))
+    off = slope_off(name, g[0], slope)
+    near(d_gate[:, 0], (slope, off + kind.rounding(slope, off)))
+    off = ref.value_off(name, g[0], value)
+    near(d_up[:, 0], (value, off + kind.rounding(value, off)))
+    assert not d_gate[:, 1:].any() and not d_up[:, 1:].any()
