@@ -437,9 +437,10 @@ int tmi_gated_ffn(tmi_ctx_t* ctx, const tmi_gated_ffn_desc_t* d, const void* x_d
 
 /* Its gradients, from the pre-activations g and u and the gradient dh of h:
  *   du = dh act(g), dg = dh u act'(g), d_x = dg gate + du up, d_gate = dg^T x, d_up = du^T x
- * in 32 bits, with dg and du rounded to dtype before the products.  d_x_dev NULL, or d_gate_dev and d_up_dev both NULL:
+ * in 32 bits, with dg and du rounded to dtype before the products; in fp16 times a power of two where the largest of
+ * them lies beyond its range or below 2^-8, so that nothing is lost but their rounding and less than 2^-17 of the largest.  d_x_dev NULL, or d_gate_dev and d_up_dev both NULL:
  * that part is not computed (x_dev, or gate_dev and up_dev, may then be NULL).  dg and du live in the scratch buffer, 4
- * (rows) (hidden_features up to whole 64s) bytes and 128 more a row, with partial sums and copies as above. */
+ * (rows) (hidden_features up to whole 64s) bytes, 128 more a row and 8256 in fp16, with partial sums and copies as above. */
 int tmi_gated_ffn_backward(tmi_ctx_t* ctx, const tmi_gated_ffn_desc_t* d, const void* x_dev, const void* gate_dev,
                            const void* up_dev, const void* pre_gate_dev, const void* pre_up_dev, const void* d_h_dev,
                            void* d_x_dev, void* d_gate_dev, void* d_up_dev);

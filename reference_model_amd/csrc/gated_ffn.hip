@@ -40,6 +40,7 @@ struct GemmFfnArgs
     uint16_t *pre_gate, *pre_up;
     float* part;               // partial sums [split][(gate, up)][M][N], where the sum is split
     const uint8_t* zeros;      // 64 bytes
+    const float* unit;         // gradients in fp16: what dp is held in units of
     int64_t ldc, ldr, ldo;     // elements
     int32_t M, N;              // results: rows and columns (features of h; d; d)
     int32_t K;                 // summed index (of one half, for d_x)
@@ -66,6 +67,10 @@ __device__ __forceinline__ int swizzle_out(int k)
 {
     return (k & 3) | (k >> 1 & 4);
 }
+
+// whether dp of this type is held in units of a power of two (gated_slope_kernel)
+template <typename T>
+constexpr bool kInUnits = !__is_same(T, bf16_t);
 
 constexpr int kGroup = 8;    // row tiles that neighbouring workgroups share column tiles over
 constexpr int kBlock = 32;   // of the summed index
@@ -491,6 +496,7 @@ __device__ __forceinline__ void gated_gemm(const GemmFfnArgs& a, int workgroup)
         }
     };
     constexpr std::integral_constant<int, 2> rounded{};
+    const float unit = kInUnits<T> && OP != OP_FORWARD ? *a.unit : 1.0f;
     auto round4 = [&](v4f v, uint32_t* w) { w[0] = pack16<T>(v[0], v[1]), w[1] = pack16<T>(v[2], v[3]); };
     if (a.splits > 1)
     {
@@ -533,7 +539,13 @@ __device__ __forceinline__ void gated_gemm(const GemmFfnArgs& a, int workgroup)
     }
     else
         through_lds(TN, rounded, [&](int c, int i, uint32_t* w) {
-            round4(acc[c][i], w);
+            if constexpr (kInUnits<T>)
+            {
+                const v4f v = acc[c][i];
+                round4(v4f{ v[0] * unit, v[1] * unit, v[2] * unit, v[3] * unit }, w);
+            }
+            else
+                round4(acc[c][i], w);
         }, [&](int64_t m, int p, v4i v) {
             uint16_t* out = a.out[0];
             if constexpr (OP == OP_DW)
@@ -625,23 +637,74 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GemmFfnArgs a)
     {
         const int half  = OP == OP_DW && m >= a.half ? 1 : 0;
         const int64_t r = m - (half ? a.half : 0);
+        if constexpr (kInUnits<T>)
+        {
+            const float unit = *a.unit;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                v[0][e] *= unit;
+        }
         if (OP == OP_DX || r < a.features)
             store(a.out[half] + r * a.ldo + n, v[0]);
     }
 }
 
-// dp: eight features of a row a thread, of both halves
+// dp: eight features of a row a thread, of both halves, rounded to 16 bits because the matrix instructions take no more: each of its elements is then off
+// by 2^-8 (bf16) or 2^-11 of itself at most, and a gradient by about sqrt(2) times what its own rounding costs.  Bound by memory: 335 MB in 64 us at 4096 x 8192.
+//
+// bf16 has the range of 32 bits, fp16 has not: dh u act'(g) may pass 65504, or lie below the least fp16 number, where the sums over it are numbers that fp16
+// holds.  Where the largest of them lies between 2^-8 and 65504 they stand as they are, and what the least fp16 numbers cannot tell apart is less than 2^-17 of
+// the largest, little beside the rounding.  Otherwise the second pass (AGAIN), which every call in fp16 launches and which returns at once (2 us) where the first one
+// does, makes dp again in units of the power of two that brings the largest to 2^14 ... 2^15; the products' results are multiplied by it.  The largest is
+// taken over finite elements; infinities and NaN stay what they are.
 struct SlopeArgs
 {
     const uint16_t *pre_gate, *pre_up, *dh;
     uint16_t* dp;
+    float *most, *unit;        // fp16: the largest |dp| of every workgroup, and the unit
     int64_t ld, ldp, units;    // elements between rows of the inputs and of dp; units: rows * half / 8
     int32_t features, half, act;
+    int32_t groups;            // workgroups of the first pass
 };
+constexpr int kSlopeGroups = 4096, kSlopeUnits = 2048, kSlopeAgain = 1024;   // workgroups at most: bf16, and fp16's two passes
+constexpr size_t kUnitBytes = (kSlopeUnits + 16) * 4;                        // of most and unit
 
-template <typename T>
+// the largest of the workgroup's (256 threads), in every thread
+__device__ __forceinline__ float most_of_all(float v, float* of_wave)
+{
+#pragma unroll
+    for (int d = 32; d; d >>= 1)
+        v = fmaxf(v, __shfl_xor(v, d));
+    if ((threadIdx.x & 63) == 0)
+        of_wave[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return fmaxf(fmaxf(of_wave[0], of_wave[1]), fmaxf(of_wave[2], of_wave[3]));
+}
+
+template <typename T, bool AGAIN>
 __global__ __launch_bounds__(256) void gated_slope_kernel(SlopeArgs a)
 {
+    static_assert(kInUnits<T> || !AGAIN, "bf16 has one pass");
+    __shared__ float of_wave[4];
+    float scale = 1.0f, most = 0.0f;    // (scale: a constant but in the second pass)
+    if constexpr (AGAIN)
+    {
+        float of[kSlopeUnits / 256];    // (all on their way at once)
+#pragma unroll
+        for (int i = 0; i < kSlopeUnits / 256; i++)
+            of[i] = a.most[i * 256 + (int)threadIdx.x < a.groups ? i * 256 + threadIdx.x : 0];
+#pragma unroll
+        for (int i = 0; i < kSlopeUnits / 256; i++)
+            most = fmaxf(most, a.groups ? of[i] : 0.0f);
+        most             = most_of_all(most, of_wave);
+        const bool first = most == 0.0f || (most >= 0x1p-8f && most < 65520.0f);    // (65520 would round to infinity)
+        const int bits   = (int)(__float_as_uint(most) >> 23), up = 141 - bits < 126 ? 141 - bits : 126;    // 2^14 / 2^(bits - 127); its reciprocal is no subnormal
+        scale            = first ? 1.0f : __uint_as_float((uint32_t)(127 + up) << 23);
+        if (blockIdx.x == 0 && threadIdx.x == 0)
+            *a.unit = 1.0f / scale;
+        if (first)
+            return;
+    }
     const int per_row = a.half / 8;
     for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < a.units; u += (int64_t)gridDim.x * 256)
     {
@@ -649,30 +712,51 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(SlopeArgs a)
         const int f     = (int)(u - m * per_row) * 8;
         const v4i g = load8(a.pre_gate + m * a.ld, f, a.features), up = load8(a.pre_up + m * a.ld, f, a.features),
                   dh = load8(a.dh + m * a.ld, f, a.features);
-        v4i dg, du;
+        float x[8], y[8];
         for_act(a.act, [&](auto ACT) {
 #pragma unroll
-            for (int p = 0; p < 4; p++)
+            for (int e = 0; e < 8; e++)
             {
-                float x[2], y[2];
-#pragma unroll
-                for (int e = 0; e < 2; e++)
-                {
-                    float value, slope;
-                    act_both<decltype(ACT)::value>(from_bits16<T>(half_of(g, 2 * p + e)), value, slope);
-                    const float d = from_bits16<T>(half_of(dh, 2 * p + e));
-                    x[e] = d * from_bits16<T>(half_of(up, 2 * p + e)) * slope;
-                    y[e] = d * value;
-                    if (f + 2 * p + e >= a.features)
-                        x[e] = 0.0f, y[e] = 0.0f;
-                }
-                dg[p] = (int)pack16<T>(x[0], x[1]);
-                du[p] = (int)pack16<T>(y[0], y[1]);
+                float value, slope;
+                act_both<decltype(ACT)::value>(from_bits16<T>(half_of(g, e)), value, slope);
+                const float d = from_bits16<T>(half_of(dh, e));
+                x[e] = d * from_bits16<T>(half_of(up, e)) * slope;
+                y[e] = d * value;
+                if (f + e >= a.features)
+                    x[e] = 0.0f, y[e] = 0.0f;
             }
         });
+        if constexpr (kInUnits<T> && !AGAIN)
+        {
+            float here = 0.0f;    // (of a number and NaN the number)
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                here = fmaxf(fmaxf(here, fabsf(x[e])), fabsf(y[e]));
+            if (here == __builtin_huge_valf())
+            {
+                here = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    here = fmaxf(here, fmaxf(fabsf(x[e]) < __builtin_huge_valf() ? fabsf(x[e]) : 0.0f, fabsf(y[e]) < __builtin_huge_valf() ? fabsf(y[e]) : 0.0f));
+            }
+            most = fmaxf(most, here);
+        }
+        v4i dg, du;
+#pragma unroll
+        for (int p = 0; p < 4; p++)
+        {
+            dg[p] = (int)pack16<T>(x[2 * p] * scale, x[2 * p + 1] * scale);
+            du[p] = (int)pack16<T>(y[2 * p] * scale, y[2 * p + 1] * scale);
+        }
         uint16_t* row = a.dp + m * a.ldp + f;
         *reinterpret_cast<v4i*>(row)          = dg;
         *reinterpret_cast<v4i*>(row + a.half) = du;
+    }
+    if constexpr (kInUnits<T> && !AGAIN)
+    {
+        most = most_of_all(most, of_wave);
+        if (threadIdx.x == 0)
+            a.most[blockIdx.x] = most;
     }
 }
 
@@ -934,7 +1018,7 @@ ForwardPlan forward_plan(const tmi_gated_ffn_desc_t& d, const void* x, const voi
 struct BackwardPlan
 {
     int64_t half, ldp;
-    size_t dp_bytes;
+    size_t dp_bytes, unit_bytes;
     int dx_blocks, dw_blocks;
     Way dx, dw;
     bool together;    // in one launch
@@ -947,6 +1031,7 @@ BackwardPlan backward_plan(const tmi_gated_ffn_desc_t& d, const void* x, const v
     // of two apart where F is one, on few channels of the memory.
     p.ldp            = 2 * p.half + 64;
     p.dp_bytes       = (size_t)d.rows * p.ldp * 2;
+    p.unit_bytes     = d.dtype == TMI_FP16 ? kUnitBytes : 0;
     p.dx_blocks      = (int)(2 * p.half / kBlock);
     p.dw_blocks      = (int)(whole_of(d.rows, kBlock) / kBlock);
     const int64_t D  = d.in_features, F = d.hidden_features;
@@ -1055,13 +1140,13 @@ const char* launch_gated_ffn(hipStream_t st, const tmi_gated_ffn_desc_t& d, cons
     return launch_product<OP_FORWARD>(st, d.dtype, a, p.way.shape, p.way.fast) ? "gated_ffn" : nullptr;
 }
 
-// dp, then copies, then the partial sums: of one product after the other, or of both
+// dp, then its unit, then copies, then the partial sums: of one product after the other, or of both
 size_t gated_ffn_backward_scratch_bytes(const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up, bool dx, bool dw)
 {
     const BackwardPlan p = backward_plan(d, x, gate, up, dx, dw);
     const size_t of_dx   = dx ? part_bytes(OP_DX, p.dx.shape, d.rows, d.in_features) : 0;
     const size_t of_dw   = dw ? part_bytes(OP_DW, p.dw.shape, 2 * p.half, d.in_features) : 0;
-    return p.dp_bytes + p.dx.bytes + p.dw.bytes + (p.together ? of_dx + of_dw : of_dx > of_dw ? of_dx : of_dw);
+    return p.dp_bytes + p.unit_bytes + p.dx.bytes + p.dw.bytes + (p.together ? of_dx + of_dw : of_dx > of_dw ? of_dx : of_dw);
 }
 
 const char* launch_gated_ffn_backward(hipStream_t st, const tmi_gated_ffn_desc_t& d, const void* x, const void* gate, const void* up,
@@ -1073,19 +1158,27 @@ const char* launch_gated_ffn_backward(hipStream_t st, const tmi_gated_ffn_desc_t
     q.pre_gate = static_cast<const uint16_t*>(pre_gate), q.pre_up = static_cast<const uint16_t*>(pre_up), q.dh = static_cast<const uint16_t*>(d_h);
     q.dp = static_cast<uint16_t*>(scratch), q.ld = d.ld_h, q.ldp = p.ldp, q.units = d.rows * (p.half / 8);
     q.features = d.hidden_features, q.half = (int32_t)p.half, q.act = d.activation;
+    q.most = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + p.dp_bytes), q.unit = q.most + kSlopeUnits;
     const int64_t groups = (q.units + 255) / 256;
-    const int grid       = (int)(groups < 4096 ? groups : 4096);
-    if (grid > 0 && d.dtype == TMI_BF16)
-        gated_slope_kernel<bf16_t><<<grid, 256, 0, st>>>(q);
-    else if (grid > 0)
-        gated_slope_kernel<_Float16><<<grid, 256, 0, st>>>(q);
+    const int64_t limit  = d.dtype == TMI_FP16 ? kSlopeUnits : kSlopeGroups;
+    q.groups             = (int32_t)(groups < limit ? groups : limit);
+    if (d.dtype == TMI_FP16)
+    {
+        if (q.groups > 0)
+            gated_slope_kernel<_Float16, false><<<q.groups, 256, 0, st>>>(q);
+        // (no rows or features: the unit of sums of nothing)
+        gated_slope_kernel<_Float16, true><<<q.groups < 1 ? 1 : q.groups < kSlopeAgain ? q.groups : kSlopeAgain, 256, 0, st>>>(q);
+    }
+    else if (q.groups > 0)
+        gated_slope_kernel<bf16_t, false><<<q.groups, 256, 0, st>>>(q);
 
     const int64_t wide = whole_of(d.in_features, 8);
-    uint16_t* copies   = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(scratch) + p.dp_bytes);
+    uint16_t* copies   = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(scratch) + p.dp_bytes + p.unit_bytes);
     GemmFfnArgs a{};
     a.row = q.dp, a.ldr = p.ldp, a.half = (int32_t)p.half, a.features = d.hidden_features;
     a.part  = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(copies) + p.dx.bytes + p.dw.bytes);
     a.zeros = static_cast<const uint8_t*>(zeros);
+    a.unit  = q.unit;
     a.N     = d.in_features;
     GemmFfnArgs of_x = a, of_w = a;
     if (d_x)

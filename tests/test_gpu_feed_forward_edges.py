@@ -1,4 +1,5 @@
-"""The feed-forward operators at the ends of their ranges: rows that lie gigabytes apart, pre-activations far out."""
+"""The feed-forward operators at the ends of their ranges: rows that lie gigabytes apart, pre-activations far out, gradients whose
+factors fp16 does not hold."""
 import math
 
 import numpy as np
@@ -71,3 +72,99 @@ def test_slopes_over_their_range(ctx, kind, name):
     off = ref.value_off(name, g[0], value)
     near(d_up[:, 0], (value, off + kind.rounding(value, off)))
     assert not d_gate[:, 1:].any() and not d_up[:, 1:].any()
+
+
+# rows, d, f: both gradients in one launch with d_x's or the weights' sums split, through registers, on copies, and one after the other with d_x in parts
+RANGE_SHAPES = {"split_dx": (40, 64, 1200), "split_dw": (1100, 72, 40), "registers": (70, 129, 65), "copies": (300, 7, 9), "apart": (2048, 1024, 4096)}
+
+
+def fp16_operands(shape, about, seed=3):
+    """dg and du beyond fp16's range on either side, or one of them beyond it and the others ordinary; the gradients are numbers that it holds"""
+    kind, rng = KINDS["fp16"], np.random.default_rng(seed)
+    m, d, f = shape
+    of_x, of_w, of_g, of_u, of_dh = {"large": (3e-4, 1e-4, 1, 100, 3000), "tiny": (300, 300, 1e-2, 3e-3, 3e-6), "ordinary": (1, d ** -0.5, 1, 1, 0.1),
+                                     "outlier": (0.05, 0.05, 1, 1, 10)}[about]
+    made = lambda std, *s: kind.wide(kind.narrow(rng.normal(0, std, s)))  # noqa: E731
+    x, gate, up, g, u, dh = made(of_x, m, d), made(of_w, f, d), made(of_w, f, d), made(of_g, m, f), made(of_u, m, f), made(of_dh, m, f)
+    if about == "outlier":
+        g[3, 5], u[3, 5], dh[3, 5] = 1, 65, 2000
+    return x, gate, up, g, u, dh
+
+
+def held_gradients(x, gate, up, g, u, dh, most):
+    """the reference where dg and du lose, besides their rounding, at most 2^-25 of the largest of them"""
+    kind = ref.Kind("fp16")
+    kind.tiny = 2.0 ** -25 * most
+    return [(w, off + KINDS["fp16"].tiny) for w, off in ref.gated_gradients(kind, "silu", x, gate, up, g, u, dh)]
+
+
+def largest(g, u, dh):
+    value, slope = ref.act("silu", g)
+    return max(np.abs(dh * value).max(), np.abs(dh * u * slope).max())
+
+
+@pytest.mark.parametrize("about", ["large", "tiny", "outlier"])
+@pytest.mark.parametrize("where", list(RANGE_SHAPES))
+def test_fp16_gradients_of_products_beyond_its_range(ctx, where, about):
+    shape = RANGE_SHAPES[where]
+    x, gate, up, g, u, dh = fp16_operands(shape, about)
+    most = largest(g, u, dh)
+    assert most > 65504 if about != "tiny" else most < 2.0 ** -22
+    got = [KINDS["fp16"].wide(v) for v in backward(ctx, KINDS["fp16"], "silu", x, gate, up, g, u, dh)]
+    # a sample of rows and of features
+    rows, features = (np.unique(np.r_[0:min(n, 40), max(n - 40, 0):n]) for n in (shape[0], shape[2]))
+    want = [held_gradients(x[rows], gate, up, g[rows], u[rows], dh[rows], most)[0], *held_gradients(x, gate[features], up[features], g[:, features], u[:, features],
+                                                                                                        dh[:, features], most)[1:]]
+    for v, w, pick in zip(got, want, (rows, features, features)):
+        near(v[pick], w)
+        assert (np.abs(w[0]) > 4 * w[1]).mean() > 0.5    # the comparison says something
+    of_x = backward(ctx, KINDS["fp16"], "silu", x, gate, up, g, u, dh, dw=False)[0]
+    assert np.isfinite(KINDS["fp16"].wide(of_x)).all()
+
+
+def test_fp16_gradients_of_nothing_and_of_infinities(ctx):
+    kind, shape = KINDS["fp16"], (40, 64, 200)
+    x, gate, up, g, u, dh = fp16_operands(shape, "large")
+    for v in backward(ctx, kind, "silu", x, gate, up, g, u, 0 * dh):
+        assert not kind.wide(v).any()
+    dh[2, 4], dh[7, 9] = np.inf, np.nan
+    got = [kind.wide(v) for v in backward(ctx, kind, "silu", x, gate, up, g, u, dh)]
+    dh[2, 4], dh[7, 9] = 0, 0
+    want = held_gradients(x, gate, up, g, u, dh, largest(g, u, dh))
+    for v, w, spoilt in zip(got, want, ((2, 7), (4, 9), (4, 9))):
+        fine = np.setdiff1d(np.arange(len(v)), spoilt)
+        assert not np.isfinite(v[list(spoilt)]).any()
+        near(v[fine], (w[0][fine], w[1][fine]))
+
+
+def test_graph_of_fp16_gradients_finds_the_range_of_every_replay():
+    kind, (m, d, f) = KINDS["fp16"], (90, 200, 136)
+    ctx, new = Context(0), lambda *s: torch.empty(*s, device="cuda", dtype=torch.float16)
+    try:
+        stream = torch.cuda.current_stream()
+        ctx.set_stream(stream.cuda_stream)
+        held, out = [new(m, d), new(f, d), new(f, d), new(m, f), new(m, f), new(m, f)], [new(m, d), new(f, d), new(f, d)]
+        desc = ctx.gated_ffn_desc(kind.dtype, capi.ACT_SILU, m, d, f)
+        fill = lambda about, seed: [t.copy_(torch.from_numpy(v)) for t, v in zip(held, fp16_operands((m, d, f), about, seed))]  # noqa: E731
+        fill("ordinary", 0)
+        ctx.gated_ffn_backward(desc, *held, *out)
+        assert ctx.sync() == capi.VALID
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        side.wait_stream(stream)
+        with torch.cuda.graph(graph, stream=side):
+            ctx.set_stream(side.cuda_stream)
+            ctx.gated_ffn_backward(desc, *held, *out)
+        ctx.set_stream(stream.cuda_stream)
+        for seed, about in enumerate(("large", "ordinary", "tiny", "outlier", "ordinary", "tiny", "large")):
+            fill(about, seed)
+            ctx.gated_ffn_backward(desc, *held, *out)
+            assert ctx.sync() == capi.VALID
+            want = [t.clone() for t in out]
+            for t in out:
+                t.fill_(77)
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(out, want):
+                assert torch.isfinite(b).all() and torch.equal(a, b)
+    finally:
+        ctx.close()
