@@ -7,7 +7,7 @@ import pytest
 
 import ffn_reference as ref
 from reference_model_amd import Context, capi
-from test_gpu_gated_ffn import KINDS, backward, near
+from test_gpu_gated_ffn import KINDS, Rows, backward, forward, near
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -168,3 +168,56 @@ def test_graph_of_fp16_gradients_finds_the_range_of_every_replay():
                 assert torch.isfinite(b).all() and torch.equal(a, b)
     finally:
         ctx.close()
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_pack_given_values_of_both_types(ctx, kind, group):
+    """rows that lie apart and side by side, infinite and NaN scales as they are, one row and column past whole tiles"""
+    kind, rng = KINDS[kind], np.random.default_rng(group)
+    for (n, k), gap in (((33, 257), 7), ((16, 128), 0), ((1, 1), 3)):
+        v, scales = rng.integers(-8, 8, (n, k)), kind.narrow(rng.normal(0, 1, (n, -(-k // group))))
+        scales[0, 0] = kind.narrow([np.inf])[0]
+        scales[-1, -1] = kind.narrow([np.nan])[0]
+        wide = np.full((n, k + gap), 99, np.int8)
+        wide[:, :k] = v
+        held, stored = ctx.upload(wide), ctx.upload(scales, kind.dtype)
+        want = ref.packed(kind, v, scales, group)
+        to = ctx.upload(np.full(want.size + 16, 0xA5, np.uint8))
+        ctx.pack_int4(ctx.int4_desc(kind.dtype, group, n, k), held, k + gap if gap else 0, stored, to)
+        assert ctx.sync() == capi.VALID
+        got = to.numpy().view(np.uint8)
+        assert np.array_equal(got[:want.size], want) and (got[want.size:] == 0xA5).all()
+        for t in (held, stored, to):
+            t.free()
+
+
+@pytest.mark.parametrize("rows", [1, 20, 70])
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_products_of_no_columns_and_of_no_rows(ctx, kind, rows):
+    """sums of nothing with 4-bit weights are 0 on the kernels of few and of more rows"""
+    kind, out = KINDS[kind], Rows(ctx, KINDS[kind], (rows, 40))
+    desc = ctx.int4_desc(kind.dtype, 64, 40, 0)
+    ctx.matvec_int4(desc, rows, None, 0, None, out.at, 0)
+    assert ctx.sync() == capi.VALID and not out.values().any()
+    again = Rows(ctx, kind, (rows, 40))
+    ctx.gated_ffn_int4(desc, capi.ACT_SIGMOID, rows, None, 0, None, None, again.at, 0)
+    assert ctx.sync() == capi.VALID and not again.values().any()
+
+
+@pytest.mark.parametrize("rows", [3, 70])
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_subnormal_operands_count(ctx, kind, rows):
+    """x below the least normal number of its type, weights that bring the sums back"""
+    kind, rng = KINDS[kind], np.random.default_rng(rows)
+    least, k, n = (2.0 ** -133, 72, 24) if kind.bf16 else (2.0 ** -24, 72, 24)
+    x = rng.integers(-60, 61, (rows, k)) * least    # exact
+    gate, up = (kind.wide(kind.narrow(rng.normal(0, 2.0 ** 60 if kind.bf16 else 100, (n, k)))) for _ in range(2))
+    for v, want in zip(forward(ctx, kind, "relu", x, gate, up)[1:], ref.gated(kind, "relu", x, gate, up)[1:]):
+        near(kind.wide(v), want)
+        assert (np.abs(want[0]) > 4 * want[1]).mean() > 0.9
+    v, scales = rng.integers(-8, 8, (n, k)), kind.narrow(rng.uniform(0.5, 1, (n, 3)) * (2.0 ** 60 if kind.bf16 else 100))
+    dev, held, out = Rows(ctx, kind, (rows, k), x), ctx.upload(ref.packed(kind, v, scales, 32)), Rows(ctx, kind, (rows, n))
+    ctx.matvec_int4(ctx.int4_desc(kind.dtype, 32, n, k), rows, dev.at, 0, held, out.at, 0)
+    assert ctx.sync() == capi.VALID
+    near(out.values(), ref.product(kind, x, ref.weights(kind, v, scales, 32)))
