@@ -398,8 +398,8 @@ int tmi_dot_product_check(tmi_ctx_t* ctx, int32_t out_dtype, int64_t n, const vo
  * TMI_ERROR with a message before anything is launched, launches on the context's stream and no wait.  Element type
  * (dtype) TMI_FP16 or TMI_BF16 for every tensor that is not packed; tensors are aligned to their elements at least (16
  * bytes for packed weights), rows may lie any number of elements apart.  Products are summed in 32 bits and results
- * rounded once, to nearest with ties to even.  Equal calls give equal bits.  A call with no rows, or no features
- * to write, does nothing.
+ * rounded once, to nearest with ties to even.  Equal calls give equal bits.  A call with no elements to write does
+ * nothing; one whose sums have no terms writes zeros (or act(0) * 0).
  *
  * Some calls use the context's scratch buffer (tmi_ctx_reserve_workspace; the rules for graphs and for several of them are
  * those of every call that does): tmi_gated_ffn_backward always; tmi_gated_ffn, tmi_matvec_int4 and tmi_gated_ffn_int4 for partial
@@ -438,9 +438,11 @@ int tmi_gated_ffn(tmi_ctx_t* ctx, const tmi_gated_ffn_desc_t* d, const void* x_d
 /* Its gradients, from the pre-activations g and u and the gradient dh of h:
  *   du = dh act(g), dg = dh u act'(g), d_x = dg gate + du up, d_gate = dg^T x, d_up = du^T x
  * in 32 bits, with dg and du rounded to dtype before the products; in fp16 times a power of two where the largest of
- * them lies beyond its range or below 2^-8, so that nothing is lost but their rounding and less than 2^-17 of the largest.  d_x_dev NULL, or d_gate_dev and d_up_dev both NULL:
- * that part is not computed (x_dev, or gate_dev and up_dev, may then be NULL).  dg and du live in the scratch buffer, 4
- * (rows) (hidden_features up to whole 64s) bytes, 128 more a row and 8256 in fp16, with partial sums and copies as above. */
+ * them lies beyond its range or below 2^-8, so that nothing is lost but their rounding and less than 2^-17 of the
+ * largest.  d_x_dev NULL, or d_gate_dev and d_up_dev both NULL: that part is not computed (x_dev, or gate_dev and up_dev,
+ * may then be NULL).  A gradient that is asked for and has elements is always written: with no rows d_gate and d_up,
+ * with no hidden features d_x, are filled with zeros.  dg and du live in the scratch buffer, 4 (rows) (hidden_features up
+ * to whole 64s) bytes, 128 more a row and 8256 in fp16, with partial sums and copies as above. */
 int tmi_gated_ffn_backward(tmi_ctx_t* ctx, const tmi_gated_ffn_desc_t* d, const void* x_dev, const void* gate_dev,
                            const void* up_dev, const void* pre_gate_dev, const void* pre_up_dev, const void* d_h_dev,
                            void* d_x_dev, void* d_gate_dev, void* d_up_dev);
@@ -477,7 +479,7 @@ int tmi_dequantize_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, const void* pa
 
 /* y = x w^T for a few rows of x (single tokens): y[m][n] = sum_k x[m][k] w[n][k], x [rows][in_features] rows ld_x apart, y
  * [rows][out_features] rows ld_y apart.  Any number of rows is taken; the weights are read once for every 16, 32 or 64 of
- * them. */
+ * them.  Products are summed over a group before its scale multiplies them. */
 int tmi_matvec_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, int32_t rows, const void* x_dev, int64_t ld_x, const void* packed_dev,
                     void* y_dev, int64_t ld_y);
 

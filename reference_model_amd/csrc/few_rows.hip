@@ -8,7 +8,8 @@
 // 16x16x32 instructions take the rows of x as first operand and the weights as second: a single row wastes 15/16 of the matrix cores, which at 512
 // weights an instruction still run four times as many weights as HBM delivers, and any other number of rows up to 16 costs the same.  4-bit
 // weights become 16-bit integers (exact; 8 or 13 instructions for eight), their products are summed in 32 bits, and the sum over a group is
-// multiplied by its scale: no weight is rounded, and an infinite or NaN x does to a row what it does in the formula.
+// multiplied by its scale: no weight is rounded, and an infinite or NaN x does to a row what it does in the formula.  (The sum of a group comes before
+// its scale: bf16 x from 5e36 on may overflow in it where x times the scaled weights would not, and given scales that are infinite meet the sum.)
 //
 // Two kernels share this.  In both, what the waves of a workgroup have summed meets in LDS in the order of the waves, so equal calls give equal bits.
 //
@@ -506,7 +507,7 @@ constexpr int kInFlight = GATED && MT > 1 ? 2 : 4;
 // What a call costs by its parts' rates, in us: the bytes of weights and x that the busiest CU takes in at 64 a clock, those that L2 gives out at 10 TB/s
 // and HBM at 6, and the vector instructions of its four SIMDs: a weight tile takes 320 clocks to unpack in bf16 and 250 in fp16, 24 for each group's
 // scale and 40 of products for each row tile, and a turn's empty places a fifth of that; 8 % of what does not bound, 1.5 us for every reading of x and 1
-// for every block.  Over 13 sizes and all their plans (8 and 16 waves, every split, 1 to 4 row tiles) its choice is within 1 % of the best on average, 3.4 % at most.
+// for every block.  Over 13 sizes and all their plans (8 and 16 waves, every split, 1, 2 and 4 row tiles) its choice is within 1 % of the best on average, 3.4 % at most.
 template <typename T, int PER, int MT, bool GATED>
 double plan(RowsArgs& a, int& waves)
 {
