@@ -567,7 +567,8 @@ __global__ __launch_bounds__(64 * WC * WR, 2) void gated_gemm_kernel(GemmFfnArgs
 }
 
 // d_x and the weights' gradients side by side in tiles of 128 x 128, where neither fills the chip: the first dx.per_xcd * 8 workgroups are d_x's.  us of both
-// gradients together and one after the other: 509 x 722 x 1930 in fp16 31 and 50, 509 x 720 x 1930 26 and 38, 64 x 512 x 2048 16 and 22.
+// gradients together and one after the other: 509 x 722 x 1930 in fp16 31 and 50 (2 to 3 more on either side for the second pass over dp), 509 x 720 x 1930 26 and
+// 38, 64 x 512 x 2048 16 and 22.
 template <typename T, bool DIRECT>
 __global__ __launch_bounds__(512, 2) void gated_gradients_kernel(GemmFfnArgs dx, GemmFfnArgs dw)
 {
