@@ -487,6 +487,69 @@ int tmi_matvec_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, int32_t rows, cons
 int tmi_gated_ffn_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, int32_t activation, int32_t rows, const void* x_dev, int64_t ld_x,
                        const void* gate_dev, const void* up_dev, void* h_dev, int64_t ld_h);
 
+/* ---- the way into a projection: root-mean-square norm, rows in 8 bits, the linear layer on them -----------
+ *
+ * Operators beside TOSA's, with no counterpart in the reference, under the conventions of the feed-forward operators above.
+ * dtype is TMI_FP16, TMI_BF16 or TMI_FP32, the type of every tensor that is said to have none of its own; tensors begin at any
+ * element, and rows lie any number of elements apart.  Sums, statistics and scales are held in 32 bits, results rounded
+ * once.  Equal calls give equal bits.
+ *
+ * A row in 8 bits is v[k] = scale * q[k], scale = max |v| / 127 in 32 bits, q = 127 v / max |v| rounded to the nearest integer (halves to even
+ * where v are 16-bit numbers; others within 2^-16 of a half to either side).  A row of zeros has scale 0; a row with an infinity or NaN has a scale
+ * that is infinite or NaN, and q = 0; max |v| below 2^-119 counts as 0.  Rows of q begin at multiples of 16 bytes: the tensor is aligned to
+ * 16 and its stride a multiple of 16 (0: the width, up to the next multiple).  The bytes that fill up a row's last 16 are zeros: the
+ * operators that write rows write them, and tmi_linear_int8 counts them as columns. */
+
+/* Row strides count elements, 0 means that rows lie side by side: ld_x for x, ld_residual for the residual, ld_sum for the sum and ld_y for the
+ * result.  Gradients have the strides of their tensors. */
+typedef struct
+{
+    int64_t ld_x, ld_residual, ld_sum, ld_y;
+    int32_t dtype;
+    int32_t rows, width;
+    float eps;           /* not negative */
+    float weight_offset; /* 0, or 1 where weights are stored as what they differ from 1 by */
+} tmi_rms_norm_desc_t;
+
+/* s = x + residual, y = s r (weight_offset + weight), r = 1 / sqrt(mean of s^2 over the row + eps).  residual_dev NULL: s = x.  sum_dev (or NULL)
+ * receives s rounded to dtype; y is computed from s before that.  rstd_dev (or NULL) receives r in 32 bits for
+ * tmi_rms_norm_backward.  sum may be x or the residual, y may be x or the residual or both; else no result overlaps an input. */
+int tmi_rms_norm(tmi_ctx_t* ctx, const tmi_rms_norm_desc_t* d, const void* x_dev, const void* residual_dev, const void* weight_dev, void* sum_dev,
+                 void* y_dev, float* rstd_dev);
+
+/* The same with y in 8 bits: q_dev, rows ld_y bytes apart, and scales_dev [rows]. */
+int tmi_rms_norm_int8(tmi_ctx_t* ctx, const tmi_rms_norm_desc_t* d, const void* x_dev, const void* residual_dev, const void* weight_dev, void* sum_dev,
+                      int8_t* q_dev, float* scales_dev);
+
+/* Gradients of tmi_rms_norm from that of y.  s_dev: the sum that was normed (x where there was no residual), rows ld_sum apart, rstd_dev as
+ * tmi_rms_norm left it.  With n = s r and g = dy (weight_offset + weight):
+ *   d_x = r (g - n mean(g n)) + d_sum, d_weight = sum over the rows of dy n
+ * d_sum_dev (or NULL): the gradient that comes to s from elsewhere.  d_x is the gradient of x and of the residual.  d_x_dev or d_weight_dev NULL:
+ * not computed.  d_x may be s, dy or d_sum.  With no rows d_weight is filled with zeros.  d_weight's sums meet in the context's
+ * scratch buffer (up to 2 MiB for every 1024 columns). */
+int tmi_rms_norm_backward(tmi_ctx_t* ctx, const tmi_rms_norm_desc_t* d, const void* s_dev, const void* weight_dev, const float* rstd_dev,
+                          const void* d_y_dev, const void* d_sum_dev, void* d_x_dev, void* d_weight_dev);
+
+/* Rows of x_dev, ld_x elements apart, into 8 bits, and back. */
+int tmi_quantize_int8(tmi_ctx_t* ctx, int32_t dtype, int32_t rows, int32_t width, const void* x_dev, int64_t ld_x, int8_t* q_dev, int64_t ld_q,
+                      float* scales_dev);
+int tmi_dequantize_int8(tmi_ctx_t* ctx, int32_t dtype, int32_t rows, int32_t width, const int8_t* q_dev, int64_t ld_q, const float* scales_dev, void* x_dev,
+                        int64_t ld_x);
+
+/* y[m][n] = x_scales[m] w_scales[n] sum_k x[m][k] w[n][k] + bias[n]: x [rows][in_features] and w [out_features][in_features] in 8 bits, y
+ * [rows][out_features] and bias (or NULL) of dtype.  ld_x and ld_w count bytes, ld_y elements.  The sum is exact: in_features is at most
+ * 131071.  It is rounded to 32 bits before it is scaled.  Some calls of more than 64 rows use the context's scratch buffer for partial sums; where it
+ * cannot grow (while a graph is captured) they go on without it, to the same bits. */
+typedef struct
+{
+    int64_t ld_x, ld_w, ld_y;
+    int32_t dtype;
+    int32_t rows, in_features, out_features;
+} tmi_linear_int8_desc_t;
+
+int tmi_linear_int8(tmi_ctx_t* ctx, const tmi_linear_int8_desc_t* d, const int8_t* x_dev, const float* x_scales_dev, const int8_t* w_dev,
+                    const float* w_scales_dev, const void* bias_dev, void* y_dev);
+
 /* ---- validation only (no launch) ---------------------------------------------------------------- */
 
 /* The checks OpConv2d / OpDepthwiseConv2d::checkTensorAttributes and the head of eval() perform

@@ -40,6 +40,7 @@ EXPORTS = [
     "tmi_ctx_set_precise_mode", "tmi_ctx_workspace_bytes", "tmi_ctx_trim_workspace",
     "tmi_int4_packed_bytes", "tmi_quantize_int4", "tmi_pack_int4", "tmi_dequantize_int4", "tmi_matvec_int4", "tmi_gated_ffn_int4",
     "tmi_gated_ffn", "tmi_gated_ffn_backward",
+    "tmi_rms_norm", "tmi_rms_norm_int8", "tmi_rms_norm_backward", "tmi_quantize_int8", "tmi_dequantize_int8", "tmi_linear_int8",
     "tmi_debug_launch_empty", "tmi_debug_tile_decode", "tmi_debug_last_launch_shape", "tmi_debug_stream", "tmi_debug_gated_ffn_plan",
 ]
 
@@ -117,6 +118,16 @@ class GatedFfnDesc(ctypes.Structure):
 
 class Int4Desc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "group", "out_features", "in_features")]
+
+
+class RmsNormDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("ld_x", "ld_residual", "ld_sum", "ld_y")] + [
+        (n, ctypes.c_int32) for n in ("dtype", "rows", "width")] + [(n, ctypes.c_float) for n in ("eps", "weight_offset")]
+
+
+class LinearInt8Desc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("ld_x", "ld_w", "ld_y")] + [
+        (n, ctypes.c_int32) for n in ("dtype", "rows", "in_features", "out_features")]
 
 
 class TmiError(RuntimeError):
@@ -198,6 +209,13 @@ def load_library() -> ctypes.CDLL:
     lib.tmi_dequantize_int4.argtypes = [vp, int4, vp, vp, i64]
     lib.tmi_matvec_int4.argtypes = [vp, int4, i32, vp, i64, vp, vp, i64]
     lib.tmi_gated_ffn_int4.argtypes = [vp, int4, i32, i32, vp, i64, vp, vp, vp, i64]
+    norm = ctypes.POINTER(RmsNormDesc)
+    lib.tmi_rms_norm.argtypes = [vp, norm] + [vp] * 6
+    lib.tmi_rms_norm_int8.argtypes = [vp, norm] + [vp] * 6
+    lib.tmi_rms_norm_backward.argtypes = [vp, norm] + [vp] * 7
+    lib.tmi_quantize_int8.argtypes = [vp, i32, i32, i32, vp, i64, vp, i64, vp]
+    lib.tmi_dequantize_int8.argtypes = [vp, i32, i32, i32, vp, i64, vp, vp, i64]
+    lib.tmi_linear_int8.argtypes = [vp, ctypes.POINTER(LinearInt8Desc)] + [vp] * 6
     lib.tmi_conv2d_check.argtypes = [vp, ctypes.POINTER(ConvDesc), i32]
     lib.tmi_rescale_check.argtypes = [vp, ctypes.POINTER(RescaleDesc), i32, i32]
     for name in EXPORTS:
@@ -211,7 +229,7 @@ def load_library() -> ctypes.CDLL:
         _calls = None
     if _calls:
         _calls.install(Context, DeviceTensor, TmiError, ctypes.ArgumentError, ConvDesc, TconvDesc, Conv3dDesc, PoolDesc, RescaleDesc,
-                       GatedFfnDesc, Int4Desc)
+                       GatedFfnDesc, Int4Desc, RmsNormDesc, LinearInt8Desc)
     _lib = lib
     return lib
 
@@ -469,6 +487,42 @@ class Context:
         return self._check(self.lib.tmi_gated_ffn_int4(self.handle, ctypes.byref(d), activation, rows, _ptr(x), ld_x, _ptr(gate), _ptr(up),
                                                        _ptr(h), ld_h))
 
+    # -- the way into a projection: the norm, rows in 8 bits, the linear layer on them ------------
+    # A row in 8 bits is scale * q; rows of q begin at multiples of 16 bytes, filled up with zeros (stride 0: the width, up to the next multiple).
+    @staticmethod
+    def rms_norm_desc(dtype, rows, width, eps, weight_offset=0.0, ld_x=0, ld_residual=0, ld_sum=0, ld_y=0) -> RmsNormDesc:
+        return RmsNormDesc(ld_x, ld_residual, ld_sum, ld_y, dtype, rows, width, eps, weight_offset)
+
+    @staticmethod
+    def linear_int8_desc(dtype, rows, in_features, out_features, ld_x=0, ld_w=0, ld_y=0) -> LinearInt8Desc:
+        return LinearInt8Desc(ld_x, ld_w, ld_y, dtype, rows, in_features, out_features)
+
+    def rms_norm(self, d: RmsNormDesc, x, residual, weight, sum, y, rstd=None) -> int:
+        """y = s / rms(s) * (weight_offset + weight), s = x + residual (None: x); sum and rstd (None: not kept) receive s and 1 / rms(s)"""
+        return self._check(self.lib.tmi_rms_norm(self.handle, ctypes.byref(d), _ptr(x), _ptr(residual), _ptr(weight), _ptr(sum), _ptr(y),
+                                                 _ptr(rstd)))
+
+    def rms_norm_int8(self, d: RmsNormDesc, x, residual, weight, sum, q, scales) -> int:
+        """rms_norm with y in 8 bits"""
+        return self._check(self.lib.tmi_rms_norm_int8(self.handle, ctypes.byref(d), _ptr(x), _ptr(residual), _ptr(weight), _ptr(sum), _ptr(q),
+                                                      _ptr(scales)))
+
+    def rms_norm_backward(self, d: RmsNormDesc, s, weight, rstd, d_y, d_sum, d_x, d_weight) -> int:
+        """the gradients of x (and the residual) and weight (None: not computed) from those of y and sum (None: it has no other use)"""
+        return self._check(self.lib.tmi_rms_norm_backward(self.handle, ctypes.byref(d), _ptr(s), _ptr(weight), _ptr(rstd), _ptr(d_y), _ptr(d_sum),
+                                                          _ptr(d_x), _ptr(d_weight)))
+
+    def quantize_int8(self, dtype, rows, width, x, ld_x, q, ld_q, scales) -> int:
+        return self._check(self.lib.tmi_quantize_int8(self.handle, dtype, rows, width, _ptr(x), ld_x, _ptr(q), ld_q, _ptr(scales)))
+
+    def dequantize_int8(self, dtype, rows, width, q, ld_q, scales, x, ld_x) -> int:
+        return self._check(self.lib.tmi_dequantize_int8(self.handle, dtype, rows, width, _ptr(q), ld_q, _ptr(scales), _ptr(x), ld_x))
+
+    def linear_int8(self, d: LinearInt8Desc, x, x_scales, w, w_scales, bias, y) -> int:
+        """y = x_scales * w_scales * (x w^T) + bias (None: without)"""
+        return self._check(self.lib.tmi_linear_int8(self.handle, ctypes.byref(d), _ptr(x), _ptr(x_scales), _ptr(w), _ptr(w_scales), _ptr(bias),
+                                                    _ptr(y)))
+
     def stream_probe(self, mode, src, dst, nbytes) -> int:
         return self._check(self.lib.tmi_debug_stream(self.handle, mode, _ptr(src), _ptr(dst), nbytes))
 
@@ -496,6 +550,9 @@ PLAIN_OPERATORS = {name: vars(Context)[name] for name in (
 
 PLAIN_FEED_FORWARD = {name: vars(Context)[name] for name in (
     "gated_ffn", "gated_ffn_backward", "quantize_int4", "dequantize_int4", "matvec_int4", "gated_ffn_int4")}
+
+PLAIN_PROJECTION = {name: vars(Context)[name] for name in (
+    "rms_norm", "rms_norm_int8", "rms_norm_backward", "quantize_int8", "dequantize_int8", "linear_int8")}
 
 
 def _stored(zp: int, dtype: int) -> int:

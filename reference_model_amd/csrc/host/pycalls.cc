@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <tuple>
+#include <type_traits>
 #include <utility>
 
 #include "tosa_mi355.h"
@@ -99,7 +100,20 @@ bool convert(PyObject* x, void*& v, Buffers& b)
     return true;
 }
 
-template <typename D>
+// the same where the entry point names the elements' type
+template <typename E>
+constexpr bool kElement = std::is_same_v<std::remove_const_t<E>, float> || std::is_same_v<std::remove_const_t<E>, int8_t>;
+template <typename E, std::enable_if_t<kElement<E>, int> = 0>
+bool convert(PyObject* x, E*& v, Buffers& b)
+{
+    const void* p;
+    if (!convert(x, p, b))
+        return false;
+    v = static_cast<E*>(const_cast<void*>(p));
+    return true;
+}
+
+template <typename D, std::enable_if_t<!kElement<D>, int> = 0>
 bool convert(PyObject* x, const D*& v, Buffers& b)
 {
     if (!PyObject_TypeCheck(x, (PyTypeObject*)g_desc<D>))
@@ -301,6 +315,13 @@ const char* const kDequant[] = { "self", "d", "packed", "w", "ld_w" };
 const char* const kMatvec[]  = { "self", "d", "rows", "x", "ld_x", "packed", "y", "ld_y" };
 const char* const kFfnInt4[] = { "self", "d", "activation", "rows", "x", "ld_x", "gate", "up", "h", "ld_h" };
 
+const char* const kNorm[]     = { "self", "d", "x", "residual", "weight", "sum", "y", "rstd" };
+const char* const kNormInt8[] = { "self", "d", "x", "residual", "weight", "sum", "q", "scales" };
+const char* const kNormBack[] = { "self", "d", "s", "weight", "rstd", "d_y", "d_sum", "d_x", "d_weight" };
+const char* const kQuant8[]   = { "self", "dtype", "rows", "width", "x", "ld_x", "q", "ld_q", "scales" };
+const char* const kDequant8[] = { "self", "dtype", "rows", "width", "q", "ld_q", "scales", "x", "ld_x" };
+const char* const kLinear8[]  = { "self", "d", "x", "x_scales", "w", "w_scales", "bias", "y" };
+
 PyMethodDef g_methods[] = {
     op<tmi_conv2d>("conv2d", kConv, "conv2d($self, d, inp, w, bias, in_zp, w_zp, out)\n--\n\nCONV2D; d: ConvDesc"),
     op<tmi_depthwise_conv2d>("depthwise_conv2d", kConv, "depthwise_conv2d($self, d, inp, w, bias, in_zp, w_zp, out)\n--\n\nDEPTHWISE_CONV2D; d: ConvDesc"),
@@ -321,6 +342,15 @@ PyMethodDef g_methods[] = {
     op<tmi_matvec_int4>("matvec_int4", kMatvec, "matvec_int4($self, d, rows, x, ld_x, packed, y, ld_y)\n--\n\ny = x w^T for a few rows of x; d: Int4Desc"),
     op<tmi_gated_ffn_int4>("gated_ffn_int4", kFfnInt4,
                            "gated_ffn_int4($self, d, activation, rows, x, ld_x, gate, up, h, ld_h)\n--\n\nthe gated block on 4-bit weights; d: Int4Desc"),
+    op<tmi_rms_norm, 1>("rms_norm", kNorm, "rms_norm($self, d, x, residual, weight, sum, y, rstd=None)\n--\n\n"
+                                           "y = s / rms(s) * (weight_offset + weight), s = x + residual; d: RmsNormDesc; sum and rstd receive s and 1 / rms(s)"),
+    op<tmi_rms_norm_int8>("rms_norm_int8", kNormInt8, "rms_norm_int8($self, d, x, residual, weight, sum, q, scales)\n--\n\nrms_norm with y in 8 bits; d: RmsNormDesc"),
+    op<tmi_rms_norm_backward>("rms_norm_backward", kNormBack, "rms_norm_backward($self, d, s, weight, rstd, d_y, d_sum, d_x, d_weight)\n--\n\n"
+                                                              "the gradients of x and weight (None: not computed) from those of y and sum; d: RmsNormDesc"),
+    op<tmi_quantize_int8>("quantize_int8", kQuant8, "quantize_int8($self, dtype, rows, width, x, ld_x, q, ld_q, scales)\n--\n\nrows into 8 bits"),
+    op<tmi_dequantize_int8>("dequantize_int8", kDequant8, "dequantize_int8($self, dtype, rows, width, q, ld_q, scales, x, ld_x)\n--\n\nrows from 8 bits"),
+    op<tmi_linear_int8>("linear_int8", kLinear8, "linear_int8($self, d, x, x_scales, w, w_scales, bias, y)\n--\n\n"
+                                                 "y = x_scales * w_scales * (x w^T) + bias on 8-bit rows; d: LinearInt8Desc"),
     { "conv2d_rescale_clamp", (PyCFunction)(void (*)())run_conv_fused, METH_FASTCALL | METH_KEYWORDS,
       "conv2d_rescale_clamp($self, d, inp, w, bias, in_zp, w_zp, r, mult, shift, out, clamp=None)\n--\n\nCONV2D + RESCALE (+ CLAMP)" },
     { "depthwise_conv2d_rescale_clamp", (PyCFunction)(void (*)())run_depthwise_fused, METH_FASTCALL | METH_KEYWORDS,
@@ -328,19 +358,23 @@ PyMethodDef g_methods[] = {
       "DEPTHWISE_CONV2D + RESCALE (+ CLAMP)" },
 };
 
-// install(Context, DeviceTensor, TmiError, ctypes.ArgumentError, ConvDesc, TconvDesc, Conv3dDesc, PoolDesc, RescaleDesc, GatedFfnDesc, Int4Desc):
+// install(Context, DeviceTensor, TmiError, ctypes.ArgumentError, ConvDesc, TconvDesc, Conv3dDesc, PoolDesc, RescaleDesc, GatedFfnDesc, Int4Desc,
+// RmsNormDesc, LinearInt8Desc):
 // the operators become methods of Context
 PyObject* install(PyObject*, PyObject* args)
 {
     PyObject *context, **kept[] = { &g_tensor, &g_error, &g_argument_error, &g_desc<tmi_conv_desc_t>, &g_desc<tmi_tconv_desc_t>,
                                     &g_desc<tmi_conv3d_desc_t>, &g_desc<tmi_pool_desc_t>, &g_desc<tmi_rescale_desc_t>,
-                                    &g_desc<tmi_gated_ffn_desc_t>, &g_desc<tmi_int4_desc_t> };
-    PyObject* got[10];
-    if (!PyArg_ParseTuple(args, "OOOOOOOOOOO", &context, &got[0], &got[1], &got[2], &got[3], &got[4], &got[5], &got[6], &got[7], &got[8], &got[9]))
+                                    &g_desc<tmi_gated_ffn_desc_t>, &g_desc<tmi_int4_desc_t>, &g_desc<tmi_rms_norm_desc_t>,
+                                    &g_desc<tmi_linear_int8_desc_t> };
+    PyObject* got[12];
+    if (!PyArg_ParseTuple(args, "OOOOOOOOOOOOO", &context, &got[0], &got[1], &got[2], &got[3], &got[4], &got[5], &got[6], &got[7], &got[8], &got[9],
+                          &got[10], &got[11]))
         return nullptr;
     const Py_ssize_t sizes[] = { sizeof(tmi_conv_desc_t), sizeof(tmi_tconv_desc_t), sizeof(tmi_conv3d_desc_t), sizeof(tmi_pool_desc_t),
-                                 sizeof(tmi_rescale_desc_t), sizeof(tmi_gated_ffn_desc_t), sizeof(tmi_int4_desc_t) };
-    for (int i = 0; i < 10; i++)
+                                 sizeof(tmi_rescale_desc_t), sizeof(tmi_gated_ffn_desc_t), sizeof(tmi_int4_desc_t),
+                                 sizeof(tmi_rms_norm_desc_t), sizeof(tmi_linear_int8_desc_t) };
+    for (int i = 0; i < 12; i++)
     {
         if (!PyType_Check(got[i]))
             return PyErr_Format(PyExc_TypeError, "install: argument %d is no type", i + 2), nullptr;

@@ -1,0 +1,441 @@
+// The root-mean-square norm with the residual's addition, in 16 or 32 bits or straight into 8 bits, and rows into 8 bits and back:
+//
+//   s = x + residual                 sum = s, rounded
+//   r = 1 / sqrt(mean(s^2) + eps)    over a row
+//   y = s r (offset + w)
+//   8 bits: scale = max |y| / 127, q = y / scale, rounded (or of x itself, without a norm)
+//
+// Bound by memory: a row is read once into registers, everything is done there, and it is written once.  In 8 bits r is in no element: max |y| is
+// r max |s (offset + w)|, so the one trip over the lanes that adds the squares finds the maximum too, q is s (offset + w) times 127 over that
+// maximum, and r only enters the scale.
+//
+// A row has 16 or 64 lanes of a wave, 256 or 1024 of a workgroup, each with P pieces of 16 bytes; longer rows are read a second time (norm_long_kernel).
+//
+// Squares and products may leave the range of 32 bits where the results do not: bf16 and 32-bit rows whose sum overflows, or is so small that digits are
+// lost, are taken again times a power of two.  That is decided for a row as a whole, from what the reduction found.
+#include "tmi_rows.h"
+
+namespace tmi
+{
+namespace
+{
+
+enum
+{
+    NORM,         // y
+    NORM_INT8,    // y in 8 bits
+    INT8          // x in 8 bits
+};
+
+struct NormArgs
+{
+    const void *x, *residual, *weight;
+    void *sum, *out;
+    float* of_row;    // 1 / rms, or the scales
+    int64_t ld_x, ld_residual, ld_sum, ld_out;
+    int64_t rows;
+    int32_t width;
+    float eps, offset;
+};
+
+constexpr float kSmall = 0x1p-80f, kUp = 0x1p100f, kDown = 0x1p-80f;
+
+// What a row's elements are multiplied by before they are taken again; 1: they are fine as they are.  `squares` and `most` as the lanes found them.
+template <typename T, int MODE>
+__device__ __forceinline__ float again_by(float squares, uint32_t most, float eps)
+{
+    if constexpr (sizeof(T) == 2 && !__is_same(T, bf16_t))
+        return 1.0f;    // fp16: squares up to 2^34 and products up to 2^33, down to 2^-48
+    else
+    {
+        const float m = __uint_as_float(most);
+        if ((MODE != INT8 && !(squares < __builtin_huge_valf())) || (MODE == NORM_INT8 && !(m < __builtin_huge_valf())))
+            return kDown;
+        if ((MODE != INT8 && squares < kSmall && eps < kSmall) || (MODE != NORM && m < kSmall && squares < 0x1p40f))
+            return kUp;
+        return 1.0f;
+    }
+}
+
+// whether products of this size need no other units
+__device__ __forceinline__ bool fine(uint32_t most)
+{
+    return __uint_as_float(most) >= kSmall && __uint_as_float(most) < __builtin_huge_valf();
+}
+
+// What becomes of a row once its sum and maximum are known
+struct OfRow
+{
+    float times;     // NORM: r; else 127 / max |y| over r, 0 where there is no such number
+    float stored;    // 1 / rms or the scale
+};
+// `by`: the row was multiplied by it for the squares, and for the maximum by the same unless `own` (that one is the first); `first`: the sum of squares before
+template <int MODE>
+__device__ __forceinline__ OfRow of_row(float squares, uint32_t most, float by, float first, bool own, int width, float eps)
+{
+    float r = 1.0f;
+    if constexpr (MODE != INT8)
+    {
+        // (the squares may have been fine where the products were not, or count for nothing beside eps; times by^2 either may be infinite)
+        if (first < __builtin_huge_valf() && (first >= kSmall || eps >= kSmall))
+            r = 1.0f / __builtin_sqrtf(first / (float)width + eps) / by;
+        else
+            r = 1.0f / __builtin_sqrtf(squares / (float)width + eps * by * by);
+    }
+    if constexpr (MODE == NORM)
+        return { r, r * by };
+    const float m     = __uint_as_float(most);
+    const bool number = m > 0x1p-119f && m < __builtin_huge_valf();    // (whose reciprocal is one too)
+    // (INT8: the maximum goes back to the row's own units)
+    return { number ? 127.0f / m : 0.0f, MODE == INT8 ? m / 127.0f / by : r * m / 127.0f * (own ? by : 1.0f) };
+}
+
+// Quotients of 16-bit operands are halves now and then, and go to the even number then.  t = v times the reciprocal of the maximum (over 127) lies in [2^e,
+// 2^(e+1)) and is off by less than 1.5 2^(e-23); a quotient that is no half is 2^(e-20) from one at least: the maximum is b 2^j and v is a 2^i with a, b <
+// 2^11 and i >= j + e - 8, so that 127 v / (b 2^j) - (k + 1/2) is a multiple of 2^(i-j-1) / b.  Rounded to a multiple of 2^(e-21) halves are halves again, and no
+// other quotient crosses one.  (32-bit operands, and what the norm makes, are as seldom a half as any number.)
+template <typename T, int MODE>
+__device__ __forceinline__ uint32_t byte_of(float v, float times)
+{
+    if constexpr (MODE == INT8 && sizeof(T) == 2)
+        return to_byte(__uint_as_float((__float_as_uint(v * times) + 2) & ~3u), 1.0f);
+    else
+        return to_byte(v, times);
+}
+
+// q of one piece, eight or four bytes
+template <typename T, typename F>
+__device__ __forceinline__ void store_int8(int8_t* row, int k, int pitch, bool zero, F&& at)
+{
+    if (k >= pitch)
+        return;
+    uint32_t v[kPiece<T> / 4];
+#pragma unroll
+    for (int i = 0; i < kPiece<T> / 4; i++)
+        v[i] = zero ? 0 : four_bytes(at(4 * i), at(4 * i + 1), at(4 * i + 2), at(4 * i + 3));    // (a NaN's lowest byte may be any)
+    __builtin_memcpy(row + k, v, sizeof(v));
+}
+
+template <typename T, int MODE, int G, int P, bool WHOLE>
+__global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(NormArgs a)
+{
+    constexpr int THREADS = G > 256 ? G : 256, ROWS = THREADS / G, V = kPiece<T>;
+    constexpr bool SUM = MODE != INT8, MOST = MODE != NORM;
+    __shared__ uint32_t slots[3][2 * (G > 64 ? G / 64 : 1)];
+    const int lane = threadIdx.x % G, width = a.width, pitch = (int)whole16(width);
+
+    v4i w[P];
+    if constexpr (MODE != INT8)
+#pragma unroll
+        for (int p = 0; p < P; p++)
+            w[p] = load_piece<T, WHOLE>(static_cast<const T*>(a.weight), (p * G + lane) * V, width);
+
+    int slot = 0;
+    for (int64_t m = (int64_t)blockIdx.x * ROWS + threadIdx.x / G; m < a.rows; m += (int64_t)gridDim.x * ROWS)
+    {
+        float s[P][V];
+        const T* row = static_cast<const T*>(a.x) + m * a.ld_x;
+        v4i raw[P], more[P];
+#pragma unroll
+        for (int p = 0; p < P; p++)
+            raw[p] = load_piece<T, WHOLE>(row, (p * G + lane) * V, width);
+        if (MODE != INT8 && a.residual)
+        {
+            const T* from = static_cast<const T*>(a.residual) + m * a.ld_residual;
+#pragma unroll
+            for (int p = 0; p < P; p++)
+                more[p] = load_piece<T, WHOLE>(from, (p * G + lane) * V, width);
+        }
+        else
+#pragma unroll
+            for (int p = 0; p < P; p++)
+                more[p] = v4i{ 0, 0, 0, 0 };
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                s[p][e] = MODE != INT8 ? piece_get<T>(raw[p], e) + piece_get<T>(more[p], e) : piece_get<T>(raw[p], e);
+
+        float squares = 0.0f;
+        uint32_t most = 0;    // (bit patterns order like the numbers, and NaN above all)
+        auto weight   = [&](int p, int e) { return a.offset + piece_get<T>(w[p], e); };
+        auto look     = [&]() {
+            squares = 0.0f, most = 0;
+#pragma unroll
+            for (int p = 0; p < P; p++)
+            {
+                float part = 0.0f;
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                {
+                    if constexpr (SUM)
+                        part = __builtin_fmaf(s[p][e], s[p][e], part);
+                    if constexpr (MOST)
+                        most = max_u32(most, __float_as_uint(MODE == INT8 ? s[p][e] : s[p][e] * weight(p, e)) & 0x7FFFFFFFu);
+                }
+                squares += part;
+            }
+        };
+        look();
+        over_row<G, SUM, MOST>(squares, most, slots[slot]);
+        slot              = 1 - slot;
+        const float first = squares, by = again_by<T, MODE>(squares, most, a.eps);
+        // (the sum leaves before a row is taken again)
+        if (MODE != INT8 && a.sum)
+#pragma unroll
+            for (int p = 0; p < P; p++)
+                store_piece<T, WHOLE>(static_cast<T*>(a.sum) + m * a.ld_sum, (p * G + lane) * V, width, piece_of<T>(s[p]));
+        bool own = false;
+        if (by != 1.0f)
+        {
+            const uint32_t before = most;
+            own                   = MODE == NORM_INT8 && fine(before);
+            auto times = [&](float f) {
+#pragma unroll
+                for (int p = 0; p < P; p++)
+#pragma unroll
+                    for (int e = 0; e < V; e++)
+                        s[p][e] *= f;
+            };
+            times(by);
+            look();
+            over_row<G, SUM, MOST>(squares, most, slots[2]);
+            if (own)
+            {
+                most = before;
+                times(1.0f / by);
+            }
+        }
+        const OfRow r = of_row<MODE>(squares, most, by, first, own, width, a.eps);
+        if (a.of_row && lane == 0)
+            a.of_row[m] = r.stored;
+#pragma unroll
+        for (int p = 0; p < P; p++)
+        {
+            const int k = (p * G + lane) * V;
+            if constexpr (MODE == NORM)
+            {
+                float y[V];
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    y[e] = s[p][e] * r.times * weight(p, e);
+                store_piece<T, WHOLE>(static_cast<T*>(a.out) + m * a.ld_out, k, width, piece_of<T>(y));
+            }
+            else
+                store_int8<T>(static_cast<int8_t*>(a.out) + m * a.ld_out, k, pitch, r.times == 0.0f,
+                              [&](int e) { return byte_of<T, MODE>(MODE == INT8 ? s[p][e] : s[p][e] * weight(p, e), r.times); });
+        }
+    }
+}
+
+// Rows that no workgroup's registers hold: read once for the sum, again if it left the range, and once more for the results.  Results may take the place of what
+// is read, so here a piece is made of its own elements alone.
+template <typename T, int MODE, bool WHOLE>
+__global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a)
+{
+    constexpr int G = 1024, V = kPiece<T>;
+    constexpr bool SUM = MODE != INT8, MOST = MODE != NORM;
+    __shared__ uint32_t slots[3][2 * (G / 64)];
+    const int width = a.width, pitch = (int)whole16(width);
+    int slot = 0;
+    for (int64_t m = blockIdx.x; m < a.rows; m += gridDim.x)
+    {
+        const T *row = static_cast<const T*>(a.x) + m * a.ld_x, *from = static_cast<const T*>(a.residual) + (a.residual ? m * a.ld_residual : 0);
+        auto piece = [&](int k, float by, float* s) {
+            const v4i raw = load_piece_alone<T, WHOLE>(row, k, width);
+            v4i more      = { 0, 0, 0, 0 };
+            if (MODE != INT8 && a.residual)
+                more = load_piece_alone<T, WHOLE>(from, k, width);
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                s[e] = (MODE != INT8 ? piece_get<T>(raw, e) + piece_get<T>(more, e) : piece_get<T>(raw, e)) * by;
+        };
+        auto weights = [&](int k, float* w) {
+            v4i v = { 0, 0, 0, 0 };
+            if constexpr (MODE != INT8)
+                v = load_piece<T, WHOLE>(static_cast<const T*>(a.weight), k, width);
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                w[e] = MODE != INT8 ? a.offset + piece_get<T>(v, e) : 1.0f;
+        };
+        float squares = 0.0f;
+        uint32_t most = 0;
+        auto look     = [&](float by) {
+            squares = 0.0f, most = 0;
+            for (int k = (int)threadIdx.x * V; k < width; k += G * V)
+            {
+                float s[V], w[V];
+                piece(k, by, s);
+                if constexpr (MOST)
+                    weights(k, w);
+                float part = 0.0f;
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                {
+                    if constexpr (SUM)
+                        part = __builtin_fmaf(s[e], s[e], part);
+                    if constexpr (MOST)
+                        most = max_u32(most, __float_as_uint(s[e] * w[e]) & 0x7FFFFFFFu);
+                }
+                squares += part;
+            }
+        };
+        look(1.0f);
+        over_row<G, SUM, MOST>(squares, most, slots[slot]);
+        slot              = 1 - slot;
+        const float first = squares, by = again_by<T, MODE>(squares, most, a.eps);
+        bool own = false;
+        if (by != 1.0f)
+        {
+            const uint32_t before = most;
+            own                   = MODE == NORM_INT8 && fine(before);
+            look(by);
+            over_row<G, SUM, MOST>(squares, most, slots[2]);
+            if (own)
+                most = before;
+        }
+        const OfRow r = of_row<MODE>(squares, most, by, first, own, width, a.eps);
+        if (a.of_row && threadIdx.x == 0)
+            a.of_row[m] = r.stored;
+        for (int k = (int)threadIdx.x * V; k < (MODE == NORM ? width : pitch); k += G * V)
+        {
+            float s[V], w[V];
+            piece(k, 1.0f, s);
+            weights(k, w);
+            if (MODE != INT8 && a.sum)
+                store_piece<T, WHOLE>(static_cast<T*>(a.sum) + m * a.ld_sum, k, width, piece_of<T>(s));
+            if constexpr (MODE == NORM)
+            {
+                float y[V];
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    y[e] = s[e] * by * r.times * w[e];
+                store_piece<T, WHOLE>(static_cast<T*>(a.out) + m * a.ld_out, k, width, piece_of<T>(y));
+            }
+            else
+                store_int8<T>(static_cast<int8_t*>(a.out) + m * a.ld_out, k, pitch, r.times == 0.0f, [&](int e) { return byte_of<T, MODE>(s[e] * (own ? 1.0f : by) * w[e], r.times); });
+        }
+    }
+}
+
+// x = scale q, rounded.  2^shift lanes have a row.
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(256) void dequantize_kernel(NormArgs a, int shift)
+{
+    constexpr int V = kPiece<T>;
+    const int per   = 1 << shift, lane = threadIdx.x & (per - 1);
+    const int64_t step = (int64_t)gridDim.x * (256 >> shift);
+    for (int64_t m = (int64_t)blockIdx.x * (256 >> shift) + (threadIdx.x >> shift); m < a.rows; m += step)
+    {
+        const int8_t* row = static_cast<const int8_t*>(a.x) + m * a.ld_x;
+        T* out            = static_cast<T*>(a.out) + m * a.ld_out;
+        const float scale = a.of_row[m];
+#pragma unroll 4
+        for (int k = lane * V; k < a.width; k += per * V)
+        {
+            int8_t q[V];
+            __builtin_memcpy(q, row + k, V);    // (rows hold whole 16 bytes)
+            float v[V];
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                v[e] = scale * (float)q[e];
+            store_piece<T, WHOLE>(out, k, a.width, piece_of<T>(v));
+        }
+    }
+}
+
+template <typename F>
+void for_type(int32_t dtype, F&& f)
+{
+    if (dtype == TMI_FP16)
+        f(_Float16{});
+    else if (dtype == TMI_BF16)
+        f(bf16_t{});
+    else
+        f(float{});
+}
+template <int N>
+constexpr std::integral_constant<int, N> number_of{};
+
+// a workgroup of 1024 has room for 16 numbers a lane beside what it read them from
+template <typename T>
+constexpr int kMostPieces = 16 * 1024 / kPiece<T>;
+
+// lanes of a row and pieces of a lane, from the pieces that a row has
+template <typename T, int MODE, bool WHOLE>
+void launch_typed(hipStream_t st, const NormArgs& a)
+{
+    const int64_t pieces = ((MODE == NORM ? a.width : whole16(a.width)) + kPiece<T> - 1) / kPiece<T>;
+    auto go = [&](auto G_tag, auto P_tag) {
+        constexpr int G = decltype(G_tag)::value, P = decltype(P_tag)::value, THREADS = G > 256 ? G : 256, ROWS = THREADS / G;
+        const int64_t groups = (a.rows + ROWS - 1) / ROWS, most = 256 * (2048 / THREADS);
+        norm_kernel<T, MODE, G, P, WHOLE><<<(int)(groups < most ? groups : most), THREADS, 0, st>>>(a);
+    };
+    if (pieces <= 16)
+        go(number_of<16>, number_of<1>);
+    else if (pieces <= 64)
+        go(number_of<64>, number_of<1>);
+    else if (pieces <= 128)
+        go(number_of<64>, number_of<2>);
+    else if (pieces <= 256)
+        go(number_of<256>, number_of<1>);
+    else if (pieces <= 512)
+        go(number_of<256>, number_of<2>);
+    else if (pieces <= 1024)
+        go(number_of<256>, number_of<4>);
+    else if (pieces <= kMostPieces<T>)
+        go(number_of<1024>, number_of<kMostPieces<T> / 1024>);
+    else
+        norm_long_kernel<T, MODE, WHOLE><<<(int)(a.rows < 512 ? a.rows : 512), 1024, 0, st>>>(a);
+}
+
+}    // namespace
+
+const char* launch_rms_norm(hipStream_t st, const tmi_rms_norm_desc_t& d, const void* x, const void* residual, const void* weight, void* sum, void* y,
+                            float* of_row, bool int8, int64_t ld_y)
+{
+    const NormArgs a{ x, residual, weight, sum, y, of_row, d.ld_x, d.ld_residual, d.ld_sum, ld_y, d.rows, d.width, d.eps, d.weight_offset };
+    for_type(d.dtype, [&](auto type) {
+        using T          = decltype(type);
+        const bool whole = whole_rows<T>(x, d.width, d.ld_x) && whole_rows<T>(weight, d.width, d.width) &&
+                           (!residual || whole_rows<T>(residual, d.width, d.ld_residual)) && (!sum || whole_rows<T>(sum, d.width, d.ld_sum)) &&
+                           (int8 || whole_rows<T>(y, d.width, ld_y));
+        if (int8)
+            whole ? launch_typed<T, NORM_INT8, true>(st, a) : launch_typed<T, NORM_INT8, false>(st, a);
+        else
+            whole ? launch_typed<T, NORM, true>(st, a) : launch_typed<T, NORM, false>(st, a);
+    });
+    return int8 ? "rms_norm_int8" : "rms_norm";
+}
+
+const char* launch_quantize_int8(hipStream_t st, int32_t dtype, int32_t rows, int32_t width, const void* x, int64_t ld_x, void* q, int64_t ld_q,
+                                 float* scales)
+{
+    const NormArgs a{ x, nullptr, nullptr, nullptr, q, scales, ld_x, 0, 0, ld_q, rows, width, 0.0f, 0.0f };
+    for_type(dtype, [&](auto type) {
+        using T = decltype(type);
+        whole_rows<T>(x, width, ld_x) ? launch_typed<T, INT8, true>(st, a) : launch_typed<T, INT8, false>(st, a);
+    });
+    return "quantize_int8";
+}
+
+const char* launch_dequantize_int8(hipStream_t st, int32_t dtype, int32_t rows, int32_t width, const void* q, int64_t ld_q, const float* scales, void* x,
+                                   int64_t ld_x)
+{
+    const NormArgs a{ q, nullptr, nullptr, nullptr, x, const_cast<float*>(scales), ld_q, 0, 0, ld_x, rows, width, 0.0f, 0.0f };
+    for_type(dtype, [&](auto type) {
+        using T   = decltype(type);
+        int shift = 4;
+        while (shift < 8 && (kPiece<T> << shift) < width)
+            shift++;
+        const int64_t groups = ((int64_t)rows + (256 >> shift) - 1) / (256 >> shift);
+        const int grid       = (int)(groups < 2048 ? groups : 2048);
+        if (whole_rows<T>(x, width, ld_x))
+            dequantize_kernel<T, true><<<grid, 256, 0, st>>>(a, shift);
+        else
+            dequantize_kernel<T, false><<<grid, 256, 0, st>>>(a, shift);
+    });
+    return "dequantize_int8";
+}
+
+}    // namespace tmi

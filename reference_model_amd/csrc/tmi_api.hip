@@ -2333,4 +2333,234 @@ int tmi_gated_ffn_backward(tmi_ctx_t* ctx, const tmi_gated_ffn_desc_t* desc, con
                                                        dw ? d_gate_dev : nullptr, dw ? d_up_dev : nullptr, ctx->workspace, ctx->pages_dev));
 }
 
+// ---- the way into a projection: the norm, rows in 8 bits, the linear layer on them ------------------------------------------
+
+static bool row_dtype(int32_t dtype)
+{
+    return ffn_dtype(dtype) || dtype == TMI_FP32;
+}
+
+static uintptr_t size_of(int32_t dtype)
+{
+    return dtype == TMI_FP32 ? 4 : 2;
+}
+
+// row_stride() of rows in 8 bits, which begin at multiples of 16 bytes
+static bool int8_stride(int64_t& ld, int64_t width, int64_t rows)
+{
+    if (ld == 0)
+        ld = whole16(width);
+    return ld % 16 == 0 && row_stride(ld, width, rows);
+}
+
+static int fail_int8_rows(tmi_ctx* ctx, const char* op, int32_t width, int64_t ld)
+{
+    return fail(ctx, "%s: rows of %d in 8 bits cannot lie %lld bytes apart (a multiple of 16 is wanted, and no overlap)", op, width, (long long)ld);
+}
+
+// `d` checked, with its row strides filled in; ld_y where y is in 8 bits
+static int validate_rms_norm(tmi_ctx* ctx, const char* op, const tmi_rms_norm_desc_t* d, bool int8, tmi_rms_norm_desc_t& out)
+{
+    if (!d)
+        return fail(ctx, "%s: null descriptor", op);
+    if (!row_dtype(d->dtype))
+        return fail(ctx, "%s: the data type must be FP16, BF16 or FP32", op);
+    if (d->rows < 0 || d->width < 0)
+        return fail(ctx, "%s: negative tensor dimension", op);
+    if (d->width > (1 << 28))
+        return fail(ctx, "%s: rows of %d elements are more than one call takes", op, d->width);
+    if (!(d->eps >= 0.0f && d->eps < __builtin_huge_valf()))
+        return fail(ctx, "%s: eps must be a number that is not negative", op);
+    if (!(__builtin_fabsf(d->weight_offset) < __builtin_huge_valf()))
+        return fail(ctx, "%s: weight_offset must be a number", op);
+    out = *d;
+    if (!row_stride(out.ld_x, d->width, d->rows) || !row_stride(out.ld_residual, d->width, d->rows) || !row_stride(out.ld_sum, d->width, d->rows) ||
+        (!int8 && !row_stride(out.ld_y, d->width, d->rows)))
+        return fail(ctx, "%s: rows of %d elements cannot lie %lld, %lld, %lld or %lld apart", op, d->width, (long long)d->ld_x, (long long)d->ld_residual,
+                    (long long)d->ld_sum, (long long)d->ld_y);
+    if (int8 && !int8_stride(out.ld_y, d->width, d->rows))
+        return fail_int8_rows(ctx, op, d->width, d->ld_y);
+    return TMI_VALID;
+}
+
+// the norm, into 16 or 32 bits with 1 / rms, or into 8 bits with scales
+static int rms_norm(tmi_ctx* ctx, const char* op, const tmi_rms_norm_desc_t* desc, bool int8, const void* x, const void* residual, const void* weight,
+                    void* sum, void* y, float* of_row)
+{
+    tmi_rms_norm_desc_t d;
+    const int rc = validate_rms_norm(ctx, op, desc, int8, d);
+    if (rc != TMI_VALID)
+        return rc;
+    // (rows of no elements still have scales)
+    const bool empty = d.rows == 0 || (d.width == 0 && !int8);
+    if (!empty && ((d.width > 0 && (!x || !weight || !y)) || (int8 && !of_row)))
+        return fail(ctx, "%s: null tensor pointer", op);
+    for (const void* p : { x, residual, weight, (const void*)sum, int8 ? nullptr : (const void*)y })
+        if (unaligned(p, size_of(d.dtype)))
+            return fail(ctx, "%s: a tensor is not aligned to its elements", op);
+    if (unaligned(of_row, 4))
+        return fail(ctx, "%s: a tensor is not aligned to its elements", op);
+    if (int8 && unaligned(y, 16))
+        return fail(ctx, "%s: rows in 8 bits are not aligned to 16 bytes", op);
+    TMI_HIP(ctx, hipSetDevice(ctx->device));
+    if (empty)
+    {
+        ctx->last_kernel = "empty";
+        return TMI_VALID;
+    }
+    if (d.width == 0)    // scales of nothing
+        return after_launch(ctx, launch_quantize_int8(ctx->stream, d.dtype, d.rows, 0, nullptr, 0, nullptr, 0, of_row));
+    return after_launch(ctx, launch_rms_norm(ctx->stream, d, x, residual, weight, sum, y, of_row, int8, d.ld_y));
+}
+
+int tmi_rms_norm(tmi_ctx_t* ctx, const tmi_rms_norm_desc_t* d, const void* x_dev, const void* residual_dev, const void* weight_dev, void* sum_dev,
+                 void* y_dev, float* rstd_dev)
+{
+    if (!ctx)
+        return TMI_ERROR;
+    return rms_norm(ctx, "rms_norm", d, false, x_dev, residual_dev, weight_dev, sum_dev, y_dev, rstd_dev);
+}
+
+int tmi_rms_norm_int8(tmi_ctx_t* ctx, const tmi_rms_norm_desc_t* d, const void* x_dev, const void* residual_dev, const void* weight_dev, void* sum_dev,
+                      int8_t* q_dev, float* scales_dev)
+{
+    if (!ctx)
+        return TMI_ERROR;
+    return rms_norm(ctx, "rms_norm_int8", d, true, x_dev, residual_dev, weight_dev, sum_dev, q_dev, scales_dev);
+}
+
+int tmi_rms_norm_backward(tmi_ctx_t* ctx, const tmi_rms_norm_desc_t* desc, const void* s_dev, const void* weight_dev, const float* rstd_dev,
+                          const void* d_y_dev, const void* d_sum_dev, void* d_x_dev, void* d_weight_dev)
+{
+    if (!ctx)
+        return TMI_ERROR;
+    tmi_rms_norm_desc_t d;
+    const int rc = validate_rms_norm(ctx, "rms_norm_backward", desc, false, d);
+    if (rc != TMI_VALID)
+        return rc;
+    // (a sum over no rows is zero, so d_weight is written all the same)
+    const bool dx = d_x_dev && d.rows > 0 && d.width > 0, dw = d_weight_dev && d.width > 0;
+    if ((dx || dw) && d.rows > 0 && (!s_dev || !weight_dev || !rstd_dev || !d_y_dev))
+        return fail(ctx, "rms_norm_backward: null tensor pointer");
+    for (const void* p : { s_dev, weight_dev, d_y_dev, d_sum_dev, (const void*)d_x_dev, (const void*)d_weight_dev })
+        if (unaligned(p, size_of(d.dtype)))
+            return fail(ctx, "rms_norm_backward: a tensor is not aligned to its elements");
+    if (unaligned(rstd_dev, 4))
+        return fail(ctx, "rms_norm_backward: a tensor is not aligned to its elements");
+    TMI_HIP(ctx, hipSetDevice(ctx->device));
+    if (!dx && !dw)
+    {
+        ctx->last_kernel = "empty";
+        return TMI_VALID;
+    }
+    const int wrc = ensure_workspace(ctx, rms_norm_backward_scratch_bytes(d, dw));
+    if (wrc != TMI_VALID)
+        return wrc;
+    return after_launch(ctx, launch_rms_norm_backward(ctx->stream, d, s_dev, weight_dev, rstd_dev, d_y_dev, d_sum_dev, dx ? d_x_dev : nullptr,
+                                                      dw ? d_weight_dev : nullptr, ctx->workspace));
+}
+
+// What quantising and the way back check in common; *empty: nothing to do
+static int check_int8_copy(tmi_ctx* ctx, const char* op, int32_t dtype, int32_t rows, int32_t width, const void* x, int64_t& ld_x, const void* q, int64_t& ld_q,
+                           const float* scales, bool into, bool* empty)
+{
+    if (!row_dtype(dtype))
+        return fail(ctx, "%s: the data type must be FP16, BF16 or FP32", op);
+    if (rows < 0 || width < 0)
+        return fail(ctx, "%s: negative tensor dimension", op);
+    if (width > (1 << 28))
+        return fail(ctx, "%s: rows of %d elements are more than one call takes", op, width);
+    if (!row_stride(ld_x, width, rows))
+        return fail(ctx, "%s: rows of %d elements cannot lie %lld apart", op, width, (long long)ld_x);
+    if (!int8_stride(ld_q, width, rows))
+        return fail_int8_rows(ctx, op, width, ld_q);
+    *empty = rows == 0 || (width == 0 && !into);    // (rows of no elements still have scales)
+    if (!*empty && ((width > 0 && (!x || !q)) || !scales))
+        return fail(ctx, "%s: null tensor pointer", op);
+    if (unaligned(x, size_of(dtype)) || unaligned(scales, 4))
+        return fail(ctx, "%s: a tensor is not aligned to its elements", op);
+    if (unaligned(q, 16))
+        return fail(ctx, "%s: rows in 8 bits are not aligned to 16 bytes", op);
+    TMI_HIP(ctx, hipSetDevice(ctx->device));
+    if (*empty)
+        ctx->last_kernel = "empty";
+    return TMI_VALID;
+}
+
+int tmi_quantize_int8(tmi_ctx_t* ctx, int32_t dtype, int32_t rows, int32_t width, const void* x_dev, int64_t ld_x, int8_t* q_dev, int64_t ld_q,
+                      float* scales_dev)
+{
+    if (!ctx)
+        return TMI_ERROR;
+    bool empty   = false;
+    const int rc = check_int8_copy(ctx, "quantize_int8", dtype, rows, width, x_dev, ld_x, q_dev, ld_q, scales_dev, true, &empty);
+    if (rc != TMI_VALID || empty)
+        return rc;
+    return after_launch(ctx, launch_quantize_int8(ctx->stream, dtype, rows, width, x_dev, ld_x, q_dev, ld_q, scales_dev));
+}
+
+int tmi_dequantize_int8(tmi_ctx_t* ctx, int32_t dtype, int32_t rows, int32_t width, const int8_t* q_dev, int64_t ld_q, const float* scales_dev, void* x_dev,
+                        int64_t ld_x)
+{
+    if (!ctx)
+        return TMI_ERROR;
+    bool empty   = false;
+    const int rc = check_int8_copy(ctx, "dequantize_int8", dtype, rows, width, x_dev, ld_x, q_dev, ld_q, scales_dev, false, &empty);
+    if (rc != TMI_VALID || empty)
+        return rc;
+    return after_launch(ctx, launch_dequantize_int8(ctx->stream, dtype, rows, width, q_dev, ld_q, scales_dev, x_dev, ld_x));
+}
+
+static int validate_linear_int8(tmi_ctx* ctx, const tmi_linear_int8_desc_t* d, tmi_linear_int8_desc_t& out)
+{
+    const char* op = "linear_int8";
+    if (!d)
+        return fail(ctx, "%s: null descriptor", op);
+    if (!row_dtype(d->dtype))
+        return fail(ctx, "%s: the data type must be FP16, BF16 or FP32", op);
+    if (d->rows < 0 || d->in_features < 0 || d->out_features < 0)
+        return fail(ctx, "%s: negative tensor dimension", op);
+    if (d->in_features > 131071)
+        return fail(ctx, "%s: sums over %d columns do not fit into 32 bits (131071 at most)", op, d->in_features);
+    out = *d;
+    if (!int8_stride(out.ld_x, d->in_features, d->rows))
+        return fail_int8_rows(ctx, op, d->in_features, d->ld_x);
+    if (!int8_stride(out.ld_w, d->in_features, d->out_features))
+        return fail_int8_rows(ctx, op, d->in_features, d->ld_w);
+    if (!row_stride(out.ld_y, d->out_features, d->rows))
+        return fail(ctx, "%s: rows of %d elements cannot lie %lld apart", op, d->out_features, (long long)d->ld_y);
+    // tiles are counted in 31 bits, and blocks of 64 rows in 16
+    if (d->rows > 65535 * 64 || d->out_features > (1 << 28) || ((int64_t)d->rows / 128 + 1) * ((int64_t)d->out_features / 128 + 1) > (int64_t(1) << 26))
+        return fail(ctx, "%s: %d rows, %d x %d weights are more than one call takes", op, d->rows, d->out_features, d->in_features);
+    return TMI_VALID;
+}
+
+int tmi_linear_int8(tmi_ctx_t* ctx, const tmi_linear_int8_desc_t* desc, const int8_t* x_dev, const float* x_scales_dev, const int8_t* w_dev,
+                    const float* w_scales_dev, const void* bias_dev, void* y_dev)
+{
+    if (!ctx)
+        return TMI_ERROR;
+    tmi_linear_int8_desc_t d;
+    const int rc = validate_linear_int8(ctx, desc, d);
+    if (rc != TMI_VALID)
+        return rc;
+    const bool empty = d.rows == 0 || d.out_features == 0;
+    if (!empty && (!y_dev || !x_scales_dev || !w_scales_dev || (d.in_features > 0 && (!x_dev || !w_dev))))
+        return fail(ctx, "linear_int8: null tensor pointer");
+    if (unaligned(y_dev, size_of(d.dtype)) || unaligned(bias_dev, size_of(d.dtype)) || unaligned(x_scales_dev, 4) || unaligned(w_scales_dev, 4))
+        return fail(ctx, "linear_int8: a tensor is not aligned to its elements");
+    if (unaligned(x_dev, 16) || unaligned(w_dev, 16))
+        return fail(ctx, "linear_int8: rows in 8 bits are not aligned to 16 bytes");
+    TMI_HIP(ctx, hipSetDevice(ctx->device));
+    if (empty)
+    {
+        ctx->last_kernel = "empty";
+        return TMI_VALID;
+    }
+    const size_t bytes = linear_int8_scratch_bytes(d);
+    const bool parts   = bytes > 0 && optional_workspace(ctx, bytes);
+    return after_launch(ctx, launch_linear_int8(ctx->stream, d, x_dev, x_scales_dev, w_dev, w_scales_dev, bias_dev, y_dev, parts ? ctx->workspace : nullptr,
+                                                ctx->pages_dev));
+}
+
 }    // extern "C"

@@ -48,6 +48,12 @@ struct ConvGeom
     int32_t M;    // depthwise channel multiplier (unused by CONV2D)
 };
 
+// Rows in 8 bits of the linear layer begin at multiples of 16 bytes, and what fills up their last 16 are zeros.
+__host__ __device__ inline int64_t whole16(int64_t width)
+{
+    return (width + 15) / 16 * 16;
+}
+
 // bf16 carried as its bit pattern
 struct bf16_t
 {
@@ -356,5 +362,22 @@ const char* launch_gated_ffn_backward(hipStream_t st, const tmi_gated_ffn_desc_t
 const char* launch_int4_pack(hipStream_t st, int32_t dtype, int32_t group, int32_t n, int32_t k, const void* w, int64_t ld, const void* scales,
                              void* packed);
 const char* launch_int4_unpack(hipStream_t st, int32_t dtype, int32_t group, int32_t n, int32_t k, const void* packed, void* w, int64_t ld);
+
+// rms_norm.hip (row strides filled in): the norm, with y and `of_row` (1 / rms or null) of dtype and 32 bits or, with `int8`, in 8 bits and scales; rows into
+// 8 bits and back
+const char* launch_rms_norm(hipStream_t st, const tmi_rms_norm_desc_t& d, const void* x, const void* residual, const void* weight, void* sum, void* y,
+                            float* of_row, bool int8, int64_t ld_y);
+const char* launch_quantize_int8(hipStream_t st, int32_t dtype, int32_t rows, int32_t width, const void* x, int64_t ld_x, void* q, int64_t ld_q,
+                                 float* scales);
+const char* launch_dequantize_int8(hipStream_t st, int32_t dtype, int32_t rows, int32_t width, const void* q, int64_t ld_q, const float* scales, void* x,
+                                   int64_t ld_x);
+// rms_norm_backward.hip: `scratch` of as many bytes as the first function says
+size_t rms_norm_backward_scratch_bytes(const tmi_rms_norm_desc_t& d, bool dw);
+const char* launch_rms_norm_backward(hipStream_t st, const tmi_rms_norm_desc_t& d, const void* s, const void* weight, const float* rstd, const void* d_y,
+                                     const void* d_sum, void* d_x, void* d_weight, void* scratch);
+// linear_int8.hip: `scratch` of as many bytes as the first function says, or nullptr: sums in one piece; zeros: 64 bytes of them
+size_t linear_int8_scratch_bytes(const tmi_linear_int8_desc_t& d);
+const char* launch_linear_int8(hipStream_t st, const tmi_linear_int8_desc_t& d, const void* x, const float* x_scales, const void* w, const float* w_scales,
+                               const void* bias, void* y, void* scratch, const void* zeros);
 
 }    // namespace tmi
