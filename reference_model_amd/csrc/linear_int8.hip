@@ -8,10 +8,11 @@
 //
 // The weights are the first operand of the instruction and x the second, so that a lane owns neighbouring features of one token.
 //
-// linear_tile_kernel: many tokens.  Workgroups that stay go through a list of tiles.  LDS is a ring of stages of 64 columns, filled straight from memory
-// four stages ahead, across the borders of tiles: while a workgroup stores one tile's results the next one's operands are on their way.
+// linear_tile_kernel: many tokens.  Workgroups that stay go through a list of tiles.  Operands go straight from memory into LDS, 128 columns of 8 rows an
+// instruction: whole cache lines (loads of 64 bytes of 16 rows bring 51 bytes a nanosecond and CU out of L2, of 128 bytes of 8 rows 136).  They are requested
+// four to two matrix instruction depths ahead, across the borders of tiles: while a workgroup stores one tile's results the next one's operands are on their way.
 //
-// linear_rows_kernel: few tokens, bound by the weights' bytes.  A workgroup has 16 or 32 weight rows, its eight waves split the columns, operands go
+// linear_rows_kernel: few tokens, bound by the weights' bytes.  A workgroup has 16 weight rows, its eight or 16 waves split the columns, operands go
 // from memory into the instruction's registers, and the sums meet in LDS.
 #include "tmi_rows.h"
 
@@ -31,15 +32,15 @@ struct LinearArgs
     int64_t ldw, ldx, ldo;   // bytes, bytes, elements
     int32_t M, N;
     int32_t K;               // columns, up to whole 16s
-    int32_t blocks;          // of 64 columns
+    int32_t blocks;          // of 64 columns, up to a whole pair
     int32_t tiles_m, tiles_n, tiles;
     int32_t splits, per_split;    // blocks of a split
     int32_t items, per_xcd;       // tiles times splits
 };
 
 constexpr int kGroup = 8;    // row tiles that neighbouring workgroups share column tiles over
-constexpr int kBlock = 64;   // columns of a stage
-constexpr int kRing  = 5;    // stages
+constexpr int kBlock = 64;   // columns of a matrix instruction
+constexpr int kPair  = 128;  // of a unit in LDS
 
 __device__ __forceinline__ v4i mma_int8(v4i a, v4i b, v4i c)
 {
@@ -62,37 +63,24 @@ __device__ __forceinline__ void store_one(void* out, int64_t at, float v)
         static_cast<uint16_t*>(out)[at] = to_bits16<T>(v);
 }
 
-// Piece c (16 bytes) of row r of a stage lies at c ^ swizzle(r).  The LDS serves 16-byte reads of 16 lanes at once, of each half wave the quads (4 lanes)
-// {0, 3, 5, 6} and then {1, 2, 4, 7}; lane l reads piece l / 16 of row l % 16.  Rows of a quad differ in r % 4, that is in which 64 of 256
-// bytes they use; of the quads of a set two are of the first piece and two of the second, and 0, 3, 2, 1 for the rows' r / 4 keeps all four apart.
+// Piece c (16 bytes) of row r (128 bytes) of a unit lies at c ^ swizzle(r).  The LDS serves 16-byte reads of 16 lanes at once, of each half wave the quads (4
+// lanes) {0, 3, 5, 6} and then {1, 2, 4, 7}; lane l reads piece l / 16 (and 4 more for the second block) of row l % 16.  Of the 16 rows of a set eight are even
+// and eight odd, which use different halves of 256 bytes; of the even ones four read one piece and four its neighbour, at r / 2 = 0, 1, 6, 7 and 2, 3, 4, 5: all
+// eight places are taken once.
 __device__ __forceinline__ int swizzle(int r)
 {
-    const int q = (r >> 2) & 3;
-    return (q ^ (q << 1)) & 3;
+    return (r >> 1) & 7;
 }
-// a pointer that is the same in every lane, where the compiler does not see it
-__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p)
+// WC x WR waves (features x tokens) that compute, of 64 features and 16 RT tokens each, and LW that load; LDS holds R pairs of blocks.  SPLIT: partial sums
+template <typename T, int WC, int WR, int RT, int LW, int R, bool SPLIT>
+__global__ __launch_bounds__(64 * (WC * WR + LW), (WC * WR + LW) / 4) void linear_tile_kernel(LinearArgs a)
 {
-    const uint64_t v  = reinterpret_cast<uint64_t>(p);
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
-    return reinterpret_cast<const uint8_t*>((uint64_t)hi << 32 | lo);
-}
-
-// WC x WR waves (features x tokens) of 64 features and 16 RT tokens each; SPLIT: partial sums
-template <typename T, int WC, int WR, int RT, bool SPLIT>
-__global__ __launch_bounds__(64 * WC * WR, 2) void linear_tile_kernel(LinearArgs a)
-{
-    constexpr int THREADS = 64 * WC * WR;
-    constexpr int BN = 64 * WC, BM = 16 * RT * WR, CT = 4;
-    constexpr int CB = BN * kBlock, STAGE = (BN + BM) * kBlock;
-    constexpr int CL = BN * 4 / THREADS, RL = BM * 4 / THREADS, LOADS = CL + RL;    // 16-byte loads of a thread and block
-    static_assert(CL * THREADS == BN * 4 && RL * THREADS == BM * 4 && (RT == 2 || RT >= CT), "a block must split evenly over the threads");
+    constexpr int CT = 4, BN = 16 * CT * WC, BM = 16 * RT * WR;
+    constexpr int PAIR = (BN + BM) * kPair;    // of LDS: the weights, then x
+    using Out = std::conditional_t<SPLIT, float, T>;    // (a partial sum is a word, as a float is)
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
 
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wc = wave % WC, wr = wave / WC;
-    const int l16 = lane & 15, q4 = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
     // Workgroups go round-robin to the 8 XCDs; each of those has a contiguous range of the list, along rows in groups of kGroup, which its workgroups go
     // through side by side.
@@ -116,78 +104,92 @@ __global__ __launch_bounds__(64 * WC * WR, 2) void linear_tile_kernel(LinearArgs
         r.block1 = SPLIT && r.block0 + a.per_split < a.blocks ? r.block0 + a.per_split : a.blocks;
         return r;
     };
+    // For results of 16 bits row 16 c + p of 32 holds feature 8 (p / 4) + 4 c + p % 4: a lane then owns eight neighbours, and four lanes 64 bytes in a row, as
+    // they do of 32 bits where row and feature are the same.
+    auto feature_of_row = [](int r) { return sizeof(Out) == 4 ? r : (r & ~31) + 8 * (r >> 2 & 3) + 4 * (r >> 4 & 1) + (r & 3); };
 
-    // ---- what is requested: 16-byte unit u = j * THREADS + tid of either operand's part of a stage -----------------------------
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave * 1024;
-    uint32_t woff[CL], xoff[RL];    // from the running addresses
-    const uint8_t *wat, *xat;
-    int ahead_item = first_item, ahead, ahead_end, astage = 0;    // the block requested next, and its stage
-    auto piece_of_unit = [&](int u) { return ((u & 3) ^ swizzle(u >> 2)) * 16; };
-    // Rows past the last repeat it and are not stored.  Row 16 c + p of 64 holds feature 16 (p / 4) + 4 c + p % 4, so that a lane owns 16 neighbours.
-    auto request_item = [&](int t) {
-        const Item it = item_of(t);
+    // Barrier p (behind the first, which says that pair 0 is there) says that pair p + 1 is there and that nobody reads pair p any more.
+    if (wave >= WC * WR)
+    {
+        // ---- waves that load: 16-byte piece u = j * 64 LW + tid of a pair, row u / 8, of the weights' rows and then of x's ------------
+        constexpr int STEP = 8 * LW, WJ = BN / STEP, XJ = BM / STEP, LOADS = WJ + XJ;
+        static_assert(WJ * STEP == BN && XJ * STEP == BM && STEP % 16 == 0, "all pieces of a thread have one place in their rows");
+        static_assert(R >= 2 && (R - 1) * LOADS < 64, "loads in flight are counted in six bits");
+        const int tid       = threadIdx.x - 64 * WC * WR, row0 = tid >> 3, piece = ((tid & 7) ^ swizzle(row0)) * 16;
+        const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + (wave - WC * WR) * 1024;
+        const uint32_t woff = (uint32_t)(feature_of_row(row0) * a.ldw), xoff = (uint32_t)(row0 * a.ldx);
+        // the item, its block that is requested next, where that lies, the last rows' offsets from there, and the place it goes to
+        int item, block, end, slot = 0;
+        const uint8_t *wat, *xat;
+        uint32_t wlast, xlast;
+        auto begin = [&](int t) {
+            const Item it       = item_of(t);
+            const int64_t lastw = a.N - 1 - it.n0, lastx = a.M - 1 - it.m0;
+            item = t, block = it.block0, end = it.block1;
+            wat = a.w + it.n0 * a.ldw + it.block0 * kBlock, xat = a.x + it.m0 * a.ldx + it.block0 * kBlock;
+            wlast = (uint32_t)((lastw < BN - 1 ? lastw : BN - 1) * a.ldw), xlast = (uint32_t)((lastx < BM - 1 ? lastx : BM - 1) * a.ldx);
+        };
+        // Past the last pair it is requested again, into places nobody reads: the loads in flight are then as many all the time.
+        auto request = [&]() {
+            const bool inside = block * kBlock + piece < a.K;
 #pragma unroll
-        for (int j = 0; j < CL; j++)
+            for (int j = 0; j < LOADS; j++)
+            {
+                // (rows past the last repeat it and are not stored; j steps are other bits of a row than the thread's, so that features add up)
+                const bool is_w    = j < WJ;
+                const uint32_t row = is_w ? woff + (uint32_t)(feature_of_row(j * STEP) * a.ldw) : xoff + (uint32_t)((j - WJ) * STEP * a.ldx);
+                const uint32_t off = (is_w ? (row < wlast ? row : wlast) : (row < xlast ? row : xlast)) + piece;
+                // (zeros where the columns end in the pair)
+                const uint8_t* src = inside ? (is_w ? wat : xat) + off : a.zeros;
+                asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds0 + slot * PAIR + j * (STEP * kPair)) : "memory");
+            }
+            slot = slot + 1 < R ? slot + 1 : 0;
+            block += 2, wat += kPair, xat += kPair;
+            if (block >= end)
+            {
+                if (item + per_turn < last_item)
+                    begin(item + per_turn);
+                else
+                    block -= 2, wat -= kPair, xat -= kPair;
+            }
+        };
+        begin(first_item);
+#pragma unroll 1
+        for (int p = 0; p < R; p++)
+            request();
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((R - 1) * LOADS) : "memory");
+#pragma unroll 1
+        for (int t = first_item; t < last_item; t += per_turn)
         {
-            const int u = j * THREADS + tid, r = u >> 2;
-            const int64_t f = (r & ~63) + 16 * (r >> 2 & 3) + 4 * (r >> 4 & 3) + (r & 3), last = a.N - 1 - it.n0;
-            woff[j] = (uint32_t)((f < last ? f : last) * a.ldw) + piece_of_unit(u);
+            const Item it = item_of(t);
+#pragma unroll 1
+            for (int n = it.block0; n < it.block1; n += 2)
+            {
+                asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((R - 2) * LOADS) : "memory");
+                request();
+            }
         }
-#pragma unroll
-        for (int j = 0; j < RL; j++)
-        {
-            const int u = j * THREADS + tid;
-            const int64_t r = u >> 2, last = a.M - 1 - it.m0;
-            xoff[j] = (uint32_t)((r < last ? r : last) * a.ldx) + piece_of_unit(u);
-        }
-        ahead = it.block0, ahead_end = it.block1;
-        wat = a.w + it.n0 * a.ldw + it.block0 * kBlock, xat = a.x + it.m0 * a.ldx + it.block0 * kBlock;
-    };
-    // load q of the block `ahead`; EDGE: the columns end in it, and zeros come from there on
-    auto request = [&](int q, auto EDGE) {
-        const bool is_w      = q < CL;
-        const int j          = is_w ? q : q - CL;
-        const uint32_t dst   = lds0 + astage * STAGE + (is_w ? 0 : CB) + j * THREADS * 16;
-        const uint8_t* base  = is_w ? wat : xat;
-        const uint32_t voff  = is_w ? woff[j] : xoff[j];
-        if constexpr (decltype(EDGE)::value)
-        {
-            const bool inside  = ahead * kBlock + piece_of_unit(j * THREADS + tid) < a.K;
-            const uint8_t* src = inside ? base + voff : a.zeros;
-            asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(dst) : "memory");
-        }
-        else
-            asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(uniform(base)), "s"(dst) : "memory");
-    };
-    // Past the last block it is requested again, into stages nobody reads: the loads in flight are then as many in every block.
-    auto advance = [&]() {
-        astage = astage + 1 < kRing ? astage + 1 : 0;
-        if (++ahead < ahead_end)
-            wat += kBlock, xat += kBlock;
-        else if (ahead_item + per_turn < last_item)
-            ahead_item += per_turn, request_item(ahead_item);
-        else
-            ahead = ahead_end - 1;
-    };
-    auto whole = [&]() { return (ahead + 1) * kBlock <= a.K; };
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        return;
+    }
 
-    // ---- what a lane reads: piece q4 of row l16 of a tile -------------------------------------------------------------------------
-    const uint32_t waddr = (wc * 64 + l16) * 64 + ((q4 ^ swizzle(l16)) * 16), xaddr = CB + (wr * 16 * RT + l16) * 64 + ((q4 ^ swizzle(l16)) * 16);
+    // ---- waves that compute: a lane reads piece q4 (and q4 + 4 in the second block) of row l16 of a tile -------------------------------
+    const int wc = wave % WC, wr = wave / WC, l16 = lane & 15, q4 = lane >> 4;
+    const uint32_t place = ((q4 ^ swizzle(l16)) * 16), waddr = (wc * 16 * CT + l16) * kPair + place, xaddr = (BN + wr * 16 * RT + l16) * kPair + place;
     v4i acc[CT][RT];
     v4i fw[2][CT], fx[RT];
-    auto read_w = [&](int set, const uint8_t* sb, int c) { fw[set][c] = *reinterpret_cast<const v4i*>(sb + waddr + c * 1024); };
-    auto read_x = [&](const uint8_t* sb, int i) { fx[i] = *reinterpret_cast<const v4i*>(sb + xaddr + i * 1024); };
+    auto read_w = [&](int set, uint32_t at, int c) { fw[set][c] = *reinterpret_cast<const v4i*>(lds + at + c * (16 * kPair)); };
+    auto read_x = [&](uint32_t at, int i) { fx[i] = *reinterpret_cast<const v4i*>(lds + at + i * (16 * kPair)); };
 
     // A block is one matrix instruction deep.  A wave takes it row tile by row tile; when a row tile is done its fragment is read from the next
-    // block, a block ahead of its use, and the column tiles' fragments into a second set.  The barrier that publishes block n + 1 stands behind
-    // the first row tile of block n; past it every wave is done with block n - 1, whose stage takes the loads of block n + 4.  Reads and
-    // loads stand behind matrix instructions one by one, and are kept there: their wait for a slot passes while the matrix cores work.
-    int cur = 0;
+    // block, a block ahead of its use, and the column tiles' fragments into a second set.  So behind the first row tile of a pair's second block all of the pair
+    // is read.  Reads stand behind matrix instructions one by one, and are kept there: their wait for a slot passes while the matrix cores work.
+    uint32_t slot = 0;    // bytes
     auto one_block = [&](auto SET) {
-        constexpr int P     = decltype(SET)::value;
-        cur                 = cur + 1 < kRing ? cur + 1 : 0;
-        const uint8_t* next = lds + cur * STAGE;
-        const bool w        = whole();
+        constexpr int P = decltype(SET)::value;    // which of the pair
+        if constexpr (P == 1)
+            slot = slot + PAIR < R * PAIR ? slot + PAIR : 0;
+        const uint32_t wat = slot + (P == 1 ? waddr : waddr ^ 64), xat = slot + (P == 1 ? xaddr : xaddr ^ 64);
 #pragma unroll
         for (int i = 0; i < RT; i++)
         {
@@ -196,53 +198,29 @@ __global__ __launch_bounds__(64 * WC * WR, 2) void linear_tile_kernel(LinearArgs
             {
                 const int c = i & 1 ? CT - 1 - k : k;    // (one operand changes at a time)
                 acc[c][i]   = mma_int8(fw[P][c], fx[i], acc[c][i]);
-                if (i > 0 && k == 1)
-#pragma unroll
-                    for (int q = 0; q < LOADS; q++)
-                        if (1 + q * (RT - 1) / LOADS == i)
-                        {
-                            if (w)
-                                request(q, std::false_type());
-                            else
-                                request(q, std::true_type());
-                        }
                 if (i > 0 && (RT >= CT ? k == 2 && i < CT : k >= 1))
-                    read_w(1 - P, next, RT >= CT ? i : k);
+                    read_w(1 - P, wat, RT >= CT ? i : k);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (i == 0)
             {
-                // (a bare barrier: the reads in flight are of the block in use)
-                asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((kRing - 3) * LOADS) : "memory");
-                read_w(1 - P, next, 0);
+                if constexpr (P == 1)
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                read_w(1 - P, wat, 0);
             }
-            read_x(next, i);
+            read_x(xat, i);
             __builtin_amdgcn_sched_barrier(0);
         }
-        advance();
     };
+    static_assert(RT == 2 || RT >= CT, "where the weights' fragments are read");
 
-    request_item(first_item);
-#pragma unroll 1
-    for (int b = 0; b < kRing - 1; b++)
-    {
-        if (whole())
-#pragma unroll
-            for (int q = 0; q < LOADS; q++)
-                request(q, std::false_type());
-        else
-#pragma unroll
-            for (int q = 0; q < LOADS; q++)
-                request(q, std::true_type());
-        advance();
-    }
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((kRing - 2) * LOADS) : "memory");
+    asm volatile("s_barrier" ::: "memory");
 #pragma unroll
     for (int c = 0; c < CT; c++)
-        read_w(0, lds, c);
+        read_w(0, waddr, c);
 #pragma unroll
     for (int i = 0; i < RT; i++)
-        read_x(lds, i);
+        read_x(xaddr, i);
     __builtin_amdgcn_sched_barrier(0);
 
 #pragma unroll 1
@@ -254,56 +232,56 @@ __global__ __launch_bounds__(64 * WC * WR, 2) void linear_tile_kernel(LinearArgs
 #pragma unroll
             for (int i = 0; i < RT; i++)
                 acc[c][i] = v4i{ 0, 0, 0, 0 };
-        int n = it.block0;
 #pragma unroll 1
-        for (; n + 1 < it.block1; n += 2)
+        for (int n = it.block0; n < it.block1; n += 2)
         {
             one_block(std::integral_constant<int, 0>());
             one_block(std::integral_constant<int, 1>());
         }
-        if (n < it.block1)
-        {
-            one_block(std::integral_constant<int, 0>());
-#pragma unroll
-            for (int c = 0; c < CT; c++)
-                fw[0][c] = fw[1][c];
-        }
 
-        // ---- results: 16 neighbours of each of a lane's rows ------------------------------------------------------------------
-        const int64_t n0 = it.n0 + wc * 64 + 16 * q4;
-        float ws[16], bs[16];
+        // ---- results: of each of a lane's rows four or two pieces of 16 bytes, of the features of_piece(0), ... on -----------------------
+        constexpr int V = kPiece<Out>, TILES = V / 4;    // (column tiles that a piece comes from)
+        auto of_piece = [&](int p) { return it.n0 + wc * 16 * CT + 16 * TILES * p + V * q4; };
+        float of_row[RT];
         if constexpr (!SPLIT)
 #pragma unroll
-            for (int e = 0; e < 16; e++)
+            for (int i = 0; i < RT; i++)
             {
-                const int64_t f = n0 + e < a.N ? n0 + e : a.N - 1;
-                ws[e] = a.w_scales[f], bs[e] = a.bias ? bias_at<T>(a.bias, f) : 0.0f;
+                const int64_t m = it.m0 + (wr * RT + i) * 16 + l16;
+                of_row[i]       = a.x_scales[m < a.M ? m : a.M - 1];
             }
 #pragma unroll
-        for (int i = 0; i < RT; i++)
+        for (int p = 0; p < CT / TILES; p++)
         {
-            const int64_t m = it.m0 + (wr * RT + i) * 16 + l16;
-            if (m >= a.M)
-                continue;
-            using Out = std::conditional_t<SPLIT, float, T>;    // (a partial sum is a word, as a float is)
-            float y[16];
-#pragma unroll
-            for (int e = 0; e < 16; e++)
-                y[e] = SPLIT ? __int_as_float(acc[e >> 2][i][e & 3]) : 0.0f;
+            const int64_t n = of_piece(p);
+            float scale[V], bias[V];
             if constexpr (!SPLIT)
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                {
+                    const int64_t f = n + e < a.N ? n + e : a.N - 1;
+                    scale[e] = a.w_scales[f], bias[e] = a.bias ? bias_at<T>(a.bias, f) : 0.0f;
+                }
+#pragma unroll
+            for (int i = 0; i < RT; i++)
             {
-                const float xs = a.x_scales[m];
+                const int64_t m = it.m0 + (wr * RT + i) * 16 + l16;
+                float y[V];
 #pragma unroll
-                for (int e = 0; e < 16; e++)
-                    y[e] = __builtin_fmaf((float)acc[e >> 2][i][e & 3] * ws[e], xs, bs[e]);
+                for (int e = 0; e < V; e++)
+                {
+                    const int sum = acc[TILES * p + e / 4][i][e & 3];
+                    if constexpr (SPLIT)
+                        y[e] = __int_as_float(sum);
+                    else
+                        y[e] = __builtin_fmaf((float)sum * scale[e], of_row[i], bias[e]);
+                }
+                Out* row = SPLIT ? reinterpret_cast<Out*>(a.part) + ((int64_t)it.split * a.M + m) * a.N : static_cast<Out*>(a.out) + m * a.ldo;
+                if (m < a.M && n < a.N)
+                    store_piece<Out, false>(row + n, 0, (int)(a.N - n < V ? a.N - n : V), piece_of<Out>(y));
             }
-            Out* row = SPLIT ? reinterpret_cast<Out*>(a.part) + ((int64_t)it.split * a.M + m) * a.N : static_cast<Out*>(a.out) + m * a.ldo;
-#pragma unroll
-            for (int p = 0; p < 16 / kPiece<Out>; p++)
-                store_piece<Out, false>(row + n0, p * kPiece<Out>, (int)(a.N - n0 < 16 ? a.N - n0 : 16), piece_of<Out>(y + p * kPiece<Out>));
         }
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 // Results of a sum that was split, four of a row a thread: integers, so the order does not matter
@@ -339,88 +317,82 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a)
     }
 }
 
-// RT tiles of 16 tokens, CT of 16 features; a wave has every eighth pair of blocks, U pairs on their way at once
-template <typename T, int RT, int CT, int U>
-__global__ __launch_bounds__(512) void linear_rows_kernel(LinearArgs a)
+// RT tiles of 16 tokens against 16 features; a wave has every pair of blocks of WAVES, U pairs on their way at once.  SPLIT: partial sums
+template <typename T, int RT, int U, int WAVES, bool SPLIT>
+__global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a)
 {
-    constexpr int WAVES = 8;
-    __shared__ v4i met[WAVES][CT * RT * 64];
+    __shared__ v4i met[WAVES][RT * 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, q4 = lane >> 4;
-    const int64_t n0 = (int64_t)blockIdx.x * (16 * CT), m0 = (int64_t)blockIdx.y * (16 * RT);
+    const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * (16 * RT);
 
-    const uint8_t *w[CT], *x[RT];    // rows past the last repeat it
-#pragma unroll
-    for (int c = 0; c < CT; c++)
-    {
-        const int64_t n = n0 + c * 16 + l16;
-        w[c]            = a.w + (n < a.N ? n : a.N - 1) * a.ldw;
-    }
+    // (rows past the last repeat it)
+    const int64_t f  = n0 + l16 < a.N ? n0 + l16 : a.N - 1;
+    const uint8_t *w = a.w + f * a.ldw, *x[RT];
 #pragma unroll
     for (int i = 0; i < RT; i++)
     {
         const int64_t m = m0 + i * 16 + l16;
         x[i]            = a.x + (m < a.M ? m : a.M - 1) * a.ldx;
     }
-    v4i acc[CT][RT];
+    v4i acc[RT];
 #pragma unroll
-    for (int c = 0; c < CT; c++)
-#pragma unroll
-        for (int i = 0; i < RT; i++)
-            acc[c][i] = v4i{ 0, 0, 0, 0 };
+    for (int i = 0; i < RT; i++)
+        acc[i] = v4i{ 0, 0, 0, 0 };
 
-    const int pairs = (a.K + 127) / 128;
+    const int pairs = a.blocks / 2, first = SPLIT ? (int)blockIdx.z * (a.per_split / 2) : 0;
+    const int last  = SPLIT && first + a.per_split / 2 < pairs ? first + a.per_split / 2 : pairs;
 #pragma unroll 1
-    for (int p = wave; p < pairs; p += WAVES * U)
+    for (int p = first + wave; p < last; p += WAVES * U)
     {
-        v4i fw[U * 2][CT], fx[U * 2][RT];
+        v4i fw[U * 2], fx[U * 2][RT];
         bool inside[U * 2];
 #pragma unroll
         for (int u = 0; u < U * 2; u++)
         {
-            const int k = (p + (u >> 1) * WAVES) * 128 + (u & 1) * 64 + q4 * 16;
-            inside[u]   = k < a.K;
-            const int at = inside[u] ? k : 0;
-#pragma unroll
-            for (int c = 0; c < CT; c++)
-                fw[u][c] = *reinterpret_cast<const v4i*>(w[c] + at);
+            const int pair = p + (u >> 1) * WAVES, k = pair * kPair + (u & 1) * kBlock + q4 * 16;
+            inside[u]      = pair < last && k < a.K;
+            const int at   = inside[u] ? k : 0;
+            fw[u]          = *reinterpret_cast<const v4i*>(w + at);
 #pragma unroll
             for (int i = 0; i < RT; i++)
                 fx[u][i] = *reinterpret_cast<const v4i*>(x[i] + at);
         }
 #pragma unroll
         for (int u = 0; u < U * 2; u++)
+        {
+            const v4i live = inside[u] ? fw[u] : v4i{ 0, 0, 0, 0 };
 #pragma unroll
-            for (int c = 0; c < CT; c++)
-            {
-                const v4i f = inside[u] ? fw[u][c] : v4i{ 0, 0, 0, 0 };
-#pragma unroll
-                for (int i = 0; i < RT; i++)
-                    acc[c][i] = mma_int8(f, fx[u][i], acc[c][i]);
-            }
+            for (int i = 0; i < RT; i++)
+                acc[i] = mma_int8(live, fx[u][i], acc[i]);
+        }
     }
 #pragma unroll
-    for (int c = 0; c < CT; c++)
-#pragma unroll
-        for (int i = 0; i < RT; i++)
-            met[wave][(c * RT + i) * 64 + lane] = acc[c][i];
+    for (int i = 0; i < RT; i++)
+        met[wave][i * 64 + lane] = acc[i];
     __syncthreads();
 #pragma unroll
-    for (int u = tid; u < CT * RT * 64; u += 64 * WAVES)
+    for (int u = tid; u < RT * 64; u += 64 * WAVES)
     {
         v4i v = met[0][u];
 #pragma unroll
         for (int k = 1; k < WAVES; k++)
             v += met[k][u];
-        const int l = u & 63, tile = u >> 6;
-        const int64_t m = m0 + (tile % RT) * 16 + (l & 15), n = n0 + (tile / RT) * 16 + 4 * (l >> 4);
+        const int l = u & 63;
+        const int64_t m = m0 + (u >> 6) * 16 + (l & 15), n = n0 + 4 * (l >> 4);
         if (m >= a.M)
             continue;
-        const float xs = a.x_scales[m];
+        const float of_row = SPLIT ? 1.0f : a.x_scales[m];
 #pragma unroll
         for (int e = 0; e < 4; e++)
             if (n + e < a.N)
-                store_one<T>(a.out, m * a.ldo + n + e, __builtin_fmaf((float)v[e] * a.w_scales[n + e], xs, a.bias ? bias_at<T>(a.bias, n + e) : 0.0f));
+            {
+                if constexpr (SPLIT)
+                    a.part[((int64_t)blockIdx.z * a.M + m) * a.N + n + e] = v[e];
+                else
+                    store_one<T>(a.out, m * a.ldo + n + e,
+                                 __builtin_fmaf((float)v[e] * a.w_scales[n + e], of_row, a.bias ? bias_at<T>(a.bias, n + e) : 0.0f));
+            }
     }
 }
 
@@ -429,57 +401,94 @@ __global__ __launch_bounds__(512) void linear_rows_kernel(LinearArgs a)
 enum
 {
     ROWS,        // linear_rows_kernel
-    TILE_256,    // 256 x 256 results, eight waves
-    TILE_128     // 128 x 128, eight waves, two workgroups a CU
+    TILE_256,    // 256 features x 128 tokens, eight waves that compute and four that load
+    TILE_128,    // 128 x 128, four and four
+    TILE_64      // 64 x 64, two and two, three workgroups a CU
 };
 struct Plan
 {
     int kind;
     int splits, per_split;
 };
-constexpr int kMostSplits = 16, kLeastBlocks = 8;
+constexpr int kMostSplits = 16;
+
+// of 64 columns, in whole pairs
+int blocks_of(int32_t columns)
+{
+    return (int)((whole16(columns) + kPair - 1) / kPair) * 2;
+}
+
+int64_t tiles_of(int64_t n, int64_t per)
+{
+    return (n + per - 1) / per;
+}
+
+// What linear_rows_kernel takes, us
+double rows_us(int64_t M, int64_t N, int blocks)
+{
+    const int rt       = M > 48 ? 4 : (int)tiles_of(M, 16);
+    const double turns = (double)tiles_of(blocks, rt > 1 ? 16 : blocks >= 64 ? 64 : 32) * (rt > 1 ? 1.0 + 0.12 * rt : 1.1);
+    const double w = (double)N * blocks * 64, x = (double)(M < 64 ? M : tiles_of(M, 64) * 64) * tiles_of(N, 16) * blocks * 64;
+    const double bytes = w * tiles_of(M, 64) / 6.2e6, all = (w * tiles_of(M, 64) + x) / 8.5e6;
+    return 2.0 + (turns > bytes ? (turns > all ? turns : all) : bytes > all ? bytes : all);
+}
+double join_us(int64_t M, int64_t N, int splits)
+{
+    return splits > 1 ? 2.3 + (double)M * N * 8 * splits / 7.5e6 : 0;
+}
 
 Plan plan_of(const tmi_linear_int8_desc_t& d)
 {
-    Plan p{};
-    const int blocks = (int)((whole16(d.in_features) + kBlock - 1) / kBlock);
-    p.splits = 1, p.per_split = blocks;
+    const int64_t M = d.rows, N = d.out_features;
+    const int blocks = blocks_of(d.in_features);
+    Plan p{ ROWS, 1, blocks };
     // (a lane's offset over a tile is held in 32 bits)
     const bool far = d.ld_x >= (int64_t(1) << 23) || d.ld_w >= (int64_t(1) << 23);
-    if (d.rows <= 64 || far || blocks == 0)
-    {
-        p.kind = ROWS;
+    if (far || blocks == 0)
         return p;
-    }
-    const int64_t big = (((int64_t)d.rows + 255) / 256) * (((int64_t)d.out_features + 255) / 256);
-    p.kind            = big >= 200 ? TILE_256 : TILE_128;
-    if (p.kind == TILE_128)
+    double least = M <= 256 ? rows_us(M, N, blocks) : 1e30;
+    auto take    = [&](int kind, double us, int splits, int per) {
+        if (us < least)
+            least = us, p = Plan{ kind, splits, per };
+    };
+    auto per_cu = [](int64_t items) { return (double)((items + 255) / 256); };
+    const int64_t t256 = tiles_of(M, 128) * tiles_of(N, 256), t128 = tiles_of(M, 128) * tiles_of(N, 128), t64 = tiles_of(M, 64) * tiles_of(N, 64);
+    take(TILE_256, 4.5 + per_cu(t256) * (blocks * (t256 >= 200 ? 0.377 : 0.29) + 2.4), 1, blocks);
+    take(TILE_128, 3.6 + per_cu(t128) * (blocks * (t128 >= 200 ? 0.22 : 0.165) + 2.4), 1, blocks);
+    for (int want = 1; want <= kMostSplits && want <= blocks / 2; want++)
     {
-        const int64_t tiles = (((int64_t)d.rows + 127) / 128) * (((int64_t)d.out_features + 127) / 128);
-        int want            = (int)(512 / tiles);
-        want = want > kMostSplits ? kMostSplits : want;
-        want = want > blocks / kLeastBlocks ? blocks / kLeastBlocks : want;
-        if (want > 1)
-        {
-            p.per_split = (blocks + want - 1) / want;
-            p.splits    = (blocks + p.per_split - 1) / p.per_split;
-        }
+        const int per = (blocks / 2 + want - 1) / want * 2, splits = (blocks + per - 1) / per;
+        const double n = per_cu(t64 * splits);
+        take(TILE_64, 3.6 + per * (0.105 * n > 0.145 ? 0.105 * n : 0.145) + 0.7 * n + join_us(M, N, splits), splits, per);
+        if (M <= 64 && splits > 1)
+            take(ROWS, rows_us(M, N * splits, per) + join_us(M, N, splits), splits, per);
     }
     return p;
 }
 
-template <typename T, int WC, int WR, int RT, bool SPLIT>
+template <typename T, int WC, int WR, int RT, int LW, int R, bool SPLIT>
 bool launch_tiles(hipStream_t st, LinearArgs a, int places)
 {
-    constexpr size_t lds = kRing * (64 * WC + 16 * RT * WR) * kBlock;
-    constexpr auto kernel = linear_tile_kernel<T, WC, WR, RT, SPLIT>;
+    constexpr int BN = 64 * WC, BM = 16 * RT * WR;
+    constexpr size_t lds  = R * (BN + BM) * kPair;
+    constexpr auto kernel = linear_tile_kernel<T, WC, WR, RT, LW, R, SPLIT>;
     if (!ensure_dynamic_lds<kernel>(lds))
         return false;
-    a.tiles_m = (a.M + 16 * RT * WR - 1) / (16 * RT * WR), a.tiles_n = (a.N + 64 * WC - 1) / (64 * WC), a.tiles = a.tiles_m * a.tiles_n;
+    a.tiles_m = (a.M + BM - 1) / BM, a.tiles_n = (a.N + BN - 1) / BN, a.tiles = a.tiles_m * a.tiles_n;
     a.items = a.tiles * a.splits, a.per_xcd = (a.items + 7) / 8;
     const int grid = a.per_xcd * 8 < places ? a.per_xcd * 8 : places;
-    kernel<<<grid, 64 * WC * WR, lds, st>>>(a);
+    kernel<<<grid, 64 * (WC * WR + LW), lds, st>>>(a);
     return true;
+}
+
+template <int N>
+constexpr std::integral_constant<int, N> number_of{};
+
+template <typename T>
+void launch_join(hipStream_t st, const LinearArgs& a)
+{
+    if (a.splits > 1)
+        linear_join_kernel<T><<<dim3((a.N + 1023) / 1024, a.M < 32768 ? a.M : 32768), 256, 0, st>>>(a);
 }
 
 template <typename T>
@@ -487,24 +496,41 @@ bool launch_typed(hipStream_t st, const LinearArgs& a, const Plan& p)
 {
     if (p.kind == ROWS)
     {
-        auto go = [&](auto kernel, int rt, int ct) { kernel<<<dim3((a.N + 16 * ct - 1) / (16 * ct), (a.M + 16 * rt - 1) / (16 * rt)), 512, 0, st>>>(a); };
-        if (a.M <= 16)
-            go(linear_rows_kernel<T, 1, 1, 4>, 1, 1);
-        else if (a.M <= 32)
-            go(linear_rows_kernel<T, 2, 1, 2>, 2, 1);
+        auto go = [&](auto SPLIT, auto RT, auto U, auto WAVES) {
+            constexpr int rt = decltype(RT)::value, waves = decltype(WAVES)::value;
+            linear_rows_kernel<T, rt, decltype(U)::value, waves, decltype(SPLIT)::value>
+                <<<dim3((a.N + 15) / 16, (a.M + 16 * rt - 1) / (16 * rt), a.splits), 64 * waves, 0, st>>>(a);
+        };
+        auto rows = [&](auto SPLIT) {
+            // Few waves and loads on their way for short columns, more for long ones.  us 1 x 1024 x 4096 with two pairs and eight waves 3.5, with two and 16 3.6,
+            // with four and eight 4.6; 1 x 8192 x 8192 14.4, 12.8 and 13.2.
+            if (a.M <= 16 && a.per_split >= 64)
+                go(SPLIT, number_of<1>, number_of<2>, number_of<16>);
+            else if (a.M <= 16)
+                go(SPLIT, number_of<1>, number_of<2>, number_of<8>);
+            else if (a.M <= 32)
+                go(SPLIT, number_of<2>, number_of<1>, number_of<8>);
+            else if (a.M <= 48)
+                go(SPLIT, number_of<3>, number_of<1>, number_of<8>);
+            else
+                go(SPLIT, number_of<4>, number_of<1>, number_of<8>);
+        };
+        if (a.splits > 1)
+            rows(std::true_type());
         else
-            go(linear_rows_kernel<T, 4, 1, 2>, 4, 1);
+            rows(std::false_type());
+        launch_join<T>(st, a);
         return true;
     }
     bool ok;
     if (p.kind == TILE_256)
-        ok = launch_tiles<T, 4, 2, 8, false>(st, a, 256);
-    else if (p.splits > 1)
-        ok = launch_tiles<float, 2, 4, 2, true>(st, a, 512);
+        ok = launch_tiles<T, 4, 2, 4, 4, 3, false>(st, a, 256);
+    else if (p.kind == TILE_128)
+        ok = launch_tiles<T, 2, 2, 4, 4, 5, false>(st, a, 256);
     else
-        ok = launch_tiles<T, 2, 4, 2, false>(st, a, 512);
-    if (ok && p.splits > 1)
-        linear_join_kernel<T><<<dim3((a.N + 1023) / 1024, a.M < 32768 ? a.M : 32768), 256, 0, st>>>(a);
+        ok = p.splits > 1 ? launch_tiles<float, 1, 2, 2, 2, 3, true>(st, a, 768) : launch_tiles<T, 1, 2, 2, 2, 3, false>(st, a, 768);
+    if (ok)
+        launch_join<T>(st, a);
     return ok;
 }
 
@@ -520,7 +546,7 @@ const char* launch_linear_int8(hipStream_t st, const tmi_linear_int8_desc_t& d, 
                                const void* bias, void* y, void* scratch, const void* zeros)
 {
     Plan p           = plan_of(d);
-    const int blocks = (int)((whole16(d.in_features) + kBlock - 1) / kBlock);
+    const int blocks = blocks_of(d.in_features);
     if (!scratch)
         p.splits = 1, p.per_split = blocks;
     LinearArgs a{};
