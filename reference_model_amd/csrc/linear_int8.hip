@@ -8,9 +8,9 @@
 //
 // The weights are the first operand of the instruction and x the second, so that a lane owns neighbouring features of one token.
 //
-// linear_tile_kernel: many tokens.  Workgroups that stay go through a list of tiles.  Operands go straight from memory into LDS, 128 columns of 8 rows an
-// instruction: whole cache lines (loads of 64 bytes of 16 rows bring 51 bytes a nanosecond and CU out of L2, of 128 bytes of 8 rows 136).  They are requested
-// four to two matrix instruction depths ahead, across the borders of tiles: while a workgroup stores one tile's results the next one's operands are on their way.
+// linear_wide_kernel, linear_tile_kernel: many tokens.  Workgroups that stay go through a list of tiles.  Operands go straight from memory into LDS, 128 columns of
+// 8 rows an instruction: whole cache lines (64 bytes of 16 rows bring 51 bytes a nanosecond and CU out of L2, 128 bytes of 8 rows 136).  They are requested a pair
+// of matrix instruction depths ahead and more, across the borders of tiles: while a workgroup stores one tile's results the next one's operands are on their way.
 //
 // linear_rows_kernel: few tokens, bound by the weights' bytes.  A workgroup has 16 weight rows, its eight or 16 waves split the columns, operands go
 // from memory into the instruction's registers, and the sums meet in LDS.
@@ -71,29 +71,25 @@ __device__ __forceinline__ int swizzle(int r)
 {
     return (r >> 1) & 7;
 }
-// WC x WR waves (features x tokens) that compute, of 64 features and 16 RT tokens each, and LW that load; LDS holds R pairs of blocks.  SPLIT: partial sums
-template <typename T, int WC, int WR, int RT, int LW, int R, bool SPLIT>
-__global__ __launch_bounds__(64 * (WC * WR + LW), (WC * WR + LW) / 4) void linear_tile_kernel(LinearArgs a)
+// The list of tiles (times splits), and where a workgroup is in it.  Workgroups go round-robin to the 8 XCDs; each of those has a contiguous range of the
+// list, along rows in groups of kGroup, which its workgroups go through side by side.
+struct Item
 {
-    constexpr int CT = 4, BN = 16 * CT * WC, BM = 16 * RT * WR;
-    constexpr int PAIR = (BN + BM) * kPair;    // of LDS: the weights, then x
-    using Out = std::conditional_t<SPLIT, float, T>;    // (a partial sum is a word, as a float is)
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-
-    // Workgroups go round-robin to the 8 XCDs; each of those has a contiguous range of the list, along rows in groups of kGroup, which its workgroups go
-    // through side by side.
-    const int per_turn = gridDim.x >> 3, first_item = (blockIdx.x & 7) * a.per_xcd + (blockIdx.x >> 3);
-    const int of_xcd = ((int)(blockIdx.x & 7) + 1) * a.per_xcd, last_item = of_xcd < a.items ? of_xcd : a.items;
-    if (first_item >= last_item)
-        return;
-    struct Item
+    int64_t m0, n0;
+    int split, block0, block1;
+};
+template <int BM, int BN, bool SPLIT>
+struct Items
+{
+    int per_turn, first, last;
+    __device__ __forceinline__ explicit Items(const LinearArgs& a)
     {
-        int64_t m0, n0;
-        int split, block0, block1;
-    };
-    auto item_of = [&](int t) {
+        per_turn = gridDim.x >> 3, first = (blockIdx.x & 7) * a.per_xcd + (blockIdx.x >> 3);
+        const int of_xcd = ((int)(blockIdx.x & 7) + 1) * a.per_xcd;
+        last = of_xcd < a.items ? of_xcd : a.items;
+    }
+    __device__ __forceinline__ Item at(const LinearArgs& a, int t) const
+    {
         Item r;
         r.split        = SPLIT ? t / a.tiles : 0;
         const int tile = t - r.split * a.tiles, in_group = kGroup * a.tiles_n, group = tile / in_group, rest = tile - group * in_group;
@@ -103,10 +99,258 @@ __global__ __launch_bounds__(64 * (WC * WR + LW), (WC * WR + LW) / 4) void linea
         r.block0 = SPLIT ? r.split * a.per_split : 0;
         r.block1 = SPLIT && r.block0 + a.per_split < a.blocks ? r.block0 + a.per_split : a.blocks;
         return r;
+    }
+};
+
+// For results of 16 bits row 16 c + p of 32 of a tile's weights holds feature 8 (p / 4) + 4 c + p % 4: a lane then owns eight neighbours, and four lanes 64 bytes in
+// a row, as they do of 32 bits where row and feature are the same.  (Rows that differ in other bits add up.)
+template <typename Out>
+__device__ __forceinline__ int feature_of_row(int r)
+{
+    return sizeof(Out) == 4 ? r : (r & ~31) + 8 * (r >> 2 & 3) + 4 * (r >> 4 & 1) + (r & 3);
+}
+// 16 bytes a lane, straight into LDS: lane l's to `to` + 16 l
+__device__ __forceinline__ void load_into_lds(const uint8_t* from, uint32_t to)
+{
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(to) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const uint8_t* p)
+{
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p;
+}
+
+// The results of a wave's CT x RT instruction tiles from feature n0 and token m0 on: of each of a lane's rows pieces of 16 bytes
+template <typename T, int CT, int RT, bool SPLIT>
+__device__ __forceinline__ void store_tile(const LinearArgs& a, const v4i (&acc)[CT][RT], int64_t n0, int64_t m0, int split, int l16, int q4)
+{
+    using Out       = std::conditional_t<SPLIT, float, T>;    // (a partial sum is a word, as a float is)
+    constexpr int V = kPiece<Out>, TILES = V / 4;             // (column tiles that a piece comes from)
+    float of_row[RT];
+    if constexpr (!SPLIT)
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+        {
+            const int64_t m = m0 + i * 16 + l16;
+            of_row[i]       = a.x_scales[m < a.M ? m : a.M - 1];
+        }
+#pragma unroll
+    for (int p = 0; p < CT / TILES; p++)
+    {
+        const int64_t n = n0 + 16 * TILES * p + V * q4;
+        float scale[V], bias[V];
+        if constexpr (!SPLIT)
+#pragma unroll
+            for (int e = 0; e < V; e++)
+            {
+                const int64_t f = n + e < a.N ? n + e : a.N - 1;
+                scale[e] = a.w_scales[f], bias[e] = a.bias ? bias_at<T>(a.bias, f) : 0.0f;
+            }
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+        {
+            const int64_t m = m0 + i * 16 + l16;
+            float y[V];
+#pragma unroll
+            for (int e = 0; e < V; e++)
+            {
+                const int sum = acc[TILES * p + e / 4][i][e & 3];
+                if constexpr (SPLIT)
+                    y[e] = __int_as_float(sum);
+                else
+                    y[e] = __builtin_fmaf((float)sum * scale[e], of_row[i], bias[e]);
+            }
+            Out* row = SPLIT ? reinterpret_cast<Out*>(a.part) + ((int64_t)split * a.M + m) * a.N : static_cast<Out*>(a.out) + m * a.ldo;
+            if (m < a.M && n < a.N)
+                store_piece<Out, false>(row + n, 0, (int)(a.N - n < V ? a.N - n : V), piece_of<Out>(y));
+        }
+    }
+}
+
+// What the waves that compute do with a pair of blocks.  A block is one matrix instruction deep; a wave takes it row tile by row tile.  When a row tile is done its
+// fragment is read from the next block, a block ahead of its use, and the column tiles' fragments into a second set.  So behind the first row tile of
+// a pair's second block all of the pair is read, and what `border` does there may say so.  Reads, and what `load` requests, stand behind matrix
+// instructions one by one, and are kept there: their wait for a slot passes while the matrix cores work.
+template <int CT, int RT>
+struct Multiply
+{
+    static_assert(RT == 2 || RT >= CT, "where the weights' fragments are read");
+    v4i acc[CT][RT], fw[2][CT], fx[RT];
+    const uint8_t* lds;
+    __device__ __forceinline__ void read_w(int set, uint32_t at, int c) { fw[set][c] = *reinterpret_cast<const v4i*>(lds + at + c * (16 * kPair)); }
+    __device__ __forceinline__ void read_x(uint32_t at, int i) { fx[i] = *reinterpret_cast<const v4i*>(lds + at + i * (16 * kPair)); }
+    __device__ __forceinline__ void first(uint32_t wat, uint32_t xat)
+    {
+#pragma unroll
+        for (int c = 0; c < CT; c++)
+            read_w(0, wat, c);
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+            read_x(xat, i);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __device__ __forceinline__ void clear()
+    {
+#pragma unroll
+        for (int c = 0; c < CT; c++)
+#pragma unroll
+            for (int i = 0; i < RT; i++)
+                acc[c][i] = v4i{ 0, 0, 0, 0 };
+    }
+    // Block P of a pair; wat and xat: where the next block's fragments are.  load(i): behind the second instruction of row tile i, from 1 on.
+    template <int P, typename B, typename L>
+    __device__ __forceinline__ void block(uint32_t wat, uint32_t xat, B&& border, L&& load)
+    {
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+        {
+#pragma unroll
+            for (int k = 0; k < CT; k++)
+            {
+                const int c = i & 1 ? CT - 1 - k : k;    // (one operand changes at a time)
+                acc[c][i]   = mma_int8(fw[P][c], fx[i], acc[c][i]);
+                if (i > 0 && k == 1)
+                    load(i);
+                if (i > 0 && (RT >= CT ? k == 2 && i < CT : k >= 1))
+                    read_w(1 - P, wat, RT >= CT ? i : k);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (i == 0)
+            {
+                if constexpr (P == 1)
+                    border();
+                read_w(1 - P, wat, 0);
+            }
+            read_x(xat, i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+};
+
+// 256 x 256 results, eight waves of 64 features x 128 tokens that load as well as compute.  LDS is a ring of five units: the weights of a pair, its x, the next
+// pair's weights and so on.  At the barrier in the second block of pair p its units are free, and pair p + 1 has landed (all but the weights of p + 2);
+// x of p + 2 goes in the place of p's weights, the weights of p + 3 in that of its x.  us 4096 x 4096 x 16384 with operands from memory 225, with the kernel below in
+// tiles of 256 x 128 262 (half as much again of the operands' bytes); where they are in the last cache 227 and 214.
+template <typename T>
+__global__ __launch_bounds__(512, 2) void linear_wide_kernel(LinearArgs a)
+{
+    constexpr int CT = 4, RT = 8, B = 256, UNIT = B * kPair, RING = 5, LOADS = B * 8 / 512;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const Items<B, B, false> items(a);
+    if (items.first >= items.last)
+        return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wc = wave & 3, wr = wave >> 2, l16 = lane & 15, q4 = lane >> 4;
+
+    // ---- what is requested: 16-byte piece u = j * 512 + tid of a unit, row u / 8 --------------------------------------------------
+    const uint32_t lds0 = lds_address(lds) + wave * 1024;
+    const int piece     = ((tid & 7) ^ swizzle(tid >> 3)) * 16;    // (64 rows are whole turns of the swizzle)
+    const uint32_t woff = (uint32_t)(feature_of_row<T>(tid >> 3) * a.ldw), xoff = (uint32_t)((tid >> 3) * a.ldx);    // of this thread's first row
+    // of the weights and of x: the item, its block that is requested next, where that lies, the last row's offset from there, and the unit it goes to
+    struct Stream
+    {
+        int item, block, end, slot;
+        const uint8_t* at;
+        uint32_t last;
     };
-    // For results of 16 bits row 16 c + p of 32 holds feature 8 (p / 4) + 4 c + p % 4: a lane then owns eight neighbours, and four lanes 64 bytes in a row, as
-    // they do of 32 bits where row and feature are the same.
-    auto feature_of_row = [](int r) { return sizeof(Out) == 4 ? r : (r & ~31) + 8 * (r >> 2 & 3) + 4 * (r >> 4 & 1) + (r & 3); };
+    Stream ws, xs;
+    auto begin = [&](auto W, int t) {
+        constexpr bool IS_W = decltype(W)::value;
+        Stream& s           = IS_W ? ws : xs;
+        const Item it       = items.at(a, t);
+        const int64_t ld = IS_W ? a.ldw : a.ldx, first = IS_W ? it.n0 : it.m0, last = (IS_W ? a.N : a.M) - 1 - first;
+        s.item = t, s.block = it.block0, s.end = it.block1;
+        s.at   = (IS_W ? a.w : a.x) + first * ld + it.block0 * kBlock;
+        s.last = (uint32_t)((last < B - 1 ? last : B - 1) * ld);
+    };
+    // load j of a stream's next unit: rows past the last repeat it and are not stored; zeros where the columns end in it (without a branch: one to each side
+    // of a load costs 50 to 100 cycles of a wave)
+    auto request = [&](auto W, int j) {
+        constexpr bool IS_W = decltype(W)::value;
+        const Stream& s     = IS_W ? ws : xs;
+        const uint32_t row  = IS_W ? woff + (uint32_t)(feature_of_row<T>(64 * j) * a.ldw) : xoff + (uint32_t)(64 * j * a.ldx);
+        const uint32_t off  = (row < s.last ? row : s.last) + piece;
+        load_into_lds(s.block * kBlock + piece < a.K ? s.at + off : a.zeros, lds0 + s.slot * UNIT + j * 8192);
+    };
+    // Past the last unit it is requested again, into places nobody reads: the loads in flight are then as many all the time.
+    auto advance = [&](auto W) {
+        Stream& s = decltype(W)::value ? ws : xs;
+        s.slot    = s.slot + 2 < RING ? s.slot + 2 : s.slot + 2 - RING;
+        s.block += 2, s.at += kPair;
+        if (__builtin_expect(s.block >= s.end, 0))
+        {
+            if (s.item + items.per_turn < items.last)
+                begin(W, s.item + items.per_turn);
+            else
+                s.block -= 2, s.at -= kPair;
+        }
+    };
+    constexpr std::true_type of_w{};
+    constexpr std::false_type of_x{};
+
+    // ---- what a lane reads: piece q4 (and q4 + 4 in the second block) of row l16 of a tile -----------------------------------------
+    const uint32_t place = (q4 ^ swizzle(l16)) * 16, waddr = (wc * 64 + l16) * kPair + place, xaddr = (wr * 128 + l16) * kPair + place;
+    Multiply<CT, RT> m;
+    m.lds     = lds;
+    int wslot = 0, xslot = 1;    // the units of the pair in use
+    auto pair = [&]() {
+        auto loads = [&](auto W) {
+            return [&](int i) {
+#pragma unroll
+                for (int j = 0; j < LOADS; j++)
+                    if (1 + j * (RT - 1) / LOADS == i)
+                        request(decltype(W){}, j);
+            };
+        };
+        m.template block<0>(wslot * UNIT + (waddr ^ 64), xslot * UNIT + (xaddr ^ 64), []() {}, loads(of_w));
+        advance(of_w);
+        wslot = wslot + 2 < RING ? wslot + 2 : wslot + 2 - RING, xslot = xslot + 2 < RING ? xslot + 2 : xslot + 2 - RING;
+        m.template block<1>(wslot * UNIT + waddr, xslot * UNIT + xaddr,
+                            []() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory"); }, loads(of_x));
+        advance(of_x);
+    };
+
+    begin(of_w, items.first), begin(of_x, items.first);
+    ws.slot = 0, xs.slot = 1;
+#pragma unroll 1
+    for (int b = 0; b < 2; b++)
+    {
+#pragma unroll
+        for (int j = 0; j < LOADS; j++)
+            request(of_w, j);
+#pragma unroll
+        for (int j = 0; j < LOADS; j++)
+            request(of_x, j);
+        advance(of_w), advance(of_x);
+    }
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
+    m.first(waddr, UNIT + xaddr);
+#pragma unroll 1
+    for (int t = items.first; t < items.last; t += items.per_turn)
+    {
+        const Item it = items.at(a, t);
+        m.clear();
+#pragma unroll 1
+        for (int n = it.block0; n < it.block1; n += 2)
+            pair();
+        store_tile<T, CT, RT, false>(a, m.acc, it.n0 + wc * 64, it.m0 + wr * 128, 0, l16, q4);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// WC x WR waves (features x tokens) that compute, of 64 features and 16 RT tokens each, and LW that load; LDS holds R pairs of blocks.  A wave that has loads to
+// request waits for each of them (some 50 cycles; 110 where two share a SIMD), which those that compute need not do here, nor wait for the loads or for their own
+// stores.  us with waves that do both 256 x 4096 x 4096 17.5 (now 12.8), 1024 x 4096 x 4096 23.7 (19.7), 512 x 8192 x 8192 40.8 (33.1).  SPLIT: partial sums.
+template <typename T, int WC, int WR, int RT, int LW, int R, bool SPLIT>
+__global__ __launch_bounds__(64 * (WC * WR + LW), (WC * WR + LW) / 4) void linear_tile_kernel(LinearArgs a)
+{
+    constexpr int CT = 4, BN = 16 * CT * WC, BM = 16 * RT * WR;
+    constexpr int PAIR = (BN + BM) * kPair;    // of LDS: the weights, then x
+    using Out          = std::conditional_t<SPLIT, float, T>;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const Items<BM, BN, SPLIT> items(a);
+    if (items.first >= items.last)
+        return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
     // Barrier p (behind the first, which says that pair 0 is there) says that pair p + 1 is there and that nobody reads pair p any more.
     if (wave >= WC * WR)
@@ -116,52 +360,49 @@ __global__ __launch_bounds__(64 * (WC * WR + LW), (WC * WR + LW) / 4) void linea
         static_assert(WJ * STEP == BN && XJ * STEP == BM && STEP % 16 == 0, "all pieces of a thread have one place in their rows");
         static_assert(R >= 2 && (R - 1) * LOADS < 64, "loads in flight are counted in six bits");
         const int tid       = threadIdx.x - 64 * WC * WR, row0 = tid >> 3, piece = ((tid & 7) ^ swizzle(row0)) * 16;
-        const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + (wave - WC * WR) * 1024;
-        const uint32_t woff = (uint32_t)(feature_of_row(row0) * a.ldw), xoff = (uint32_t)(row0 * a.ldx);
+        const uint32_t lds0 = lds_address(lds) + (wave - WC * WR) * 1024;
+        const uint32_t woff = (uint32_t)(feature_of_row<Out>(row0) * a.ldw), xoff = (uint32_t)(row0 * a.ldx);
         // the item, its block that is requested next, where that lies, the last rows' offsets from there, and the place it goes to
         int item, block, end, slot = 0;
         const uint8_t *wat, *xat;
         uint32_t wlast, xlast;
         auto begin = [&](int t) {
-            const Item it       = item_of(t);
+            const Item it       = items.at(a, t);
             const int64_t lastw = a.N - 1 - it.n0, lastx = a.M - 1 - it.m0;
             item = t, block = it.block0, end = it.block1;
             wat = a.w + it.n0 * a.ldw + it.block0 * kBlock, xat = a.x + it.m0 * a.ldx + it.block0 * kBlock;
             wlast = (uint32_t)((lastw < BN - 1 ? lastw : BN - 1) * a.ldw), xlast = (uint32_t)((lastx < BM - 1 ? lastx : BM - 1) * a.ldx);
         };
-        // Past the last pair it is requested again, into places nobody reads: the loads in flight are then as many all the time.
+        // (rows past the last, columns behind the last and pairs past the last as in the kernel above)
         auto request = [&]() {
             const bool inside = block * kBlock + piece < a.K;
 #pragma unroll
             for (int j = 0; j < LOADS; j++)
             {
-                // (rows past the last repeat it and are not stored; j steps are other bits of a row than the thread's, so that features add up)
                 const bool is_w    = j < WJ;
-                const uint32_t row = is_w ? woff + (uint32_t)(feature_of_row(j * STEP) * a.ldw) : xoff + (uint32_t)((j - WJ) * STEP * a.ldx);
+                const uint32_t row = is_w ? woff + (uint32_t)(feature_of_row<Out>(j * STEP) * a.ldw) : xoff + (uint32_t)((j - WJ) * STEP * a.ldx);
                 const uint32_t off = (is_w ? (row < wlast ? row : wlast) : (row < xlast ? row : xlast)) + piece;
-                // (zeros where the columns end in the pair)
-                const uint8_t* src = inside ? (is_w ? wat : xat) + off : a.zeros;
-                asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds0 + slot * PAIR + j * (STEP * kPair)) : "memory");
+                load_into_lds(inside ? (is_w ? wat : xat) + off : a.zeros, lds0 + slot * PAIR + j * (STEP * kPair));
             }
             slot = slot + 1 < R ? slot + 1 : 0;
             block += 2, wat += kPair, xat += kPair;
             if (block >= end)
             {
-                if (item + per_turn < last_item)
-                    begin(item + per_turn);
+                if (item + items.per_turn < items.last)
+                    begin(item + items.per_turn);
                 else
                     block -= 2, wat -= kPair, xat -= kPair;
             }
         };
-        begin(first_item);
+        begin(items.first);
 #pragma unroll 1
         for (int p = 0; p < R; p++)
             request();
         asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((R - 1) * LOADS) : "memory");
 #pragma unroll 1
-        for (int t = first_item; t < last_item; t += per_turn)
+        for (int t = items.first; t < items.last; t += items.per_turn)
         {
-            const Item it = item_of(t);
+            const Item it = items.at(a, t);
 #pragma unroll 1
             for (int n = it.block0; n < it.block1; n += 2)
             {
@@ -175,112 +416,26 @@ __global__ __launch_bounds__(64 * (WC * WR + LW), (WC * WR + LW) / 4) void linea
 
     // ---- waves that compute: a lane reads piece q4 (and q4 + 4 in the second block) of row l16 of a tile -------------------------------
     const int wc = wave % WC, wr = wave / WC, l16 = lane & 15, q4 = lane >> 4;
-    const uint32_t place = ((q4 ^ swizzle(l16)) * 16), waddr = (wc * 16 * CT + l16) * kPair + place, xaddr = (BN + wr * 16 * RT + l16) * kPair + place;
-    v4i acc[CT][RT];
-    v4i fw[2][CT], fx[RT];
-    auto read_w = [&](int set, uint32_t at, int c) { fw[set][c] = *reinterpret_cast<const v4i*>(lds + at + c * (16 * kPair)); };
-    auto read_x = [&](uint32_t at, int i) { fx[i] = *reinterpret_cast<const v4i*>(lds + at + i * (16 * kPair)); };
-
-    // A block is one matrix instruction deep.  A wave takes it row tile by row tile; when a row tile is done its fragment is read from the next
-    // block, a block ahead of its use, and the column tiles' fragments into a second set.  So behind the first row tile of a pair's second block all of the pair
-    // is read.  Reads stand behind matrix instructions one by one, and are kept there: their wait for a slot passes while the matrix cores work.
+    const uint32_t place = (q4 ^ swizzle(l16)) * 16, waddr = (wc * 16 * CT + l16) * kPair + place, xaddr = (BN + wr * 16 * RT + l16) * kPair + place;
+    Multiply<CT, RT> m;
+    m.lds         = lds;
     uint32_t slot = 0;    // bytes
-    auto one_block = [&](auto SET) {
-        constexpr int P = decltype(SET)::value;    // which of the pair
-        if constexpr (P == 1)
-            slot = slot + PAIR < R * PAIR ? slot + PAIR : 0;
-        const uint32_t wat = slot + (P == 1 ? waddr : waddr ^ 64), xat = slot + (P == 1 ? xaddr : xaddr ^ 64);
-#pragma unroll
-        for (int i = 0; i < RT; i++)
-        {
-#pragma unroll
-            for (int k = 0; k < CT; k++)
-            {
-                const int c = i & 1 ? CT - 1 - k : k;    // (one operand changes at a time)
-                acc[c][i]   = mma_int8(fw[P][c], fx[i], acc[c][i]);
-                if (i > 0 && (RT >= CT ? k == 2 && i < CT : k >= 1))
-                    read_w(1 - P, wat, RT >= CT ? i : k);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            if (i == 0)
-            {
-                if constexpr (P == 1)
-                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                read_w(1 - P, wat, 0);
-            }
-            read_x(xat, i);
-            __builtin_amdgcn_sched_barrier(0);
-        }
+    auto pair     = [&]() {
+        m.template block<0>(slot + (waddr ^ 64), slot + (xaddr ^ 64), []() {}, [](int) {});
+        slot = slot + PAIR < R * PAIR ? slot + PAIR : 0;
+        m.template block<1>(slot + waddr, slot + xaddr, []() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }, [](int) {});
     };
-    static_assert(RT == 2 || RT >= CT, "where the weights' fragments are read");
-
     asm volatile("s_barrier" ::: "memory");
-#pragma unroll
-    for (int c = 0; c < CT; c++)
-        read_w(0, waddr, c);
-#pragma unroll
-    for (int i = 0; i < RT; i++)
-        read_x(xaddr, i);
-    __builtin_amdgcn_sched_barrier(0);
-
+    m.first(waddr, xaddr);
 #pragma unroll 1
-    for (int t = first_item; t < last_item; t += per_turn)
+    for (int t = items.first; t < items.last; t += items.per_turn)
     {
-        const Item it = item_of(t);
-#pragma unroll
-        for (int c = 0; c < CT; c++)
-#pragma unroll
-            for (int i = 0; i < RT; i++)
-                acc[c][i] = v4i{ 0, 0, 0, 0 };
+        const Item it = items.at(a, t);
+        m.clear();
 #pragma unroll 1
         for (int n = it.block0; n < it.block1; n += 2)
-        {
-            one_block(std::integral_constant<int, 0>());
-            one_block(std::integral_constant<int, 1>());
-        }
-
-        // ---- results: of each of a lane's rows four or two pieces of 16 bytes, of the features of_piece(0), ... on -----------------------
-        constexpr int V = kPiece<Out>, TILES = V / 4;    // (column tiles that a piece comes from)
-        auto of_piece = [&](int p) { return it.n0 + wc * 16 * CT + 16 * TILES * p + V * q4; };
-        float of_row[RT];
-        if constexpr (!SPLIT)
-#pragma unroll
-            for (int i = 0; i < RT; i++)
-            {
-                const int64_t m = it.m0 + (wr * RT + i) * 16 + l16;
-                of_row[i]       = a.x_scales[m < a.M ? m : a.M - 1];
-            }
-#pragma unroll
-        for (int p = 0; p < CT / TILES; p++)
-        {
-            const int64_t n = of_piece(p);
-            float scale[V], bias[V];
-            if constexpr (!SPLIT)
-#pragma unroll
-                for (int e = 0; e < V; e++)
-                {
-                    const int64_t f = n + e < a.N ? n + e : a.N - 1;
-                    scale[e] = a.w_scales[f], bias[e] = a.bias ? bias_at<T>(a.bias, f) : 0.0f;
-                }
-#pragma unroll
-            for (int i = 0; i < RT; i++)
-            {
-                const int64_t m = it.m0 + (wr * RT + i) * 16 + l16;
-                float y[V];
-#pragma unroll
-                for (int e = 0; e < V; e++)
-                {
-                    const int sum = acc[TILES * p + e / 4][i][e & 3];
-                    if constexpr (SPLIT)
-                        y[e] = __int_as_float(sum);
-                    else
-                        y[e] = __builtin_fmaf((float)sum * scale[e], of_row[i], bias[e]);
-                }
-                Out* row = SPLIT ? reinterpret_cast<Out*>(a.part) + ((int64_t)it.split * a.M + m) * a.N : static_cast<Out*>(a.out) + m * a.ldo;
-                if (m < a.M && n < a.N)
-                    store_piece<Out, false>(row + n, 0, (int)(a.N - n < V ? a.N - n : V), piece_of<Out>(y));
-            }
-        }
+            pair();
+        store_tile<T, CT, RT, SPLIT>(a, m.acc, it.n0 + wc * 16 * CT, it.m0 + wr * 16 * RT, it.split, l16, q4);
     }
 }
 
@@ -401,8 +556,8 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a)
 enum
 {
     ROWS,        // linear_rows_kernel
-    TILE_256,    // 256 features x 128 tokens, eight waves that compute and four that load
-    TILE_128,    // 128 x 128, four and four
+    TILE_256,    // linear_wide_kernel
+    TILE_128,    // linear_tile_kernel: 128 x 128, four waves that compute and four that load
     TILE_64      // 64 x 64, two and two, three workgroups a CU
 };
 struct Plan
@@ -452,8 +607,8 @@ Plan plan_of(const tmi_linear_int8_desc_t& d)
             least = us, p = Plan{ kind, splits, per };
     };
     auto per_cu = [](int64_t items) { return (double)((items + 255) / 256); };
-    const int64_t t256 = tiles_of(M, 128) * tiles_of(N, 256), t128 = tiles_of(M, 128) * tiles_of(N, 128), t64 = tiles_of(M, 64) * tiles_of(N, 64);
-    take(TILE_256, 4.5 + per_cu(t256) * (blocks * (t256 >= 200 ? 0.377 : 0.29) + 2.4), 1, blocks);
+    const int64_t t256 = tiles_of(M, 256) * tiles_of(N, 256), t128 = tiles_of(M, 128) * tiles_of(N, 128), t64 = tiles_of(M, 64) * tiles_of(N, 64);
+    take(TILE_256, 4.0 + per_cu(t256) * (blocks * (t256 >= 200 ? 0.76 : 0.57) + 7.0), 1, blocks);
     take(TILE_128, 3.6 + per_cu(t128) * (blocks * (t128 >= 200 ? 0.22 : 0.165) + 2.4), 1, blocks);
     for (int want = 1; want <= kMostSplits && want <= blocks / 2; want++)
     {
@@ -466,19 +621,23 @@ Plan plan_of(const tmi_linear_int8_desc_t& d)
     return p;
 }
 
-template <typename T, int WC, int WR, int RT, int LW, int R, bool SPLIT>
-bool launch_tiles(hipStream_t st, LinearArgs a, int places)
+// `places`: workgroups that are there at once
+template <auto Kernel>
+bool launch_list(hipStream_t st, LinearArgs a, int bm, int bn, int threads, size_t lds, int places)
 {
-    constexpr int BN = 64 * WC, BM = 16 * RT * WR;
-    constexpr size_t lds  = R * (BN + BM) * kPair;
-    constexpr auto kernel = linear_tile_kernel<T, WC, WR, RT, LW, R, SPLIT>;
-    if (!ensure_dynamic_lds<kernel>(lds))
+    if (!ensure_dynamic_lds<Kernel>(lds))
         return false;
-    a.tiles_m = (a.M + BM - 1) / BM, a.tiles_n = (a.N + BN - 1) / BN, a.tiles = a.tiles_m * a.tiles_n;
+    a.tiles_m = (a.M + bm - 1) / bm, a.tiles_n = (a.N + bn - 1) / bn, a.tiles = a.tiles_m * a.tiles_n;
     a.items = a.tiles * a.splits, a.per_xcd = (a.items + 7) / 8;
     const int grid = a.per_xcd * 8 < places ? a.per_xcd * 8 : places;
-    kernel<<<grid, 64 * (WC * WR + LW), lds, st>>>(a);
+    Kernel<<<grid, threads, lds, st>>>(a);
     return true;
+}
+template <typename T, int WC, int WR, int RT, int LW, int R, bool SPLIT>
+bool launch_tiles(hipStream_t st, const LinearArgs& a, int places)
+{
+    constexpr int BN = 64 * WC, BM = 16 * RT * WR;
+    return launch_list<linear_tile_kernel<T, WC, WR, RT, LW, R, SPLIT>>(st, a, BM, BN, 64 * (WC * WR + LW), R * (BN + BM) * kPair, places);
 }
 
 template <int N>
@@ -524,7 +683,7 @@ bool launch_typed(hipStream_t st, const LinearArgs& a, const Plan& p)
     }
     bool ok;
     if (p.kind == TILE_256)
-        ok = launch_tiles<T, 4, 2, 4, 4, 3, false>(st, a, 256);
+        ok = launch_list<linear_wide_kernel<T>>(st, a, 256, 256, 512, 5 * 256 * kPair, 256);
     else if (p.kind == TILE_128)
         ok = launch_tiles<T, 2, 2, 4, 4, 5, false>(st, a, 256);
     else
