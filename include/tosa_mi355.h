@@ -526,7 +526,7 @@ int tmi_rms_norm_int8(tmi_ctx_t* ctx, const tmi_rms_norm_desc_t* d, const void* 
  *   d_x = r (g - n mean(g n)) + d_sum, d_weight = sum over the rows of dy n
  * d_sum_dev (or NULL): the gradient that comes to s from elsewhere.  d_x is the gradient of x and of the residual.  d_x_dev or d_weight_dev NULL:
  * not computed.  d_x may be s, dy or d_sum.  With no rows d_weight is filled with zeros.  d_weight's sums meet in the context's
- * scratch buffer (up to 2 MiB for every 1024 columns). */
+ * scratch buffer (up to 1 MiB for every 1024 columns). */
 int tmi_rms_norm_backward(tmi_ctx_t* ctx, const tmi_rms_norm_desc_t* d, const void* s_dev, const void* weight_dev, const float* rstd_dev,
                           const void* d_y_dev, const void* d_sum_dev, void* d_x_dev, void* d_weight_dev);
 

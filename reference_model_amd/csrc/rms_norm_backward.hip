@@ -7,6 +7,10 @@
 // columns are added over the rows that its workgroup has, without leaving the registers; the workgroups' sums meet in the scratch buffer, [workgroup][width]
 // in 32 bits, and a second kernel adds those in order, so that equal calls give equal bits.
 //
+// 8192 x 4096 in bf16 with d_weight: 46.6 us, 4.3 TB/s (the second kernel 4.8 of them), with d_sum too 55.3; without d_weight 38.1, 5.3 TB/s.  131072 x 128:
+// 25.5.  Waves of a row wait for each other at its sum; a row's loads before the sum of the one ahead of it (prefetched in registers) gave 48.3, a wave for
+// a whole row, whose registers then overflow, 59.4.
+//
 // A row has 16 or 64 lanes of a wave, 256 or 1024 of a workgroup, each with P pieces of 16 bytes.  Longer rows are read twice: once for the means, once by
 // column tiles with the means given.
 #include "tmi_rows.h"
@@ -28,14 +32,14 @@ struct BackArgs
     float offset;
 };
 
-// GIVEN: the means are, and blockIdx.y is a column tile of G P pieces
-template <typename T, int G, int P, bool WHOLE, bool GIVEN>
-__global__ __launch_bounds__(G > 256 ? G : 256) void norm_backward_kernel(BackArgs a)
+// THREADS / G rows at once.  GIVEN: the means are, and blockIdx.y is a column tile of G P pieces
+template <typename T, int THREADS, int G, int P, bool WHOLE, bool GIVEN>
+__global__ __launch_bounds__(THREADS) void norm_backward_kernel(BackArgs a)
 {
-    constexpr int THREADS = G > 256 ? G : 256, ROWS = THREADS / G, V = kPiece<T>;
-    __shared__ uint32_t slots[2][2 * (G > 64 ? G / 64 : 1)];
-    __shared__ float met[ROWS > 1 ? ROWS * G * P * V : 1];
-    const int lane = threadIdx.x % G, width = a.width, first = GIVEN ? (int)blockIdx.y * (G * P * V) : 0;
+    constexpr int ROWS = THREADS / G, V = kPiece<T>, COLUMNS = G * P * V;
+    __shared__ uint32_t slots[2][ROWS][2 * (G > 64 ? G / 64 : 1)];
+    __shared__ __align__(16) float met[ROWS > 1 ? THREADS * V : 1];
+    const int lane = threadIdx.x % G, group = threadIdx.x / G, width = a.width, first = GIVEN ? (int)blockIdx.y * COLUMNS : 0;
     auto at = [&](int p) { return first + (p * G + lane) * V; };
 
     v4i w[P];
@@ -49,8 +53,11 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_backward_kernel(BackAr
             dw[p][e] = 0.0f;
     }
     int slot = 0;
-    for (int64_t m = (int64_t)blockIdx.x * ROWS + threadIdx.x / G; m < a.rows; m += (int64_t)gridDim.x * ROWS)
+    // (the groups of a workgroup go round together, for its barriers; one whose rows are done takes the last row again, and drops what it makes)
+    for (int64_t m0 = (int64_t)blockIdx.x * ROWS; m0 < a.rows; m0 += (int64_t)gridDim.x * ROWS)
     {
+        const bool live = m0 + group < a.rows;
+        const int64_t m = live ? m0 + group : a.rows - 1;
         // (with the means given no barrier stands between a row's reads and its writes)
         auto load = [&](const void* from, int64_t ld, int p) {
             const T* row = static_cast<const T*>(from) + m * ld;
@@ -88,10 +95,16 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_backward_kernel(BackAr
                     part = __builtin_fmaf(piece_get<T>(dy[p], e) * (a.offset + piece_get<T>(w[p], e)), piece_get<T>(s[p], e) * r, part);
                 mean += part;
             }
-            over_row<G, true, false>(mean, none, slots[slot]);
+            over_row<G, true, false>(mean, none, slots[slot][group]);
             slot = 1 - slot;
             mean /= (float)width;
+            // (the pieces wait as they came: as floats they would take twice the registers)
+#pragma unroll
+            for (int p = 0; p < P; p++)
+                asm volatile("" : "+v"(s[p]), "+v"(dy[p]), "+v"(w[p]));
         }
+        if (!live)
+            continue;
 #pragma unroll
         for (int p = 0; p < P; p++)
         {
@@ -112,27 +125,31 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_backward_kernel(BackAr
     float* part = a.part + (int64_t)blockIdx.x * width;
     if constexpr (ROWS > 1)
     {
-        // the workgroup's rows, in order
+        // the groups' sums, in order
 #pragma unroll
         for (int p = 0; p < P; p++)
-#pragma unroll
-            for (int e = 0; e < V; e++)
-                met[(threadIdx.x / G) * (G * P * V) + (p * G + lane) * V + e] = dw[p][e];
-        __syncthreads();
-        for (int k = threadIdx.x; k < G * P * V && k < width; k += THREADS)
         {
-            float sum = 0.0f;
+            __syncthreads();
 #pragma unroll
-            for (int g = 0; g < ROWS; g++)
-                sum += met[g * (G * P * V) + k];
-            part[k] = sum;
+            for (int e = 0; e < V; e += 4)
+                *reinterpret_cast<v4i*>(met + (group * G + lane) * V + e) = piece_of<float>(&dw[p][e]);
+            __syncthreads();
+            for (int k = threadIdx.x; k < G * V && p * G * V + k < width; k += THREADS)
+            {
+                float sum = 0.0f;
+#pragma unroll 4
+                for (int g = 0; g < ROWS; g++)
+                    sum += met[g * G * V + k];
+                part[p * G * V + k] = sum;
+            }
         }
     }
     else
 #pragma unroll
         for (int p = 0; p < P; p++)
-            store_piece<float, false>(part, at(p), width, piece_of<float>(&dw[p][0])),
-                V == 8 ? store_piece<float, false>(part, at(p) + 4, width, piece_of<float>(&dw[p][V - 4])) : void();
+#pragma unroll
+            for (int e = 0; e < V; e += 4)
+                store_piece<float, false>(part, at(p) + e, width, piece_of<float>(&dw[p][e]));
 }
 
 // The means of rows that are too long for the kernel above
@@ -164,14 +181,15 @@ __global__ __launch_bounds__(1024) void norm_mean_kernel(BackArgs a)
     }
 }
 
-// The workgroups' sums: 32 columns and 32 parts of the list a workgroup
+// The workgroups' sums: 32 columns and 32 parts of the list a workgroup (with 16 and 64 the same, with 8 and 128 2.5 us more at 8192 x 4096)
 template <typename T>
 __global__ __launch_bounds__(1024) void norm_join_kernel(BackArgs a)
 {
-    __shared__ float met[32][33];
-    const int column = threadIdx.x & 31, share = threadIdx.x >> 5;
-    const int64_t k  = (int64_t)blockIdx.x * 32 + column;
-    const int each   = (a.groups + 31) / 32, end = (share + 1) * each < a.groups ? (share + 1) * each : a.groups;
+    constexpr int COLUMNS = 32, SHARES = 1024 / COLUMNS;
+    __shared__ float met[SHARES][COLUMNS + 1];
+    const int column = threadIdx.x % COLUMNS, share = threadIdx.x / COLUMNS;
+    const int64_t k  = (int64_t)blockIdx.x * COLUMNS + column;
+    const int each   = (a.groups + SHARES - 1) / SHARES, end = (share + 1) * each < a.groups ? (share + 1) * each : a.groups;
     float sum        = 0.0f;
     if (k < a.width)
 #pragma unroll 8
@@ -182,7 +200,7 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(BackArgs a)
     if (share != 0 || k >= a.width)
         return;
 #pragma unroll
-    for (int i = 1; i < 32; i++)
+    for (int i = 1; i < SHARES; i++)
         sum += met[i][column];
     if constexpr (sizeof(T) == 4)
         static_cast<T*>(a.dw)[k] = sum;
@@ -194,9 +212,9 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(BackArgs a)
 // column and tensor that it reads of its rows.
 struct BackPlan
 {
-    int lanes, pieces, groups, tiles;    // tiles > 1: long rows
+    int threads, lanes, pieces, groups, tiles;    // tiles > 1: long rows
 };
-BackPlan back_plan(int32_t dtype, int64_t rows, int64_t width)
+BackPlan back_plan(int32_t dtype, int64_t rows, int64_t width, bool dw)
 {
     const int v           = dtype == TMI_FP32 ? 4 : 8;
     const int64_t pieces  = (width + v - 1) / v;
@@ -213,8 +231,13 @@ BackPlan back_plan(int32_t dtype, int64_t rows, int64_t width)
         p.lanes = 1024, p.pieces = pieces <= 1024 ? 1 : 2;
         p.tiles = (int)((pieces + 2047) / 2048);
     }
-    const int threads = p.lanes > 256 ? p.lanes : 256, at_once = threads / p.lanes;
-    const int64_t need = (rows + at_once - 1) / at_once, most = 256 * (512 / threads > 1 ? 512 / threads : 1) / (p.tiles < 4 ? p.tiles : 4);
+    // A workgroup's sums are written and read again, and few of them make a short second kernel: 256 workgroups of 1024 threads, one for a CU.  (us with them,
+    // and with 512 of 256 threads: 8192 x 4096 bf16 46.6 and 48.4, 509 x 1930 fp32 9.5 and 11.9, 131072 x 128 bf16 25.5 and 27.5.)  Too few rows to give every
+    // CU such a workgroup have ones of 256 threads: 64 x 4096 6.5 and with 1024 threads 8.1, 128 x 4096 7.5 and 8.3, but 256 x 4096 9.4 and 8.7.  Without
+    // d_weight there are no sums, and each workgroup has its own rows: 8192 x 4096 38.1, with 256 workgroups 41.8.
+    p.threads = p.lanes == 1024 || (dw && rows * p.lanes > 48 * 1024) ? 1024 : 256;
+    const int at_once  = p.threads / p.lanes;
+    const int64_t need = (rows + at_once - 1) / at_once, most = dw ? 256 / (p.tiles < 4 ? p.tiles : 4) : 1 << 20;
     p.groups = (int)(need < most ? need : most);
     return p;
 }
@@ -222,22 +245,27 @@ BackPlan back_plan(int32_t dtype, int64_t rows, int64_t width)
 template <typename T, bool WHOLE>
 void launch_typed(hipStream_t st, const BackArgs& a, const BackPlan& p)
 {
-    auto go = [&](auto kernel) { kernel<<<dim3(p.groups, p.tiles), p.lanes > 256 ? p.lanes : 256, 0, st>>>(a); };
+    auto go = [&](auto kernel) { kernel<<<dim3(p.groups, p.tiles), p.threads, 0, st>>>(a); };
     if (p.groups > 0)
     {
+        const bool many = p.threads == 1024;
         if (p.tiles > 1)
         {
-            norm_mean_kernel<T, WHOLE><<<(int)(a.rows < 512 ? a.rows : 512), 1024, 0, st>>>(a);
-            go(norm_backward_kernel<T, 1024, 2, WHOLE, true>);
+            norm_mean_kernel<T, WHOLE><<<(int)(a.rows < (1 << 20) ? a.rows : 1 << 20), 1024, 0, st>>>(a);
+            go(norm_backward_kernel<T, 1024, 1024, 2, WHOLE, true>);
         }
         else if (p.lanes == 16)
-            go(norm_backward_kernel<T, 16, 1, WHOLE, false>);
+            many ? go(norm_backward_kernel<T, 1024, 16, 1, WHOLE, false>) : go(norm_backward_kernel<T, 256, 16, 1, WHOLE, false>);
+        else if (p.lanes == 64 && p.pieces == 1)
+            many ? go(norm_backward_kernel<T, 1024, 64, 1, WHOLE, false>) : go(norm_backward_kernel<T, 256, 64, 1, WHOLE, false>);
         else if (p.lanes == 64)
-            p.pieces == 1 ? go(norm_backward_kernel<T, 64, 1, WHOLE, false>) : go(norm_backward_kernel<T, 64, 2, WHOLE, false>);
+            many ? go(norm_backward_kernel<T, 1024, 64, 2, WHOLE, false>) : go(norm_backward_kernel<T, 256, 64, 2, WHOLE, false>);
+        else if (p.lanes == 256 && p.pieces == 1)
+            many ? go(norm_backward_kernel<T, 1024, 256, 1, WHOLE, false>) : go(norm_backward_kernel<T, 256, 256, 1, WHOLE, false>);
         else if (p.lanes == 256)
-            p.pieces == 1 ? go(norm_backward_kernel<T, 256, 1, WHOLE, false>) : go(norm_backward_kernel<T, 256, 2, WHOLE, false>);
+            many ? go(norm_backward_kernel<T, 1024, 256, 2, WHOLE, false>) : go(norm_backward_kernel<T, 256, 256, 2, WHOLE, false>);
         else
-            p.pieces == 1 ? go(norm_backward_kernel<T, 1024, 1, WHOLE, false>) : go(norm_backward_kernel<T, 1024, 2, WHOLE, false>);
+            p.pieces == 1 ? go(norm_backward_kernel<T, 1024, 1024, 1, WHOLE, false>) : go(norm_backward_kernel<T, 1024, 1024, 2, WHOLE, false>);
     }
     if (a.dw)
         norm_join_kernel<T><<<(a.width + 31) / 32, 1024, 0, st>>>(a);
@@ -252,14 +280,14 @@ size_t mean_bytes(const BackPlan& p, int64_t rows)
 
 size_t rms_norm_backward_scratch_bytes(const tmi_rms_norm_desc_t& d, bool dw)
 {
-    const BackPlan p = back_plan(d.dtype, d.rows, d.width);
+    const BackPlan p = back_plan(d.dtype, d.rows, d.width, dw);
     return mean_bytes(p, d.rows) + (dw ? (size_t)p.groups * d.width * 4 : 0);
 }
 
 const char* launch_rms_norm_backward(hipStream_t st, const tmi_rms_norm_desc_t& d, const void* s, const void* weight, const float* rstd, const void* d_y,
                                      const void* d_sum, void* d_x, void* d_weight, void* scratch)
 {
-    const BackPlan p = back_plan(d.dtype, d.rows, d.width);
+    const BackPlan p = back_plan(d.dtype, d.rows, d.width, d_weight);
     float* mean      = static_cast<float*>(scratch);
     const BackArgs a{ s, weight, d_y, d_sum, rstd, d_x, d_weight, mean, mean + mean_bytes(p, d.rows) / 4, d.ld_sum, d.ld_y, d.ld_x, d.rows, d.width,
                       p.groups, d.weight_offset };

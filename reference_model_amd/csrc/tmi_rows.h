@@ -143,7 +143,7 @@ __device__ __forceinline__ void over_row(float& sum, uint32_t& most, uint32_t* s
     if constexpr (G > 64)
     {
         constexpr int W = G / 64;
-        const int wave  = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int wave  = __builtin_amdgcn_readfirstlane(threadIdx.x % G >> 6);
         if ((threadIdx.x & 63) == 0)
         {
             if constexpr (SUM)
