@@ -526,7 +526,8 @@ int tmi_rms_norm_int8(tmi_ctx_t* ctx, const tmi_rms_norm_desc_t* d, const void* 
  *   d_x = r (g - n mean(g n)) + d_sum, d_weight = sum over the rows of dy n
  * d_sum_dev (or NULL): the gradient that comes to s from elsewhere.  d_x is the gradient of x and of the residual.  d_x_dev or d_weight_dev NULL:
  * not computed.  d_x may be s, dy or d_sum.  With no rows d_weight is filled with zeros.  d_weight's sums meet in the context's
- * scratch buffer (up to 1 MiB for every 1024 columns). */
+ * scratch buffer (tmi_ctx_reserve_workspace; up to 1 MiB for every 1024 columns), and rows of more than 8192 elements (fp32), or 16384, need it
+ * for their means: a captured call for which it would have to grow is refused. */
 int tmi_rms_norm_backward(tmi_ctx_t* ctx, const tmi_rms_norm_desc_t* d, const void* s_dev, const void* weight_dev, const float* rstd_dev,
                           const void* d_y_dev, const void* d_sum_dev, void* d_x_dev, void* d_weight_dev);
 
@@ -538,8 +539,8 @@ int tmi_dequantize_int8(tmi_ctx_t* ctx, int32_t dtype, int32_t rows, int32_t wid
 
 /* y[m][n] = x_scales[m] w_scales[n] sum_k x[m][k] w[n][k] + bias[n]: x [rows][in_features] and w [out_features][in_features] in 8 bits, y
  * [rows][out_features] and bias (or NULL) of dtype.  ld_x and ld_w count bytes, ld_y elements.  The sum is exact: in_features is at most
- * 131071.  It is rounded to 32 bits before it is scaled.  Some calls of more than 64 rows use the context's scratch buffer for partial sums; where it
- * cannot grow (while a graph is captured) they go on without it, to the same bits. */
+ * 131071.  It is rounded to 32 bits before it is scaled.  Some calls split it, and use the context's scratch buffer for the parts; where
+ * that cannot grow (while a graph is captured) they go on without it, to the same bits. */
 typedef struct
 {
     int64_t ld_x, ld_w, ld_y;
@@ -616,6 +617,10 @@ int tmi_debug_tile_decode(int64_t grid, uint32_t n_ocb, uint32_t tiles_x, uint32
  * Used by the unit tests, which choose their sizes by it. */
 int tmi_debug_gated_ffn_plan(const tmi_gated_ffn_desc_t* d, const void* x_dev, const void* gate_dev, const void* up_dev, int32_t product,
                              int64_t* out8);
+
+/* Host arithmetic only: out2 receives the rows of tmi_linear_int8's tiles (0: the kernel of few rows has the call) and into how many parts its
+ * sums are split, given scratch.  TMI_ERROR where the call is refused.  Used by the unit tests, which choose their sizes by it. */
+int tmi_debug_linear_int8_plan(const tmi_linear_int8_desc_t* d, int64_t* out2);
 
 /* Library build identification, e.g. "tosa_mi355 gfx950". */
 const char* tmi_version(void);

@@ -42,6 +42,7 @@ EXPORTS = [
     "tmi_gated_ffn", "tmi_gated_ffn_backward",
     "tmi_rms_norm", "tmi_rms_norm_int8", "tmi_rms_norm_backward", "tmi_quantize_int8", "tmi_dequantize_int8", "tmi_linear_int8",
     "tmi_debug_launch_empty", "tmi_debug_tile_decode", "tmi_debug_last_launch_shape", "tmi_debug_stream", "tmi_debug_gated_ffn_plan",
+    "tmi_debug_linear_int8_plan",
 ]
 
 NOALLOC_SCRATCH_BYTES = 16 << 20  # TMI_NOALLOC_SCRATCH_BYTES
@@ -215,6 +216,7 @@ def load_library() -> ctypes.CDLL:
     lib.tmi_rms_norm_backward.argtypes = [vp, norm] + [vp] * 7
     lib.tmi_quantize_int8.argtypes = [vp, i32, i32, i32, vp, i64, vp, i64, vp]
     lib.tmi_dequantize_int8.argtypes = [vp, i32, i32, i32, vp, i64, vp, vp, i64]
+    lib.tmi_debug_linear_int8_plan.argtypes = [ctypes.POINTER(LinearInt8Desc), ctypes.POINTER(i64)]
     lib.tmi_linear_int8.argtypes = [vp, ctypes.POINTER(LinearInt8Desc)] + [vp] * 6
     lib.tmi_conv2d_check.argtypes = [vp, ctypes.POINTER(ConvDesc), i32]
     lib.tmi_rescale_check.argtypes = [vp, ctypes.POINTER(RescaleDesc), i32, i32]

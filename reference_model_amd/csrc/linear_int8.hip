@@ -578,11 +578,12 @@ int64_t tiles_of(int64_t n, int64_t per)
     return (n + per - 1) / per;
 }
 
-// What linear_rows_kernel takes, us
+// What linear_rows_kernel takes, us: the turns of a workgroup's waves, the weights' bytes out of memory, or all bytes out of the L2s, whichever is longest.  (1 x
+// 16384 x 1024, 64 workgroups of four long turns: 11.3, split in four 8.5)
 double rows_us(int64_t M, int64_t N, int blocks)
 {
     const int rt       = M > 48 ? 4 : (int)tiles_of(M, 16);
-    const double turns = (double)tiles_of(blocks, rt > 1 ? 16 : blocks >= 64 ? 64 : 32) * (rt > 1 ? 1.0 + 0.12 * rt : 1.1);
+    const double turns = (double)tiles_of(blocks, rt > 1 ? 16 : blocks >= 64 ? 64 : 32) * (rt > 1 ? 1.0 + 0.12 * rt : blocks >= 64 ? 2.2 : 1.1);
     const double w = (double)N * blocks * 64, x = (double)(M < 64 ? M : tiles_of(M, 64) * 64) * tiles_of(N, 16) * blocks * 64;
     const double bytes = w * tiles_of(M, 64) / 6.2e6, all = (w * tiles_of(M, 64) + x) / 8.5e6;
     return 2.0 + (turns > bytes ? (turns > all ? turns : all) : bytes > all ? bytes : all);
@@ -592,6 +593,21 @@ double join_us(int64_t M, int64_t N, int splits)
     return splits > 1 ? 2.3 + (double)M * N * 8 * splits / 7.5e6 : 0;
 }
 
+// The kernel, and into how many parts its columns are split, with the least time by a model of each: a fixed part, and for each tile that a CU goes through its
+// blocks' time and its border's.  Many tiles run at a lower clock, and share the L2s' bytes.  Measured, us rows x in_features x out_features:
+//
+//                         rows   tiles of 64, split in 1, 2, 4   of 128   of 256
+//     16 x 4096 x 4096     6.6     12.2    10.3     9.6           13.7
+//     33 x 4096 x 4096     8.9     12.7    10.7    10.4           14.6
+//     64 x 4096 x 4096    12.4     12.7    11.1    11.4           15.0
+//    128 x 4096 x 4096    21.1     13.0    12.1    14.9           15.7
+//    256 x 4096 x 4096    38.5     13.6    16.6    21.0           16.1     42
+//    512 x 4096 x 4096             18.5    25.6                   16.5     42
+//   2048 x 4096 x 4096             57.7                           37.3     48.6
+//   4096 x 4096 x 4096            105                             67.7     58.3
+//   1500 x 8192 x 8192            160                            100.2     91.0
+//   1000 x 777 x 9000              23.2                           22.7     19.2
+//   300 x 16384 x 1024    65.6     37.5    23.5    21.1           43.4    142
 Plan plan_of(const tmi_linear_int8_desc_t& d)
 {
     const int64_t M = d.rows, N = d.out_features;
@@ -694,6 +710,13 @@ bool launch_typed(hipStream_t st, const LinearArgs& a, const Plan& p)
 }
 
 }    // namespace
+
+void linear_int8_plan(const tmi_linear_int8_desc_t& d, int64_t* out2)
+{
+    const Plan p           = plan_of(d);
+    constexpr int tokens[] = { 0, 256, 128, 64 };
+    out2[0] = tokens[p.kind], out2[1] = p.splits;
+}
 
 size_t linear_int8_scratch_bytes(const tmi_linear_int8_desc_t& d)
 {

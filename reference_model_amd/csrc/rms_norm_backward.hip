@@ -8,8 +8,8 @@
 // in 32 bits, and a second kernel adds those in order, so that equal calls give equal bits.
 //
 // 8192 x 4096 in bf16 with d_weight: 46.6 us, 4.3 TB/s (the second kernel 4.8 of them), with d_sum too 55.3; without d_weight 38.1, 5.3 TB/s.  131072 x 128:
-// 25.5.  Waves of a row wait for each other at its sum; a row's loads before the sum of the one ahead of it (prefetched in registers) gave 48.3, a wave for
-// a whole row, whose registers then overflow, 59.4.
+// 25.5.  A row's loads before the sum of the one ahead of it gave the same 46.2, and 1 us more where a workgroup has one or two rows; a wave for a whole row,
+// whose registers then overflow, 59.4.
 //
 // A row has 16 or 64 lanes of a wave, 256 or 1024 of a workgroup, each with P pieces of 16 bytes.  Longer rows are read twice: once for the means, once by
 // column tiles with the means given.

@@ -2529,9 +2529,18 @@ static int validate_linear_int8(tmi_ctx* ctx, const tmi_linear_int8_desc_t* d, t
         return fail_int8_rows(ctx, op, d->in_features, d->ld_w);
     if (!row_stride(out.ld_y, d->out_features, d->rows))
         return fail(ctx, "%s: rows of %d elements cannot lie %lld apart", op, d->out_features, (long long)d->ld_y);
-    // tiles are counted in 31 bits, and blocks of 64 rows in 16
-    if (d->rows > 65535 * 64 || d->out_features > (1 << 28) || ((int64_t)d->rows / 128 + 1) * ((int64_t)d->out_features / 128 + 1) > (int64_t(1) << 26))
+    // tiles are counted in 31 bits, blocks of 64 rows in 16, and threads of 16 features' workgroups in 32
+    if (d->rows > 65535 * 64 || d->out_features > (1 << 25) || ((int64_t)d->rows / 128 + 1) * ((int64_t)d->out_features / 128 + 1) > (int64_t(1) << 26))
         return fail(ctx, "%s: %d rows, %d x %d weights are more than one call takes", op, d->rows, d->out_features, d->in_features);
+    return TMI_VALID;
+}
+
+int tmi_debug_linear_int8_plan(const tmi_linear_int8_desc_t* desc, int64_t* out2)
+{
+    tmi_linear_int8_desc_t d;
+    if (!out2 || validate_linear_int8(nullptr, desc, d) != TMI_VALID)
+        return TMI_ERROR;
+    linear_int8_plan(d, out2);
     return TMI_VALID;
 }
 
