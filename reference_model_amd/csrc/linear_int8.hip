@@ -119,32 +119,56 @@ __device__ __forceinline__ uint32_t lds_address(const uint8_t* p)
     return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p;
 }
 
-// The results of a wave's CT x RT instruction tiles from feature n0 and token m0 on: of each of a lane's rows pieces of 16 bytes
-template <typename T, int CT, int RT, bool SPLIT>
-__device__ __forceinline__ void store_tile(const LinearArgs& a, const v4i (&acc)[CT][RT], int64_t n0, int64_t m0, int split, int l16, int q4)
+// A lane's part of what a wave's CT x RT instruction tiles from feature n0 and token m0 on are multiplied by: asked for before their sum and used behind it (us
+// asked for behind it 777 x 1111 x 2731 13.6, now 12.6; 1 x 4096 x 4096 6.7 and 6.4; 2048 x 4096 x 4096 37.5 and 36.8).
+template <typename T, int CT, int RT>
+struct Scales
 {
-    using Out       = std::conditional_t<SPLIT, float, T>;    // (a partial sum is a word, as a float is)
-    constexpr int V = kPiece<Out>, TILES = V / 4;             // (column tiles that a piece comes from)
-    float of_row[RT];
-    if constexpr (!SPLIT)
+    static constexpr int V = CT == 1 ? 4 : kPiece<T>, TILES = V / 4;    // (neighbours that a lane has, and column tiles that they come from)
+    float of_row[RT], scale[CT * 4];
+    using Bits = std::conditional_t<sizeof(T) == 4, float, uint16_t>;
+    Bits bias[CT * 4];
+    __device__ __forceinline__ void ask(const LinearArgs& a, int64_t n0, int64_t m0, int l16, int q4)
+    {
 #pragma unroll
         for (int i = 0; i < RT; i++)
         {
             const int64_t m = m0 + i * 16 + l16;
             of_row[i]       = a.x_scales[m < a.M ? m : a.M - 1];
         }
+        // (no bias: other bits of that size, which are not used.  Loads in a branch would be waited for at its end)
+        const Bits* from = static_cast<const Bits*>(a.bias ? a.bias : a.w_scales);
+#pragma unroll
+        for (int p = 0; p < CT / TILES; p++)
+#pragma unroll
+            for (int e = 0; e < V; e++)
+            {
+                const int64_t n = n0 + 16 * TILES * p + V * q4 + e, f = n < a.N ? n : a.N - 1;
+                scale[p * V + e] = a.w_scales[f], bias[p * V + e] = from[f];
+            }
+    }
+    __device__ __forceinline__ float of(const LinearArgs& a, int sum, int at, int i) const
+    {
+        float b;
+        if constexpr (sizeof(T) == 4)
+            b = bias[at];
+        else
+            b = from_bits16<T>(bias[at]);
+        return __builtin_fmaf((float)sum * scale[at], of_row[i], a.bias ? b : 0.0f);
+    }
+};
+
+// The results of those tiles: of each of a lane's rows pieces of 16 bytes
+template <typename T, int CT, int RT, bool SPLIT>
+__device__ __forceinline__ void store_tile(const LinearArgs& a, const v4i (&acc)[CT][RT], const Scales<T, CT, RT>& scales, int64_t n0, int64_t m0, int split, int l16,
+                                           int q4)
+{
+    using Out       = std::conditional_t<SPLIT, float, T>;    // (a partial sum is a word, as a float is)
+    constexpr int V = kPiece<Out>, TILES = V / 4;
 #pragma unroll
     for (int p = 0; p < CT / TILES; p++)
     {
         const int64_t n = n0 + 16 * TILES * p + V * q4;
-        float scale[V], bias[V];
-        if constexpr (!SPLIT)
-#pragma unroll
-            for (int e = 0; e < V; e++)
-            {
-                const int64_t f = n + e < a.N ? n + e : a.N - 1;
-                scale[e] = a.w_scales[f], bias[e] = a.bias ? bias_at<T>(a.bias, f) : 0.0f;
-            }
 #pragma unroll
         for (int i = 0; i < RT; i++)
         {
@@ -157,7 +181,7 @@ __device__ __forceinline__ void store_tile(const LinearArgs& a, const v4i (&acc)
                 if constexpr (SPLIT)
                     y[e] = __int_as_float(sum);
                 else
-                    y[e] = __builtin_fmaf((float)sum * scale[e], of_row[i], bias[e]);
+                    y[e] = scales.of(a, sum, p * V + e, i);
             }
             Out* row = SPLIT ? reinterpret_cast<Out*>(a.part) + ((int64_t)split * a.M + m) * a.N : static_cast<Out*>(a.out) + m * a.ldo;
             if (m < a.M && n < a.N)
@@ -332,14 +356,16 @@ __global__ __launch_bounds__(512, 2) void linear_wide_kernel(LinearArgs a)
 #pragma unroll 1
         for (int n = it.block0; n < it.block1; n += 2)
             pair();
-        store_tile<T, CT, RT, false>(a, m.acc, it.n0 + wc * 64, it.m0 + wr * 128, 0, l16, q4);
+        Scales<T, CT, RT> scales;
+        scales.ask(a, it.n0 + wc * 64, it.m0 + wr * 128, l16, q4);
+        store_tile<T, CT, RT, false>(a, m.acc, scales, it.n0 + wc * 64, it.m0 + wr * 128, 0, l16, q4);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 // WC x WR waves (features x tokens) that compute, of 64 features and 16 RT tokens each, and LW that load; LDS holds R pairs of blocks.  A wave that has loads to
 // request waits for each of them (some 50 cycles; 110 where two share a SIMD), which those that compute need not do here, nor wait for the loads or for their own
-// stores.  us with waves that do both 256 x 4096 x 4096 17.5 (now 12.8), 1024 x 4096 x 4096 23.7 (19.7), 512 x 8192 x 8192 40.8 (33.1).  SPLIT: partial sums.
+// stores.  us with waves that do both 256 x 4096 x 4096 17.5 (now 12.5), 1024 x 4096 x 4096 23.7 (19.3), 512 x 8192 x 8192 40.8 (32.5).  SPLIT: partial sums.
 template <typename T, int WC, int WR, int RT, int LW, int R, bool SPLIT>
 __global__ __launch_bounds__(64 * (WC * WR + LW), (WC * WR + LW) / 4) void linear_tile_kernel(LinearArgs a)
 {
@@ -431,11 +457,14 @@ __global__ __launch_bounds__(64 * (WC * WR + LW), (WC * WR + LW) / 4) void linea
     for (int t = items.first; t < items.last; t += items.per_turn)
     {
         const Item it = items.at(a, t);
+        Scales<T, CT, RT> scales;
+        if constexpr (!SPLIT)
+            scales.ask(a, it.n0 + wc * 16 * CT, it.m0 + wr * 16 * RT, l16, q4);
         m.clear();
 #pragma unroll 1
         for (int n = it.block0; n < it.block1; n += 2)
             pair();
-        store_tile<T, CT, RT, SPLIT>(a, m.acc, it.n0 + wc * 16 * CT, it.m0 + wr * 16 * RT, it.split, l16, q4);
+        store_tile<T, CT, RT, SPLIT>(a, m.acc, scales, it.n0 + wc * 16 * CT, it.m0 + wr * 16 * RT, it.split, l16, q4);
     }
 }
 
@@ -495,6 +524,13 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a)
     for (int i = 0; i < RT; i++)
         acc[i] = v4i{ 0, 0, 0, 0 };
 
+    // (of the result that thread tid < 64 RT adds up)
+    static_assert(RT <= WAVES, "a result a thread");
+    const int64_t m = m0 + (wave < RT ? wave : 0) * 16 + l16, n = n0 + 4 * q4;
+    Scales<T, 1, 1> scales;
+    if constexpr (!SPLIT)
+        scales.ask(a, n, m - l16, l16, 0);
+
     const int pairs = a.blocks / 2, first = SPLIT ? (int)blockIdx.z * (a.per_split / 2) : 0;
     const int last  = SPLIT && first + a.per_split / 2 < pairs ? first + a.per_split / 2 : pairs;
 #pragma unroll 1
@@ -526,29 +562,23 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a)
     for (int i = 0; i < RT; i++)
         met[wave][i * 64 + lane] = acc[i];
     __syncthreads();
+    if (tid >= RT * 64)
+        return;
+    v4i v = met[0][tid];
 #pragma unroll
-    for (int u = tid; u < RT * 64; u += 64 * WAVES)
-    {
-        v4i v = met[0][u];
+    for (int k = 1; k < WAVES; k++)
+        v += met[k][tid];
+    if (m >= a.M)
+        return;
 #pragma unroll
-        for (int k = 1; k < WAVES; k++)
-            v += met[k][u];
-        const int l = u & 63;
-        const int64_t m = m0 + (u >> 6) * 16 + (l & 15), n = n0 + 4 * (l >> 4);
-        if (m >= a.M)
-            continue;
-        const float of_row = SPLIT ? 1.0f : a.x_scales[m];
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (n + e < a.N)
-            {
-                if constexpr (SPLIT)
-                    a.part[((int64_t)blockIdx.z * a.M + m) * a.N + n + e] = v[e];
-                else
-                    store_one<T>(a.out, m * a.ldo + n + e,
-                                 __builtin_fmaf((float)v[e] * a.w_scales[n + e], of_row, a.bias ? bias_at<T>(a.bias, n + e) : 0.0f));
-            }
-    }
+    for (int e = 0; e < 4; e++)
+        if (n + e < a.N)
+        {
+            if constexpr (SPLIT)
+                a.part[((int64_t)blockIdx.z * a.M + m) * a.N + n + e] = v[e];
+            else
+                store_one<T>(a.out, m * a.ldo + n + e, scales.of(a, v[e], e, 0));
+        }
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
@@ -597,17 +627,17 @@ double join_us(int64_t M, int64_t N, int splits)
 // blocks' time and its border's.  Many tiles run at a lower clock, and share the L2s' bytes.  Measured, us rows x in_features x out_features:
 //
 //                         rows   tiles of 64, split in 1, 2, 4   of 128   of 256
-//     16 x 4096 x 4096     6.6     12.2    10.3     9.6           13.7
-//     33 x 4096 x 4096     8.9     12.7    10.7    10.4           14.6
-//     64 x 4096 x 4096    12.4     12.7    11.1    11.4           15.0
-//    128 x 4096 x 4096    21.1     13.0    12.1    14.9           15.7
-//    256 x 4096 x 4096    38.5     13.6    16.6    21.0           16.1     42
-//    512 x 4096 x 4096             18.5    25.6                   16.5     42
-//   2048 x 4096 x 4096             57.7                           37.3     48.6
-//   4096 x 4096 x 4096            105                             67.7     58.3
-//   1500 x 8192 x 8192            160                            100.2     91.0
-//   1000 x 777 x 9000              23.2                           22.7     19.2
-//   300 x 16384 x 1024    65.6     37.5    23.5    21.1           43.4    142
+//     16 x 4096 x 4096     6.5     11.7    10.4     9.7           13.6
+//     33 x 4096 x 4096     8.5     12.0    10.8    10.5           14.2
+//     64 x 4096 x 4096    11.9     12.1    11.3    11.5           14.5
+//    128 x 4096 x 4096    20.9     12.5    12.4    15.2           15.2
+//    256 x 4096 x 4096    38.9     13.4    16.8    21.1           15.7     41.3
+//    512 x 4096 x 4096             17.0    24.5                   15.9     41.5
+//   2048 x 4096 x 4096             52.7                           33.4     43.9
+//   4096 x 4096 x 4096             98.5                           63.1     55.8
+//   1500 x 8192 x 8192            150                             97.1     87.2
+//   1000 x 777 x 9000              21.9                           20.8     18.2
+//   300 x 16384 x 1024    64.9     35.6    23.4    21.0           42.6    141
 Plan plan_of(const tmi_linear_int8_desc_t& d)
 {
     const int64_t M = d.rows, N = d.out_features;
