@@ -618,9 +618,9 @@ int tmi_debug_tile_decode(int64_t grid, uint32_t n_ocb, uint32_t tiles_x, uint32
 int tmi_debug_gated_ffn_plan(const tmi_gated_ffn_desc_t* d, const void* x_dev, const void* gate_dev, const void* up_dev, int32_t product,
                              int64_t* out8);
 
-/* Host arithmetic only: out2 receives the rows of tmi_linear_int8's tiles (0: the kernel of few rows has the call) and into how many parts its
- * sums are split, given scratch.  TMI_ERROR where the call is refused.  Used by the unit tests, which choose their sizes by it. */
-int tmi_debug_linear_int8_plan(const tmi_linear_int8_desc_t* d, int64_t* out2);
+/* Host arithmetic only: out3 receives the rows and features of tmi_linear_int8's tiles (0 rows: the kernel of few rows has the call) and into how
+ * many parts its sums are split, given scratch.  TMI_ERROR where the call is refused.  Used by the unit tests, which choose their sizes by it. */
+int tmi_debug_linear_int8_plan(const tmi_linear_int8_desc_t* d, int64_t* out3);
 
 /* Library build identification, e.g. "tosa_mi355 gfx950". */
 const char* tmi_version(void);

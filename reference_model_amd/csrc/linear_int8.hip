@@ -366,7 +366,8 @@ __global__ __launch_bounds__(512, 2) void linear_wide_kernel(LinearArgs a)
 
 // WC x WR waves (features x tokens) that compute, of 64 features and 16 RT tokens each, and LW that load; LDS holds R pairs of blocks.  A wave that has loads to
 // request waits for each of them (some 50 cycles; 110 where two share a SIMD), which those that compute need not do here, nor wait for the loads or for their own
-// stores.  us with waves that do both 256 x 4096 x 4096 17.5 (now 12.5), 1024 x 4096 x 4096 23.7 (19.3), 512 x 8192 x 8192 40.8 (32.5).  SPLIT: partial sums.
+// stores.  us with waves that do both 256 x 4096 x 4096 17.5 (now 10.6), 1024 x 4096 x 4096 23.7 (19.8), 512 x 8192 x 8192 40.8 (32.5).  Tiles of 64 with two waves
+// that load and three workgroups a CU 13.4 at 256 x 4096 x 4096, one workgroup of eight pairs 11.2.  SPLIT: partial sums.
 template <typename T, int WC, int WR, int RT, int LW, int R, bool SPLIT>
 __global__ __launch_bounds__(64 * (WC * WR + LW), (WC * WR + LW) / 4) void linear_tile_kernel(LinearArgs a)
 {
@@ -590,7 +591,8 @@ enum
     ROWS,        // linear_rows_kernel
     TILE_256,    // linear_wide_kernel
     TILE_128,    // linear_tile_kernel: 128 x 128, four waves that compute and four that load
-    TILE_64      // 64 x 64, two and two, three workgroups a CU
+    TILE_LONG,   // 128 tokens x 64 features, four and four, two workgroups a CU
+    TILE_64      // 64 x 64, two and four, two workgroups a CU
 };
 struct Plan
 {
@@ -617,29 +619,31 @@ double rows_us(int64_t M, int64_t N, int blocks)
     const int rt       = M > 48 ? 4 : (int)tiles_of(M, 16);
     const double turns = (double)tiles_of(blocks, rt > 1 ? 16 : blocks >= 64 ? 64 : 32) * (rt > 1 ? 1.0 + 0.12 * rt : blocks >= 64 ? 2.2 : 1.1);
     const double w = (double)N * blocks * 64, x = (double)(M < 64 ? M : tiles_of(M, 64) * 64) * tiles_of(N, 16) * blocks * 64;
-    const double bytes = w * tiles_of(M, 64) / 6.2e6, all = (w * tiles_of(M, 64) + x) / 8.5e6;
+    const double bytes = w * tiles_of(M, 64) / 6.2e6, all = (w * tiles_of(M, 64) + x) / 7.6e6;
     return 2.0 + (turns > bytes ? (turns > all ? turns : all) : bytes > all ? bytes : all);
 }
 double join_us(int64_t M, int64_t N, int splits)
 {
-    return splits > 1 ? 2.3 + (double)M * N * 8 * splits / 7.5e6 : 0;
+    return splits > 1 ? 3.3 + (double)M * N * 8 * splits / 4e6 : 0;
 }
 
 // The kernel, and into how many parts its columns are split, with the least time by a model of each: a fixed part, and for each tile that a CU goes through its
 // blocks' time and its border's.  Many tiles run at a lower clock, and share the L2s' bytes.  Measured, us rows x in_features x out_features:
 //
-//                         rows   tiles of 64, split in 1, 2, 4   of 128   of 256
-//     16 x 4096 x 4096     6.5     11.7    10.4     9.7           13.6
-//     33 x 4096 x 4096     8.5     12.0    10.8    10.5           14.2
-//     64 x 4096 x 4096    11.9     12.1    11.3    11.5           14.5
-//    128 x 4096 x 4096    20.9     12.5    12.4    15.2           15.2
-//    256 x 4096 x 4096    38.9     13.4    16.8    21.1           15.7     41.3
-//    512 x 4096 x 4096             17.0    24.5                   15.9     41.5
-//   2048 x 4096 x 4096             52.7                           33.4     43.9
-//   4096 x 4096 x 4096             98.5                           63.1     55.8
-//   1500 x 8192 x 8192            150                             97.1     87.2
-//   1000 x 777 x 9000              21.9                           20.8     18.2
-//   300 x 16384 x 1024    64.9     35.6    23.4    21.0           42.6    141
+//                         rows   tiles of 64, split in 1, 2, 4   128 x 64   128     256
+//     16 x 4096 x 4096     6.4      9.6     9.5     9.4          11.8     13.5    38
+//     33 x 4096 x 4096     8.7     10.0     9.9    10.2          12.1     14.2    38
+//     64 x 4096 x 4096    12.1     10.0    10.3    11.3          12.2     14.4    39
+//    256 x 4096 x 4096    39.3     10.6    16.1    19.8          13.2     15.6    41
+//    512 x 4096 x 4096             16.6    24.5                  14.3     16.3    41
+//    768 x 4096 x 4096             21.6                          21.5     17.0    42
+//   2048 x 4096 x 4096             54.3                          44.8     35.2    47
+//   4096 x 4096 x 4096            104                            84       64.4    56.6
+//   1500 x 8192 x 8192            156                           128       99.4    88.7
+//    300 x 1111 x 5003    17.7      8.6    18.5    20.9           7.8     10.1    24
+//   2048 x 1024 x 1024              7.9    20.5                   6.7      8.5    17
+//   1000 x 777 x 9000              23.4                          19.7     20.9    18.2
+//    300 x 16384 x 1024   64.6     27.8    19.9    19.4          37.4     42.7   142
 Plan plan_of(const tmi_linear_int8_desc_t& d)
 {
     const int64_t M = d.rows, N = d.out_features;
@@ -654,15 +658,18 @@ Plan plan_of(const tmi_linear_int8_desc_t& d)
         if (us < least)
             least = us, p = Plan{ kind, splits, per };
     };
+    auto tiles  = [&](int bm, int bn) { return tiles_of(M, bm) * tiles_of(N, bn); };
     auto per_cu = [](int64_t items) { return (double)((items + 255) / 256); };
-    const int64_t t256 = tiles_of(M, 256) * tiles_of(N, 256), t128 = tiles_of(M, 128) * tiles_of(N, 128), t64 = tiles_of(M, 64) * tiles_of(N, 64);
+    const int64_t t256 = tiles(256, 256), t128 = tiles(128, 128), t64 = tiles(64, 64);
+    const double n_long = per_cu(tiles(128, 64));
     take(TILE_256, 4.0 + per_cu(t256) * (blocks * (t256 >= 200 ? 0.76 : 0.57) + 7.0), 1, blocks);
-    take(TILE_128, 3.6 + per_cu(t128) * (blocks * (t128 >= 200 ? 0.22 : 0.165) + 2.4), 1, blocks);
+    take(TILE_128, 3.6 + per_cu(t128) * (blocks * (t128 >= 200 ? 0.2 : 0.16) + 2.4), 1, blocks);
+    take(TILE_LONG, 3.6 + n_long * (blocks * 0.13 + (n_long > 1 ? 1.4 : 1.0)), 1, blocks);
     for (int want = 1; want <= kMostSplits && want <= blocks / 2; want++)
     {
         const int per = (blocks / 2 + want - 1) / want * 2, splits = (blocks + per - 1) / per;
         const double n = per_cu(t64 * splits);
-        take(TILE_64, 3.6 + per * (0.105 * n > 0.145 ? 0.105 * n : 0.145) + 0.7 * n + join_us(M, N, splits), splits, per);
+        take(TILE_64, 3.6 + per * (n > 1 ? 0.085 * n : 0.09) + 0.7 * n + join_us(M, N, splits), splits, per);
         if (M <= 64 && splits > 1)
             take(ROWS, rows_us(M, N * splits, per) + join_us(M, N, splits), splits, per);
     }
@@ -734,8 +741,10 @@ bool launch_typed(hipStream_t st, const LinearArgs& a, const Plan& p)
         ok = launch_list<linear_wide_kernel<T>>(st, a, 256, 256, 512, 5 * 256 * kPair, 256);
     else if (p.kind == TILE_128)
         ok = launch_tiles<T, 2, 2, 4, 4, 5, false>(st, a, 256);
+    else if (p.kind == TILE_LONG)
+        ok = launch_tiles<T, 1, 4, 2, 4, 3, false>(st, a, 512);
     else
-        ok = p.splits > 1 ? launch_tiles<float, 1, 2, 2, 2, 3, true>(st, a, 768) : launch_tiles<T, 1, 2, 2, 2, 3, false>(st, a, 768);
+        ok = p.splits > 1 ? launch_tiles<float, 1, 2, 2, 4, 4, true>(st, a, 512) : launch_tiles<T, 1, 2, 2, 4, 4, false>(st, a, 512);
     if (ok)
         launch_join<T>(st, a);
     return ok;
@@ -743,11 +752,12 @@ bool launch_typed(hipStream_t st, const LinearArgs& a, const Plan& p)
 
 }    // namespace
 
-void linear_int8_plan(const tmi_linear_int8_desc_t& d, int64_t* out2)
+void linear_int8_plan(const tmi_linear_int8_desc_t& d, int64_t* out3)
 {
-    const Plan p           = plan_of(d);
-    constexpr int tokens[] = { 0, 256, 128, 64 };
-    out2[0] = tokens[p.kind], out2[1] = p.splits;
+    const Plan p             = plan_of(d);
+    constexpr int tokens[]   = { 0, 256, 128, 128, 64 };
+    constexpr int features[] = { 16, 256, 128, 64, 64 };
+    out3[0] = tokens[p.kind], out3[1] = features[p.kind], out3[2] = p.splits;
 }
 
 size_t linear_int8_scratch_bytes(const tmi_linear_int8_desc_t& d)

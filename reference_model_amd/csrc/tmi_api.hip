@@ -2535,12 +2535,12 @@ static int validate_linear_int8(tmi_ctx* ctx, const tmi_linear_int8_desc_t* d, t
     return TMI_VALID;
 }
 
-int tmi_debug_linear_int8_plan(const tmi_linear_int8_desc_t* desc, int64_t* out2)
+int tmi_debug_linear_int8_plan(const tmi_linear_int8_desc_t* desc, int64_t* out3)
 {
     tmi_linear_int8_desc_t d;
-    if (!out2 || validate_linear_int8(nullptr, desc, d) != TMI_VALID)
+    if (!out3 || validate_linear_int8(nullptr, desc, d) != TMI_VALID)
         return TMI_ERROR;
-    linear_int8_plan(d, out2);
+    linear_int8_plan(d, out3);
     return TMI_VALID;
 }
 

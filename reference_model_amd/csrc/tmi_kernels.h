@@ -376,7 +376,7 @@ size_t rms_norm_backward_scratch_bytes(const tmi_rms_norm_desc_t& d, bool dw);
 const char* launch_rms_norm_backward(hipStream_t st, const tmi_rms_norm_desc_t& d, const void* s, const void* weight, const float* rstd, const void* d_y,
                                      const void* d_sum, void* d_x, void* d_weight, void* scratch);
 // linear_int8.hip: `scratch` of as many bytes as the first function says, or nullptr: sums in one piece; zeros: 64 bytes of them
-void linear_int8_plan(const tmi_linear_int8_desc_t& d, int64_t* out2);
+void linear_int8_plan(const tmi_linear_int8_desc_t& d, int64_t* out3);
 size_t linear_int8_scratch_bytes(const tmi_linear_int8_desc_t& d);
 const char* launch_linear_int8(hipStream_t st, const tmi_linear_int8_desc_t& d, const void* x, const float* x_scales, const void* w, const float* w_scales,
                                const void* bias, void* y, void* scratch, const void* zeros);

@@ -10,10 +10,10 @@ from reference_model_amd import Context, TmiError, capi  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
-# rows, out_features, in_features of every kernel of the linear layer: rows of its tiles (0: the one of few rows), and whether the sum is split
-KINDS_OF_FORMS = [((1, 1000, 700), 0, False), ((9, 200, 16400), 0, True), ((20, 300, 500), 0, False), ((40, 300, 500), 0, False), ((60, 300, 500), 0, False),
-                  ((30, 100, 9000), 0, True), ((300, 500, 200), 64, False), ((200, 300, 5000), 64, True), ((900, 4000, 1000), 128, False),
-                  ((3600, 3700, 700), 256, False)]
+# rows, out_features, in_features of every kernel of the linear layer: rows (0: the one of few rows) and features of its tiles, and whether the sum is split
+KINDS_OF_FORMS = [((1, 1000, 700), 0, 16, False), ((9, 200, 16400), 0, 16, True), ((20, 300, 500), 0, 16, False), ((40, 300, 500), 0, 16, False),
+                  ((60, 300, 500), 0, 16, False), ((30, 100, 9000), 0, 16, True), ((300, 500, 200), 64, 64, False), ((200, 300, 12000), 64, 64, True),
+                  ((300, 5003, 1111), 128, 64, False), ((500, 4000, 1000), 128, 64, False), ((900, 4000, 1000), 128, 128, False), ((3600, 3700, 700), 256, 256, False)]
 FORMS = [f[0] for f in KINDS_OF_FORMS]
 
 
@@ -183,7 +183,7 @@ def test_every_form_into_two_graphs_that_take_turns(ctx, shape):
         assert torch.equal(a.y, want[0])
 
 
-@pytest.mark.parametrize("shape", [f[0] for f in KINDS_OF_FORMS if f[2]], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("shape", [f[0] for f in KINDS_OF_FORMS if f[3]], ids=lambda s: "x".join(map(str, s)))
 def test_sums_in_one_piece_where_the_scratch_buffer_cannot_grow(shape):
     c = Context(0)
     try:
@@ -323,9 +323,10 @@ def test_8_bits_beyond_32_bits(ctx):
     near(wide(back), want, kind.rounding(want))
 
 
-@pytest.mark.parametrize("shape,ld_x,ld_w,ld_y", [((3, 50, 40), 1 << 31, 1 << 27, 1 << 31), ((300, 300, 96), (1 << 23) - 16, (1 << 23) - 16, 1 << 24),
-                                                  ((200, 300, 5000), (1 << 23) - 16, 1 << 13, 1 << 25), ((900, 4000, 1000), 5 << 20, 1 << 12, 5 << 20),
-                                                  ((3600, 3700, 192), 5 << 18, 5 << 18, 5 << 18)], ids=["few", "64", "split", "128", "256"])
+@pytest.mark.parametrize("shape,ld_x,ld_w,ld_y", [
+    ((3, 50, 40), 1 << 31, 1 << 27, 1 << 31), ((300, 300, 96), (1 << 23) - 16, (1 << 23) - 16, 1 << 24), ((200, 300, 12000), (1 << 23) - 16, 1 << 14, 1 << 25),
+    ((500, 4000, 1000), 9 << 20, 1 << 12, 9 << 20), ((900, 4000, 1000), 5 << 20, 1 << 12, 5 << 20), ((3600, 3700, 192), 5 << 18, 5 << 18, 5 << 18)],
+    ids=["few", "64", "split", "128x64", "128", "256"])
 def test_linear_beyond_32_bits(ctx, shape, ld_x, ld_w, ld_y):
     """tensors of more than 4 GiB each but the weights of some"""
     kind, (m, n, k) = KINDS["bf16"], shape

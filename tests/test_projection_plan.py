@@ -8,14 +8,14 @@ from projection_plan import plan  # noqa: E402
 
 
 def test_every_kernel_is_reached():
-    seen = {(p.tile, p.splits > 1) for p in (plan(*s) for s in sizes.FEW + sizes.MANY + use.FORMS)}
-    assert seen == {(0, False), (0, True), (64, False), (64, True), (128, False), (256, False)}
+    seen = {(p.tile, p.features, p.splits > 1) for p in (plan(*s) for s in sizes.FEW + sizes.MANY + use.FORMS)}
+    assert seen == {(0, 16, False), (0, 16, True), (64, 64, False), (64, 64, True), (128, 64, False), (128, 128, False), (256, 256, False)}
 
 
-@pytest.mark.parametrize("shape,tile,split", use.KINDS_OF_FORMS)
-def test_forms(shape, tile, split):
+@pytest.mark.parametrize("shape,tile,features,split", use.KINDS_OF_FORMS)
+def test_forms(shape, tile, features, split):
     p = plan(*shape)
-    assert p.tile == tile and (p.splits > 1) == split
+    assert (p.tile, p.features) == (tile, features) and (p.splits > 1) == split
 
 
 def test_rows_that_lie_far_apart_are_no_tiles():
@@ -30,7 +30,7 @@ def test_few_rows_are_no_large_tiles():
             for m in (1, 16, 33):
                 p = plan(m, n, k)
                 assert p.tile <= 64 and 1 <= p.splits <= 16
-            assert plan(m, n, 0) == (0, 1)
+            assert plan(m, n, 0) == (0, 16, 1)
 
 
 def test_none_where_the_call_is_refused():
