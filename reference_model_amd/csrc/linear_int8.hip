@@ -470,36 +470,32 @@ __global__ __launch_bounds__(64 * (WC * WR + LW), (WC * WR + LW) / 4) void linea
     }
 }
 
-// Results of a sum that was split, four of a row a thread: integers, so the order does not matter.  Its launch and its reads take 2.5 to 3 us where there is little of it
-template <typename T>
+// Results of a sum that was split into up to J parts, four of a row a thread: integers, so the order does not matter.  All parts are asked for at once (past the
+// last one it again): one after the other 128 x 16384 x 1024 in eight parts took 13.3 us, now 11.6, 72 x 3646 x 201 in 15 11.1 and 7.6.
+template <typename T, int J>
 __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a)
 {
-    const int64_t n = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (n >= a.N)
+    const int64_t own = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (own >= a.N)
         return;
-    const int live      = a.N - n < 4 ? (int)(a.N - n) : 4;
-    const int64_t plane = (int64_t)a.M * a.N;
+    // (a row's last thread has its last four, some of which are its neighbour's; the buffer has room for four of a shorter row behind its end)
+    const int64_t n = own + 4 <= a.N ? own : a.N >= 4 ? a.N - 4 : 0, plane = (int64_t)a.M * a.N;
     for (int64_t m = blockIdx.y; m < a.M; m += gridDim.y)
     {
-        v4i v = { 0, 0, 0, 0 };
-        for (int s = 0; s < a.splits; s++)
-        {
-            const int32_t* at = a.part + s * plane + m * a.N + n;
-            v4i t             = { 0, 0, 0, 0 };
-            if (live == 4)
-                __builtin_memcpy(&t, at, 16);
-            else
+        Scales<T, 1, 1> scales;
+        scales.ask(a, n, m, 0, 0);
+        v4i t[J], v = { 0, 0, 0, 0 };
 #pragma unroll
-                for (int e = 0; e < 3; e++)
-                    if (e < live)
-                        t[e] = at[e];
-            v += t;
-        }
-        const float xs = a.x_scales[m];
+        for (int s = 0; s < J; s++)
+            __builtin_memcpy(&t[s], a.part + (s < a.splits ? s : a.splits - 1) * plane + m * a.N + n, 16);
+#pragma unroll
+        for (int s = 0; s < J; s++)
+            if (s < a.splits)
+                v += t[s];
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            if (e < live)
-                store_one<T>(a.out, m * a.ldo + n + e, __builtin_fmaf((float)v[e] * a.w_scales[n + e], xs, a.bias ? bias_at<T>(a.bias, n + e) : 0.0f));
+            if (n + e >= own && n + e < a.N)
+                store_one<T>(a.out, m * a.ldo + n + e, scales.of(a, v[e], e, 0));
     }
 }
 
@@ -590,7 +586,8 @@ enum
 {
     ROWS,        // linear_rows_kernel
     TILE_256,    // linear_wide_kernel
-    TILE_128,    // linear_tile_kernel: 128 x 128, four waves that compute and four that load
+    TILE_BROAD,  // linear_tile_kernel: 128 tokens x 256 features, eight waves that compute and four that load
+    TILE_128,    // 128 x 128, four and four
     TILE_LONG,   // 128 tokens x 64 features, four and four, two workgroups a CU
     TILE_64      // 64 x 64, two and four, two workgroups a CU
 };
@@ -613,37 +610,40 @@ int64_t tiles_of(int64_t n, int64_t per)
 }
 
 // What linear_rows_kernel takes, us: the turns of a workgroup's waves, the weights' bytes out of memory, or all bytes out of the L2s, whichever is longest.  (1 x
-// 16384 x 1024, 64 workgroups of four long turns: 11.3, split in four 8.5)
+// 16384 x 1024, 64 workgroups of four long turns: 11.2, split in four 7.6)
 double rows_us(int64_t M, int64_t N, int blocks)
 {
     const int rt       = M > 48 ? 4 : (int)tiles_of(M, 16);
-    const double turns = (double)tiles_of(blocks, rt > 1 ? 16 : blocks >= 64 ? 64 : 32) * (rt > 1 ? 1.0 + 0.12 * rt : blocks >= 64 ? 2.2 : 1.1);
+    const double turns = (double)tiles_of(blocks, rt > 1 ? 16 : blocks >= 64 ? 64 : 32) * (rt > 1 ? 0.45 * rt : blocks >= 64 ? 2.2 : 1.1);
     const double w = (double)N * blocks * 64, x = (double)(M < 64 ? M : tiles_of(M, 64) * 64) * tiles_of(N, 16) * blocks * 64;
     const double bytes = w * tiles_of(M, 64) / 6.2e6, all = (w * tiles_of(M, 64) + x) / 7.6e6;
     return 2.0 + (turns > bytes ? (turns > all ? turns : all) : bytes > all ? bytes : all);
 }
 double join_us(int64_t M, int64_t N, int splits)
 {
-    return splits > 1 ? 3.3 + (double)M * N * 8 * splits / 4e6 : 0;
+    return splits > 1 ? 2.2 + (double)M * N * 8 * splits / 3.6e6 : 0;
 }
 
 // The kernel, and into how many parts its columns are split, with the least time by a model of each: a fixed part, and for each tile that a CU goes through its
-// blocks' time and its border's.  Many tiles run at a lower clock, and share the L2s' bytes.  Measured, us rows x in_features x out_features:
+// blocks' time and its border's.  Many tiles run at a lower clock, and share the L2s' bytes.  Of 40
+// drawn sizes its choice is within 0.2 % of the best of all on average, and 14 % at most.  Measured, us rows x in_features x out_features:
 //
-//                         rows   tiles of 64, split in 1, 2, 4   128 x 64   128     256
-//     16 x 4096 x 4096     6.4      9.6     9.5     9.4          11.8     13.5    38
-//     33 x 4096 x 4096     8.7     10.0     9.9    10.2          12.1     14.2    38
-//     64 x 4096 x 4096    12.1     10.0    10.3    11.3          12.2     14.4    39
-//    256 x 4096 x 4096    39.3     10.6    16.1    19.8          13.2     15.6    41
-//    512 x 4096 x 4096             16.6    24.5                  14.3     16.3    41
-//    768 x 4096 x 4096             21.6                          21.5     17.0    42
-//   2048 x 4096 x 4096             54.3                          44.8     35.2    47
-//   4096 x 4096 x 4096            104                            84       64.4    56.6
-//   1500 x 8192 x 8192            156                           128       99.4    88.7
-//    300 x 1111 x 5003    17.7      8.6    18.5    20.9           7.8     10.1    24
-//   2048 x 1024 x 1024              7.9    20.5                   6.7      8.5    17
-//   1000 x 777 x 9000              23.4                          19.7     20.9    18.2
-//    300 x 16384 x 1024   64.6     27.8    19.9    19.4          37.4     42.7   142
+//                         rows   tiles of 64, split in 1, 2, 4   128 x 64   128     128 x 256   256
+//     16 x 4096 x 4096     6.4      9.6     9.5     9.4          11.8     13.5                 38
+//     33 x 4096 x 4096     8.7     10.0     9.9    10.2          12.1     14.2                 38
+//     64 x 4096 x 4096    11.9     10.0    10.0    10.5          12.3     14.4                 39
+//    256 x 4096 x 4096    39.3     10.6    16.1    19.8          13.2     15.6                 41
+//    512 x 4096 x 4096             16.6    24.5                  14.3     16.3                 41
+//   1024 x 4096 x 4096             30.4    42.8                  23.3     20.1      25.0       43
+//   1536 x 4096 x 4096             41.6    58.9                  33.6     31.8      28.2       45
+//   2048 x 4096 x 4096             54.3    75.5                  44.8     36.0      34.1       47
+//   4096 x 4096 x 4096            104                            84       65        62.6       57.5
+//   1500 x 8192 x 8192            156                           128      100       110         89
+//    300 x 1111 x 5003    17.7      8.6    18.5    20.9           7.8     10.1                 24
+//   2048 x 1024 x 1024              7.9    20.5                   6.7      8.5                 17
+//   1000 x 777 x 9000              23.4                          19.7     20.9                 18.2
+//    300 x 16384 x 1024   65.7     27.7    20.0    19.3          37.4     42.8                141
+//     64 x 4096 x 1024    11.4     10.0     9.4     8.2          10.8     14.3                 39      (rows, split in four: 7.9)
 Plan plan_of(const tmi_linear_int8_desc_t& d)
 {
     const int64_t M = d.rows, N = d.out_features;
@@ -660,9 +660,10 @@ Plan plan_of(const tmi_linear_int8_desc_t& d)
     };
     auto tiles  = [&](int bm, int bn) { return tiles_of(M, bm) * tiles_of(N, bn); };
     auto per_cu = [](int64_t items) { return (double)((items + 255) / 256); };
-    const int64_t t256 = tiles(256, 256), t128 = tiles(128, 128), t64 = tiles(64, 64);
+    const int64_t t256 = tiles(256, 256), t_broad = tiles(128, 256), t128 = tiles(128, 128), t64 = tiles(64, 64);
     const double n_long = per_cu(tiles(128, 64));
     take(TILE_256, 4.0 + per_cu(t256) * (blocks * (t256 >= 200 ? 0.76 : 0.57) + 7.0), 1, blocks);
+    take(TILE_BROAD, 3.6 + per_cu(t_broad) * (blocks * (t_broad >= 200 ? 0.41 : 0.3) + 3.6), 1, blocks);
     take(TILE_128, 3.6 + per_cu(t128) * (blocks * (t128 >= 200 ? 0.2 : 0.16) + 2.4), 1, blocks);
     take(TILE_LONG, 3.6 + n_long * (blocks * 0.13 + (n_long > 1 ? 1.4 : 1.0)), 1, blocks);
     for (int want = 1; want <= kMostSplits && want <= blocks / 2; want++)
@@ -670,7 +671,7 @@ Plan plan_of(const tmi_linear_int8_desc_t& d)
         const int per = (blocks / 2 + want - 1) / want * 2, splits = (blocks + per - 1) / per;
         const double n = per_cu(t64 * splits);
         take(TILE_64, 3.6 + per * (n > 1 ? 0.085 * n : 0.09) + 0.7 * n + join_us(M, N, splits), splits, per);
-        if (M <= 64 && splits > 1)
+        if (M <= 256 && splits > 1)
             take(ROWS, rows_us(M, N * splits, per) + join_us(M, N, splits), splits, per);
     }
     return p;
@@ -701,8 +702,13 @@ constexpr std::integral_constant<int, N> number_of{};
 template <typename T>
 void launch_join(hipStream_t st, const LinearArgs& a)
 {
-    if (a.splits > 1)
-        linear_join_kernel<T><<<dim3((a.N + 1023) / 1024, a.M < 32768 ? a.M : 32768), 256, 0, st>>>(a);
+    const dim3 grid((a.N + 1023) / 1024, a.M < 32768 ? a.M : 32768);
+    if (a.splits > 8)
+        linear_join_kernel<T, kMostSplits><<<grid, 256, 0, st>>>(a);
+    else if (a.splits > 4)
+        linear_join_kernel<T, 8><<<grid, 256, 0, st>>>(a);
+    else if (a.splits > 1)
+        linear_join_kernel<T, 4><<<grid, 256, 0, st>>>(a);
 }
 
 template <typename T>
@@ -739,6 +745,8 @@ bool launch_typed(hipStream_t st, const LinearArgs& a, const Plan& p)
     bool ok;
     if (p.kind == TILE_256)
         ok = launch_list<linear_wide_kernel<T>>(st, a, 256, 256, 512, 5 * 256 * kPair, 256);
+    else if (p.kind == TILE_BROAD)
+        ok = launch_tiles<T, 4, 2, 4, 4, 3, false>(st, a, 256);
     else if (p.kind == TILE_128)
         ok = launch_tiles<T, 2, 2, 4, 4, 5, false>(st, a, 256);
     else if (p.kind == TILE_LONG)
@@ -755,15 +763,15 @@ bool launch_typed(hipStream_t st, const LinearArgs& a, const Plan& p)
 void linear_int8_plan(const tmi_linear_int8_desc_t& d, int64_t* out3)
 {
     const Plan p             = plan_of(d);
-    constexpr int tokens[]   = { 0, 256, 128, 128, 64 };
-    constexpr int features[] = { 16, 256, 128, 64, 64 };
+    constexpr int tokens[]   = { 0, 256, 128, 128, 128, 64 };
+    constexpr int features[] = { 16, 256, 256, 128, 64, 64 };
     out3[0] = tokens[p.kind], out3[1] = features[p.kind], out3[2] = p.splits;
 }
 
 size_t linear_int8_scratch_bytes(const tmi_linear_int8_desc_t& d)
 {
     const Plan p = plan_of(d);
-    return p.splits > 1 ? (size_t)p.splits * d.rows * d.out_features * 4 : 0;
+    return p.splits > 1 ? (size_t)p.splits * d.rows * d.out_features * 4 + 16 : 0;
 }
 
 const char* launch_linear_int8(hipStream_t st, const tmi_linear_int8_desc_t& d, const void* x, const float* x_scales, const void* w, const float* w_scales,

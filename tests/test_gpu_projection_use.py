@@ -5,6 +5,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import projection_reference as ref  # noqa: E402
+from projection_plan import plan  # noqa: E402
 from projection_reference import KINDS, near  # noqa: E402
 from reference_model_amd import Context, TmiError, capi  # noqa: E402
 
@@ -13,7 +14,8 @@ pytestmark = pytest.mark.gpu
 # rows, out_features, in_features of every kernel of the linear layer: rows (0: the one of few rows) and features of its tiles, and whether the sum is split
 KINDS_OF_FORMS = [((1, 1000, 700), 0, 16, False), ((9, 200, 16400), 0, 16, True), ((20, 300, 500), 0, 16, False), ((40, 300, 500), 0, 16, False),
                   ((60, 300, 500), 0, 16, False), ((30, 100, 9000), 0, 16, True), ((300, 500, 200), 64, 64, False), ((200, 300, 12000), 64, 64, True),
-                  ((300, 5003, 1111), 128, 64, False), ((500, 4000, 1000), 128, 64, False), ((900, 4000, 1000), 128, 128, False), ((3600, 3700, 700), 256, 256, False)]
+                  ((300, 5003, 1111), 128, 64, False), ((500, 4000, 1000), 128, 64, False), ((900, 4000, 1000), 128, 128, False),
+                  ((2000, 4090, 1000), 128, 256, False), ((3600, 3700, 700), 256, 256, False)]
 FORMS = [f[0] for f in KINDS_OF_FORMS]
 
 
@@ -211,6 +213,18 @@ def test_sums_in_one_piece_where_the_scratch_buffer_cannot_grow(shape):
         c.close()
 
 
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 63, 1023, 1025])
+@pytest.mark.parametrize("m", [1, 9, 70])
+def test_split_sums_of_any_width(ctx, m, n):
+    """joined in fours, of which a row's last begin inside its neighbour's"""
+    for k in (5000, 9000, 60000):
+        assert plan(m, n, k).splits > 1
+        p = Product(ctx, (m, n, k), n + k, "bf16")
+        p.call()
+        assert ctx.sync() == capi.VALID
+        p.check()
+
+
 def test_gradients_that_need_scratch_are_refused_where_it_cannot_grow():
     c = Context(0)
     try:
@@ -325,8 +339,9 @@ def test_8_bits_beyond_32_bits(ctx):
 
 @pytest.mark.parametrize("shape,ld_x,ld_w,ld_y", [
     ((3, 50, 40), 1 << 31, 1 << 27, 1 << 31), ((300, 300, 96), (1 << 23) - 16, (1 << 23) - 16, 1 << 24), ((200, 300, 12000), (1 << 23) - 16, 1 << 14, 1 << 25),
-    ((500, 4000, 1000), 9 << 20, 1 << 12, 9 << 20), ((900, 4000, 1000), 5 << 20, 1 << 12, 5 << 20), ((3600, 3700, 192), 5 << 18, 5 << 18, 5 << 18)],
-    ids=["few", "64", "split", "128x64", "128", "256"])
+    ((500, 4000, 1000), 9 << 20, 1 << 12, 9 << 20), ((900, 4000, 1000), 5 << 20, 1 << 12, 5 << 20),
+    ((2000, 4090, 1000), 5 << 19, 1 << 12, 5 << 19), ((3600, 3700, 192), 5 << 18, 5 << 18, 5 << 18)],
+    ids=["few", "64", "split", "128x64", "128", "128x256", "256"])
 def test_linear_beyond_32_bits(ctx, shape, ld_x, ld_w, ld_y):
     """tensors of more than 4 GiB each but the weights of some"""
     kind, (m, n, k) = KINDS["bf16"], shape
