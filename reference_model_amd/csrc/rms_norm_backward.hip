@@ -32,6 +32,8 @@ struct BackArgs
     float offset;
 };
 
+constexpr int kMostGroups = 256;    // workgroups that leave sums
+
 // THREADS / G rows at once.  GIVEN: the means are, and blockIdx.y is a column tile of G P pieces
 template <typename T, int THREADS, int G, int P, bool WHOLE, bool GIVEN>
 __global__ __launch_bounds__(THREADS) void norm_backward_kernel(BackArgs a)
@@ -189,12 +191,25 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(BackArgs a)
     __shared__ float met[SHARES][COLUMNS + 1];
     const int column = threadIdx.x % COLUMNS, share = threadIdx.x / COLUMNS;
     const int64_t k  = (int64_t)blockIdx.x * COLUMNS + column;
-    const int each   = (a.groups + SHARES - 1) / SHARES, end = (share + 1) * each < a.groups ? (share + 1) * each : a.groups;
-    float sum        = 0.0f;
-    if (k < a.width)
-#pragma unroll 8
-        for (int g = share * each; g < end; g++)
-            sum += a.part[(int64_t)g * a.width + k];
+    constexpr int MOST = kMostGroups / SHARES;
+    const int each = (a.groups + SHARES - 1) / SHARES, first = share * each;
+    const int64_t column_of = k < a.width ? k : a.width - 1;
+    // (all of them asked for at once, past the last one it again: one after the other 509 x 1930 9.5 us, now 9.0)
+    float sum = 0.0f;
+    if (a.groups > 0)    // (no rows: zeros)
+    {
+        float t[MOST];
+#pragma unroll
+        for (int i = 0; i < MOST; i++)
+        {
+            const int g = i < each && first + i < a.groups ? first + i : a.groups - 1;
+            t[i]        = a.part[(int64_t)g * a.width + column_of];
+        }
+#pragma unroll
+        for (int i = 0; i < MOST; i++)
+            if (i < each && first + i < a.groups)
+                sum += t[i];
+    }
     met[share][column] = sum;
     __syncthreads();
     if (share != 0 || k >= a.width)
@@ -232,12 +247,12 @@ BackPlan back_plan(int32_t dtype, int64_t rows, int64_t width, bool dw)
         p.tiles = (int)((pieces + 2047) / 2048);
     }
     // A workgroup's sums are written and read again, and few of them make a short second kernel: 256 workgroups of 1024 threads, one for a CU.  (us with them,
-    // and with 512 of 256 threads: 8192 x 4096 bf16 46.6 and 48.4, 509 x 1930 fp32 9.5 and 11.9, 131072 x 128 bf16 25.5 and 27.5.)  Too few rows to give every
+    // and with 512 of 256 threads: 8192 x 4096 bf16 46.6 and 48.4, 509 x 1930 fp32 9.0 and 11.9, 131072 x 128 bf16 25.5 and 27.5.)  Too few rows to give every
     // CU such a workgroup have ones of 256 threads: 64 x 4096 6.5 and with 1024 threads 8.1, 128 x 4096 7.5 and 8.3, but 256 x 4096 9.4 and 8.7.  Without
     // d_weight there are no sums, and each workgroup has its own rows: 8192 x 4096 38.1, with 256 workgroups 41.8.
     p.threads = p.lanes == 1024 || (dw && rows * p.lanes > 48 * 1024) ? 1024 : 256;
     const int at_once  = p.threads / p.lanes;
-    const int64_t need = (rows + at_once - 1) / at_once, most = dw ? 256 / (p.tiles < 4 ? p.tiles : 4) : 1 << 20;
+    const int64_t need = (rows + at_once - 1) / at_once, most = dw ? kMostGroups / (p.tiles < 4 ? p.tiles : 4) : 1 << 20;
     p.groups = (int)(need < most ? need : most);
     return p;
 }
