@@ -609,24 +609,23 @@ int64_t tiles_of(int64_t n, int64_t per)
     return (n + per - 1) / per;
 }
 
-// What linear_rows_kernel takes, us: the turns of a workgroup's waves, the weights' bytes out of memory, or all bytes out of the L2s, whichever is longest.  (1 x
-// 16384 x 1024, 64 workgroups of four long turns: 11.2, split in four 7.6)
+// What linear_rows_kernel takes, us: a CU's bytes, of x too, at 28 or 33 a nanosecond (45 where few CUs ask), or all weights out of memory, whichever is longer.  (1 x 16384 x 1024, 64
+// workgroups: 11.2, split in four 7.6; 1 x 17776 x 5008, where some CUs have two: 22.5 and 18.0)
 double rows_us(int64_t M, int64_t N, int blocks)
 {
-    const int rt       = M > 48 ? 4 : (int)tiles_of(M, 16);
-    const double turns = (double)tiles_of(blocks, rt > 1 ? 16 : blocks >= 64 ? 64 : 32) * (rt > 1 ? 0.45 * rt : blocks >= 64 ? 2.2 : 1.1);
-    const double w = (double)N * blocks * 64, x = (double)(M < 64 ? M : tiles_of(M, 64) * 64) * tiles_of(N, 16) * blocks * 64;
-    const double bytes = w * tiles_of(M, 64) / 6.2e6, all = (w * tiles_of(M, 64) + x) / 7.6e6;
-    return 2.0 + (turns > bytes ? (turns > all ? turns : all) : bytes > all ? bytes : all);
+    const int64_t groups = tiles_of(N, 16) * tiles_of(M, 64);
+    const double of_cu   = (double)tiles_of(groups, 256) * (16 + (M < 64 ? M : 64)) * blocks * 64 / (groups <= 32 ? 45e3 : M <= 16 ? 28e3 : 33e3);
+    const double all     = (double)N * blocks * 64 * tiles_of(M, 64) / 6.2e6;
+    return 2.0 + (of_cu > all ? of_cu : all);
 }
 double join_us(int64_t M, int64_t N, int splits)
 {
-    return splits > 1 ? 2.2 + (double)M * N * 8 * splits / 3.6e6 : 0;
+    return splits > 1 ? 3.0 + (double)M * N * 8 * splits / 3.6e6 : 0;
 }
 
 // The kernel, and into how many parts its columns are split, with the least time by a model of each: a fixed part, and for each tile that a CU goes through its
-// blocks' time and its border's.  Many tiles run at a lower clock, and share the L2s' bytes.  Of 40
-// drawn sizes its choice is within 0.2 % of the best of all on average, and 14 % at most.  Measured, us rows x in_features x out_features:
+// blocks' time and its border's.  Many tiles run at a lower clock, and share the L2s' bytes.  Of 81
+// drawn sizes its choice is within 1.3 % of the best of all on average, and 17 % at most.  Measured, us rows x in_features x out_features:
 //
 //                         rows   tiles of 64, split in 1, 2, 4   128 x 64   128     128 x 256   256
 //     16 x 4096 x 4096     6.4      9.6     9.5     9.4          11.8     13.5                 38
@@ -654,8 +653,12 @@ Plan plan_of(const tmi_linear_int8_desc_t& d)
     if (far || blocks == 0)
         return p;
     double least = M <= 256 ? rows_us(M, N, blocks) : 1e30;
-    auto take    = [&](int kind, double us, int splits, int per) {
-        if (us < least)
+    const double memory = 3.6 + (double)(M + N) * blocks * 64 / 6e6;    // (tiles: no faster than their operands come)
+    auto take           = [&](int kind, double us, int splits, int per) {
+        if (kind != ROWS && us < memory)
+            us = memory;
+        us += join_us(M, N, splits);
+        if (us * (splits > 1 ? 1.1 : 1.0) < least)    // (split where that is clearly less)
             least = us, p = Plan{ kind, splits, per };
     };
     auto tiles  = [&](int bm, int bn) { return tiles_of(M, bm) * tiles_of(N, bn); };
@@ -670,9 +673,9 @@ Plan plan_of(const tmi_linear_int8_desc_t& d)
     {
         const int per = (blocks / 2 + want - 1) / want * 2, splits = (blocks + per - 1) / per;
         const double n = per_cu(t64 * splits);
-        take(TILE_64, 3.6 + per * (n > 1 ? 0.085 * n : 0.09) + 0.7 * n + join_us(M, N, splits), splits, per);
+        take(TILE_64, 3.6 + per * (n > 1 ? 0.085 * n : 0.09) + 0.7 * n, splits, per);
         if (M <= 256 && splits > 1)
-            take(ROWS, rows_us(M, N * splits, per) + join_us(M, N, splits), splits, per);
+            take(ROWS, rows_us(M, N * splits, per), splits, per);
     }
     return p;
 }

