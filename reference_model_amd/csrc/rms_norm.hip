@@ -9,7 +9,7 @@
 // r max |s (offset + w)|, so the one trip over the lanes that adds the squares finds the maximum too, q is s (offset + w) times 127 over that
 // maximum, and r only enters the scale.
 //
-// A row has 16 or 64 lanes of a wave, 256 or 1024 of a workgroup, each with P pieces of 16 bytes; longer rows are read a second time (norm_long_kernel).
+// A row has 8 to 64 lanes of a wave, 256 or 1024 of a workgroup, each with P pieces of 16 bytes; longer rows are read a second time (norm_long_kernel).
 // us and TB/s: 4096 x 8192 fp16 with residual and sum 48.2, 5.6 (a copy of as many bytes runs at 6.1); 131072 x 128 bf16 12 to 13.5, 5.3; 4096 x 4096 bf16 with residual and
 // sum 25.9, 5.2, into 8 bits 24.8, 4.7; 16384 x 4096 bf16 into 8 bits 37.7, 5.3, and back 36 to 38, 5.4; one row of 4096 3.2.  Rows of 4095 elements, read in words:
 // 32.2 for 25.9, 29.5 for 24.8, 41.8 for 37.7.  Rows of 8-byte stores: 16 bytes joined from two lanes gave the same (36.5 for 36.4).
@@ -365,20 +365,25 @@ constexpr std::integral_constant<int, N> number_of{};
 template <typename T>
 constexpr int kMostPieces = 16 * 1024 / kPiece<T>;
 
-// lanes of a row and pieces of a lane, from the pieces that a row has
+// lanes of a row and pieces of a lane, from the pieces that a row has.  (us with lanes of a row for 16 or 64 pieces at least: 262144 x 64 bf16 21.0, with 8 lanes 13.5;
+// 44157 x 168 16.2, with 32 9.3)
 template <typename T, int MODE, bool WHOLE>
 void launch_typed(hipStream_t st, const NormArgs& a)
 {
     const int64_t pieces = ((MODE == NORM ? a.width : whole16(a.width)) + kPiece<T> - 1) / kPiece<T>;
     auto go = [&](auto G_tag, auto P_tag) {
         constexpr int G = decltype(G_tag)::value, P = decltype(P_tag)::value, THREADS = G > 256 ? G : 256, ROWS = THREADS / G;
-        // (short rows: as many workgroups as there are at once, which keep the weights; longer ones a workgroup each.  us 131072 x 128 12.1 and 12.8, 16384 x
-        // 4096 into 8 bits 38.4 and 36.4, 8192 x 4096 with a residual 51.0 and 46.7)
-        const int64_t groups = (a.rows + ROWS - 1) / ROWS, most = G == 16 ? 2048 : 1 << 20;
+        // (short rows: as many workgroups as there are at once, which keep the weights; longer ones a workgroup each.  us 131072 x 128 12.1 and 12.8, 44157 x 168
+        // 9.4 and 10.3, 16384 x 4096 into 8 bits 38.4 and 36.4, 8192 x 4096 with a residual 51.0 and 46.7)
+        const int64_t groups = (a.rows + ROWS - 1) / ROWS, most = G <= 32 ? 2048 : 1 << 20;
         norm_kernel<T, MODE, G, P, WHOLE><<<(int)(groups < most ? groups : most), THREADS, 0, st>>>(a);
     };
-    if (pieces <= 16)
+    if (pieces <= 8)
+        go(number_of<8>, number_of<1>);
+    else if (pieces <= 16)
         go(number_of<16>, number_of<1>);
+    else if (pieces <= 32)
+        go(number_of<32>, number_of<1>);
     else if (pieces <= 64)
         go(number_of<64>, number_of<1>);
     else if (pieces <= 128)

@@ -11,7 +11,7 @@
 // 25.5.  A row's loads before the sum of the one ahead of it gave the same 46.2, and 1 us more where a workgroup has one or two rows; a wave for a whole row,
 // whose registers then overflow, 59.4.
 //
-// A row has 16 or 64 lanes of a wave, 256 or 1024 of a workgroup, each with P pieces of 16 bytes.  Longer rows are read twice: once for the means, once by
+// A row has 8 to 64 lanes of a wave, 256 or 1024 of a workgroup, each with P pieces of 16 bytes.  Longer rows are read twice: once for the means, once by
 // column tiles with the means given.
 #include "tmi_rows.h"
 
@@ -223,7 +223,8 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(BackArgs a)
         static_cast<uint16_t*>(a.dw)[k] = to_bits16<T>(sum);
 }
 
-// Lanes of a row, its pieces a lane, and how many workgroups share the rows.  Each of those leaves 4 bytes a column for the second kernel, against b bytes a
+// Lanes of a row (us with 16 at least 262144 x 64 bf16 34.0, with eight 26.6; with 64 instead of 32 44157 x 168 23.2 and 16.2), its pieces a lane, and how many
+// workgroups share the rows.  Each of those leaves 4 bytes a column for the second kernel, against b bytes a
 // column and tensor that it reads of its rows.
 struct BackPlan
 {
@@ -235,8 +236,12 @@ BackPlan back_plan(int32_t dtype, int64_t rows, int64_t width, bool dw)
     const int64_t pieces  = (width + v - 1) / v;
     BackPlan p{};
     p.tiles = 1;
-    if (pieces <= 16)
+    if (pieces <= 8)
+        p.lanes = 8, p.pieces = 1;
+    else if (pieces <= 16)
         p.lanes = 16, p.pieces = 1;
+    else if (pieces <= 32)
+        p.lanes = 32, p.pieces = 1;
     else if (pieces <= 128)
         p.lanes = 64, p.pieces = pieces <= 64 ? 1 : 2;
     else if (pieces <= 512)
@@ -269,8 +274,12 @@ void launch_typed(hipStream_t st, const BackArgs& a, const BackPlan& p)
             norm_mean_kernel<T, WHOLE><<<(int)(a.rows < (1 << 20) ? a.rows : 1 << 20), 1024, 0, st>>>(a);
             go(norm_backward_kernel<T, 1024, 1024, 2, WHOLE, true>);
         }
+        else if (p.lanes == 8)
+            many ? go(norm_backward_kernel<T, 1024, 8, 1, WHOLE, false>) : go(norm_backward_kernel<T, 256, 8, 1, WHOLE, false>);
         else if (p.lanes == 16)
             many ? go(norm_backward_kernel<T, 1024, 16, 1, WHOLE, false>) : go(norm_backward_kernel<T, 256, 16, 1, WHOLE, false>);
+        else if (p.lanes == 32)
+            many ? go(norm_backward_kernel<T, 1024, 32, 1, WHOLE, false>) : go(norm_backward_kernel<T, 256, 32, 1, WHOLE, false>);
         else if (p.lanes == 64 && p.pieces == 1)
             many ? go(norm_backward_kernel<T, 1024, 64, 1, WHOLE, false>) : go(norm_backward_kernel<T, 256, 64, 1, WHOLE, false>);
         else if (p.lanes == 64)

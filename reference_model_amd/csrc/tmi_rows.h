@@ -94,7 +94,7 @@ __device__ __forceinline__ void store_piece(T* row, int k, int width, v4i v)
     }
 }
 
-// ---- over the G lanes of a row: 16 or 64 of a wave, or all of a workgroup ------------------------------------------------------
+// ---- over the G lanes of a row: 8 to 64 of a wave, or all of a workgroup ------------------------------------------------------
 template <int CTRL>
 __device__ __forceinline__ uint32_t from_lane(uint32_t v)
 {
@@ -104,8 +104,8 @@ __device__ __forceinline__ uint32_t max_u32(uint32_t a, uint32_t b)
 {
     return a > b ? a : b;
 }
-// within 16 lanes: the neighbour, the other pair, the other four, the other eight
-template <bool SUM, bool MOST>
+// within 16 lanes (or eight): the neighbour, the other pair, the other four, the other eight
+template <bool SUM, bool MOST, int G = 16>
 __device__ __forceinline__ void over_16(float& sum, uint32_t& most)
 {
     auto step = [&](auto CTRL) {
@@ -117,7 +117,19 @@ __device__ __forceinline__ void over_16(float& sum, uint32_t& most)
     step(std::integral_constant<int, 0xB1>());
     step(std::integral_constant<int, 0x4E>());
     step(std::integral_constant<int, 0x141>());
-    step(std::integral_constant<int, 0x140>());
+    if constexpr (G == 16)
+        step(std::integral_constant<int, 0x140>());
+}
+// within 32: the other 16, lane l ^ 16
+template <bool SUM, bool MOST>
+__device__ __forceinline__ void over_32(float& sum, uint32_t& most)
+{
+    over_16<SUM, MOST>(sum, most);
+    auto other = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_ds_swizzle((int)v, 0x401F); };
+    if constexpr (SUM)
+        sum += __uint_as_float(other(__float_as_uint(sum)));
+    if constexpr (MOST)
+        most = max_u32(most, other(most));
 }
 template <bool SUM, bool MOST>
 __device__ __forceinline__ void over_64(float& sum, uint32_t& most)
@@ -136,8 +148,10 @@ __device__ __forceinline__ void over_64(float& sum, uint32_t& most)
 template <int G, bool SUM, bool MOST>
 __device__ __forceinline__ void over_row(float& sum, uint32_t& most, uint32_t* slot)
 {
-    if constexpr (G == 16)
-        over_16<SUM, MOST>(sum, most);
+    if constexpr (G <= 16)
+        over_16<SUM, MOST, G>(sum, most);
+    else if constexpr (G == 32)
+        over_32<SUM, MOST>(sum, most);
     else
         over_64<SUM, MOST>(sum, most);
     if constexpr (G > 64)
