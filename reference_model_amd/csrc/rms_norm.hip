@@ -366,7 +366,7 @@ template <typename T>
 constexpr int kMostPieces = 16 * 1024 / kPiece<T>;
 
 // lanes of a row and pieces of a lane, from the pieces that a row has.  (us with lanes of a row for 16 or 64 pieces at least: 262144 x 64 bf16 21.0, with 8 lanes 13.5;
-// 44157 x 168 16.2, with 32 9.3)
+// 44157 x 168 16.2, with 32 9.3; 16384 x 1088 with residual and sum, 256 lanes of a piece 34.3, 64 of three 29.3, but one row of 1536 2.9 and 3.1)
 template <typename T, int MODE, bool WHOLE>
 void launch_typed(hipStream_t st, const NormArgs& a)
 {
@@ -388,6 +388,8 @@ void launch_typed(hipStream_t st, const NormArgs& a)
         go(number_of<64>, number_of<1>);
     else if (pieces <= 128)
         go(number_of<64>, number_of<2>);
+    else if (pieces <= 192 && a.rows > 256)
+        go(number_of<64>, number_of<3>);
     else if (pieces <= 256)
         go(number_of<256>, number_of<1>);
     else if (pieces <= 512)

@@ -167,6 +167,17 @@ def test_results_in_place_of_operands(ctx, name, shape):
     assert torch.equal(call.q.m, want.q.m) and torch.equal(call.scales.m, want.scales.m) and torch.equal(call.sum.m, want.sum.m)
 
 
+@pytest.mark.parametrize("shape", [(600, 24), (600, 61), (300, 200), (300, 255), (300, 1030), (257, 1101), (300, 1536), (260, 520), (270, 767)],
+                         ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("name", list(KINDS))
+def test_rows_that_share_a_wave_or_have_three_pieces_a_lane(ctx, name, shape):
+    """enough of them for every workgroup to have several"""
+    test_norm(ctx, name, shape)
+    test_norm_in_8_bits(ctx, name, shape)
+    test_rows_into_8_bits(ctx, name, shape)
+    test_results_in_place_of_operands(ctx, name, shape)
+
+
 @pytest.mark.parametrize("width", [48, 1000, 4096, 20000])
 @pytest.mark.parametrize("size", [2.0 ** 120, 2.0 ** 70, 2.0 ** -70, 2.0 ** -110])
 @pytest.mark.parametrize("name", ["bf16", "fp32"])

@@ -91,6 +91,13 @@ def test_results_in_place_of_operands(ctx, name, shape):
         assert torch.equal(call.dx.m, want.dx.m) and torch.equal(call.dw.m, want.dw.m)
 
 
+@pytest.mark.parametrize("shape", [(9000, 24), (5000, 61), (5000, 200), (2000, 255)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("name", list(KINDS))
+def test_short_rows_that_share_a_wave(ctx, name, shape):
+    test_gradients(ctx, name, shape)
+    test_results_in_place_of_operands(ctx, name, shape)
+
+
 @pytest.mark.parametrize("residual", [False, True])
 @pytest.mark.parametrize("shape", [(5, 24), (3, 300)], ids=lambda s: "x".join(map(str, s)))
 def test_against_differences(ctx, shape, residual):
