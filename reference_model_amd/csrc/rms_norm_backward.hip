@@ -136,14 +136,34 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(BackArgs a)
             for (int e = 0; e < V; e += 4)
                 *reinterpret_cast<v4i*>(met + (group * G + lane) * V + e) = piece_of<float>(&dw[p][e]);
             __syncthreads();
-            for (int k = threadIdx.x; k < G * V && p * G * V + k < width; k += THREADS)
+            if constexpr (G * V < THREADS)
             {
-                float sum = 0.0f;
-#pragma unroll 4
-                for (int g = 0; g < ROWS; g++)
-                    sum += met[g * G * V + k];
+                // V groups a thread, and then what those are (all of them one after the other took up to 0.5 us more)
+                constexpr int PARTS = ROWS / V;
+                const int k = threadIdx.x % (G * V), of = threadIdx.x / (G * V);
+                float sum   = met[of * V * (G * V) + k];
+#pragma unroll
+                for (int g = 1; g < V; g++)
+                    sum += met[(of * V + g) * (G * V) + k];
+                __syncthreads();
+                met[threadIdx.x] = sum;
+                __syncthreads();
+                if (of != 0 || p * G * V + k >= width)
+                    continue;
+#pragma unroll
+                for (int i = 1; i < PARTS; i++)
+                    sum += met[i * (G * V) + k];
                 part[p * G * V + k] = sum;
             }
+            else
+                for (int k = threadIdx.x; k < G * V && p * G * V + k < width; k += THREADS)
+                {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int g = 0; g < ROWS; g++)
+                        sum += met[g * G * V + k];
+                    part[p * G * V + k] = sum;
+                }
         }
     }
     else
@@ -223,7 +243,7 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(BackArgs a)
         static_cast<uint16_t*>(a.dw)[k] = to_bits16<T>(sum);
 }
 
-// Lanes of a row (us with 16 at least 262144 x 64 bf16 34.0, with eight 26.6; with 64 instead of 32 44157 x 168 23.2 and 16.2), its pieces a lane, and how many
+// Lanes of a row (us with 16 at least 262144 x 64 bf16 34.0, with eight 25.8; with 64 instead of 32 44157 x 168 23.2 and 16.4), its pieces a lane, and how many
 // workgroups share the rows.  Each of those leaves 4 bytes a column for the second kernel, against b bytes a
 // column and tensor that it reads of its rows.
 struct BackPlan
