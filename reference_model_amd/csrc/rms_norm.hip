@@ -71,7 +71,31 @@ struct OfRow
 {
     float times;     // NORM: r; else 127 / max |y| over r, 0 where there is no such number
     float stored;    // 1 / rms or the scale
+    float unit;      // max |y| over 127 r where quotients may be halves that `times` does not send to the even number, else 0
 };
+
+// 127 / m rounded up.  What the norm makes are products of 16-bit numbers, exact in 32 bits more often than not, and halves of a row's maximum among them: 20 to 50
+// in 4096 x 4096 bf16 with a residual, half of which a rounded reciprocal sends to the odd number.  127 v / m is half an odd number k where 254 v = k m: v = m / 2, or 127
+// divides m.  Rounded up, v = m / 2 becomes 63.5 or more, and so 64, the even one.
+__device__ __forceinline__ float reciprocal_up(float m)
+{
+    const float f = 127.0f / m;
+    return __builtin_fmaf(f, m, -127.0f) < 0.0f ? __uint_as_float(__float_as_uint(f) + 1) : f;
+}
+// Other halves are in rows whose m has m / 127 in 17 bits, which is what this gives then (1 / 127 in 32 bits is off by 2^-28 of itself), and 0 of any other: one in
+// 127, 3 % where neither x nor the weights have more than eight bits.  There the quotient's error, v less a multiple of that, is exact in 32 bits, and added to it.
+// us into 8 bits with both, and with 127 / m as it is: 131072 x 128 13.1 and 12.8, 4096 x 4096 with residual and sum 24.2 and 24.3, 16384 x 4096 40.3 and 40.1.  A test of each
+// quotient for being near a half took 14.1, 24.5 and 43.5.
+__device__ __forceinline__ float whole_127th(float m)
+{
+    const float u = m * (1.0f / 127.0f);
+    return __builtin_fmaf(u, 127.0f, -m) == 0.0f ? u : 0.0f;
+}
+__device__ __forceinline__ uint32_t nearest_byte(float v, float times, float unit)
+{
+    const float t = v * times;
+    return to_byte(__builtin_fmaf(__builtin_fmaf(-t, unit, v), times, t), 1.0f);
+}
 // `by`: the row was multiplied by it for the squares, and for the maximum by the same unless `own` (that one is the first); `first`: the sum of squares before
 template <int MODE>
 __device__ __forceinline__ OfRow of_row(float squares, uint32_t most, float by, float first, bool own, int width, float eps)
@@ -86,17 +110,19 @@ __device__ __forceinline__ OfRow of_row(float squares, uint32_t most, float by, 
             r = 1.0f / __builtin_sqrtf(squares / (float)width + eps * by * by);
     }
     if constexpr (MODE == NORM)
-        return { r, r * by };
+        return { r, r * by, 0.0f };
     const float m     = __uint_as_float(most);
     const bool number = m > 0x1p-119f && m < __builtin_huge_valf();    // (whose reciprocal is one too)
     // (INT8: the maximum goes back to the row's own units)
-    return { number ? 127.0f / m : 0.0f, MODE == INT8 ? m / 127.0f / by : r * m / 127.0f * (own ? by : 1.0f) };
+    if constexpr (MODE == INT8)
+        return { number ? 127.0f / m : 0.0f, m / 127.0f / by, 0.0f };
+    return { number ? reciprocal_up(m) : 0.0f, r * m / 127.0f * (own ? by : 1.0f), whole_127th(m) };
 }
 
 // Quotients of 16-bit operands are halves now and then, and go to the even number then.  t = v times the reciprocal of the maximum (over 127) lies in [2^e,
 // 2^(e+1)) and is off by less than 1.5 2^(e-23); a quotient that is no half is 2^(e-20) from one at least: the maximum is b 2^j and v is a 2^i with a, b <
 // 2^11 and i >= j + e - 8, so that 127 v / (b 2^j) - (k + 1/2) is a multiple of 2^(i-j-1) / b.  Rounded to a multiple of 2^(e-21) halves are halves again, and no
-// other quotient crosses one.  (32-bit operands, and what the norm makes, are as seldom a half as any number.)
+// other quotient crosses one.  (32-bit operands are as seldom a half as any number.)
 template <typename T, int MODE>
 __device__ __forceinline__ uint32_t byte_of(float v, float times)
 {
@@ -106,16 +132,23 @@ __device__ __forceinline__ uint32_t byte_of(float v, float times)
         return to_byte(v, times);
 }
 
-// q of one piece, eight or four bytes
-template <typename T, typename F>
-__device__ __forceinline__ void store_int8(int8_t* row, int k, int pitch, bool zero, F&& at)
+// q of one piece, eight or four bytes; at(e): its elements
+template <typename T, int MODE, typename F>
+__device__ __forceinline__ void store_int8(int8_t* row, int k, int pitch, const OfRow& r, F&& at)
 {
     if (k >= pitch)
         return;
-    uint32_t v[kPiece<T> / 4];
+    uint32_t b[kPiece<T>], v[kPiece<T> / 4];
+#pragma unroll
+    for (int e = 0; e < kPiece<T>; e++)
+        b[e] = byte_of<T, MODE>(at(e), r.times);
+    if (MODE == NORM_INT8 && __builtin_expect(r.unit != 0.0f, 0))
+#pragma unroll
+        for (int e = 0; e < kPiece<T>; e++)
+            b[e] = nearest_byte(at(e), r.times, r.unit);
 #pragma unroll
     for (int i = 0; i < kPiece<T> / 4; i++)
-        v[i] = zero ? 0 : four_bytes(at(4 * i), at(4 * i + 1), at(4 * i + 2), at(4 * i + 3));    // (a NaN's lowest byte may be any)
+        v[i] = r.times == 0.0f ? 0 : four_bytes(b[4 * i], b[4 * i + 1], b[4 * i + 2], b[4 * i + 3]);    // (a NaN's lowest byte may be any)
     __builtin_memcpy(row + k, v, sizeof(v));
 }
 
@@ -225,8 +258,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(NormArgs a)
                 store_piece<T, WHOLE>(static_cast<T*>(a.out) + m * a.ld_out, k, width, piece_of<T>(y));
             }
             else
-                store_int8<T>(static_cast<int8_t*>(a.out) + m * a.ld_out, k, pitch, r.times == 0.0f,
-                              [&](int e) { return byte_of<T, MODE>(MODE == INT8 ? s[p][e] : s[p][e] * weight(p, e), r.times); });
+                store_int8<T, MODE>(static_cast<int8_t*>(a.out) + m * a.ld_out, k, pitch, r, [&](int e) { return MODE == INT8 ? s[p][e] : s[p][e] * weight(p, e); });
         }
     }
 }
@@ -317,7 +349,7 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a)
                 store_piece<T, WHOLE>(static_cast<T*>(a.out) + m * a.ld_out, k, width, piece_of<T>(y));
             }
             else
-                store_int8<T>(static_cast<int8_t*>(a.out) + m * a.ld_out, k, pitch, r.times == 0.0f, [&](int e) { return byte_of<T, MODE>(s[e] * (own ? 1.0f : by) * w[e], r.times); });
+                store_int8<T, MODE>(static_cast<int8_t*>(a.out) + m * a.ld_out, k, pitch, r, [&](int e) { return s[e] * (own ? 1.0f : by) * w[e]; });
         }
     }
 }

@@ -184,10 +184,11 @@ __device__ __forceinline__ void over_row(float& sum, uint32_t& most, uint32_t* s
 }
 
 // ---- 8 bits ---------------------------------------------------------------------------------------------------------------------
-// v rounded to the nearest integer (ties to even) in a word's lowest byte, |v| <= 127: 1.5 2^23 + v has no finer digits
+// v scale rounded to the nearest integer (ties to even) in a word's lowest byte, up to 127: 1.5 2^23 + that has no finer digits
+constexpr float kByteZero = 12582912.0f;
 __device__ __forceinline__ uint32_t to_byte(float v, float scale)
 {
-    return __float_as_uint(__builtin_fmaf(v, scale, 12582912.0f));
+    return __float_as_uint(__builtin_fmaf(v, scale, kByteZero));
 }
 __device__ __forceinline__ uint32_t four_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
 {
