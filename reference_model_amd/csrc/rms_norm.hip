@@ -14,8 +14,8 @@
 // sum 25.9, 5.2, into 8 bits 24.8, 4.7; 16384 x 4096 bf16 into 8 bits 37.7, 5.3, and back 36 to 38, 5.4; one row of 4096 3.2.  Rows of 4095 elements, read in words:
 // 32.2 for 25.9, 29.5 for 24.8, 41.8 for 37.7.  Rows of 8-byte stores: 16 bytes joined from two lanes gave the same (36.5 for 36.4).
 //
-// Squares and products may leave the range of 32 bits where the results do not: bf16 and 32-bit rows whose sum overflows, or is so small that digits are
-// lost, are taken again times a power of two.  That is decided for a row as a whole, from what the reduction found.
+// Squares and products may leave the range of 32 bits where the results do not: bf16 and 32-bit rows whose sum or maximum overflows, or is so small that digits are
+// lost, are taken again times a power of two, each in its own units.  That is decided for a row as a whole, from what the reduction found.
 #include "tmi_rows.h"
 
 namespace tmi
@@ -43,27 +43,46 @@ struct NormArgs
 
 constexpr float kSmall = 0x1p-80f, kUp = 0x1p100f, kDown = 0x1p-80f;
 
-// What a row's elements are multiplied by before they are taken again; 1: they are fine as they are.  `squares` and `most` as the lanes found them.
-template <typename T, int MODE>
-__device__ __forceinline__ float again_by(float squares, uint32_t most, float eps)
-{
-    if constexpr (sizeof(T) == 2 && !__is_same(T, bf16_t))
-        return 1.0f;    // fp16: squares up to 2^34 and products up to 2^33, down to 2^-48
-    else
-    {
-        const float m = __uint_as_float(most);
-        if ((MODE != INT8 && !(squares < __builtin_huge_valf())) || (MODE == NORM_INT8 && !(m < __builtin_huge_valf())))
-            return kDown;
-        if ((MODE != INT8 && squares < kSmall && eps < kSmall) || (MODE != NORM && m < kSmall && squares < 0x1p40f))
-            return kUp;
-        return 1.0f;
-    }
-}
+constexpr int kUpProducts = 200, kDownProducts = -130;    // (exponents: products under 2^-80, and up to 2^256, become numbers of the usual size)
 
 // whether products of this size need no other units
 __device__ __forceinline__ bool fine(uint32_t most)
 {
     return __uint_as_float(most) >= kSmall && __uint_as_float(most) < __builtin_huge_valf();
+}
+
+// (fp16: squares up to 2^34 and products up to 2^33, down to 2^-48)
+template <typename T>
+constexpr bool kLeavesRange = !__is_same(T, _Float16);
+// Whether a row's sum or its maximum, as the lanes found them, have to be taken again
+template <typename T, int MODE>
+__device__ __forceinline__ bool leaves_range(float squares, uint32_t most, float eps)
+{
+    if constexpr (!kLeavesRange<T>)
+        return false;
+    else if constexpr (MODE == INT8)
+        return most != 0 && __uint_as_float(most) < kSmall;
+    else
+        return !(squares < __builtin_huge_valf()) || (squares < kSmall && eps < kSmall) || (MODE == NORM_INT8 && !fine(most));
+}
+// What the elements are multiplied by before their squares are added again; 1: those are fine.  (So small a sum is taken again for the products' sake too: zero
+// is then a row of zeros)
+template <int MODE>
+__device__ __forceinline__ float squares_again(float squares)
+{
+    return MODE == INT8 || (squares >= kSmall && squares < __builtin_huge_valf()) ? 1.0f : squares < kSmall ? kUp : kDown;
+}
+// The units, 2 to the minus this, in which the products are taken again; 0: they are fine, or all zero
+template <int MODE>
+__device__ __forceinline__ int products_again(float squares, uint32_t most)
+{
+    return MODE == NORM || fine(most) || (MODE == NORM_INT8 && squares == 0.0f) ? 0 : __uint_as_float(most) < kSmall ? kUpProducts : kDownProducts;
+}
+// s w 2^units, wherever s and w are in the range; rounded once.  (The compiler is not to keep the parts of rows and weights in registers, which halved the waves a SIMD)
+__device__ __forceinline__ float product_in(float s, float w, int units)
+{
+    asm volatile("" : "+v"(s), "+v"(w));
+    return __builtin_ldexpf(__builtin_amdgcn_frexp_mantf(s) * __builtin_amdgcn_frexp_mantf(w), __builtin_amdgcn_frexp_expf(s) + __builtin_amdgcn_frexp_expf(w) + units);
 }
 
 // What becomes of a row once its sum and maximum are known
@@ -96,27 +115,34 @@ __device__ __forceinline__ uint32_t nearest_byte(float v, float times, float uni
     const float t = v * times;
     return to_byte(__builtin_fmaf(__builtin_fmaf(-t, unit, v), times, t), 1.0f);
 }
-// `by`: the row was multiplied by it for the squares, and for the maximum by the same unless `own` (that one is the first); `first`: the sum of squares before
+// `by`: what the row was multiplied by for the squares, `first`: their sum before that; `units`: of the maximum
 template <int MODE>
-__device__ __forceinline__ OfRow of_row(float squares, uint32_t most, float by, float first, bool own, int width, float eps)
+__device__ __forceinline__ OfRow of_row(float squares, uint32_t most, float by, float first, int units, int width, float eps)
 {
-    float r = 1.0f;
+    float r = 1.0f, of_r = 1.0f;    // 1 / rms is r of_r
     if constexpr (MODE != INT8)
     {
-        // (the squares may have been fine where the products were not, or count for nothing beside eps; times by^2 either may be infinite)
+        // (so small a sum counts for nothing beside an eps of the usual size, which times by^2 may be infinite)
         if (first < __builtin_huge_valf() && (first >= kSmall || eps >= kSmall))
-            r = 1.0f / __builtin_sqrtf(first / (float)width + eps) / by;
+            r = 1.0f / __builtin_sqrtf(first / (float)width + eps);
         else
-            r = 1.0f / __builtin_sqrtf(squares / (float)width + eps * by * by);
+            r = 1.0f / __builtin_sqrtf(squares / (float)width + eps * by * by), of_r = by;
     }
     if constexpr (MODE == NORM)
-        return { r, r * by, 0.0f };
+        return { r, r * of_r, 0.0f };
     const float m     = __uint_as_float(most);
     const bool number = m > 0x1p-119f && m < __builtin_huge_valf();    // (whose reciprocal is one too)
-    // (INT8: the maximum goes back to the row's own units)
+    float scale       = MODE == INT8 ? m / 127.0f : r * m / 127.0f;
+    if (by != 1.0f || units != 0)
+    {
+        // (r may be large where the maximum is small, or their product no number in these units)
+        const float mant = MODE == INT8 ? scale : __builtin_amdgcn_frexp_mantf(r) * __builtin_amdgcn_frexp_mantf(m) / 127.0f;
+        const int exp    = MODE == INT8 ? 0 : __builtin_amdgcn_frexp_expf(r) + __builtin_amdgcn_frexp_expf(of_r) - 1 + __builtin_amdgcn_frexp_expf(m);
+        scale            = __builtin_ldexpf(mant, exp - units);
+    }
     if constexpr (MODE == INT8)
-        return { number ? 127.0f / m : 0.0f, m / 127.0f / by, 0.0f };
-    return { number ? reciprocal_up(m) : 0.0f, r * m / 127.0f * (own ? by : 1.0f), whole_127th(m) };
+        return { number ? 127.0f / m : 0.0f, scale, 0.0f };
+    return { number ? reciprocal_up(m) : 0.0f, scale, whole_127th(m) };
 }
 
 // Quotients of 16-bit operands are halves now and then, and go to the even number then.  t = v times the reciprocal of the maximum (over 127) lies in [2^e,
@@ -152,12 +178,13 @@ __device__ __forceinline__ void store_int8(int8_t* row, int k, int pitch, const 
     __builtin_memcpy(row + k, v, sizeof(v));
 }
 
+// (what is taken again may cost no wave: 4096 x 8191 bf16 with residual and sum into 8 bits 61.2 us, and three waves a SIMD instead of four 71.4)
 template <typename T, int MODE, int G, int P, bool WHOLE>
-__global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(NormArgs a)
+__global__ __launch_bounds__(G > 256 ? G : 256, G == 256 && P == 4 && kLeavesRange<T> ? 4 : 1) void norm_kernel(NormArgs a)
 {
     constexpr int THREADS = G > 256 ? G : 256, ROWS = THREADS / G, V = kPiece<T>;
     constexpr bool SUM = MODE != INT8, MOST = MODE != NORM;
-    __shared__ uint32_t slots[3][2 * (G > 64 ? G / 64 : 1)];
+    __shared__ uint32_t slots[4][2 * (G > 64 ? G / 64 : 1)];
     const int lane = threadIdx.x % G, width = a.width, pitch = (int)whole16(width);
 
     v4i w[P];
@@ -195,70 +222,95 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(NormArgs a)
         float squares = 0.0f;
         uint32_t most = 0;    // (bit patterns order like the numbers, and NaN above all)
         auto weight   = [&](int p, int e) { return a.offset + piece_get<T>(w[p], e); };
-        auto look     = [&]() {
-            squares = 0.0f, most = 0;
+        auto add      = [&](float by) {
+            squares = 0.0f;
 #pragma unroll
             for (int p = 0; p < P; p++)
             {
                 float part = 0.0f;
 #pragma unroll
                 for (int e = 0; e < V; e++)
-                {
-                    if constexpr (SUM)
-                        part = __builtin_fmaf(s[p][e], s[p][e], part);
-                    if constexpr (MOST)
-                        most = max_u32(most, __float_as_uint(MODE == INT8 ? s[p][e] : s[p][e] * weight(p, e)) & 0x7FFFFFFFu);
-                }
+                    part = __builtin_fmaf(s[p][e] * by, s[p][e] * by, part);
                 squares += part;
             }
         };
-        look();
+        auto product = [&](int p, int e) { return MODE == INT8 ? s[p][e] : s[p][e] * weight(p, e); };
+        if constexpr (SUM)
+            add(1.0f);
+        if constexpr (MOST)
+#pragma unroll
+            for (int p = 0; p < P; p++)
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    most = max_u32(most, __float_as_uint(product(p, e)) & 0x7FFFFFFFu);
         over_row<G, SUM, MOST>(squares, most, slots[slot]);
-        slot              = 1 - slot;
-        const float first = squares, by = again_by<T, MODE>(squares, most, a.eps);
+        slot = 1 - slot;
         // (the sum leaves before a row is taken again)
         if (MODE != INT8 && a.sum)
 #pragma unroll
             for (int p = 0; p < P; p++)
                 store_piece<T, WHOLE>(static_cast<T*>(a.sum) + m * a.ld_sum, (p * G + lane) * V, width, piece_of<T>(s[p]));
-        bool own = false;
-        if (by != 1.0f)
+        const float first = squares;
+        float by          = 1.0f;
+        int units         = 0;
+        if (__builtin_expect(leaves_range<T, MODE>(squares, most, a.eps), 0))
         {
-            const uint32_t before = most;
-            own                   = MODE == NORM_INT8 && fine(before);
-            auto times = [&](float f) {
+            by = squares_again<MODE>(squares);
+            if (by != 1.0f)
+            {
+                uint32_t none = 0;
+                add(by);
+                over_row<G, true, false>(squares, none, slots[2]);
+            }
+            units = products_again<MODE>(squares, most);
+            if (units != 0)
+            {
+                // (from here on the elements are the products)
+                float none = 0.0f;
+                most       = 0;
 #pragma unroll
                 for (int p = 0; p < P; p++)
 #pragma unroll
                     for (int e = 0; e < V; e++)
-                        s[p][e] *= f;
-            };
-            times(by);
-            look();
-            over_row<G, SUM, MOST>(squares, most, slots[2]);
-            if (own)
-            {
-                most = before;
-                times(1.0f / by);
+                    {
+                        s[p][e] = product_in(s[p][e], MODE == INT8 ? 1.0f : weight(p, e), units);
+                        most    = max_u32(most, __float_as_uint(s[p][e]) & 0x7FFFFFFFu);
+                    }
+                over_row<G, false, true>(none, most, slots[3]);
             }
+            if constexpr (MODE == NORM)
+#pragma unroll
+                for (int p = 0; p < P; p++)
+#pragma unroll
+                    for (int e = 0; e < V; e++)
+                        s[p][e] *= by;
         }
-        const OfRow r = of_row<MODE>(squares, most, by, first, own, width, a.eps);
+        const OfRow r = of_row<MODE>(squares, most, by, first, units, width, a.eps);
         if (a.of_row && lane == 0)
             a.of_row[m] = r.stored;
+        if constexpr (MODE == NORM)
 #pragma unroll
-        for (int p = 0; p < P; p++)
-        {
-            const int k = (p * G + lane) * V;
-            if constexpr (MODE == NORM)
+            for (int p = 0; p < P; p++)
             {
                 float y[V];
 #pragma unroll
                 for (int e = 0; e < V; e++)
                     y[e] = s[p][e] * r.times * weight(p, e);
-                store_piece<T, WHOLE>(static_cast<T*>(a.out) + m * a.ld_out, k, width, piece_of<T>(y));
+                store_piece<T, WHOLE>(static_cast<T*>(a.out) + m * a.ld_out, (p * G + lane) * V, width, piece_of<T>(y));
+            }
+        else
+        {
+            int8_t* to = static_cast<int8_t*>(a.out) + m * a.ld_out;
+            if (MODE == NORM_INT8 && __builtin_expect(units != 0, 0))
+            {
+#pragma unroll
+                for (int p = 0; p < P; p++)
+                    store_int8<T, MODE>(to, (p * G + lane) * V, pitch, r, [&](int e) { return s[p][e]; });
             }
             else
-                store_int8<T, MODE>(static_cast<int8_t*>(a.out) + m * a.ld_out, k, pitch, r, [&](int e) { return MODE == INT8 ? s[p][e] : s[p][e] * weight(p, e); });
+#pragma unroll
+                for (int p = 0; p < P; p++)
+                    store_int8<T, MODE>(to, (p * G + lane) * V, pitch, r, [&](int e) { return product(p, e); });
         }
     }
 }
@@ -271,20 +323,20 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a)
 {
     constexpr int G = 1024, V = kPiece<T>;
     constexpr bool SUM = MODE != INT8, MOST = MODE != NORM;
-    __shared__ uint32_t slots[3][2 * (G / 64)];
+    __shared__ uint32_t slots[4][2 * (G / 64)];
     const int width = a.width, pitch = (int)whole16(width);
     int slot = 0;
     for (int64_t m = blockIdx.x; m < a.rows; m += gridDim.x)
     {
         const T *row = static_cast<const T*>(a.x) + m * a.ld_x, *from = static_cast<const T*>(a.residual) + (a.residual ? m * a.ld_residual : 0);
-        auto piece = [&](int k, float by, float* s) {
+        auto piece = [&](int k, float* s) {
             const v4i raw = load_piece_alone<T, WHOLE>(row, k, width);
             v4i more      = { 0, 0, 0, 0 };
             if (MODE != INT8 && a.residual)
                 more = load_piece_alone<T, WHOLE>(from, k, width);
 #pragma unroll
             for (int e = 0; e < V; e++)
-                s[e] = (MODE != INT8 ? piece_get<T>(raw, e) + piece_get<T>(more, e) : piece_get<T>(raw, e)) * by;
+                s[e] = MODE != INT8 ? piece_get<T>(raw, e) + piece_get<T>(more, e) : piece_get<T>(raw, e);
         };
         auto weights = [&](int k, float* w) {
             v4i v = { 0, 0, 0, 0 };
@@ -296,47 +348,58 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a)
         };
         float squares = 0.0f;
         uint32_t most = 0;
-        auto look     = [&](float by) {
-            squares = 0.0f, most = 0;
+        // (the squares of the row times `by`, and the products in `units`; without units as they are)
+        auto look = [&](auto with_sum, auto with_most, float by, int units) {
             for (int k = (int)threadIdx.x * V; k < width; k += G * V)
             {
                 float s[V], w[V];
-                piece(k, by, s);
-                if constexpr (MOST)
+                piece(k, s);
+                if constexpr (decltype(with_most)::value)
                     weights(k, w);
                 float part = 0.0f;
 #pragma unroll
                 for (int e = 0; e < V; e++)
                 {
-                    if constexpr (SUM)
-                        part = __builtin_fmaf(s[e], s[e], part);
-                    if constexpr (MOST)
-                        most = max_u32(most, __float_as_uint(s[e] * w[e]) & 0x7FFFFFFFu);
+                    if constexpr (decltype(with_sum)::value)
+                        part = __builtin_fmaf(s[e] * by, s[e] * by, part);
+                    if constexpr (decltype(with_most)::value)
+                        most = max_u32(most, __float_as_uint(units == 0 ? s[e] * w[e] : product_in(s[e], w[e], units)) & 0x7FFFFFFFu);
                 }
                 squares += part;
             }
         };
-        look(1.0f);
+        look(std::bool_constant<SUM>(), std::bool_constant<MOST>(), 1.0f, 0);
         over_row<G, SUM, MOST>(squares, most, slots[slot]);
         slot              = 1 - slot;
-        const float first = squares, by = again_by<T, MODE>(squares, most, a.eps);
-        bool own = false;
-        if (by != 1.0f)
+        const float first = squares;
+        float by          = 1.0f;
+        int units         = 0;
+        if (__builtin_expect(leaves_range<T, MODE>(squares, most, a.eps), 0))
         {
-            const uint32_t before = most;
-            own                   = MODE == NORM_INT8 && fine(before);
-            look(by);
-            over_row<G, SUM, MOST>(squares, most, slots[2]);
-            if (own)
-                most = before;
+            by = squares_again<MODE>(squares);
+            if (by != 1.0f)
+            {
+                uint32_t none = 0;
+                squares       = 0.0f;
+                look(std::true_type(), std::false_type(), by, 0);
+                over_row<G, true, false>(squares, none, slots[2]);
+            }
+            units = products_again<MODE>(squares, most);
+            if (units != 0)
+            {
+                float none = 0.0f;
+                most       = 0;
+                look(std::false_type(), std::true_type(), 1.0f, units);
+                over_row<G, false, true>(none, most, slots[3]);
+            }
         }
-        const OfRow r = of_row<MODE>(squares, most, by, first, own, width, a.eps);
+        const OfRow r = of_row<MODE>(squares, most, by, first, units, width, a.eps);
         if (a.of_row && threadIdx.x == 0)
             a.of_row[m] = r.stored;
         for (int k = (int)threadIdx.x * V; k < (MODE == NORM ? width : pitch); k += G * V)
         {
             float s[V], w[V];
-            piece(k, 1.0f, s);
+            piece(k, s);
             weights(k, w);
             if (MODE != INT8 && a.sum)
                 store_piece<T, WHOLE>(static_cast<T*>(a.sum) + m * a.ld_sum, k, width, piece_of<T>(s));
@@ -349,7 +412,13 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a)
                 store_piece<T, WHOLE>(static_cast<T*>(a.out) + m * a.ld_out, k, width, piece_of<T>(y));
             }
             else
-                store_int8<T, MODE>(static_cast<int8_t*>(a.out) + m * a.ld_out, k, pitch, r, [&](int e) { return s[e] * (own ? 1.0f : by) * w[e]; });
+            {
+                int8_t* to = static_cast<int8_t*>(a.out) + m * a.ld_out;
+                if (__builtin_expect(units != 0, 0))
+                    store_int8<T, MODE>(to, k, pitch, r, [&](int e) { return product_in(s[e], w[e], units); });
+                else
+                    store_int8<T, MODE>(to, k, pitch, r, [&](int e) { return s[e] * w[e]; });
+            }
         }
     }
 }

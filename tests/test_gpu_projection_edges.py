@@ -1,4 +1,5 @@
-"""Where the operators on the way into a projection can go wrong and a bound on roundings would not show it: halves on the way into 8 bits."""
+"""Where the operators on the way into a projection can go wrong and a bound on roundings would not show it: halves on the way into 8 bits, and products
+beyond the range of 32 bits there."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -62,3 +63,43 @@ def test_halves_of_any_maximum_go_to_even(ctx, name, shape):
         # (v and the maximum are as they stand: what is left is the reciprocal's last place, two halves of one)
         assert ((q - v * 127 / most).abs() <= 0.5 + 127 * 2 * ref.EPS).all()
     assert seen > 0
+
+
+def check_norm8(ctx, kind, x, weight, eps):
+    call = Call(ctx, kind, x, None, weight, eps)
+    call.norm8()
+    y = ref.norm(kind, x, None, weight, eps, 0.0)[1][0]
+    ref.check_int8(call.q.values(), call.scales.values()[0], y, (ref.depth(x.shape[1]) / 2 + 10) * ref.EPS, x.shape[1])
+
+
+# x and weights times these: squares that leave the range beside products that do not, both, products alone at either end, and rows that are next to nothing
+FACTORS = [(2.0 ** 70, 2.0 ** 50), (2.0 ** 110, 2.0 ** 100), (2.0 ** 120, 2.0 ** 120), (2.0 ** 100, 2.0 ** -110), (2.0 ** 40, 2.0 ** 110), (2.0 ** -30, 2.0 ** -80),
+           (2.0 ** -60, 2.0 ** 100), (2.0 ** -122, 2.0 ** -60), (2.0 ** -120, 2.0 ** -100), (2.0 ** -122, 2.0 ** 110)]
+
+
+@pytest.mark.parametrize("width", [48, 1000, 4096, 20000])
+@pytest.mark.parametrize("factors", FACTORS, ids=lambda f: f"{f[0]:.0e}-{f[1]:.0e}")
+@pytest.mark.parametrize("name", ["bf16", "fp32"])
+def test_products_beyond_the_range_into_8_bits(ctx, name, factors, width):
+    """the scale is a number wherever y is; every other row is of the usual size"""
+    kind = KINDS[name]
+    x, _, weight = operands(kind, 6, width, 12, residual=False)
+    x[::2] *= factors[0]
+    weight = (weight * factors[1]).to(kind.t).double()
+    for eps in (0.0, 1e-5):
+        if eps and factors[0] < 2.0 ** -100:
+            continue    # (y of those rows is nothing beside eps)
+        check_norm8(ctx, kind, x.to(kind.t).double(), weight, eps)
+
+
+@pytest.mark.parametrize("width", [48, 1000, 4096, 20000])
+@pytest.mark.parametrize("name", ["bf16", "fp32"])
+def test_rows_that_span_the_range_into_8_bits(ctx, name, width):
+    """one element makes the squares leave the range, and the others, of every size, make the row's maximum"""
+    kind = KINDS[name]
+    for first, of_first, others, of_others in ((2.0 ** 66, 0.0, 2.0 ** -69, 2.0 ** 100), (2.0 ** 127, 2.0 ** -10, 8.0, 2.0 ** 125), (2.0 ** 127, 0.0, 2.0 ** -40, 2.0 ** 40),
+                                               (2.0 ** -42, 0.0, 2.0 ** -100, 2.0 ** -20), (2.0 ** -10, 0.0, 2.0 ** -90, 2.0 ** -10)):
+        x, _, weight = operands(kind, 5, width, 13, residual=False)
+        x, weight = x * others, weight * of_others
+        x[:, 7], weight[7] = first, of_first
+        check_norm8(ctx, kind, x.to(kind.t).double(), weight.to(kind.t).double(), 0.0)
