@@ -203,14 +203,16 @@ __global__ __launch_bounds__(1024) void norm_mean_kernel(BackArgs a)
     }
 }
 
-// The workgroups' sums: 32 columns and 32 parts of the list a workgroup (with 16 and 64 the same, with 8 and 128 2.5 us more at 8192 x 4096)
+// The workgroups' sums: 32 columns and 32 parts of the list a workgroup (with 16 and 64 the same, with 8 and 128 2.5 us more at 8192 x 4096).  Of a grid's two
+// dimensions none has more than kJoinGrid workgroups: the threads of one are counted in 32 bits, and 2^28 columns have 2^33.
+constexpr int kJoinGrid = 1 << 20;
 template <typename T>
 __global__ __launch_bounds__(1024) void norm_join_kernel(BackArgs a)
 {
     constexpr int COLUMNS = 32, SHARES = 1024 / COLUMNS;
     __shared__ float met[SHARES][COLUMNS + 1];
     const int column = threadIdx.x % COLUMNS, share = threadIdx.x / COLUMNS;
-    const int64_t k  = (int64_t)blockIdx.x * COLUMNS + column;
+    const int64_t k  = ((int64_t)blockIdx.y * kJoinGrid + blockIdx.x) * COLUMNS + column;
     constexpr int MOST = kMostGroups / SHARES;
     const int each = (a.groups + SHARES - 1) / SHARES, first = share * each;
     const int64_t column_of = k < a.width ? k : a.width - 1;
@@ -312,7 +314,10 @@ void launch_typed(hipStream_t st, const BackArgs& a, const BackPlan& p)
             p.pieces == 1 ? go(norm_backward_kernel<T, 1024, 1024, 1, WHOLE, false>) : go(norm_backward_kernel<T, 1024, 1024, 2, WHOLE, false>);
     }
     if (a.dw)
-        norm_join_kernel<T><<<(a.width + 31) / 32, 1024, 0, st>>>(a);
+    {
+        const int groups = (a.width + 31) / 32;
+        norm_join_kernel<T><<<dim3(groups < kJoinGrid ? groups : kJoinGrid, (groups + kJoinGrid - 1) / kJoinGrid), 1024, 0, st>>>(a);
+    }
 }
 
 size_t mean_bytes(const BackPlan& p, int64_t rows)

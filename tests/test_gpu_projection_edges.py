@@ -1,5 +1,5 @@
-"""Where the operators on the way into a projection can go wrong and a bound on roundings would not show it: halves on the way into 8 bits, and products
-beyond the range of 32 bits there."""
+"""Where the operators on the way into a projection can go wrong and a bound on roundings would not show it: halves on the way into 8 bits, products beyond
+the range of 32 bits there, and the widest rows."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -103,3 +103,18 @@ def test_rows_that_span_the_range_into_8_bits(ctx, name, width):
         x, weight = x * others, weight * of_others
         x[:, 7], weight[7] = first, of_first
         check_norm8(ctx, kind, x.to(kind.t).double(), weight.to(kind.t).double(), 0.0)
+
+
+@pytest.mark.parametrize("name", ["bf16", "fp32"])
+def test_gradients_of_the_widest_rows(ctx, name):
+    """more columns than 2^32 threads have at 32 threads a column; whole numbers and halves, exact in every type"""
+    kind, rows, width = KINDS[name], 2, (1 << 27) + 40
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    new = lambda: torch.randint(-3, 4, (rows, width), generator=gen, device="cuda", dtype=torch.int8).to(kind.t)  # noqa: E731
+    s, dy, w = new(), new(), torch.ones(width, device="cuda", dtype=kind.t)
+    r = torch.tensor([0.5, 2.0], device="cuda")
+    dw = torch.full((width + 8,), ref.CANARY, device="cuda", dtype=kind.t)
+    ctx.rms_norm_backward(ctx.rms_norm_desc(kind.dtype, rows, width, 1e-5), s, w, r, dy, None, None, dw)
+    assert ctx.sync() == capi.VALID and (dw[width:] == ref.CANARY).all()
+    want = s[0] * dy[0] * 0.5 + s[1] * dy[1] * 2    # (at most 22.5 in halves)
+    assert torch.equal(dw[:width], want)
