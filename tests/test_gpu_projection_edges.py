@@ -1,11 +1,11 @@
 """Where the operators on the way into a projection can go wrong and a bound on roundings would not show it: halves on the way into 8 bits, products beyond
-the range of 32 bits there, and the widest rows."""
+the range of 32 bits there, the widest rows, and gradients that are whole numbers, so that no row may be lost."""
 import pytest
 
 torch = pytest.importorskip("torch")
 
 import projection_reference as ref  # noqa: E402
-from projection_reference import KINDS  # noqa: E402
+from projection_reference import KINDS, Held, near  # noqa: E402
 from reference_model_amd import Context, capi  # noqa: E402
 from test_gpu_rms_norm import Call, operands  # noqa: E402
 
@@ -118,3 +118,32 @@ def test_gradients_of_the_widest_rows(ctx, name):
     assert ctx.sync() == capi.VALID and (dw[width:] == ref.CANARY).all()
     want = s[0] * dy[0] * 0.5 + s[1] * dy[1] * 2    # (at most 22.5 in halves)
     assert torch.equal(dw[:width], want)
+
+
+@pytest.mark.parametrize("shape", [(1, 24), (31, 24), (20000, 24), (9000, 24), (9001, 64), (5000, 61), (5000, 200), (4999, 255), (3000, 300), (2100, 1030), (1500, 4104),
+                                   (1025, 2048), (1100, 9000), (700, 17000), (65, 17000), (300, 40003)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("name", list(KINDS))
+def test_every_row_counts_once_in_the_weights_gradient(ctx, name, shape):
+    """terms of +-1 and +-2: their sums are whole numbers that 32 bits hold exactly whatever their order, and a result is the sum rounded once.  A lost or repeated
+    row is off by one or two in every column, in fp32 and fp16 always (sums below 2048), in bf16 where a sum is below 256, as most are."""
+    kind, (rows, width) = KINDS[name], shape
+    gen = torch.Generator().manual_seed(rows + width)
+    one = lambda: torch.randint(0, 2, shape, generator=gen) * 2.0 - 1  # noqa: E731
+    s, dy, r = one() * 4, one() * (torch.randint(0, 2, (rows, 1), generator=gen) + 1), torch.full((rows,), 0.25)
+    want = (s * dy).double().sum(0) / 4
+    assert want.abs().max() < 2048 and (want.abs() < 256).any()
+    for gap, lead in ((0, 0), (3, 1)):
+        hold = lambda v: Held(shape, kind.t, gap, lead, v)  # noqa: E731, B023
+        ds, ddy, dx = hold(s), hold(dy), hold(torch.zeros(shape))
+        w, dw = Held((1, width), kind.t, 0, lead, torch.ones(1, width)), Held((1, width), kind.t, 0, lead)
+        ld = width + gap
+        desc = ctx.rms_norm_desc(kind.dtype, rows, width, 1e-5, 0.0, ld, 0, ld, ld)
+        for to in (dx.at, None):
+            dw.m.fill_(ref.CANARY)
+            ctx.rms_norm_backward(desc, ds.at, w.at, r.cuda(), ddy.at, None, to, dw.at)
+            assert ctx.sync() == capi.VALID and torch.equal(dw.values()[0], want.to(kind.t).double())
+        # and in d_x: dy / 4 - s / 16 mean(dy s / 4), whose mean is a whole number over width
+        mean = (s * dy).double().sum(1, keepdim=True) / 4 / width
+        dx_want = (dy.double() - s.double() / 4 * mean) / 4
+        off = 4 * ref.EPS * (dy.double().abs() + mean.abs())
+        near(dx.values(), dx_want, off + kind.rounding(dx_want, off))
