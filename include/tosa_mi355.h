@@ -495,11 +495,11 @@ int tmi_gated_ffn_int4(tmi_ctx_t* ctx, const tmi_int4_desc_t* d, int32_t activat
  * once.  Equal calls give equal bits.
  *
  * A row in 8 bits is v[k] = scale * q[k], scale = max |v| / 127 in 32 bits, q = 127 v / max |v| rounded to the nearest integer (halves to even
- * where v are 16-bit numbers, and out of the norm where s (weight_offset + weight) and its maximum are exact in 32 bits; others within 2^-16 of a
- * half to either side).  A row of zeros has scale 0; a row with an infinity or NaN has a scale
- * that is infinite or NaN, and q = 0; max |v| below 2^-119 counts as 0.  Rows of q begin at multiples of 16 bytes: the tensor is aligned to
- * 16 and its stride a multiple of 16 (0: the width, up to the next multiple).  The bytes that fill up a row's last 16 are zeros: the
- * operators that write rows write them, and tmi_linear_int8 counts them as columns. */
+ * where v are 16-bit numbers, and out of the norm where s (weight_offset + weight) and its maximum are exact in 32 bits; others within 2^-17 of a
+ * half to either side, out of the norm within 2^-14).  A row of zeros has scale 0; a row with an infinity or NaN has a scale that is infinite or
+ * NaN, and q = 0.  Where max |v| is below 2^-119 the scale is a multiple of 2^-149 and has fewer digits; where that is 0 so is q.
+ * Rows of q begin at multiples of 16 bytes: the tensor is aligned to 16 and its stride a multiple of 16 (0: the width, up to the next multiple).  The
+ * bytes that fill up a row's last 16 are zeros: the operators that write rows write them, and tmi_linear_int8 counts them as columns. */
 
 /* Row strides count elements, 0 means that rows lie side by side: ld_x for x, ld_residual for the residual, ld_sum for the sum and ld_y for the
  * result.  Gradients have the strides of their tensors. */

@@ -43,12 +43,14 @@ struct NormArgs
 
 constexpr float kSmall = 0x1p-80f, kUp = 0x1p100f, kDown = 0x1p-80f;
 
-constexpr int kUpProducts = 200, kDownProducts = -130;    // (exponents: products under 2^-80, and up to 2^256, become numbers of the usual size)
+// (products this small may have a scale of 0: times 2^-64, the least 1 / rms of squares that 32 bits hold, and over 127)
+constexpr float kSmallProduct = 0x1p-77f;
+constexpr int kUpProducts = 200, kDownProducts = -130;    // (exponents: products under that, and up to 2^256, become numbers of the usual size)
 
 // whether products of this size need no other units
 __device__ __forceinline__ bool fine(uint32_t most)
 {
-    return __uint_as_float(most) >= kSmall && __uint_as_float(most) < __builtin_huge_valf();
+    return __uint_as_float(most) >= kSmallProduct && __uint_as_float(most) < __builtin_huge_valf();
 }
 
 // (fp16: squares up to 2^34 and products up to 2^33, down to 2^-48)
@@ -61,7 +63,7 @@ __device__ __forceinline__ bool leaves_range(float squares, uint32_t most, float
     if constexpr (!kLeavesRange<T>)
         return false;
     else if constexpr (MODE == INT8)
-        return most != 0 && __uint_as_float(most) < kSmall;
+        return most != 0 && __uint_as_float(most) < kSmallProduct;
     else
         return !(squares < __builtin_huge_valf()) || (squares < kSmall && eps < kSmall) || (MODE == NORM_INT8 && !fine(most));
 }
@@ -76,7 +78,7 @@ __device__ __forceinline__ float squares_again(float squares)
 template <int MODE>
 __device__ __forceinline__ int products_again(float squares, uint32_t most)
 {
-    return MODE == NORM || fine(most) || (MODE == NORM_INT8 && squares == 0.0f) ? 0 : __uint_as_float(most) < kSmall ? kUpProducts : kDownProducts;
+    return MODE == NORM || fine(most) || (MODE == NORM_INT8 && squares == 0.0f) ? 0 : __uint_as_float(most) < kSmallProduct ? kUpProducts : kDownProducts;
 }
 // s w 2^units, wherever s and w are in the range; rounded once.  (The compiler is not to keep the parts of rows and weights in registers, which halved the waves a SIMD)
 __device__ __forceinline__ float product_in(float s, float w, int units)
@@ -131,7 +133,7 @@ __device__ __forceinline__ OfRow of_row(float squares, uint32_t most, float by, 
     if constexpr (MODE == NORM)
         return { r, r * of_r, 0.0f };
     const float m     = __uint_as_float(most);
-    const bool number = m > 0x1p-119f && m < __builtin_huge_valf();    // (whose reciprocal is one too)
+    bool number       = m > 0x1p-119f && m < __builtin_huge_valf();    // (whose reciprocal is one too)
     float scale       = MODE == INT8 ? m / 127.0f : r * m / 127.0f;
     if (by != 1.0f || units != 0)
     {
@@ -139,6 +141,7 @@ __device__ __forceinline__ OfRow of_row(float squares, uint32_t most, float by, 
         const float mant = MODE == INT8 ? scale : __builtin_amdgcn_frexp_mantf(r) * __builtin_amdgcn_frexp_mantf(m) / 127.0f;
         const int exp    = MODE == INT8 ? 0 : __builtin_amdgcn_frexp_expf(r) + __builtin_amdgcn_frexp_expf(of_r) - 1 + __builtin_amdgcn_frexp_expf(m);
         scale            = __builtin_ldexpf(mant, exp - units);
+        number           = number && scale != 0.0f;
     }
     if constexpr (MODE == INT8)
         return { number ? 127.0f / m : 0.0f, scale, 0.0f };

@@ -1,11 +1,11 @@
 """Where the operators on the way into a projection can go wrong and a bound on roundings would not show it: halves on the way into 8 bits, products beyond
-the range of 32 bits there, the widest rows, and gradients that are whole numbers, so that no row may be lost."""
+the range of 32 bits there, scales that 32 bits hardly hold, the widest rows, and gradients that are whole numbers, so that no row may be lost."""
 import pytest
 
 torch = pytest.importorskip("torch")
 
 import projection_reference as ref  # noqa: E402
-from projection_reference import KINDS, Held, near  # noqa: E402
+from projection_reference import KINDS, Held, held8, near  # noqa: E402
 from reference_model_amd import Context, capi  # noqa: E402
 from test_gpu_rms_norm import Call, operands  # noqa: E402
 
@@ -147,3 +147,32 @@ def test_every_row_counts_once_in_the_weights_gradient(ctx, name, shape):
         dx_want = (dy.double() - s.double() / 4 * mean) / 4
         off = 4 * ref.EPS * (dy.double().abs() + mean.abs())
         near(dx.values(), dx_want, off + kind.rounding(dx_want, off))
+
+
+@pytest.mark.parametrize("width", [7, 48, 4096, 20000])
+@pytest.mark.parametrize("size", [2.0 ** -118, 2.0 ** -125, 2.0 ** -130, 2.0 ** -140, 2.0 ** -149])
+@pytest.mark.parametrize("name", ["bf16", "fp32"])
+def test_scales_that_32_bits_hardly_hold(ctx, name, size, width):
+    """a scale is the nearest number that 32 bits hold, below 2^-126 a multiple of 2^-149; where that is 0 so is q, else q is as of any row"""
+    kind = KINDS[name]
+    x, _, weight = operands(kind, 5, width, 14, residual=False)
+
+    def check(q, scales, v, rel, off_q):
+        most = v.abs().amax(1)
+        assert ((scales - most / 127).abs() <= rel * most / 127 + 2.0 ** -150 * (1 + 2.0 ** -20)).all()
+        assert (q[scales == 0] == 0).all() and (q[:, width:] == 0).all()
+        live = scales > 0
+        t = v[live] * 127 / most[live][:, None]
+        assert ((q[live][:, :width] - t).abs() <= 0.5 + off_q).all() and (q[live].abs().amax(1) == 127).all()
+
+    small = (x * size).to(kind.t).double()
+    dev, q, scales = Held(x.shape, kind.t, 0, 0, small), held8(5, width), Held((1, 5), torch.float32)
+    ctx.quantize_int8(kind.dtype, 5, width, dev.at, 0, q.at, 0, scales.at)
+    assert ctx.sync() == capi.VALID
+    # (127 over the maximum is rounded, and the product joins its rounding to a whole number: 2^-17 of 127)
+    check(q.values(), scales.values()[0], small, 2 * ref.EPS, 0.0 if name == "bf16" else 2.0 ** -17)
+    # the same sizes out of the norm: weights that small
+    w = (weight * size).to(kind.t).double()
+    call = Call(ctx, kind, x, None, w)
+    call.norm8()
+    check(call.q.values(), call.scales.values()[0], ref.norm(kind, x, None, w, 1e-5, 0.0)[1][0], (ref.depth(width) / 2 + 10) * ref.EPS, 127 * 8 * ref.EPS)
