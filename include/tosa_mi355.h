@@ -540,8 +540,8 @@ int tmi_dequantize_int8(tmi_ctx_t* ctx, int32_t dtype, int32_t rows, int32_t wid
 
 /* y[m][n] = x_scales[m] w_scales[n] sum_k x[m][k] w[n][k] + bias[n]: x [rows][in_features] and w [out_features][in_features] in 8 bits, y
  * [rows][out_features] and bias (or NULL) of dtype.  ld_x and ld_w count bytes, ld_y elements.  The sum is exact: in_features is at most
- * 131071.  It is rounded to 32 bits before it is scaled.  Some calls split it, and use the context's scratch buffer for the parts; where
- * that cannot grow (while a graph is captured) they go on without it, to the same bits. */
+ * 131071.  It is rounded to 32 bits, then multiplied by w's scale and then by x's, each product in 32 bits.  Some calls split the sum, and use the
+ * context's scratch buffer for the parts; where that cannot grow (while a graph is captured) they go on without it, to the same bits. */
 typedef struct
 {
     int64_t ld_x, ld_w, ld_y;

@@ -253,8 +253,10 @@ struct Multiply
 
 // 256 x 256 results, eight waves of 64 features x 128 tokens that load as well as compute.  LDS is a ring of five units: the weights of a pair, its x, the next
 // pair's weights and so on.  At the barrier in the second block of pair p its units are free, and pair p + 1 has landed (all but the weights of p + 2);
-// x of p + 2 goes in the place of p's weights, the weights of p + 3 in that of its x.  us 4096 x 4096 x 16384 with operands from memory 225, with the kernel below in
-// tiles of 256 x 128 262 (half as much again of the operands' bytes); where they are in the last cache 227 and 214.
+// x of p + 2 goes in the place of p's weights, the weights of p + 3 in that of its x.  With the kernel below in tiles of 256 x 128
+// 4096 x 4096 x 16384 took 262 us when this took 225 (half as much again of the operands' bytes), but 214 for 227 where the operands lay in the last cache.
+// Operands from memory, on random bits: 239 to 250 us from run to run, 232 at the least; on zeros 201.  A dispatch is 447 thousand cycles: the matrix cores are busy 59 % of them,
+// the LDS serves reads in 22 %, without conflicts; a wave waits 37 % of its time to issue anything and 3 % for LDS.  The clock falls from 2.2 GHz to 1.8 on random bits.
 template <typename T>
 __global__ __launch_bounds__(512, 2) void linear_wide_kernel(LinearArgs a)
 {
@@ -726,7 +728,8 @@ bool launch_typed(hipStream_t st, const LinearArgs& a, const Plan& p)
         };
         auto rows = [&](auto SPLIT) {
             // Few waves and loads on their way for short columns, more for long ones.  us 1 x 1024 x 4096 with two pairs and eight waves 3.5, with two and 16 3.6,
-            // with four and eight 4.6; 1 x 8192 x 8192 14.4, 12.8 and 13.2.
+            // with four and eight 4.6; 1 x 8192 x 8192 14.4, 12.8 and 13.2.  With more tiles of tokens one pair and eight waves: 33 x 1111 x 5003 5.7, with two pairs
+            // 7.2, with 16 waves 6.6; 24 x 4096 x 4096 8.5, 9.0 and 8.7; 48 x 4096 x 4096 11.0, 11.2 and 11.3; 64 x 4096 x 1024 in four 9.0, 10.5 and 9.2.
             if (a.M <= 16 && a.per_split >= 64)
                 go(SPLIT, number_of<1>, number_of<2>, number_of<16>);
             else if (a.M <= 16)

@@ -10,9 +10,10 @@
 // maximum, and r only enters the scale.
 //
 // A row has 8 to 64 lanes of a wave, 256 or 1024 of a workgroup, each with P pieces of 16 bytes; longer rows are read a second time (norm_long_kernel).
-// us and TB/s: 4096 x 8192 fp16 with residual and sum 48.2, 5.6 (a copy of as many bytes runs at 6.1); 131072 x 128 bf16 12 to 13.5, 5.3; 4096 x 4096 bf16 with residual and
-// sum 25.9, 5.2, into 8 bits 24.8, 4.7; 16384 x 4096 bf16 into 8 bits 37.7, 5.3, and back 36 to 38, 5.4; one row of 4096 3.2.  Rows of 4095 elements, read in words:
-// 32.2 for 25.9, 29.5 for 24.8, 41.8 for 37.7.  Rows of 8-byte stores: 16 bytes joined from two lanes gave the same (36.5 for 36.4).
+// us and TB/s: 4096 x 8192 fp16 with residual and sum 48.2, 5.6 (a copy of as many bytes runs at 6.1); 131072 x 128 bf16 12 to 13, 5.3; 4096 x 4096 bf16 with residual and
+// sum 25.9, 5.2, into 8 bits 24.5, 4.8; 16384 x 4096 bf16 into 8 bits 37.4, 5.4 (38 to 46 right behind the way back, whose results are on their way to memory then), and back 37.5,
+// 5.4 (29 behind the way there, which leaves part of q in the last cache); one row of 4096 2.9.  Rows of 4095 elements, read in words: 32.1 for 25.9, 29.7 for 24.5, 40.1
+// for 37.4.  Rows of 8-byte stores: 16 bytes joined from two lanes gave the same (36.5 for 36.4).
 //
 // Squares and products may leave the range of 32 bits where the results do not: bf16 and 32-bit rows whose sum or maximum overflows, or is so small that digits are
 // lost, are taken again times a power of two, each in its own units.  That is decided for a row as a whole, from what the reduction found.
@@ -318,7 +319,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G == 256 && P == 4 && kLeavesRan
     }
 }
 
-// Rows that no workgroup's registers hold: read once for the sum, again if it left the range, and once more for the results (1024 x 40000 bf16 with residual and sum 87
+// Rows that no workgroup's registers hold: read once for the sum, again if it left the range, and once more for the results (1024 x 40000 bf16 with residual and sum 86
 // us, 3.8 TB/s of the bytes that one reading would take).  Results may take the place of what
 // is read, so here a piece is made of its own elements alone.
 template <typename T, int MODE, bool WHOLE>

@@ -9,7 +9,8 @@
 //
 // 8192 x 4096 in bf16 with d_weight: 46.6 us, 4.3 TB/s (the second kernel 4.8 of them), with d_sum too 55.3; without d_weight 38.1, 5.3 TB/s.  131072 x 128:
 // 25.5.  A row's loads before the sum of the one ahead of it gave the same 46.2, and 1 us more where a workgroup has one or two rows; a wave for a whole row,
-// whose registers then overflow, 59.4.
+// whose registers then overflow, 59.4.  Rows of 4095 elements, read in words: 57.4 with d_weight, where 4096 take 45.5 in the same run.  1024 x 40000, read twice: 87.4, 2.8 TB/s of
+// the bytes that one reading would take.
 //
 // A row has 8 to 64 lanes of a wave, 256 or 1024 of a workgroup, each with P pieces of 16 bytes.  Longer rows are read twice: once for the means, once by
 // column tiles with the means given.
